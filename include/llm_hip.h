@@ -136,6 +136,74 @@ int llm_sampler_state(llm_model *m, unsigned long long *rng);
 
 void llm_close(llm_model *m);
 
+/* ---- operators on device memory -----------------------------------------------------------------------------
+ *
+ * What a serving program that keeps its own tensors calls next to the token loop: K and V rows written into a cache of
+ * 8 bits and read back, attention for a tree of drafted tokens over a cache, log probabilities of given tokens.  The
+ * model calls the same kernels (llm_set_kv, llm_verify, llm_score).
+ *
+ * Every address is device memory (checked), all on one device, which need not be the current one.  The launches go to
+ * `stream` (a hipStream_t of that device; NULL: its default stream) and nothing is synchronized, allocated or kept, so a
+ * call can be captured into a graph.  Scratch memory is the caller's: calls that may overlap need one each.
+ * Returns 0, or -1 with a message on stderr; nothing is launched then. */
+enum { LLM_F32 = 0, LLM_BF16 = 1, LLM_I8 = 2, LLM_E4M3 = 3 };
+
+/* The K and V rows of n_seq sequences, ctx positions and n_kv heads of hs values (a multiple of 16, at most 256).  fp32
+ * and bf16 rows hold the values.  int8 and e4m3 rows hold codes, and k_scale / v_scale a float per row: value = code *
+ * scale.  Strides are in values (of K and V alike) and in floats (of the scales); the values of a row lie together, rows
+ * start at multiples of 4 bytes, and a position's stride is at most 16 MiB. */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;  /* NULL for fp32 and bf16 */
+    int type, n_seq, n_kv, hs, ctx;
+    int64_t seq, head, pos;       /* strides of k and v */
+    int64_t s_seq, s_head, s_pos; /* strides of the scales */
+} llm_kv;
+
+/* Rows of activations, fp32 or bf16: row (sequence, token, head) at p + its strides (in values; multiples of 4, the
+ * address too). */
+typedef struct {
+    void *p;
+    int type;
+    int64_t seq, tok, head;
+} llm_rows;
+
+/* Rows of K and V into the cache: token t < n[b] (n NULL: max_n, else at most max_n) of sequence b at position pos[b] + t.
+ * Positions outside 0 .. ctx - 1 are not written.  int8: scale = amax / 127 rounded to fp32, code = the quotient value /
+ * scale, exact, rounded half to even; e4m3: amax / 448, the quotient rounded to e4m3 half to even.  A row of zeros has
+ * scale 0; a row that holds an infinity or a NaN gets scale NaN and reads back as NaN.  pos and n: n_seq ints each. */
+int llm_kv_write(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos, const int *n, int max_n,
+                 void *stream);
+/* The values of positions pos[b] .. pos[b] + n[b] - 1 into rows 0 .. n[b] - 1 of k and v, rounded to their type.  Rows
+ * behind n[b] or whose position lies outside the cache are left as they were. */
+int llm_kv_read(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos, const int *n, int max_n,
+                void *stream);
+
+/* Attention of the n[b] <= max_n <= 64 newest tokens of every sequence over its cache (n NULL: max_n each).  Token i of
+ * sequence b has its K and V rows at position lens[b] + i; it sees positions 0 .. lens[b] - 1 and the new tokens j whose
+ * bit j is set in mask[b * max_n + i] (a drafted tree: its ancestors and itself; mask NULL: j <= i, a chain; max_n 1: the
+ * decode step).  out[b][i][h] = sum_p softmax_p(scale q.k_p) v_p over the kv head h / (n_heads / n_kv), in fp32, rounded to
+ * out's type (q's type).  A token that sees nothing gets zeros.  Rows behind n[b] are left as they were; positions from ctx
+ * on are not seen.  What is not seen has no influence, infinities and NaN included; a new token whose V row holds one makes
+ * the tokens that see it NaN.  n_heads / n_kv is at most 64.  max_len is the host's upper bound of lens[] (lens above it
+ * are right too, slower); `work` has llm_tree_attention_work() bytes, 16-byte aligned. */
+size_t llm_tree_attention_work(const llm_kv *c, int n_heads, int max_n, int max_len);
+int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_rows *out, int n_heads, const int *lens, const int *n,
+                       const uint64_t *mask, int max_n, int max_len, float scale, void *work, size_t work_bytes,
+                       void *stream);
+
+/* Log probabilities over `rows` rows of `vocab` logits (type LLM_F32 or LLM_BF16, `stride` values from row to row), of
+ * y = logit / temperature (1e-30 to 1e30): lse = log sum exp y, entropy = -sum p log p (nats), logp[r][i] = y[tokens[r][i]] - lse for
+ * n_tokens tokens a row (an id outside 0 .. vocab - 1: -infinity), and the `top` <= 32 largest logits of the row in
+ * descending order (equal ones, and NaN, which count as the largest: lowest index first) with their log probabilities.
+ * Masked logits of -infinity have probability 0.  A row with +infinity or NaN, or of -infinity alone, has NaN for its
+ * results (lse of -infinity alone: -infinity).  entropy and lse may be NULL, logp with n_tokens 0 and the two top arrays with top 0.  `work` has
+ * llm_logprobs_work() bytes, 16-byte aligned. */
+size_t llm_logprobs_work(int rows, int vocab, int top);
+int llm_logprobs(const void *logits, int type, int rows, int vocab, int64_t stride, float temperature, const int *tokens,
+                 int n_tokens, float *logp, float *entropy, float *lse, int top, int *top_ids, float *top_logp, void *work,
+                 size_t work_bytes, void *stream);
+
 /* ---- test hooks: no counterpart in the reference; they expose single device stages so the tests can
  * hold each one against the oracle (like the reference's FPGA_CHECK side-by-side check, qwen.c:464-472) --- */
 

@@ -29,6 +29,17 @@ class LlmInfo(C.Structure):
                 ("gemv_bytes_per_token", C.c_double), ("weight_bytes", C.c_double)]
 
 
+class LlmKv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("type", C.c_int), ("n_seq", C.c_int), ("n_kv", C.c_int), ("hs", C.c_int), ("ctx", C.c_int),
+                ("seq", C.c_int64), ("head", C.c_int64), ("pos", C.c_int64),
+                ("s_seq", C.c_int64), ("s_head", C.c_int64), ("s_pos", C.c_int64)]
+
+
+class LlmRows(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("type", C.c_int), ("seq", C.c_int64), ("tok", C.c_int64), ("head", C.c_int64)]
+
+
 class LlmTiming(C.Structure):
     _fields_ = [("n_prompt", C.c_int), ("n_generated", C.c_int), ("n_forward", C.c_int),
                 ("prompt_ms", C.c_double), ("decode_ms", C.c_double)]
@@ -93,6 +104,15 @@ def lib():
     L.mvh_seq_sum.argtypes = [vp, i32, i32, i32, vp]
     L.llm_set_strict.argtypes = [vp, i32]
     L.llm_get_strict.argtypes = [vp]
+    pkv, prows = C.POINTER(LlmKv), C.POINTER(LlmRows)
+    L.llm_kv_write.argtypes = [pkv, prows, prows, vp, vp, i32, vp]
+    L.llm_kv_read.argtypes = [pkv, prows, prows, vp, vp, i32, vp]
+    L.llm_tree_attention_work.argtypes = [pkv, i32, i32, i32]
+    L.llm_tree_attention_work.restype = sz
+    L.llm_tree_attention.argtypes = [pkv, prows, prows, i32, vp, vp, vp, i32, i32, C.c_float, vp, sz, vp]
+    L.llm_logprobs_work.argtypes = [i32, i32, i32]
+    L.llm_logprobs_work.restype = sz
+    L.llm_logprobs.argtypes = [vp, i32, i32, i32, C.c_int64, C.c_float, vp, i32, vp, vp, vp, i32, vp, vp, vp, sz, vp]
     _lib = L
     return L
 
@@ -184,6 +204,151 @@ def ref_expf(x, host=False):
     if fn(_ptr(x), x.size, _ptr(y)) != 0:
         raise RuntimeError("mvh_ref_expf failed")
     return y
+
+
+# ---- operators on device memory (torch tensors) -----------------------------------------------------------
+
+_torch = None
+
+
+def _types():
+    """torch and its types' LLM_* numbers (torch is imported by the first call that is given its tensors)"""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch, {torch.float32: 0, torch.bfloat16: 1, torch.int8: 2, torch.float8_e4m3fn: 3}
+    return _torch
+
+
+def _stream(t):
+    return _torch[0].cuda.current_stream(t.device).cuda_stream
+
+
+def _ints(name, t, shape, device, dtype=None):
+    """the address of a contiguous int32 tensor of this shape (None: NULL)"""
+    if t is None:
+        return None
+    if t.dtype != (dtype or _torch[0].int32) or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name}: a contiguous {dtype or 'int32'} tensor of {shape} on {device} is needed")
+    return t.data_ptr()
+
+
+def _kv(k, v, k_scale, v_scale):
+    """the cache of tensors [seqs, kv heads, positions, head size] (any strides, a row's values together) and, for int8 and
+    e4m3, scales [seqs, kv heads, positions]"""
+    torch, types = _types()
+    ty, shape, st = types.get(k.dtype), k.shape, k.stride()
+    if ty is None or v.dtype != k.dtype or v.shape != shape or len(shape) != 4 or v.device != k.device or not k.is_cuda:
+        raise ValueError("k and v: device tensors [seqs, kv heads, positions, head size] of one type (float32, bfloat16, "
+                         "int8, float8_e4m3fn) are needed")
+    b, h, ctx, hs = shape
+    # (a dimension of one has no stride that counts)
+    def strides(s, inner):
+        return s[0] if b > 1 else 0, s[1] if h > 1 else 0, s[2] if ctx > 1 else inner
+    if strides(v.stride(), hs) != strides(st, hs) or (hs > 1 and (st[3] != 1 or v.stride()[3] != 1)):
+        raise ValueError("k and v: equal strides with a row's values together are needed")
+    if ty < 2:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("scales belong to int8 and e4m3 caches")
+        return LlmKv(k.data_ptr(), v.data_ptr(), None, None, ty, b, h, hs, ctx, *strides(st, hs), 0, 0, 1)
+    for s in (k_scale, v_scale):
+        if s is None or s.dtype != torch.float32 or s.shape != shape[:3] or s.device != k.device:
+            raise ValueError("an int8 or e4m3 cache needs float32 scales [seqs, kv heads, positions]")
+    ss = strides(k_scale.stride(), 1)
+    if strides(v_scale.stride(), 1) != ss:
+        raise ValueError("k_scale and v_scale: equal strides are needed")
+    return LlmKv(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, b, h, hs, ctx,
+                 *strides(st, hs), *ss)
+
+
+def _rows(name, x, shape, device):
+    """rows [seqs, tokens, heads, head size], float32 or bfloat16, a row's values together"""
+    ty = _torch[1].get(x.dtype)
+    if ty is None or ty > 1 or x.shape != shape or x.device != device or (shape[3] > 1 and x.stride(3) != 1):
+        raise ValueError(f"{name}: float32 or bfloat16 rows {tuple(shape)} on {device} are needed")
+    st = x.stride()
+    return LlmRows(x.data_ptr(), ty, *(st[i] if shape[i] > 1 else 0 for i in range(3)))
+
+
+def kv_write(k_rows, v_rows, k, v, pos, n=None, k_scale=None, v_scale=None):
+    """Rows [seqs, tokens, kv heads, head size] into the cache (llm_kv_write): token t < n[b] of sequence b at position
+    pos[b] + t.  The cache: k and v [seqs, kv heads, positions, head size] of float32, bfloat16, int8 or float8_e4m3fn, the
+    last two with float32 scales [seqs, kv heads, positions]."""
+    c = _kv(k, v, k_scale, v_scale)
+    b, h, _, hs = k.shape
+    t = k_rows.shape[1]
+    kr, vr = _rows("k_rows", k_rows, (b, t, h, hs), k.device), _rows("v_rows", v_rows, (b, t, h, hs), k.device)
+    if lib().llm_kv_write(C.byref(c), C.byref(kr), C.byref(vr), _ints("pos", pos, (b,), k.device),
+                          _ints("n", n, (b,), k.device), t, _stream(k)) != 0:
+        raise RuntimeError("llm_kv_write failed")
+
+
+def kv_read(k, v, pos, tokens, n=None, k_scale=None, v_scale=None, out=None, dtype=None):
+    """The values of positions pos[b] .. pos[b] + n[b] - 1 (n None: `tokens` each) as rows [seqs, tokens, kv heads, head
+    size] of K and V (llm_kv_read), float32 or `dtype`; new tensors (rows that are not read: zero) or `out`, a pair (such
+    rows left as they were)."""
+    torch, _ = _types()
+    c = _kv(k, v, k_scale, v_scale)
+    b, h, _, hs = k.shape
+    if out is None:
+        out = [torch.zeros(b, tokens, h, hs, dtype=dtype or torch.float32, device=k.device) for _ in range(2)]
+    kr, vr = _rows("out", out[0], (b, tokens, h, hs), k.device), _rows("out", out[1], (b, tokens, h, hs), k.device)
+    if lib().llm_kv_read(C.byref(c), C.byref(kr), C.byref(vr), _ints("pos", pos, (b,), k.device),
+                         _ints("n", n, (b,), k.device), tokens, _stream(k)) != 0:
+        raise RuntimeError("llm_kv_read failed")
+    return out[0], out[1]
+
+
+def tree_attention(q, k, v, lens, n=None, mask=None, k_scale=None, v_scale=None, scale=None, max_len=None, out=None):
+    """Attention of the newest tokens of every sequence over its cache (llm_tree_attention).  q [seqs, tokens <= 64, heads,
+    head size] float32 or bfloat16; the cache as in kv_write; token i of sequence b has its rows at position lens[b] + i and
+    sees the positions before lens[b] and the new tokens of mask[b, i]'s bits (int64; None: a chain).  n[b] tokens count
+    (None: all); scale None: head size ** -0.5; max_len: the host's bound of lens (None: the cache's positions).  Returns
+    `out`, or a new tensor (rows behind n[b]: zero)."""
+    torch, _ = _types()
+    c = _kv(k, v, k_scale, v_scale)
+    b, t, heads, hs = q.shape
+    if b != c.n_seq or hs != c.hs:
+        raise ValueError(f"q: {tuple(q.shape)} over a cache {tuple(k.shape)}")
+    qr = _rows("q", q, q.shape, k.device)
+    if out is None:
+        out = (torch.empty if n is None else torch.zeros)(b, t, heads, hs, dtype=q.dtype, device=k.device)
+    orow = _rows("out", out, q.shape, k.device)
+    L, cp = lib(), C.byref(c)
+    bound = c.ctx if max_len is None else max_len
+    need = L.llm_tree_attention_work(cp, heads, t, bound)
+    work = torch.empty(need, dtype=torch.uint8, device=k.device) if need else None
+    if L.llm_tree_attention(cp, C.byref(qr), C.byref(orow), heads, _ints("lens", lens, (b,), k.device),
+                            _ints("n", n, (b,), k.device), _ints("mask", mask, (b, t), k.device, torch.int64), t, bound,
+                            hs ** -0.5 if scale is None else scale, work.data_ptr() if need else None, need,
+                            _stream(k)) != 0:
+        raise RuntimeError("llm_tree_attention failed")
+    return out
+
+
+def logprobs(logits, tokens=None, top=0, temperature=1.0):
+    """Log probabilities of logits / temperature (llm_logprobs): logits [rows, vocab] float32 or bfloat16 (any row stride),
+    tokens [rows, count] int32.  Returns (logp [rows, count] of the tokens, entropy [rows], top_ids [rows, top] and top_logp
+    [rows, top] of the largest logits in descending order, lse [rows])."""
+    torch, types = _types()
+    rows, vocab = logits.shape
+    ty, dev = types.get(logits.dtype), logits.device
+    if ty is None or ty > 1 or not logits.is_cuda or (vocab > 1 and logits.stride(1) != 1):
+        raise ValueError("logits: float32 or bfloat16 rows on the device are needed")
+    count = tokens.shape[1] if tokens is not None else 0
+    f32 = torch.float32
+    logp, top_logp = torch.empty(rows, count, dtype=f32, device=dev), torch.empty(rows, top, dtype=f32, device=dev)
+    top_ids = torch.empty(rows, top, dtype=torch.int32, device=dev)
+    entropy, lse = torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev)
+    L = lib()
+    need = L.llm_logprobs_work(rows, vocab, top)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    if rows and L.llm_logprobs(logits.data_ptr(), ty, rows, vocab, logits.stride(0) if rows > 1 else vocab, temperature,
+                               _ints("tokens", tokens, (rows, count), dev), count, logp.data_ptr(), entropy.data_ptr(),
+                               lse.data_ptr(), top, top_ids.data_ptr(), top_logp.data_ptr(),
+                               work.data_ptr() if need else None, need, _stream(logits)) != 0:
+        raise RuntimeError("llm_logprobs failed")
+    return logp, entropy, top_ids, top_logp, lse
 
 
 # ---- drop-in driver API -----------------------------------------------------------------------------------
