@@ -174,23 +174,23 @@ typedef struct {
  * scale 0; a row that holds an infinity or a NaN gets scale NaN and reads back as NaN.  pos and n: n_seq ints each. */
 int llm_kv_write(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos, const int *n, int max_n,
                  void *stream);
-/* The values of positions pos[b] .. pos[b] + n[b] - 1 into rows 0 .. n[b] - 1 of k and v, rounded to their type.  Rows
- * behind n[b] or whose position lies outside the cache are left as they were. */
+/* The values of positions pos[b] .. pos[b] + n[b] - 1 into rows 0 .. n[b] - 1 of k and v, rounded to their type.  The
+ * rows behind n[b], and those whose position lies outside the cache, are left as they were, or zeroed (zero_rest). */
 int llm_kv_read(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos, const int *n, int max_n,
-                void *stream);
+                int zero_rest, void *stream);
 
 /* Attention of the n[b] <= max_n <= 64 newest tokens of every sequence over its cache (n NULL: max_n each).  Token i of
  * sequence b has its K and V rows at position lens[b] + i; it sees positions 0 .. lens[b] - 1 and the new tokens j whose
  * bit j is set in mask[b * max_n + i] (a drafted tree: its ancestors and itself; mask NULL: j <= i, a chain; max_n 1: the
  * decode step).  out[b][i][h] = sum_p softmax_p(scale q.k_p) v_p over the kv head h / (n_heads / n_kv), in fp32, rounded to
- * out's type (q's type).  A token that sees nothing gets zeros.  Rows behind n[b] are left as they were; positions from ctx
- * on are not seen.  What is not seen has no influence, infinities and NaN included; a new token whose V row holds one makes
+ * out's type (q's type).  A token that sees nothing gets zeros.  Rows behind n[b] are left as they were, or zeroed
+ * (zero_rest); positions from ctx on are not seen.  What is not seen has no influence, infinities and NaN included; a new token whose V row holds one makes
  * the tokens that see it NaN.  n_heads / n_kv is at most 64.  max_len is the host's upper bound of lens[] (lens above it
  * are right too, slower); `work` has llm_tree_attention_work() bytes, 16-byte aligned. */
 size_t llm_tree_attention_work(const llm_kv *c, int n_heads, int max_n, int max_len);
 int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_rows *out, int n_heads, const int *lens, const int *n,
-                       const uint64_t *mask, int max_n, int max_len, float scale, void *work, size_t work_bytes,
-                       void *stream);
+                       const uint64_t *mask, int max_n, int max_len, float scale, int zero_rest, void *work,
+                       size_t work_bytes, void *stream);
 
 /* Log probabilities over `rows` rows of `vocab` logits (type LLM_F32 or LLM_BF16, `stride` values from row to row), of
  * y = logit / temperature (1e-30 to 1e30): lse = log sum exp y, entropy = -sum p log p (nats), logp[r][i] = y[tokens[r][i]] - lse for

@@ -10,6 +10,7 @@ The directory name is not a Python identifier, so callers load this file by path
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -104,12 +105,11 @@ def lib():
     L.mvh_seq_sum.argtypes = [vp, i32, i32, i32, vp]
     L.llm_set_strict.argtypes = [vp, i32]
     L.llm_get_strict.argtypes = [vp]
-    pkv, prows = C.POINTER(LlmKv), C.POINTER(LlmRows)
-    L.llm_kv_write.argtypes = [pkv, prows, prows, vp, vp, i32, vp]
-    L.llm_kv_read.argtypes = [pkv, prows, prows, vp, vp, i32, vp]
-    L.llm_tree_attention_work.argtypes = [pkv, i32, i32, i32]
+    L.llm_kv_write.argtypes = [vp, vp, vp, vp, vp, i32, vp]
+    L.llm_kv_read.argtypes = [vp, vp, vp, vp, vp, i32, i32, vp]
+    L.llm_tree_attention_work.argtypes = [vp, i32, i32, i32]
     L.llm_tree_attention_work.restype = sz
-    L.llm_tree_attention.argtypes = [pkv, prows, prows, i32, vp, vp, vp, i32, i32, C.c_float, vp, sz, vp]
+    L.llm_tree_attention.argtypes = [vp, vp, vp, i32, vp, vp, vp, i32, i32, C.c_float, i32, vp, sz, vp]
     L.llm_logprobs_work.argtypes = [i32, i32, i32]
     L.llm_logprobs_work.restype = sz
     L.llm_logprobs.argtypes = [vp, i32, i32, i32, C.c_int64, C.c_float, vp, i32, vp, vp, vp, i32, vp, vp, vp, sz, vp]
@@ -207,8 +207,12 @@ def ref_expf(x, host=False):
 
 
 # ---- operators on device memory (torch tensors) -----------------------------------------------------------
+# (a call's host time is most of a small call's: the C structs are packed in one step, and what the library checks by
+# itself, that every address is memory of one device, is not checked here again)
 
 _torch = None
+_PACK_KV = struct.Struct("4P5i4x6q").pack
+_PACK_ROWS = struct.Struct("Pi4x3q").pack
 
 
 def _types():
@@ -221,65 +225,67 @@ def _types():
 
 
 def _stream(t):
-    return _torch[0].cuda.current_stream(t.device).cuda_stream
+    """the current stream of a tensor's device"""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError("device tensors are needed")
+    return _torch[0].cuda.current_stream(dev).cuda_stream
 
 
-def _ints(name, t, shape, device, dtype=None):
-    """the address of a contiguous int32 tensor of this shape (None: NULL)"""
+def _ints(name, t, count, dtype):
+    """the address of `count` contiguous integers (None: NULL)"""
     if t is None:
         return None
-    if t.dtype != (dtype or _torch[0].int32) or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name}: a contiguous {dtype or 'int32'} tensor of {shape} on {device} is needed")
+    if t.dtype is not dtype or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{name}: {count} contiguous {dtype} are needed")
     return t.data_ptr()
 
 
 def _kv(k, v, k_scale, v_scale):
-    """the cache of tensors [seqs, kv heads, positions, head size] (any strides, a row's values together) and, for int8 and
-    e4m3, scales [seqs, kv heads, positions]"""
-    torch, types = _types()
-    ty, shape, st = types.get(k.dtype), k.shape, k.stride()
-    if ty is None or v.dtype != k.dtype or v.shape != shape or len(shape) != 4 or v.device != k.device or not k.is_cuda:
-        raise ValueError("k and v: device tensors [seqs, kv heads, positions, head size] of one type (float32, bfloat16, "
-                         "int8, float8_e4m3fn) are needed")
+    """llm_kv of tensors [seqs, kv heads, positions, head size] (any strides, a row's values together) and, for int8 and
+    e4m3, scales [seqs, kv heads, positions]; and its dimensions"""
+    shape, types = k.shape, _types()[1]
+    ty = types.get(k.dtype)
+    if ty is None or v.dtype is not k.dtype or v.shape != shape or len(shape) != 4:
+        raise ValueError("k and v: tensors [seqs, kv heads, positions, head size] of one type (float32, bfloat16, int8, "
+                         "float8_e4m3fn) are needed")
     b, h, ctx, hs = shape
     # (a dimension of one has no stride that counts)
     def strides(s, inner):
         return s[0] if b > 1 else 0, s[1] if h > 1 else 0, s[2] if ctx > 1 else inner
-    if strides(v.stride(), hs) != strides(st, hs) or (hs > 1 and (st[3] != 1 or v.stride()[3] != 1)):
+    st, sv = k.stride(), v.stride()
+    if st[3] != 1 or sv[3] != 1 or (st != sv and strides(st, hs) != strides(sv, hs)):
         raise ValueError("k and v: equal strides with a row's values together are needed")
     if ty < 2:
         if k_scale is not None or v_scale is not None:
             raise ValueError("scales belong to int8 and e4m3 caches")
-        return LlmKv(k.data_ptr(), v.data_ptr(), None, None, ty, b, h, hs, ctx, *strides(st, hs), 0, 0, 1)
-    for s in (k_scale, v_scale):
-        if s is None or s.dtype != torch.float32 or s.shape != shape[:3] or s.device != k.device:
-            raise ValueError("an int8 or e4m3 cache needs float32 scales [seqs, kv heads, positions]")
-    ss = strides(k_scale.stride(), 1)
-    if strides(v_scale.stride(), 1) != ss:
+        return _PACK_KV(k.data_ptr(), v.data_ptr(), 0, 0, ty, b, h, hs, ctx, *strides(st, hs), 0, 0, 1), shape
+    if k_scale is None or v_scale is None or k_scale.shape != shape[:3] or v_scale.shape != shape[:3] or \
+            k_scale.dtype is not _torch[0].float32 or v_scale.dtype is not _torch[0].float32:
+        raise ValueError("an int8 or e4m3 cache needs float32 scales [seqs, kv heads, positions]")
+    ss, sv = k_scale.stride(), v_scale.stride()
+    if ss != sv and strides(ss, 1) != strides(sv, 1):
         raise ValueError("k_scale and v_scale: equal strides are needed")
-    return LlmKv(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, b, h, hs, ctx,
-                 *strides(st, hs), *ss)
+    return _PACK_KV(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, b, h, hs, ctx,
+                    *strides(st, hs), *strides(ss, 1)), shape
 
 
-def _rows(name, x, shape, device):
-    """rows [seqs, tokens, heads, head size], float32 or bfloat16, a row's values together"""
-    ty = _torch[1].get(x.dtype)
-    if ty is None or ty > 1 or x.shape != shape or x.device != device or (shape[3] > 1 and x.stride(3) != 1):
-        raise ValueError(f"{name}: float32 or bfloat16 rows {tuple(shape)} on {device} are needed")
-    st = x.stride()
-    return LlmRows(x.data_ptr(), ty, *(st[i] if shape[i] > 1 else 0 for i in range(3)))
+def _rows(name, x, b, t, h, hs):
+    """llm_rows of a tensor [b, t, h, hs], float32 or bfloat16, a row's values together"""
+    ty, st = _torch[1].get(x.dtype, 4), x.stride()
+    if ty > 1 or x.shape != (b, t, h, hs) or st[3] != 1:
+        raise ValueError(f"{name}: float32 or bfloat16 rows {(b, t, h, hs)} are needed")
+    return _PACK_ROWS(x.data_ptr(), ty, st[0] if b > 1 else 0, st[1] if t > 1 else 0, st[2] if h > 1 else 0)
 
 
 def kv_write(k_rows, v_rows, k, v, pos, n=None, k_scale=None, v_scale=None):
     """Rows [seqs, tokens, kv heads, head size] into the cache (llm_kv_write): token t < n[b] of sequence b at position
     pos[b] + t.  The cache: k and v [seqs, kv heads, positions, head size] of float32, bfloat16, int8 or float8_e4m3fn, the
     last two with float32 scales [seqs, kv heads, positions]."""
-    c = _kv(k, v, k_scale, v_scale)
-    b, h, _, hs = k.shape
-    t = k_rows.shape[1]
-    kr, vr = _rows("k_rows", k_rows, (b, t, h, hs), k.device), _rows("v_rows", v_rows, (b, t, h, hs), k.device)
-    if lib().llm_kv_write(C.byref(c), C.byref(kr), C.byref(vr), _ints("pos", pos, (b,), k.device),
-                          _ints("n", n, (b,), k.device), t, _stream(k)) != 0:
+    c, (b, h, _, hs) = _kv(k, v, k_scale, v_scale)
+    t, i32 = k_rows.shape[1], _torch[0].int32
+    if lib().llm_kv_write(c, _rows("k_rows", k_rows, b, t, h, hs), _rows("v_rows", v_rows, b, t, h, hs),
+                          _ints("pos", pos, b, i32), _ints("n", n, b, i32), t, _stream(k)) != 0:
         raise RuntimeError("llm_kv_write failed")
 
 
@@ -287,14 +293,12 @@ def kv_read(k, v, pos, tokens, n=None, k_scale=None, v_scale=None, out=None, dty
     """The values of positions pos[b] .. pos[b] + n[b] - 1 (n None: `tokens` each) as rows [seqs, tokens, kv heads, head
     size] of K and V (llm_kv_read), float32 or `dtype`; new tensors (rows that are not read: zero) or `out`, a pair (such
     rows left as they were)."""
-    torch, _ = _types()
-    c = _kv(k, v, k_scale, v_scale)
-    b, h, _, hs = k.shape
-    if out is None:
-        out = [torch.zeros(b, tokens, h, hs, dtype=dtype or torch.float32, device=k.device) for _ in range(2)]
-    kr, vr = _rows("out", out[0], (b, tokens, h, hs), k.device), _rows("out", out[1], (b, tokens, h, hs), k.device)
-    if lib().llm_kv_read(C.byref(c), C.byref(kr), C.byref(vr), _ints("pos", pos, (b,), k.device),
-                         _ints("n", n, (b,), k.device), tokens, _stream(k)) != 0:
+    c, (b, h, _, hs) = _kv(k, v, k_scale, v_scale)
+    torch, fresh = _torch[0], out is None
+    if fresh:
+        out = torch.empty(2, b, tokens, h, hs, dtype=dtype or torch.float32, device=k.device).unbind()
+    if lib().llm_kv_read(c, _rows("out", out[0], b, tokens, h, hs), _rows("out", out[1], b, tokens, h, hs),
+                         _ints("pos", pos, b, torch.int32), _ints("n", n, b, torch.int32), tokens, fresh, _stream(k)) != 0:
         raise RuntimeError("llm_kv_read failed")
     return out[0], out[1]
 
@@ -304,24 +308,19 @@ def tree_attention(q, k, v, lens, n=None, mask=None, k_scale=None, v_scale=None,
     head size] float32 or bfloat16; the cache as in kv_write; token i of sequence b has its rows at position lens[b] + i and
     sees the positions before lens[b] and the new tokens of mask[b, i]'s bits (int64; None: a chain).  n[b] tokens count
     (None: all); scale None: head size ** -0.5; max_len: the host's bound of lens (None: the cache's positions).  Returns
-    `out`, or a new tensor (rows behind n[b]: zero)."""
-    torch, _ = _types()
-    c = _kv(k, v, k_scale, v_scale)
-    b, t, heads, hs = q.shape
-    if b != c.n_seq or hs != c.hs:
-        raise ValueError(f"q: {tuple(q.shape)} over a cache {tuple(k.shape)}")
-    qr = _rows("q", q, q.shape, k.device)
-    if out is None:
-        out = (torch.empty if n is None else torch.zeros)(b, t, heads, hs, dtype=q.dtype, device=k.device)
-    orow = _rows("out", out, q.shape, k.device)
-    L, cp = lib(), C.byref(c)
-    bound = c.ctx if max_len is None else max_len
-    need = L.llm_tree_attention_work(cp, heads, t, bound)
+    a new tensor (rows behind n[b]: zero), or `out` (such rows left as they were)."""
+    c, (b, _, ctx, hs) = _kv(k, v, k_scale, v_scale)
+    torch, fresh = _torch[0], out is None
+    t, heads = q.shape[1:3]
+    if fresh:
+        out = torch.empty(b, t, heads, hs, dtype=q.dtype, device=k.device)
+    L, bound = lib(), ctx if max_len is None else max_len
+    need = L.llm_tree_attention_work(c, heads, t, bound)
     work = torch.empty(need, dtype=torch.uint8, device=k.device) if need else None
-    if L.llm_tree_attention(cp, C.byref(qr), C.byref(orow), heads, _ints("lens", lens, (b,), k.device),
-                            _ints("n", n, (b,), k.device), _ints("mask", mask, (b, t), k.device, torch.int64), t, bound,
-                            hs ** -0.5 if scale is None else scale, work.data_ptr() if need else None, need,
-                            _stream(k)) != 0:
+    if L.llm_tree_attention(c, _rows("q", q, b, t, heads, hs), _rows("out", out, b, t, heads, hs), heads,
+                            _ints("lens", lens, b, torch.int32), _ints("n", n, b, torch.int32),
+                            _ints("mask", mask, b * t, torch.int64), t, bound, hs ** -0.5 if scale is None else scale, fresh,
+                            work.data_ptr() if need else None, need, _stream(k)) != 0:
         raise RuntimeError("llm_tree_attention failed")
     return out
 
@@ -332,23 +331,26 @@ def logprobs(logits, tokens=None, top=0, temperature=1.0):
     [rows, top] of the largest logits in descending order, lse [rows])."""
     torch, types = _types()
     rows, vocab = logits.shape
-    ty, dev = types.get(logits.dtype), logits.device
-    if ty is None or ty > 1 or not logits.is_cuda or (vocab > 1 and logits.stride(1) != 1):
-        raise ValueError("logits: float32 or bfloat16 rows on the device are needed")
+    ty, st = types.get(logits.dtype, 4), logits.stride()
+    if ty > 1 or (vocab > 1 and st[1] != 1) or (tokens is not None and (tokens.dim() != 2 or tokens.shape[0] != rows)):
+        raise ValueError("logits: float32 or bfloat16 rows [rows, vocab], tokens: [rows, count] are needed")
     count = tokens.shape[1] if tokens is not None else 0
-    f32 = torch.float32
-    logp, top_logp = torch.empty(rows, count, dtype=f32, device=dev), torch.empty(rows, top, dtype=f32, device=dev)
-    top_ids = torch.empty(rows, top, dtype=torch.int32, device=dev)
-    entropy, lse = torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev)
     L = lib()
     need = L.llm_logprobs_work(rows, vocab, top)
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    if rows and L.llm_logprobs(logits.data_ptr(), ty, rows, vocab, logits.stride(0) if rows > 1 else vocab, temperature,
-                               _ints("tokens", tokens, (rows, count), dev), count, logp.data_ptr(), entropy.data_ptr(),
-                               lse.data_ptr(), top, top_ids.data_ptr(), top_logp.data_ptr(),
-                               work.data_ptr() if need else None, need, _stream(logits)) != 0:
+    # one allocation: the results, and the scratch memory behind them
+    at = rows * (2 + 2 * top + count)
+    at += -at % 4
+    mem = torch.empty(at + need // 4, dtype=torch.float32, device=logits.device)
+    entropy, lse, ids, top_logp, logp, _ = mem.split_with_sizes(
+        (rows, rows, rows * top, rows * top, rows * count, mem.numel() - rows * (2 + 2 * top + count)))
+    ids = ids.view(torch.int32)
+    p = mem.data_ptr()
+    if rows and L.llm_logprobs(logits.data_ptr(), ty, rows, vocab, st[0] if rows > 1 else vocab, temperature,
+                               _ints("tokens", tokens, rows * count, torch.int32) if count else None, count,
+                               p + 4 * rows * (2 + 2 * top), p, p + 4 * rows, top, p + 8 * rows, p + 4 * rows * (2 + top),
+                               p + 4 * at if need else None, need, _stream(logits)) != 0:
         raise RuntimeError("llm_logprobs failed")
-    return logp, entropy, top_ids, top_logp, lse
+    return logp.view(rows, count), entropy, ids.view(rows, top), top_logp.view(rows, top), lse
 
 
 # ---- drop-in driver API -----------------------------------------------------------------------------------

@@ -16,7 +16,7 @@ struct KvArgs {
     int64_t seq, head, pos, s_seq, s_head, s_pos; // cache
     int64_t r_seq[2], r_tok[2], r_head[2];        // rows, of K and V
     const int *at, *n;
-    int n_kv, hs, ctx, max_n;
+    int n_kv, hs, ctx, max_n, zero_rest;
     uint32_t rows; // n_seq * max_n * n_kv
 };
 
@@ -127,8 +127,12 @@ __global__ void __launch_bounds__(256) k_kv_read(KvArgs a) {
     if (item >= a.rows) return;
     const uint32_t h = item % a.n_kv, bt = item / a.n_kv, t = bt % a.max_n, b = bt / a.max_n;
     const int64_t p = (int64_t)a.at[b] + t;
-    if ((a.n && (int)t >= a.n[b]) || p < 0 || p >= a.ctx) return;
     uint8_t *dst = a.side[side].r + b * a.r_seq[side] + t * a.r_tok[side] + h * a.r_head[side];
+    if ((a.n && (int)t >= a.n[b]) || p < 0 || p >= a.ctx) {
+        if (a.zero_rest)
+            for (int e = 4 * l; e < a.hs; e += 64) put4<RT>(dst + (size_t)e * RS, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        return;
+    }
     const uint8_t *src = a.side[side].c + b * a.seq + h * a.head + p * a.pos;
     float s = 1.0f;
     if constexpr (CS == 1) s = a.side[side].s[b * a.s_seq + h * a.s_head + p * a.s_pos];
@@ -163,7 +167,7 @@ __global__ void __launch_bounds__(256) k_kv_read(KvArgs a) {
 }
 
 int kv_rows(const char *who, bool write, const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos,
-            const int *n, int max_n, void *stream) {
+            const int *n, int max_n, int zero_rest, void *stream) {
     if (!c || !k || !v || max_n < 0) {
         fprintf(stderr, "%s: bad arguments\n", who);
         return -1;
@@ -197,7 +201,7 @@ int kv_rows(const char *who, bool write, const llm_kv *c, const llm_rows *k, con
     }
     a.at = pos;
     a.n = n;
-    a.n_kv = c->n_kv, a.hs = c->hs, a.ctx = c->ctx, a.max_n = max_n;
+    a.n_kv = c->n_kv, a.hs = c->hs, a.ctx = c->ctx, a.max_n = max_n, a.zero_rest = zero_rest;
     a.rows = (uint32_t)rows;
     void (*kern)(KvArgs) = nullptr;
 #define KV_PICK(C, R)                                                                 \
@@ -259,10 +263,10 @@ bool op_check_rows(const llm_rows *r, const char *what, OpDevice *dev, const cha
 
 extern "C" int llm_kv_write(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos, const int *n, int max_n,
                             void *stream) {
-    return kv_rows("llm_kv_write", true, c, k, v, pos, n, max_n, stream);
+    return kv_rows("llm_kv_write", true, c, k, v, pos, n, max_n, 0, stream);
 }
 
 extern "C" int llm_kv_read(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos, const int *n, int max_n,
-                           void *stream) {
-    return kv_rows("llm_kv_read", false, c, k, v, pos, n, max_n, stream);
+                           int zero_rest, void *stream) {
+    return kv_rows("llm_kv_read", false, c, k, v, pos, n, max_n, zero_rest, stream);
 }

@@ -17,7 +17,7 @@ struct TreeArgs {
     int64_t o_seq, o_tok, o_head;
     const int *lens, *n;
     const uint64_t *mask;
-    int n_seq, n_kv, hs, ctx, group, max_n;
+    int n_seq, n_kv, hs, ctx, group, max_n, zero_rest;
     int splits;                    // slices of a sequence's positions, at most
     float c;                       // softmax scale * log2(e)
     float *ml, *acc;               // slices: [seq][kv head][slice][row] (max, sum), the same with hs sums of values

@@ -103,8 +103,8 @@ extern "C" size_t llm_tree_attention_work(const llm_kv *c, int n_heads, int max_
 }
 
 extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_rows *out, int n_heads, const int *lens,
-                                  const int *n, const uint64_t *mask, int max_n, int max_len, float scale, void *work,
-                                  size_t work_bytes, void *stream) {
+                                  const int *n, const uint64_t *mask, int max_n, int max_len, float scale, int zero_rest,
+                                  void *work, size_t work_bytes, void *stream) {
     const char *who = "llm_tree_attention";
     if (c && !op_check_cache(c, nullptr, who)) return -1;
     if (!c || !q || !out || !tree_shape_ok(c, n_heads, max_n)) {
@@ -145,7 +145,7 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
     a.o_seq = out->seq * qs, a.o_tok = out->tok * qs, a.o_head = out->head * qs;
     a.lens = lens, a.n = n, a.mask = mask;
     a.n_seq = c->n_seq, a.n_kv = c->n_kv, a.hs = c->hs, a.ctx = c->ctx;
-    a.group = n_heads / c->n_kv, a.max_n = max_n, a.splits = p.splits;
+    a.group = n_heads / c->n_kv, a.max_n = max_n, a.splits = p.splits, a.zero_rest = zero_rest;
     a.c = scale * 1.44269504088896340736f;
     a.acc = (float *)work; // (rows of hs values, hs a multiple of 16: 16-byte aligned)
     a.ml = (float *)work + (p.bytes / 4 / (c->hs + 2)) * c->hs;

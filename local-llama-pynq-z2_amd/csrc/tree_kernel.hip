@@ -140,6 +140,15 @@ __global__ void __launch_bounds__(256) k_tree_attention(TreeArgs a) {
     const int end = min((int64_t)len + nn, (int64_t)a.ctx), rows = nn * a.group, row0 = blockIdx.y * 16 * R;
     int steps;
     const int slices = tree_slices(end, TP, a.splits, &steps);
+    if (a.zero_rest && split_id == 0) { // the rows behind the last token
+        for (int e = threadIdx.x * 4; e < 16 * R * a.hs; e += 1024) {
+            const int row = row0 + e / a.hs, t = row / a.group, d = e - (row - row0) * a.hs;
+            if (row < rows || row >= a.max_n * a.group) continue;
+            uint8_t *op = a.o + b * a.o_seq + t * a.o_tok + (h * a.group + row - t * a.group) * a.o_head;
+            if constexpr (QT == LLM_F32) *(float4 *)(op + (size_t)d * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            else *(uint2 *)(op + (size_t)d * 2) = make_uint2(0, 0);
+        }
+    }
     if (row0 >= rows || split_id >= slices) return;
     const int all = (end + TP - 1) / TP, first = split_id * steps, last = min(first + steps, all);
 

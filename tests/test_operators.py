@@ -31,7 +31,7 @@ def write(c, r=None, v=None, n=1):
 def attend(c, q=None, out=None, heads=4, n=1, work=0):
     q = q or rows()
     return pkg().lib().llm_tree_attention(C.byref(c), C.byref(q), C.byref(out or q), heads, 0x10000, None, None, n, 10, 0.1,
-                                          None, work, None)
+                                          0, None, work, None)
 
 
 def logp(type=F32, rows=1, vocab=100, stride=100, t=1.0, n=0, top=0, p=0x10000):
