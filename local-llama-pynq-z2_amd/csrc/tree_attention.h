@@ -18,30 +18,27 @@ struct TreeArgs {
     const int *lens, *n;
     const uint64_t *mask;
     int n_seq, n_kv, hs, ctx, group, max_n, zero_rest;
-    int splits;                    // slices of a sequence's positions, at most
-    float c;                       // softmax scale * log2(e)
+    int splits, quantum;           // slices of a sequence's positions: at most, and their steps
+    float c;                       // |softmax scale| * log2(e), positive
+    int negate;                    // the scale is negative: the queries change their sign
     float *ml, *acc;               // slices: [seq][kv head][slice][row] (max, sum), the same with hs sums of values
 };
 
-// A wave's step over the positions, a block's four waves side by side.
-__host__ __device__ constexpr int tree_positions(int hsp, int type) {
-    return hsp * (type == LLM_F32 ? 4 : type == LLM_BF16 ? 2 : 1) <= 128 ? 64 : 32;
+// Positions of a step.  Few rows: a wave's step, its rows held in registers; many rows: the block's, in LDS.
+__host__ __device__ constexpr int tree_positions(int hsp, int type, bool many) {
+    return many || hsp * (type == LLM_F32 ? 4 : type == LLM_BF16 ? 2 : 1) <= 128 ? 64 : 32;
 }
-// Slices of `end` positions: a block's four waves have a step each at least; none is empty.
-__host__ __device__ inline int tree_slices(int end, int tp, int splits, int *steps) {
-    const int all = (end + tp - 1) / tp;
-    int s = (all + 3) / 4;
-    if (s > splits) s = splits;
-    if (s < 1) s = 1;
-    *steps = (all + s - 1) / s;
-    if (*steps < 1) *steps = 1;
-    s = (all + *steps - 1) / *steps;
-    return s < 1 ? 1 : s;
+// Slices of `end` positions in steps of tp: of `quantum` steps, more where that gives more than `splits`; none is empty.
+__host__ __device__ inline int tree_slices(int end, int tp, int splits, int quantum, int *steps) {
+    const int all = max((end + tp - 1) / tp, 1);
+    *steps = max(quantum, (all + splits - 1) / splits);
+    return (all + *steps - 1) / *steps;
 }
 
 typedef void (*TreeKernel)(TreeArgs);
-// The kernel for caches of `type` and queries of `q_type`, `tiles` tiles of 16 rows a wave, and its LDS bytes.
-TreeKernel tree_kernel_64(int type, int q_type, int tiles, size_t *lds);
-TreeKernel tree_kernel_128(int type, int q_type, int tiles, size_t *lds);
-TreeKernel tree_kernel_192(int type, int q_type, int tiles, size_t *lds);
-TreeKernel tree_kernel_256(int type, int q_type, int tiles, size_t *lds);
+// The kernel for caches of `type` and queries of `q_type`, `tiles` tiles of 16 rows a wave, its waves taking positions
+// (many 0) or rows (many 1), and its LDS bytes.
+TreeKernel tree_kernel_64(int type, int q_type, int tiles, int many, size_t *lds);
+TreeKernel tree_kernel_128(int type, int q_type, int tiles, int many, size_t *lds);
+TreeKernel tree_kernel_192(int type, int q_type, int tiles, int many, size_t *lds);
+TreeKernel tree_kernel_256(int type, int q_type, int tiles, int many, size_t *lds);

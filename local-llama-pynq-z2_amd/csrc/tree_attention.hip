@@ -2,6 +2,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "device.h"
 #include "operators.h"
@@ -11,19 +12,31 @@ namespace {
 
 constexpr int TREE_MAX_SPLITS = 128;
 
-// A row's slices joined: weights exp2(max_s - max), the four waves every fourth slice each.
+// A row's slices joined: weights exp2(max_s - max).  A thread takes four values of every (1024 / hs)-th slice, eight
+// slices' loads at once.
 template <int QT>
 __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
-    __shared__ float sm_f[TREE_MAX_SPLITS];
-    __shared__ float sm_o[3][256];
+    __shared__ float sm_f[TREE_MAX_SPLITS + 64]; // (a group's last loads may be past the last slice: weight 0)
+    __shared__ float4 sm_o[256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     const int len = min(max(a.lens[b], 0), a.ctx), nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n;
     int steps;
-    const int slices = tree_slices((int)min((int64_t)len + nn, (int64_t)a.ctx), tp, a.splits, &steps);
+    const int slices = tree_slices((int)min((int64_t)len + nn, (int64_t)a.ctx), tp, a.splits, a.quantum, &steps);
     if (slices == 1 || row >= nn * a.group) return;
     const int64_t stride = (int64_t)a.max_n * a.group, base = ((int64_t)b * a.n_kv + h) * a.splits * stride + row;
-    // every wave forms the weights; the loads of the values do not wait for them
+    const int per = a.hs / 4, groups = 256 / per, g = threadIdx.x / per, d = 4 * (threadIdx.x - g * per);
+    constexpr int U = 8;
+    float4 v[U];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int s = s0 + u * groups;
+            v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (g < groups && s < slices) v[u] = *(const float4 *)(a.acc + (base + s * stride) * a.hs + d);
+        }
+    };
+    load(g); // (the first values do not wait for the weights)
     float m[TREE_MAX_SPLITS / 64], l[TREE_MAX_SPLITS / 64], mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < TREE_MAX_SPLITS / 64; i++) {
@@ -42,51 +55,63 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
         if (wave == 0) sm_f[lane + 64 * i] = f;
     }
     sum = wave_sum(sum);
+    if (wave == 0) sm_f[lane + TREE_MAX_SPLITS] = 0.0f;
     __syncthreads();
-    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = wave; s < slices; s += 4) {
-        const float f = sm_f[s];
-        const float *acc = a.acc + (base + s * stride) * a.hs;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = g; s0 < slices; s0 += U * groups) {
+        if (s0 != g) load(s0);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < a.hs) o[i] += acc[lane + 64 * i] * f;
+        for (int u = 0; u < U; u++) {
+            const float f = sm_f[min(s0 + u * groups, TREE_MAX_SPLITS)];
+            o.x += v[u].x * f, o.y += v[u].y * f, o.z += v[u].z * f, o.w += v[u].w * f;
+        }
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (wave) sm_o[wave - 1][lane + 64 * i] = o[i];
+    sm_o[threadIdx.x] = o;
     __syncthreads();
-    if (wave) return;
-    const int t = row / a.group, g = row - t * a.group;
-    uint8_t *op = a.o + b * a.o_seq + t * a.o_tok + (h * a.group + g) * a.o_head;
+    if (g) return;
+    for (int k = 1; k < groups; k++) {
+        const float4 x = sm_o[k * per + threadIdx.x];
+        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+    }
+    const int t = row / a.group, gr = row - t * a.group;
+    uint8_t *op = a.o + b * a.o_seq + t * a.o_tok + (h * a.group + gr) * a.o_head;
     const float il = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int d = lane + 64 * i;
-        if (d >= a.hs) continue;
-        const float v = (((o[i] + sm_o[0][d]) + sm_o[1][d]) + sm_o[2][d]) * il;
-        if constexpr (QT == LLM_F32) ((float *)op)[d] = v;
-        else ((__bf16 *)op)[d] = (__bf16)v;
+    o = make_float4(o.x * il, o.y * il, o.z * il, o.w * il);
+    if constexpr (QT == LLM_F32) *(float4 *)(op + (size_t)d * 4) = o;
+    else {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        *(uint2 *)(op + (size_t)d * 2) = make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector((f2){o.x, o.y}, b2)),
+                                                    __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){o.z, o.w}, b2)));
     }
 }
 
 struct TreePlan {
-    int hsp, tp, tiles, row_blocks, splits;
+    int hsp, tp, many, tiles, row_blocks, splits, quantum;
     size_t bytes;
 };
 
-// How a call is cut: rows of a kv head in tiles of 16, one tile a wave up to 16 rows and two from there where the registers
-// allow it; positions in slices until the grid has two blocks a CU.
+// How a call is cut.  Up to 32 rows a kv head: the block's waves share the positions, with one or two tiles of 16 rows
+// each.  More rows: the waves share the rows, and the cache's rows go through LDS.  (Not for fp32 caches, whose rows need
+// no conversion, and head sizes above 128, whose rows do not fit twice.)  Positions in slices, the same number of steps
+// for every sequence, until the grid has two blocks a CU; eight for several sequences, whose lengths the host does not
+// know.
 TreePlan tree_plan(const llm_kv *c, int n_heads, int max_n, int max_len) {
     TreePlan p;
     p.hsp = (c->hs + 63) / 64 * 64;
-    p.tp = tree_positions(p.hsp, c->type);
     const int group = n_heads / c->n_kv, rows = group * max_n;
-    p.tiles = rows > 16 && p.hsp <= 128 ? 2 : 1;
-    p.row_blocks = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
+    p.many = rows > 32 && p.hsp <= 128 && c->type != LLM_F32;
+    p.tp = tree_positions(p.hsp, c->type, p.many);
+    p.tiles = rows > (p.many ? 64 : 16) && p.hsp <= 128 ? 2 : 1;
+    const int per_block = 16 * p.tiles * (p.many ? 4 : 1);
+    p.row_blocks = (rows + per_block - 1) / per_block;
     const int64_t end = std::min<int64_t>((int64_t)std::max(max_len, 0) + max_n, c->ctx);
-    const int64_t steps = (end + p.tp - 1) / p.tp, blocks = (int64_t)c->n_seq * c->n_kv * p.row_blocks;
-    const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(blocks, 1));
-    p.splits = (int)std::max<int64_t>(1, std::min({want, (steps + 3) / 4, (int64_t)TREE_MAX_SPLITS}));
+    const int64_t steps = std::max<int64_t>((end + p.tp - 1) / p.tp, 1), blocks = (int64_t)c->n_seq * c->n_kv * p.row_blocks;
+    const int64_t least = p.many ? 2 : 4; // steps of a slice (few rows: one a wave)
+    const int64_t want = std::max<int64_t>(1, (c->n_seq > 1 ? 2048 : 512) / std::max<int64_t>(blocks, 1));
+    const int64_t cap = std::min({want, (steps + least - 1) / least, (int64_t)TREE_MAX_SPLITS});
+    p.quantum = (int)std::max<int64_t>((steps + cap - 1) / cap, 1);
+    p.splits = (int)((steps + p.quantum - 1) / p.quantum);
     p.bytes = p.splits > 1 ? (size_t)c->n_seq * c->n_kv * p.splits * rows * (c->hs + 2) * 4 : 0;
     return p;
 }
@@ -118,6 +143,10 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
     if (!op_check_rows(q, "q", &dev, who) || !op_check_rows(out, "out", &dev, who) || !dev.holds(lens, "lens") ||
         (n && !dev.holds(n, "n")) || (mask && !dev.holds(mask, "mask")))
         return -1;
+    if (!std::isfinite(scale)) {
+        fprintf(stderr, "%s: scale %g\n", who, scale);
+        return -1;
+    }
     if (q->type != out->type) {
         fprintf(stderr, "%s: q and out of different types\n", who);
         return -1;
@@ -145,13 +174,16 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
     a.o_seq = out->seq * qs, a.o_tok = out->tok * qs, a.o_head = out->head * qs;
     a.lens = lens, a.n = n, a.mask = mask;
     a.n_seq = c->n_seq, a.n_kv = c->n_kv, a.hs = c->hs, a.ctx = c->ctx;
-    a.group = n_heads / c->n_kv, a.max_n = max_n, a.splits = p.splits, a.zero_rest = zero_rest;
-    a.c = scale * 1.44269504088896340736f;
+    a.group = n_heads / c->n_kv, a.max_n = max_n, a.splits = p.splits, a.quantum = p.quantum;
+    a.zero_rest = zero_rest;
+    // (a scale of 0 as one so small that every weight is 1)
+    a.c = std::max(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
+    a.negate = scale < 0.0f;
     a.acc = (float *)work; // (rows of hs values, hs a multiple of 16: 16-byte aligned)
     a.ml = (float *)work + (p.bytes / 4 / (c->hs + 2)) * c->hs;
     size_t lds = 0;
     auto *pick = p.hsp == 64 ? tree_kernel_64 : p.hsp == 128 ? tree_kernel_128 : p.hsp == 192 ? tree_kernel_192 : tree_kernel_256;
-    TreeKernel kern = pick(c->type, q->type, p.tiles, &lds);
+    TreeKernel kern = pick(c->type, q->type, p.tiles, p.many, &lds);
     if (!kern) {
         fprintf(stderr, "%s: internal error: no kernel\n", who);
         return -1;

@@ -1,17 +1,20 @@
 // Attention of drafted tokens over a cache, head sizes up to TREE_HSP (a multiple of 64; this file is compiled for each).
 //
-// The rows of a kv head are its query heads' tokens (row = token * group + head of the group), in tiles of 16; a wave takes
-// one or two tiles over every fourth step of TP positions of its block's slice, with one running maximum and sum a row.
-// Everything stays in registers, nothing crosses lanes but the maximum:
-//   scores  S^T = K Q^T: K rows are the A operand, lane 16 j + n has 16-byte pieces of position n (piece j of every four),
-//           so a row's bytes are read whole and once; Q's lanes hold the same values of row n.  The lane then owns the
-//           scores of row n at positions 4 j + i of every 16.
+// The rows of a kv head are its query heads' tokens (row = token * group + head of the group), in tiles of 16 on the
+// 16 x 16 matrix instructions, with one running maximum and sum a row over the positions:
+//   scores  S^T = K Q^T: K rows are the A operand, the queries B.  A lane 16 j + n then owns the scores of row n at
+//           positions 4 j + i of every 16.
 //   values  O^T += V^T P^T: its own probabilities are the B operand as they are (eight positions: 4 j + i of two tiles of
-//           16).  A's lane n needs those positions of one dimension: it reads 4 or 8 neighbouring dimensions of each of the
-//           positions and pairs the registers of two positions, which transposes for nothing.
-// int8 and e4m3 codes and bf16 values are exact in bf16, so the products run on v_mfma_f32_16x16x32_bf16 with the fp32 side
-// (queries, probabilities * V scale) in bf16 pieces: three hold all 24 bits; 16-bit queries are one, their probabilities
-// two (2^-16, against the output's 2^-9).  fp32 caches take v_mfma_f32_16x16x4_f32.
+//           16); V, A, has those positions of one dimension in a lane.
+// Few rows (k_tree_attention): the block's four waves share the positions; K and V go from memory to the registers where
+// they are used.  Many rows (k_tree_rows): the waves share the rows; each step's K and V are converted once and read by
+// all four from LDS.
+//
+// Operands.  int8 and e4m3 codes are exact in fp16, and the fp32 side is held in two fp16 pieces (22 bits): a query row is
+// scaled by a power of two to the top of fp16's range first, and so are the weights p * V scale, by the largest V scale met
+// (a running exponent, as the maximum is running).  bf16 caches: three bf16 pieces.  16-bit queries are one piece; their
+// weights one in fp16 (half a step 2^-11, against the output's 2^-8) and two in bf16.  fp32 caches: v_mfma_f32_16x16x4_f32.
+// Maxima, sums and outputs are fp32.
 #include <type_traits>
 
 #include "device.h"
@@ -28,36 +31,53 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 constexpr int HSP = TREE_HSP;
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u; // a buffer offset past every resource here: the load returns zero
 
-// a float pair in bf16, rounded; exact for codes
-__device__ __forceinline__ uint32_t bf2(float x, float y) {
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t bf2(float x, float y) { // a float pair in bf16, rounded
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2));
 }
 __device__ __forceinline__ float lo16(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi16(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
-// x and y as NP bf16 pieces, each word a pair
-template <int NP>
+
+// x and y as NP 16-bit pieces (bf16 caches: bf16, 8-bit caches: fp16), each word a pair
+template <int CT, int NP>
 __device__ __forceinline__ void split(float x, float y, uint32_t *p) {
 #pragma unroll
     for (int i = 0; i < NP; i++) {
-        p[i] = bf2(x, y);
-        if (i + 1 < NP) x -= lo16(p[i]), y -= hi16(p[i]);
+        if constexpr (CT == LLM_BF16) {
+            p[i] = bf2(x, y);
+            if (i + 1 < NP) x -= lo16(p[i]), y -= hi16(p[i]);
+        } else {
+            const f16x2 h = __builtin_convertvector((f32x2){x, y}, f16x2);
+            p[i] = __builtin_bit_cast(uint32_t, h);
+            if (i + 1 < NP) x = fmaf((float)h[0], -1.0f, x), y = fmaf((float)h[1], -1.0f, y);
+        }
     }
 }
-template <int CT, int BYTE>
-__device__ __forceinline__ float code(uint32_t w) { // byte BYTE's value
-    if constexpr (CT == LLM_I8) return (float)(int8_t)(w >> (8 * BYTE));
-    else {
-        const auto f = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, BYTE >= 2);
-        return f[BYTE & 1];
-    }
-}
+// Two codes (word W of u: bytes 2 W and 2 W + 1) as an fp16 pair.  int8 (its sign bit flipped before, flip_sign): 0x64 over
+// the byte is 1024 + code + 128.
 template <int CT>
-__device__ __forceinline__ void codes4(uint32_t w, uint32_t *p) { // four codes as two bf16 pairs
-    p[0] = bf2(code<CT, 0>(w), code<CT, 1>(w));
-    p[1] = bf2(code<CT, 2>(w), code<CT, 3>(w));
+__device__ __forceinline__ uint32_t flip_sign(uint32_t u) { return CT == LLM_I8 ? u ^ 0x80808080u : u; }
+template <int CT, int W>
+__device__ __forceinline__ uint32_t codes2(uint32_t u) {
+    if constexpr (CT == LLM_I8) {
+        const uint32_t h = __builtin_amdgcn_perm(0x64646464u, u, W ? 0x04030402u : 0x04010400u);
+        const f16x2 c = __builtin_bit_cast(f16x2, h) - (f16x2){(_Float16)1152.0f, (_Float16)1152.0f};
+        return __builtin_bit_cast(uint32_t, c);
+    } else {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u, 1.0f, W));
+    }
+}
+// The pairs (a0, a1) of bytes 2 H and 2 H + 1: pieces of V at two positions, by dimension.
+template <int CT, int H>
+__device__ __forceinline__ void pairs2(uint32_t a0, uint32_t a1, uint32_t *p) {
+    const uint32_t m = flip_sign<CT>(__builtin_amdgcn_perm(a1, a0, H ? 0x07030602u : 0x05010400u));
+    p[0] = codes2<CT, 0>(m);
+    p[1] = codes2<CT, 1>(m);
 }
 
-// An operand of a product over 32 terms: eight values a lane.  fp32: as they are, else NP bf16 pieces.
+// An operand of a product over 32 terms: eight values a lane.  fp32: as they are, else NP 16-bit pieces.
 template <int CT, int NP>
 struct Frag {
     typename std::conditional<CT == LLM_F32, float[8], u32x4[NP]>::type v;
@@ -69,9 +89,14 @@ __device__ __forceinline__ f32x4 product(const Frag<CT, 1> &a, const Frag<CT, NP
         for (int i = 0; i < 8; i++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], d, 0, 0, 0);
     } else {
 #pragma unroll
-        for (int p = NP - 1; p >= 0; p--) // smallest pieces first
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v[0]),
-                                                        __builtin_bit_cast(bf16x8, b.v[p]), d, 0, 0, 0);
+        for (int p = NP - 1; p >= 0; p--) { // smallest pieces first
+            if constexpr (CT == LLM_BF16)
+                d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v[0]),
+                                                            __builtin_bit_cast(bf16x8, b.v[p]), d, 0, 0, 0);
+            else
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v[0]),
+                                                           __builtin_bit_cast(f16x8, b.v[p]), d, 0, 0, 0);
+        }
     }
     return d;
 }
@@ -82,12 +107,18 @@ __device__ __forceinline__ void fill(Frag<CT, NP> &f, const float (&x)[8]) {
         if constexpr (CT == LLM_F32) f.v[i] = x[i], f.v[i + 1] = x[i + 1];
         else {
             uint32_t p[NP];
-            split<NP>(x[i], x[i + 1], p);
+            split<CT, NP>(x[i], x[i + 1], p);
 #pragma unroll
             for (int k = 0; k < NP; k++) f.v[k][i / 2] = p[k];
         }
     }
 }
+
+// The power of two that takes a magnitude to [2^14, 2^15) (magnitudes below 2^-112 to less, infinities: 2^-127 and NaN), and
+// its inverse, from the magnitude's exponent field.
+__device__ __forceinline__ uint32_t exponent(float x) { return (__float_as_uint(x) >> 23) & 0xff; }
+__device__ __forceinline__ float power_to(uint32_t e) { return __uint_as_float(min(268u - e, 253u) << 23); }
+__device__ __forceinline__ float power_from(uint32_t e) { return __uint_as_float((254u - min(268u - e, 253u)) << 23); }
 
 // Over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
 template <typename F>
@@ -106,117 +137,255 @@ __device__ __forceinline__ void wave_lds_fence() { // this wave's LDS stores bef
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int CT, int QT, int R>
-struct TreeShape {
+template <int CT, int QT>
+struct TreePieces {
     static constexpr int ES = CT == LLM_F32 ? 4 : CT == LLM_BF16 ? 2 : 1;
-    static constexpr int TP = tree_positions(HSP, CT), NT = TP / 16; // positions a step, their tiles of 16
-    static constexpr int KL = HSP * ES / 64;                         // 16-byte pieces of a K row a lane
-    static constexpr int KS = HSP / 32;                              // products of a score
-    static constexpr int VW = HSP % 128 ? 4 : 8;                     // neighbouring dimensions a lane of V
-    static constexpr int VC = HSP / (16 * VW), VR = VW * ES / 4;     // runs of them, a run's registers
-    static constexpr int NPQ = QT == LLM_BF16 ? 1 : 3, NPP = QT == LLM_BF16 ? 2 : 3;
-    static constexpr size_t LDS = (size_t)2 * R * (HSP / 16) * 64 * 16 + 4 * R * 16 * 8 + 4 * 2 * 64 * 4;
+    static constexpr bool SCALED = ES == 1;
+    static constexpr int Q = QT == LLM_BF16 ? 1 : SCALED ? 2 : 3;                // of a query
+    static constexpr int P = QT == LLM_BF16 ? (SCALED ? 1 : 2) : SCALED ? 2 : 3; // of a weight
 };
 
-template <int CT, int QT, int R>
-__global__ void __launch_bounds__(256) k_tree_attention(TreeArgs a) {
-    using Sh = TreeShape<CT, QT, R>;
-    constexpr int ES = Sh::ES, TP = Sh::TP, NT = Sh::NT, KL = Sh::KL, KS = Sh::KS, VW = Sh::VW, VC = Sh::VC, VR = Sh::VR;
-    constexpr int NPQ = Sh::NPQ, NPP = Sh::NPP;
-    constexpr bool SCALED = ES == 1;
-    extern __shared__ __align__(16) uint8_t lds[];
-    f32x4 *const sm_o = (f32x4 *)lds;                                        // [2][R][HSP / 16][64]
-    float *const sm_ml = (float *)(lds + (size_t)2 * R * (HSP / 16) * 64 * 16); // [4][R][16][2]
-    float *const sm_s = sm_ml + 4 * R * 16 * 2;                              // [4][2][64]
+// The dimension of value i = 4 q4 .. 4 q4 + 3 of lane group j in product s.  From memory, a lane's 16-byte pieces of a K row
+// are its own (piece j of every four); from LDS, rows are in order.
+template <int CT, bool LDS>
+__device__ __forceinline__ int dim_of(int s, int j, int q4) {
+    if constexpr (LDS || CT == LLM_BF16) return 32 * s + 8 * j + 4 * q4;
+    else if constexpr (CT == LLM_F32) return 32 * s + 16 * q4 + 4 * j;
+    else return 64 * (s / 2) + 16 * j + 8 * (s % 2) + 4 * q4;
+}
 
-    const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// Where a block works: sequence, kv head, slice, and how many positions and rows there are.
+struct Place {
+    int b, h, split, len, end, rows, slices, first, last;
+};
+template <int QT>
+__device__ __forceinline__ bool place(const TreeArgs &a, int tp, int row0, int block_rows, Place &p) {
     int id = blockIdx.x;
-    const int split_id = id % a.splits;
+    p.split = id % a.splits;
     id /= a.splits;
-    const int h = id % a.n_kv, b = id / a.n_kv;
-    const int len = min(max(a.lens[b], 0), a.ctx);
-    const int nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n;
-    const int end = min((int64_t)len + nn, (int64_t)a.ctx), rows = nn * a.group, row0 = blockIdx.y * 16 * R;
+    p.h = id % a.n_kv;
+    p.b = id / a.n_kv;
+    p.len = min(max(a.lens[p.b], 0), a.ctx);
+    const int nn = a.n ? min(max(a.n[p.b], 0), a.max_n) : a.max_n;
+    p.end = (int)min((int64_t)p.len + nn, (int64_t)a.ctx);
+    p.rows = nn * a.group;
     int steps;
-    const int slices = tree_slices(end, TP, a.splits, &steps);
-    if (a.zero_rest && split_id == 0) { // the rows behind the last token
-        for (int e = threadIdx.x * 4; e < 16 * R * a.hs; e += 1024) {
+    p.slices = tree_slices(p.end, tp, a.splits, a.quantum, &steps);
+    if (a.zero_rest && p.split == 0 && row0 + block_rows > p.rows) { // the rows behind the last token
+        for (int e = threadIdx.x * 4; e < block_rows * a.hs; e += 1024) {
             const int row = row0 + e / a.hs, t = row / a.group, d = e - (row - row0) * a.hs;
-            if (row < rows || row >= a.max_n * a.group) continue;
-            uint8_t *op = a.o + b * a.o_seq + t * a.o_tok + (h * a.group + row - t * a.group) * a.o_head;
+            if (row < p.rows || row >= a.max_n * a.group) continue;
+            uint8_t *op = a.o + p.b * a.o_seq + t * a.o_tok + (p.h * a.group + row - t * a.group) * a.o_head;
             if constexpr (QT == LLM_F32) *(float4 *)(op + (size_t)d * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             else *(uint2 *)(op + (size_t)d * 2) = make_uint2(0, 0);
         }
     }
-    if (row0 >= rows || split_id >= slices) return;
-    const int all = (end + TP - 1) / TP, first = split_id * steps, last = min(first + steps, all);
+    const int all = (p.end + tp - 1) / tp;
+    p.first = p.split * steps;
+    p.last = min(p.first + steps, all);
+    return row0 < p.rows && p.split < p.slices;
+}
 
-    // the rows of this wave's tiles: queries, and what each sees among the new tokens
-    Frag<CT, NPQ> qf[R][KS];
-    uint64_t sees[R];
+// The queries of row `row` (none from p.rows on: zeros, nothing seen) as the operand of its scores.  Returns what takes a
+// score to the exponent of 2.
+template <int CT, int QT, bool LDS, int NP>
+__device__ __forceinline__ float load_queries(const TreeArgs &a, const Place &p, int row, Frag<CT, NP> (&qf)[HSP / 32],
+                                              uint64_t &sees) {
+    const int j = (threadIdx.x & 63) >> 4, t = row / a.group, g = row - t * a.group;
+    const bool ok = row < p.rows;
+    sees = 0;
+    if (ok) sees = a.mask ? a.mask[(int64_t)p.b * a.max_n + t] : ~(uint64_t)0 >> (63 - t);
+    const uint8_t *qp = a.q + p.b * a.q_seq + (ok ? t * a.q_tok + (p.h * a.group + g) * a.q_head : 0);
+    float x[HSP / 32][8], mx = 0.0f;
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int row = row0 + 16 * r + n, t = row / a.group, g = row - t * a.group;
-        const bool ok = row < rows;
-        sees[r] = 0;
-        if (ok) sees[r] = a.mask ? a.mask[(int64_t)b * a.max_n + t] : ~(uint64_t)0 >> (63 - t);
-        const uint8_t *qp = a.q + b * a.q_seq + (ok ? t * a.q_tok + (h * a.group + g) * a.q_head : 0);
+    for (int s = 0; s < HSP / 32; s++)
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            float x[8];
-#pragma unroll
-            for (int q4 = 0; q4 < 2; q4++) {
-                // the lane's values of product s are those of its pieces of K
-                const int d = CT == LLM_F32 ? 32 * s + 16 * q4 + 4 * j
-                              : CT == LLM_BF16 ? 32 * s + 8 * j + 4 * q4 : 64 * (s / 2) + 16 * j + 8 * (s % 2) + 4 * q4;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (ok && d < a.hs) {
-                    if constexpr (QT == LLM_F32) v = *(const float4 *)(qp + (size_t)d * 4);
-                    else {
-                        const uint2 u = *(const uint2 *)(qp + (size_t)d * 2);
-                        v = make_float4(lo16(u.x), hi16(u.x), lo16(u.y), hi16(u.y));
-                    }
+        for (int q4 = 0; q4 < 2; q4++) {
+            const int d = dim_of<CT, LDS>(s, j, q4);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (ok && d < a.hs) {
+                if constexpr (QT == LLM_F32) v = *(const float4 *)(qp + (size_t)d * 4);
+                else {
+                    const uint2 u = *(const uint2 *)(qp + (size_t)d * 2);
+                    v = make_float4(lo16(u.x), hi16(u.x), lo16(u.y), hi16(u.y));
                 }
-                x[4 * q4] = v.x, x[4 * q4 + 1] = v.y, x[4 * q4 + 2] = v.z, x[4 * q4 + 3] = v.w;
             }
-            fill(qf[r][s], x);
+            x[s][4 * q4] = v.x, x[s][4 * q4 + 1] = v.y, x[s][4 * q4 + 2] = v.z, x[s][4 * q4 + 3] = v.w;
+            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
         }
+    float to = 1.0f, from = 1.0f;
+    if constexpr (TreePieces<CT, QT>::SCALED) {
+        const uint32_t e = exponent(over_groups(mx, fmax_));
+        to = power_to(e);
+        from = power_from(e);
     }
+    if (a.negate) to = -to;
+#pragma unroll
+    for (int s = 0; s < HSP / 32; s++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[s][i] *= to;
+        fill(qf[s], x[s]);
+    }
+    return fmaxf(a.c * from, 1e-37f);
+}
 
-    const uint8_t *const kb = a.k + b * a.seq + h * a.head, *const vb = a.v + b * a.seq + h * a.head;
+// What row `sees` of a step's positions at its edge: bit 4 t + i.
+template <int N>
+__device__ __forceinline__ uint32_t seen_bits(const Place &p, int p0, uint64_t sees) {
+    const int j = (threadIdx.x & 63) >> 4;
+    uint32_t vis = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int at = p0 + 16 * (i / 4) + 4 * j + i % 4;
+        const bool v = at < p.len || (at < p.end && ((sees >> (at - p.len)) & 1));
+        vis |= (uint32_t)v << i;
+    }
+    return vis;
+}
+
+// A step's scores x (with the K scales, if any) into the weights of its values: the running maximum m (exponents of 2) and
+// sum l of the row; `sv` (in LDS) the V scales times their common power, at 16 t + i; o and l are rescaled when the maximum or, by `oe`, that
+// power has moved.
+template <int NT, int CT, int NPP, int DT>
+__device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *sv, bool edge, uint32_t vis, float oe,
+                                        float &m, float &l, f32x4 (&o)[DT], Frag<CT, NPP> (&pf)[NT / 2]) {
+    constexpr bool SCALED = CT == LLM_I8 || CT == LLM_E4M3;
+    if (edge)
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!((vis >> (4 * t + i)) & 1)) x[t][i] = -INFINITY;
+    float mx = x[0][0];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mx = fmaxf(mx, x[t][i]);
+    mx = over_groups(mx, fmax_);
+    const float mn = fmaxf(m, mx * cq), mu = mn == -INFINITY ? 0.0f : mn;
+    if (__any(mn > m || oe != 1.0f)) {
+        const float al = __builtin_amdgcn_exp2f(m - mu), ao = al * oe;
+        l *= al;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[d][i] *= ao;
+        m = mn;
+    }
+#pragma unroll
+    for (int u = 0; u < NT / 2; u++) {
+        float w[8];
+        f32x4 s4;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int t = 2 * u + i / 4;
+            w[i] = __builtin_amdgcn_exp2f(fmaf(x[t][i % 4], cq, -mu));
+            l += w[i];
+            if constexpr (SCALED) {
+                if (i % 4 == 0) s4 = *(const f32x4 *)(sv + 16 * t);
+                w[i] *= s4[i % 4];
+                if (edge && !((vis >> (8 * u + i)) & 1)) w[i] = 0.0f; // (0 * a scale that is not finite)
+            }
+        }
+        fill(pf[u], w);
+    }
+}
+
+// Sums of row `row` at dimensions d .. d + 3: the output where there is one slice, else this slice's partial sums.
+template <int QT>
+__device__ __forceinline__ void put_values(const TreeArgs &a, const Place &p, int row, int d, float4 y) {
+    if (d >= a.hs) return;
+    if (p.slices > 1) {
+        const int64_t part = (((int64_t)p.b * a.n_kv + p.h) * a.splits + p.split) * a.max_n * a.group + row;
+        *(float4 *)(a.acc + part * a.hs + d) = y;
+        return;
+    }
+    const int t = row / a.group, g = row - t * a.group;
+    uint8_t *op = a.o + p.b * a.o_seq + t * a.o_tok + (p.h * a.group + g) * a.o_head;
+    if constexpr (QT == LLM_F32) *(float4 *)(op + (size_t)d * 4) = y;
+    else *(uint2 *)(op + (size_t)d * 2) = make_uint2(bf2(y.x, y.y), bf2(y.z, y.w));
+}
+__device__ __forceinline__ void put_sums(const TreeArgs &a, const Place &p, int row, float m, float l) {
+    const int64_t part = (((int64_t)p.b * a.n_kv + p.h) * a.splits + p.split) * a.max_n * a.group + row;
+    a.ml[2 * part] = m;
+    a.ml[2 * part + 1] = l;
+}
+// what takes the sums of a row to its output (a row that sees nothing has the sum 0)
+__device__ __forceinline__ float to_output(const Place &p, float l) {
+    return p.slices > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+}
+
+// A step's rows through buffers that hold its positions and no more: what lies past them reads as zero.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t step_rsrc(const void *base, int64_t stride, int step, int tp,
+                                                            const Place &p) {
+    const int left = step < p.last ? min(tp, p.end - step * tp) : 0;
+    return __builtin_amdgcn_make_buffer_rsrc((void *)((const uint8_t *)base + (int64_t)step * tp * stride), 0,
+                                             (int)(left * stride), 0x00020000);
+}
+
+// ---- few rows: the waves share the positions
+
+template <int CT, int QT, int R>
+struct TreeShape {
+    static constexpr int ES = TreePieces<CT, QT>::ES;
+    static constexpr int TP = tree_positions(HSP, CT, false), NT = TP / 16; // positions a step, their tiles of 16
+    static constexpr int KL = HSP * ES / 64;                                // 16-byte pieces of a K row a lane
+    static constexpr int KS = HSP / 32;                                     // products of a score
+    static constexpr int VW = HSP % 128 ? 4 : 8;                            // neighbouring dimensions a lane of V
+    static constexpr int VC = HSP / (16 * VW), VR = VW * ES / 4;            // runs of them, a run's registers
+    static constexpr size_t LDS = (size_t)2 * R * (HSP / 16) * 64 * 16 + 4 * R * 16 * 8 + 4 * 2 * 64 * 4;
+};
+
+// K's lane 16 j + n has 16-byte pieces of position n (piece j of every four), so a row's bytes are read whole and once.  V's
+// lane n reads 4 or 8 neighbouring dimensions of its eight positions and pairs the registers of two positions, which
+// transposes for nothing.  The next step's loads go out as soon as a step's registers are used.
+template <int CT, int QT, int R>
+__global__ void __launch_bounds__(256, CT != LLM_F32 && R == 1 && HSP <= 128 ? 2 : 1) k_tree_attention(TreeArgs a) {
+    using Sh = TreeShape<CT, QT, R>;
+    using Pc = TreePieces<CT, QT>;
+    constexpr int ES = Sh::ES, TP = Sh::TP, NT = Sh::NT, KL = Sh::KL, KS = Sh::KS, VW = Sh::VW, VC = Sh::VC, VR = Sh::VR;
+    constexpr bool SCALED = Pc::SCALED;
+    extern __shared__ __align__(16) uint8_t lds[];
+    f32x4 *const sm_o = (f32x4 *)lds;                                           // [2][R][HSP / 16][64]
+    float *const sm_ml = (float *)(lds + (size_t)2 * R * (HSP / 16) * 64 * 16); // [4][R][16][2]
+    float *const sm_s = sm_ml + 4 * R * 16 * 2;                                 // [4][2][64]
+
+    const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row0 = blockIdx.y * 16 * R;
+    Place p;
+    if (!place<QT>(a, TP, row0, 16 * R, p)) return;
+
+    const uint8_t *const kb = a.k + p.b * a.seq + p.h * a.head, *const vb = a.v + p.b * a.seq + p.h * a.head;
     const float *ksb = nullptr, *vsb = nullptr;
     if constexpr (SCALED) {
-        ksb = a.ks + b * a.s_seq + h * a.s_head;
-        vsb = a.vs + b * a.s_seq + h * a.s_head;
+        ksb = a.ks + p.b * a.s_seq + p.h * a.s_head;
+        vsb = a.vs + p.b * a.s_seq + p.h * a.s_head;
     }
     const uint32_t ps = (uint32_t)a.pos, hb = (uint32_t)(a.hs * ES);
     u32x4 kr[NT][KL];
     uint32_t vr[TP / 4][VC][VR];
     uint32_t skr = 0, svr = 0;
-
-    // A step's rows through buffers that hold its positions and no more: what lies past them reads as zero.
-    auto rsrc = [&](const void *p, int64_t stride, int step) {
-        const int left = step < last ? min(TP, end - step * TP) : 0;
-        return __builtin_amdgcn_make_buffer_rsrc((void *)((const uint8_t *)p + (int64_t)step * TP * stride), 0,
-                                                 (int)(left * stride), 0x00020000);
-    };
     auto load_k = [&](int step) {
-        const auto rs = rsrc(kb, a.pos, step);
+        const auto rs = step_rsrc(kb, a.pos, step, TP, p);
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int p = 0; p < KL; p++) {
-                const uint32_t at = 64 * p + 16 * j;
+            for (int i = 0; i < KL; i++) {
+                const uint32_t at = 64 * i + 16 * j;
                 const auto x = __builtin_amdgcn_raw_buffer_load_b128(
                     rs, (int)(at < hb ? (16 * t + n) * ps + at : OUT_OF_RANGE), 0, 0);
-                kr[t][p] = (u32x4){x[0], x[1], x[2], x[3]};
+                kr[t][i] = (u32x4){x[0], x[1], x[2], x[3]};
             }
         if constexpr (SCALED)
-            skr = __builtin_amdgcn_raw_buffer_load_b32(rsrc(ksb, a.s_pos * 4, step), (int)(lane * (uint32_t)a.s_pos * 4), 0, 0);
+            skr = __builtin_amdgcn_raw_buffer_load_b32(step_rsrc(ksb, a.s_pos * 4, step, TP, p),
+                                                       (int)(lane * (uint32_t)a.s_pos * 4), 0, 0);
     };
     auto load_v = [&](int step) {
-        const auto rs = rsrc(vb, a.pos, step);
+        const auto rs = step_rsrc(vb, a.pos, step, TP, p);
+        if constexpr (SCALED)
+            svr = __builtin_amdgcn_raw_buffer_load_b32(step_rsrc(vsb, a.s_pos * 4, step, TP, p),
+                                                       (int)(lane * (uint32_t)a.s_pos * 4), 0, 0);
 #pragma unroll
         for (int x = 0; x < TP / 4; x++)
 #pragma unroll
@@ -229,43 +398,36 @@ __global__ void __launch_bounds__(256) k_tree_attention(TreeArgs a) {
                     vr[x][c][0] = u[0], vr[x][c][1] = u[1];
                 } else {
 #pragma unroll
-                    for (int p = 0; p < VR / 4; p++) {
-                        const auto u = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(off + 16 * p), 0, 0);
+                    for (int i = 0; i < VR / 4; i++) {
+                        const auto u = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(off + 16 * i), 0, 0);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) vr[x][c][4 * p + k] = u[k];
+                        for (int k = 0; k < 4; k++) vr[x][c][4 * i + k] = u[k];
                     }
                 }
             }
-        if constexpr (SCALED)
-            svr = __builtin_amdgcn_raw_buffer_load_b32(rsrc(vsb, a.s_pos * 4, step), (int)(lane * (uint32_t)a.s_pos * 4), 0, 0);
     };
+    int step = p.first + wave;
+    load_k(step); // (a wave without a step loads nothing)
+    load_v(step);
 
-    f32x4 o[R][VC][VW];
-    float m[R], l[R];
+    Frag<CT, Pc::Q> qf[R][KS];
+    uint64_t sees[R];
+    float cq[R], m[R], l[R];
+    f32x4 o[R][VC * VW];
 #pragma unroll
     for (int r = 0; r < R; r++) {
+        cq[r] = load_queries<CT, QT, false>(a, p, row0 + 16 * r + n, qf[r], sees[r]);
         m[r] = -INFINITY;
         l[r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < VC; c++)
-#pragma unroll
-            for (int e = 0; e < VW; e++) o[r][c][e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int d = 0; d < VC * VW; d++) o[r][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
     float *const my_s = sm_s + wave * 128;
+    uint32_t ve = 20; // exponent field of the largest V scale (at least 2^-107)
 
-    int step = first + wave;
-    if (step < last) {
-        load_k(step);
-        load_v(step);
-    }
-    for (; step < last; step += 4) {
+    for (; step < p.last; step += 4) {
         const int p0 = step * TP;
-        const bool edge = p0 + TP > len; // new tokens or the end among the positions
-        if constexpr (SCALED) {
-            my_s[lane] = __uint_as_float(skr);
-            my_s[64 + lane] = __uint_as_float(svr);
-            wave_lds_fence();
-        }
+        const bool edge = p0 + TP > p.len; // new tokens or the end among the positions
         f32x4 x[R][NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -280,33 +442,35 @@ __global__ void __launch_bounds__(256) k_tree_attention(TreeArgs a) {
                 } else if constexpr (CT == LLM_BF16) {
                     kf.v[0] = kr[t][s];
                 } else {
-                    uint32_t p[4];
-                    codes4<CT>(kr[t][s / 2][2 * (s % 2)], p);
-                    codes4<CT>(kr[t][s / 2][2 * (s % 2) + 1], p + 2);
-                    kf.v[0] = (u32x4){p[0], p[1], p[2], p[3]};
+                    const uint32_t u0 = flip_sign<CT>(kr[t][s / 2][2 * (s % 2)]), u1 = flip_sign<CT>(kr[t][s / 2][2 * (s % 2) + 1]);
+                    kf.v[0] = (u32x4){codes2<CT, 0>(u0), codes2<CT, 1>(u0), codes2<CT, 0>(u1), codes2<CT, 1>(u1)};
                 }
 #pragma unroll
                 for (int r = 0; r < R; r++) x[r][t] = product(kf, qf[r][s], x[r][t]);
             }
         }
+        float oe = 1.0f;
+        if constexpr (SCALED) {
+            my_s[lane] = __uint_as_float(skr);
+            const float sv = __uint_as_float(svr);
+            const uint32_t e0 = ve;
+            ve = max(ve, exponent(wave_max(sv < INFINITY ? sv : 0.0f)));
+            if (ve != e0) oe = power_from(e0) * power_to(ve);
+            my_s[64 + lane] = sv * power_to(ve);
+            wave_lds_fence();
+        }
         load_k(step + 4);
 
-        uint32_t vis[R]; // edge: bit 4 t + i, whether the row sees the position
+        uint32_t vis[R];
         uint64_t bad = 0; // edge, fp32 and bf16: new tokens whose V row is not finite
 #pragma unroll
         for (int r = 0; r < R; r++) vis[r] = 0;
         if (edge) {
 #pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int i = 0; i < TP / 4; i++) {
-                    const int p = p0 + 16 * (i / 4) + 4 * j + i % 4;
-                    const bool v = p < len || (p < end && ((sees[r] >> (p - len)) & 1));
-                    vis[r] |= (uint32_t)v << i;
-                }
+            for (int r = 0; r < R; r++) vis[r] = seen_bits<TP / 4>(p, p0, sees[r]);
             if constexpr (!SCALED) {
                 // a value that is not finite would reach the rows that do not see it as 0 * inf: taken out here, and
-                // the rows that do see it become NaN at the end
+                // the rows that do see it become NaN
 #pragma unroll
                 for (int i = 0; i < TP / 4; i++) {
                     const int q = p0 + 16 * (i / 4) + i % 4; // of lane group 0
@@ -319,12 +483,12 @@ __global__ void __launch_bounds__(256) k_tree_attention(TreeArgs a) {
                             if constexpr (CT == LLM_F32) nf |= (u & 0x7f800000u) == 0x7f800000u;
                             else nf |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
                         }
-                    nf = nf && q + 4 * j >= len;
+                    nf = nf && q + 4 * j >= p.len;
                     const uint64_t any = __ballot(nf);
                     if (any) {
 #pragma unroll
                         for (int g = 0; g < 4; g++)
-                            if ((any >> (16 * g)) & 0xffff) bad |= (uint64_t)1 << (q + 4 * g - len);
+                            if ((any >> (16 * g)) & 0xffff) bad |= (uint64_t)1 << (q + 4 * g - p.len);
                         if ((any >> (16 * j)) & 0xffff)
 #pragma unroll
                             for (int c = 0; c < VC; c++)
@@ -335,96 +499,54 @@ __global__ void __launch_bounds__(256) k_tree_attention(TreeArgs a) {
             }
         }
 
-        Frag<CT, NPP> pf[R][NT / 2];
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            float mx = -INFINITY;
+        if constexpr (SCALED)
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                f32x4 sk = (f32x4){a.c, a.c, a.c, a.c};
-                if constexpr (SCALED) {
-                    const f32x4 s4 = *(const f32x4 *)(my_s + 16 * t + 4 * j);
+                const f32x4 sk = *(const f32x4 *)(my_s + 16 * t + 4 * j);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sk[i] = s4[i] * a.c;
-                }
+                for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[r][t][i] *= sk[i];
-                if (edge)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (!((vis[r] >> (4 * t + i)) & 1)) x[r][t][i] = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, x[r][t][i]);
+                    for (int i = 0; i < 4; i++) x[r][t][i] *= sk[i];
             }
-            mx = over_groups(mx, fmax_);
-            const float mn = fmaxf(m[r], mx), mu = mn == -INFINITY ? 0.0f : mn;
-            if (__any(mn > m[r])) {
-                const float al = __builtin_amdgcn_exp2f(m[r] - mu);
-                l[r] *= al;
+        Frag<CT, Pc::P> pf[R][NT / 2];
 #pragma unroll
-                for (int c = 0; c < VC; c++)
-#pragma unroll
-                    for (int e = 0; e < VW; e++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) o[r][c][e][i] *= al;
-                m[r] = mn;
-            }
-            float w[TP / 4];
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    w[4 * t + i] = __builtin_amdgcn_exp2f(x[r][t][i] - mu);
-                    l[r] += w[4 * t + i];
-                }
-            if constexpr (SCALED) {
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const f32x4 s4 = *(const f32x4 *)(my_s + 64 + 16 * t + 4 * j);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) w[4 * t + i] *= s4[i];
-                }
-                if (edge) // (0 * a scale that is not finite)
-#pragma unroll
-                    for (int i = 0; i < TP / 4; i++)
-                        if (!((vis[r] >> i) & 1)) w[i] = 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < NT / 2; u++) {
-                float y[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = w[8 * u + i];
-                fill(pf[r][u], y);
-            }
+        for (int r = 0; r < R; r++) {
+            weights(x[r], cq[r], my_s + 64 + 4 * j, edge, vis[r], oe, m[r], l[r], o[r], pf[r]);
             if (!SCALED && (sees[r] & bad)) l[r] = NAN;
         }
 
 #pragma unroll
         for (int u = 0; u < NT / 2; u++)
 #pragma unroll
-            for (int c = 0; c < VC; c++)
+            for (int c = 0; c < VC; c++) {
+                Frag<CT, 1> vf[VW];
 #pragma unroll
-                for (int e = 0; e < VW; e++) {
-                    Frag<CT, 1> vf;
+                for (int i = 0; i < 8; i += 2) {
+                    const uint32_t *v0 = vr[8 * u + i][c], *v1 = vr[8 * u + i + 1][c];
+                    if constexpr (CT == LLM_F32) {
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const uint32_t *v0 = vr[8 * u + i][c], *v1 = vr[8 * u + i + 1][c];
-                        if constexpr (CT == LLM_F32) {
-                            vf.v[i] = __uint_as_float(v0[e]), vf.v[i + 1] = __uint_as_float(v1[e]);
-                        } else if constexpr (CT == LLM_BF16) {
-                            vf.v[0][i / 2] = e % 2 ? __builtin_amdgcn_perm(v1[e / 2], v0[e / 2], 0x07060302)
-                                                   : __builtin_amdgcn_perm(v1[e / 2], v0[e / 2], 0x05040100);
-                        } else {
-                            const uint32_t a0 = v0[e / 4], a1 = v1[e / 4];
-                            vf.v[0][i / 2] = e % 4 == 0   ? bf2(code<CT, 0>(a0), code<CT, 0>(a1))
-                                             : e % 4 == 1 ? bf2(code<CT, 1>(a0), code<CT, 1>(a1))
-                                             : e % 4 == 2 ? bf2(code<CT, 2>(a0), code<CT, 2>(a1))
-                                                          : bf2(code<CT, 3>(a0), code<CT, 3>(a1));
+                        for (int e = 0; e < VW; e++)
+                            vf[e].v[i] = __uint_as_float(v0[e]), vf[e].v[i + 1] = __uint_as_float(v1[e]);
+                    } else if constexpr (CT == LLM_BF16) {
+#pragma unroll
+                        for (int e = 0; e < VW; e++)
+                            vf[e].v[0][i / 2] = __builtin_amdgcn_perm(v1[e / 2], v0[e / 2], e % 2 ? 0x07060302 : 0x05040100);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VW; e += 4) {
+                            uint32_t q[4];
+                            pairs2<CT, 0>(v0[e / 4], v1[e / 4], q);
+                            pairs2<CT, 1>(v0[e / 4], v1[e / 4], q + 2);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) vf[e + k].v[0][i / 2] = q[k];
                         }
                     }
-#pragma unroll
-                    for (int r = 0; r < R; r++) o[r][c][e] = product(vf, pf[r][u], o[r][c][e]);
                 }
+#pragma unroll
+                for (int e = 0; e < VW; e++)
+#pragma unroll
+                    for (int r = 0; r < R; r++) o[r][c * VW + e] = product(vf[e], pf[r][u], o[r][c * VW + e]);
+            }
         load_v(step + 4);
     }
 
@@ -447,86 +569,294 @@ __global__ void __launch_bounds__(256) k_tree_attention(TreeArgs a) {
             lw[w] = sm_ml[((w * R + r) * 16 + n) * 2 + 1];
         }
         const float mn = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3])), mu = mn == -INFINITY ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m[r] - mu);
+        const float al = __builtin_amdgcn_exp2f(m[r] - mu) * (SCALED ? power_from(ve) : 1.0f);
         l[r] = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; w++) l[r] += lw[w] * __builtin_amdgcn_exp2f(mw[w] - mu);
         m[r] = mn;
 #pragma unroll
-        for (int c = 0; c < VC; c++)
+        for (int d = 0; d < VC * VW; d++)
 #pragma unroll
-            for (int e = 0; e < VW; e++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[r][c][e][i] *= al;
+            for (int i = 0; i < 4; i++) o[r][d][i] *= al;
     }
-    auto slot = [&](int s, int r, int c, int e) -> f32x4 & { return sm_o[((s * R + r) * (HSP / 16) + c * VW + e) * 64 + lane]; };
+    auto slot = [&](int s, int r, int d) -> f32x4 & { return sm_o[((s * R + r) * (HSP / 16) + d) * 64 + lane]; };
 #pragma unroll
     for (int half = 2; half; half >>= 1) {
         if (wave >= half && wave < 2 * half)
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int c = 0; c < VC; c++)
-#pragma unroll
-                    for (int e = 0; e < VW; e++) slot(wave - half, r, c, e) = o[r][c][e];
+                for (int d = 0; d < VC * VW; d++) slot(wave - half, r, d) = o[r][d];
         __syncthreads();
         if (wave < half)
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int c = 0; c < VC; c++)
-#pragma unroll
-                    for (int e = 0; e < VW; e++) o[r][c][e] += slot(wave, r, c, e);
+                for (int d = 0; d < VC * VW; d++) o[r][d] += slot(wave, r, d);
         __syncthreads();
     }
     if (wave) return;
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const int row = row0 + 16 * r + n, t = row / a.group, g = row - t * a.group;
-        if (row >= rows) continue;
-        // a row that sees nothing has the sum 0
-        const float il = slices > 1 ? 1.0f : l[r] == 0.0f ? 0.0f : 1.0f / l[r];
-        const int64_t part = (((int64_t)b * a.n_kv + h) * a.splits + split_id) * a.max_n * a.group + row;
-        if (slices > 1 && j == 0) {
-            a.ml[2 * part] = m[r];
-            a.ml[2 * part + 1] = l[r];
-        }
-        uint8_t *op = a.o + b * a.o_seq + t * a.o_tok + (h * a.group + g) * a.o_head;
+        const int row = row0 + 16 * r + n;
+        if (row >= p.rows) continue;
+        const float il = to_output(p, l[r]);
+        if (p.slices > 1 && j == 0) put_sums(a, p, row, m[r], l[r]);
 #pragma unroll
         for (int c = 0; c < VC; c++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int d = c * 16 * VW + VW * (4 * j + i);
-                if (d >= a.hs) continue;
+            for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int e = 0; e < VW; e += 4) {
-                    const float4 y = make_float4(o[r][c][e][i] * il, o[r][c][e + 1][i] * il, o[r][c][e + 2][i] * il,
-                                                 o[r][c][e + 3][i] * il);
-                    if (slices > 1) *(float4 *)(a.acc + part * a.hs + d + e) = y;
-                    else if constexpr (QT == LLM_F32) *(float4 *)(op + (size_t)(d + e) * 4) = y;
-                    else *(uint2 *)(op + (size_t)(d + e) * 2) = make_uint2(bf2(y.x, y.y), bf2(y.z, y.w));
+                    const f32x4 *y = &o[r][c * VW + e];
+                    put_values<QT>(a, p, row, c * 16 * VW + VW * (4 * j + i) + e,
+                                   make_float4(y[0][i] * il, y[1][i] * il, y[2][i] * il, y[3][i] * il));
                 }
-            }
     }
 }
+
+// ---- many rows: the waves share the rows
+
+#if TREE_HSP <= 128
+// A step in LDS, 16-bit values: K rows in order, V transposed, its positions in the order of the weights' lanes (unit u, j
+// of eight: positions 4 j + i of tiles 2 u and 2 u + 1).  Rows are padded by 16 bytes, so that the sixteen rows of a read
+// start in different banks.
+struct __align__(16) TreeStep {
+    static constexpr int KP = HSP * 2 + 16, VP = 128 + 16; // bytes of a row
+    uint8_t k[64 * KP], v[HSP * VP];
+    float s[2][64]; // K scales, V scales times a power of two
+    uint32_t e, pad[3]; // that power's exponent field (power_to)
+};
+
+template <int CT, int QT, int R>
+__global__ void __launch_bounds__(256, 2) k_tree_rows(TreeArgs a) {
+    using Pc = TreePieces<CT, QT>;
+    constexpr int ES = Pc::ES, KS = HSP / 32, DT = HSP / 16;
+    constexpr int KN = HSP * ES / 16, KL = 64 * KN / 256; // 16-byte pieces of a K row, of a thread
+    constexpr int VN = HSP / 4;                           // runs of four dimensions: a thread takes one, at eight positions
+    constexpr bool SCALED = Pc::SCALED;
+    __shared__ TreeStep sm[2];
+    __shared__ uint32_t sm_bad[2]; // new tokens whose V row is not finite
+
+    const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row0 = blockIdx.y * 64 * R, my_row0 = row0 + wave * 16 * R;
+    Place p;
+    if (!place<QT>(a, 64, row0, 64 * R, p)) return;
+
+    const uint8_t *const kb = a.k + p.b * a.seq + p.h * a.head, *const vb = a.v + p.b * a.seq + p.h * a.head;
+    const float *ksb = nullptr, *vsb = nullptr;
+    if constexpr (SCALED) {
+        ksb = a.ks + p.b * a.s_seq + p.h * a.s_head;
+        vsb = a.vs + p.b * a.s_seq + p.h * a.s_head;
+    }
+    const uint32_t ps = (uint32_t)a.pos, hb = (uint32_t)(a.hs * ES);
+    const int vu = threadIdx.x / VN, vc = threadIdx.x % VN; // V: unit (u = vu / 4, j = vu % 4) and run
+    const bool has_v = VN == 32 || threadIdx.x < 8 * VN;
+    u32x4 kr[KL];
+    uint32_t vr[8][ES], sr = 0, next_e = 20; // (the largest V scale's exponent field, at least 2^-107; wave 1 keeps it)
+    auto load = [&](int step) {
+        const auto rk = step_rsrc(kb, a.pos, step, 64, p);
+#pragma unroll
+        for (int i = 0; i < KL; i++) {
+            const uint32_t piece = threadIdx.x + 256 * i, at = piece % KN * 16;
+            const auto x = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(at < hb ? piece / KN * ps + at : OUT_OF_RANGE), 0, 0);
+            kr[i] = (u32x4){x[0], x[1], x[2], x[3]};
+        }
+        const auto rv = step_rsrc(vb, a.pos, step, 64, p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t pos = 32 * (vu / 4) + 16 * (i / 4) + 4 * (vu % 4) + i % 4;
+            const int off = (int)(has_v && 4 * ES * vc < hb ? pos * ps + 4 * ES * vc : OUT_OF_RANGE);
+            if constexpr (ES == 1) vr[i][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, off, 0, 0);
+            else {
+                const auto x = __builtin_amdgcn_raw_buffer_load_b64(rv, off, 0, 0);
+                vr[i][0] = x[0], vr[i][1] = x[1];
+            }
+        }
+        if constexpr (SCALED) // (waves 0 and 1: K's, V's)
+            if (wave < 2)
+                sr = __builtin_amdgcn_raw_buffer_load_b32(step_rsrc(wave ? vsb : ksb, a.s_pos * 4, step, 64, p),
+                                                          (int)(lane * (uint32_t)a.s_pos * 4), 0, 0);
+    };
+    auto store = [&](int step, TreeStep &st) {
+#pragma unroll
+        for (int i = 0; i < KL; i++) {
+            const uint32_t piece = threadIdx.x + 256 * i;
+            uint8_t *to = st.k + piece / KN * TreeStep::KP + piece % KN * (32 / ES);
+            if constexpr (CT == LLM_BF16) *(u32x4 *)to = kr[i];
+            else {
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t u0 = flip_sign<CT>(kr[i][2 * k]), u1 = flip_sign<CT>(kr[i][2 * k + 1]);
+                    *(u32x4 *)(to + 16 * k) = (u32x4){codes2<CT, 0>(u0), codes2<CT, 1>(u0), codes2<CT, 0>(u1), codes2<CT, 1>(u1)};
+                }
+            }
+        }
+        if (has_v) {
+            if constexpr (CT == LLM_BF16) {
+                if (step * 64 + 64 > p.len && step < p.last) { // (see k_tree_attention)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int at = step * 64 + 32 * (vu / 4) + 16 * (i / 4) + 4 * (vu % 4) + i % 4 - p.len;
+                        bool nf = false;
+#pragma unroll
+                        for (int k = 0; k < ES; k++)
+                            nf |= (vr[i][k] & 0x7f80u) == 0x7f80u || (vr[i][k] & 0x7f800000u) == 0x7f800000u;
+                        // (only the values that are not finite have to go; the row's others make its readers NaN too)
+                        if (nf && at >= 0) {
+                            atomicOr(&sm_bad[at / 32], 1u << (at % 32));
+#pragma unroll
+                            for (int k = 0; k < ES; k++) vr[i][k] = 0;
+                        }
+                    }
+                }
+            }
+            u32x4 w[4];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                if constexpr (CT == LLM_BF16) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e][i / 2] = __builtin_amdgcn_perm(vr[i + 1][e / 2], vr[i][e / 2], e % 2 ? 0x07060302 : 0x05040100);
+                } else {
+                    uint32_t q[4];
+                    pairs2<CT, 0>(vr[i][0], vr[i + 1][0], q);
+                    pairs2<CT, 1>(vr[i][0], vr[i + 1][0], q + 2);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e][i / 2] = q[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) *(u32x4 *)(st.v + (4 * vc + e) * TreeStep::VP + 16 * vu) = w[e];
+        }
+        if constexpr (SCALED)
+            if (wave < 2) {
+                float s = __uint_as_float(sr);
+                if (wave) {
+                    next_e = max(next_e, exponent(wave_max(s < INFINITY ? s : 0.0f)));
+                    s *= power_to(next_e);
+                    if (lane == 0) st.e = next_e;
+                }
+                st.s[wave][lane] = s;
+            }
+    };
+
+    load(p.first);
+    if (threadIdx.x < 2) sm_bad[threadIdx.x] = 0;
+    Frag<CT, Pc::Q> qf[R][KS];
+    uint64_t sees[R];
+    float cq[R], m[R], l[R];
+    f32x4 o[R][DT];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        cq[r] = load_queries<CT, QT, true>(a, p, my_row0 + 16 * r + n, qf[r], sees[r]);
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[r][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    uint32_t ve = 20;
+    const bool works = my_row0 < p.rows; // (a wave without rows still loads and stores)
+    __syncthreads();
+    store(p.first, sm[0]);
+    load(p.first + 1);
+    __syncthreads();
+
+    for (int step = p.first; step < p.last; step++) {
+        const TreeStep &st = sm[(step - p.first) & 1];
+        if (works) {
+            const bool edge = step * 64 + 64 > p.len;
+            f32x4 x[R][4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+#pragma unroll
+                for (int r = 0; r < R; r++) x[r][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    Frag<CT, 1> kf;
+                    kf.v[0] = *(const u32x4 *)(st.k + (16 * t + n) * TreeStep::KP + 64 * s + 16 * j);
+#pragma unroll
+                    for (int r = 0; r < R; r++) x[r][t] = product(kf, qf[r][s], x[r][t]);
+                }
+            }
+            float oe = 1.0f;
+            if constexpr (SCALED) {
+                const uint32_t e1 = __builtin_amdgcn_readfirstlane(st.e);
+                if (ve != e1) oe = power_from(ve) * power_to(e1);
+                ve = e1;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const f32x4 sk = *(const f32x4 *)&st.s[0][16 * t + 4 * j];
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[r][t][i] *= sk[i];
+                }
+            }
+            Frag<CT, Pc::P> pf[R][2];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                uint32_t vis = 0;
+                if (edge) vis = seen_bits<16>(p, step * 64, sees[r]);
+                weights(x[r], cq[r], &st.s[1][4 * j], edge, vis, oe, m[r], l[r], o[r], pf[r]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    Frag<CT, 1> vf;
+                    vf.v[0] = *(const u32x4 *)(st.v + (16 * d + n) * TreeStep::VP + 64 * u + 16 * j);
+#pragma unroll
+                    for (int r = 0; r < R; r++) o[r][d] = product(vf, pf[r][u], o[r][d]);
+                }
+        }
+        store(step + 1, sm[(step + 1 - p.first) & 1]);
+        load(step + 2);
+        __syncthreads();
+    }
+    if (!works) return;
+    const uint64_t bad = CT == LLM_BF16 ? (uint64_t)sm_bad[1] << 32 | sm_bad[0] : 0;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        l[r] = over_groups(l[r], fadd_);
+        if (sees[r] & bad) l[r] = NAN;
+        const int row = my_row0 + 16 * r + n;
+        if (row >= p.rows) continue;
+        const float il = to_output(p, l[r]) * (SCALED ? power_from(ve) : 1.0f);
+        if (p.slices > 1 && j == 0) put_sums(a, p, row, m[r], l[r]);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const f32x4 y = o[r][d];
+            put_values<QT>(a, p, row, 16 * d + 4 * j, make_float4(y[0] * il, y[1] * il, y[2] * il, y[3] * il));
+        }
+    }
+}
+#endif
 
 } // namespace
 
 #define TREE_NAME2(n) tree_kernel_##n
 #define TREE_NAME(n) TREE_NAME2(n)
 
-TreeKernel TREE_NAME(TREE_HSP)(int type, int q_type, int tiles, size_t *lds) {
-#define TREE_PICK(C, Q, T)                           \
-    if (type == C && q_type == Q && tiles == T) {    \
-        *lds = TreeShape<C, Q, T>::LDS;              \
-        return k_tree_attention<C, Q, T>;            \
+TreeKernel TREE_NAME(TREE_HSP)(int type, int q_type, int tiles, int many, size_t *lds) {
+#define TREE_PICK(C, Q, T)                                \
+    if (!many && type == C && q_type == Q && tiles == T) { \
+        *lds = TreeShape<C, Q, T>::LDS;                   \
+        return k_tree_attention<C, Q, T>;                 \
     }
 #define TREE_PICK_Q(C, T) TREE_PICK(C, LLM_F32, T) TREE_PICK(C, LLM_BF16, T)
     TREE_PICK_Q(LLM_F32, 1) TREE_PICK_Q(LLM_BF16, 1) TREE_PICK_Q(LLM_I8, 1) TREE_PICK_Q(LLM_E4M3, 1)
 #if TREE_HSP <= 128
     TREE_PICK_Q(LLM_F32, 2) TREE_PICK_Q(LLM_BF16, 2) TREE_PICK_Q(LLM_I8, 2) TREE_PICK_Q(LLM_E4M3, 2)
+#define TREE_PICK_M(C, Q, T)                             \
+    if (many && type == C && q_type == Q && tiles == T) { \
+        *lds = 0;                                        \
+        return k_tree_rows<C, Q, T>;                     \
+    }
+#define TREE_PICK_MQ(C, T) TREE_PICK_M(C, LLM_F32, T) TREE_PICK_M(C, LLM_BF16, T)
+    TREE_PICK_MQ(LLM_BF16, 1) TREE_PICK_MQ(LLM_I8, 1) TREE_PICK_MQ(LLM_E4M3, 1)
+    TREE_PICK_MQ(LLM_BF16, 2) TREE_PICK_MQ(LLM_I8, 2) TREE_PICK_MQ(LLM_E4M3, 2)
 #endif
     return nullptr;
-#undef TREE_PICK
-#undef TREE_PICK_Q
 }

@@ -3,10 +3,14 @@ in float64.
 
 Tolerances.  u = 2^-24, half a step of fp32.
   cache rows: none; scales and codes are those of the definition.
-  attention: a score is a sum of hs products, each operand held to 24 bits: off by at most (hs + 8) u scale sum |q k|.  A
+  attention: a score is a sum of hs products, the query held to 22 bits at least (4 u): off by at most (hs + 8) u scale
+    sum |q k|.  A
     weight is then off by a factor of e^(2 d), d the largest such error of the row, a sum over L positions by L u, and
-    everything else (exponential, scales, joins) by 64 u; so is the output, relative to sum p |v|.  bf16: the weights of 16
-    bits (2^-16), and the output's half step, 2^-8 of its value.
+    everything else (exponential, scales, joins) by 64 u; so is the output, relative to sum p |v|.  bf16: the weights'
+    half step in fp16 (8-bit caches, 2^-11) or in two bf16 pieces (2^-16), and the output's, 2^-8 of its value.
+    8-bit caches: the weights p sv are fp16 pieces, scaled so that the largest V scale lands in [2^14, 2^15).  The last
+    piece has steps of 2^-24, so it is off by at most 2^-25 and a term code * w by |code| 2^-25 / (2^14 / max sv) <=
+    2^-39 max |v|: L of those.  (It is all there is in a dimension where the tokens that count have the code 0.)
   log probabilities: exponents off by 4 u |x - max| / T, the sum's terms by their number in a thread's chain and 64 joins
     and roundings, the result by its own rounding."""
 import math
@@ -154,7 +158,7 @@ def tree_masks(g, b, t):
     return mask
 
 
-def attention_check(q, kval, vval, lens, n, mask, scale, got, cache_len):
+def attention_check(q, kval, vval, lens, n, mask, scale, got, cache_len, cache):
     """got against float64 over the values kval, vval [b][h][ctx][hs] (float64, CPU)"""
     b, t, heads, hs = q.shape
     h = kval.shape[1]
@@ -179,7 +183,9 @@ def attention_check(q, kval, vval, lens, n, mask, scale, got, cache_len):
                 rel = 2 * d + (len(seen) + 64) * U
                 tol = rel * (p @ vv.abs())
                 if q.dtype == torch.bfloat16:
-                    tol = tol + 2.0 ** -16 * (p @ vv.abs()) + 2.0 ** -8 * want.abs()
+                    tol = tol + (2.0 ** -11 if cache in ("int8", "e4m3") else 2.0 ** -16) * (p @ vv.abs()) + 2.0 ** -8 * want.abs()
+                if cache in ("int8", "e4m3"):
+                    tol = tol + len(seen) * 2.0 ** -39 * float(vval[i, hd // (heads // h)].abs().max())
                 err = (got[i, j, hd].double().cpu() - want).abs()
                 assert (err <= tol + 1e-37).all(), (i, j, hd, float((err / (tol + 1e-37)).max()))
 
@@ -216,7 +222,7 @@ def attention_case(cache, rows, b, heads, h, hs, ctx, lens, t, n=None, layout="h
     m = torch.from_numpy(np.array(mask, np.uint64).view(np.int64)).to(DEV)
     got = pkg().tree_attention(q.to(DEV), k, v, it(lens), None if n is None else it(n), m, k_scale=ks, v_scale=vs,
                                max_len=max_len)
-    attention_check(q, vals[0], vals[1], lens, nn, mask, hs ** -0.5, got, ctx)
+    attention_check(q, vals[0], vals[1], lens, nn, mask, hs ** -0.5, got, ctx, cache)
     return got
 
 
