@@ -18,6 +18,7 @@ struct TreeArgs {
     const int *lens, *n;
     const uint64_t *mask;
     int n_seq, n_kv, hs, ctx, group, max_n, zero_rest;
+    int row_blocks, block_rows;    // blocks that share a kv head's rows, rows of each
     int splits, quantum;           // slices of a sequence's positions: at most, and their steps
     float c;                       // |softmax scale| * log2(e), positive
     int negate;                    // the scale is negative: the queries change their sign
@@ -25,7 +26,7 @@ struct TreeArgs {
 };
 
 // Positions of a step.  Few rows: a wave's step, its rows held in registers; many rows: the block's, in LDS.
-__host__ __device__ constexpr int tree_positions(int hsp, int type, bool many) {
+__host__ __device__ constexpr int tree_positions(int hsp, int type, int many) {
     return many || hsp * (type == LLM_F32 ? 4 : type == LLM_BF16 ? 2 : 1) <= 128 ? 64 : 32;
 }
 // Slices of `end` positions in steps of tp: of `quantum` steps, more where that gives more than `splits`; none is empty.
@@ -37,7 +38,7 @@ __host__ __device__ inline int tree_slices(int end, int tp, int splits, int quan
 
 typedef void (*TreeKernel)(TreeArgs);
 // The kernel for caches of `type` and queries of `q_type`, `tiles` tiles of 16 rows a wave, its waves taking positions
-// (many 0) or rows (many 1), and its LDS bytes.
+// (many 0) or rows (many: 4 or 8 waves), and its LDS bytes.
 TreeKernel tree_kernel_64(int type, int q_type, int tiles, int many, size_t *lds);
 TreeKernel tree_kernel_128(int type, int q_type, int tiles, int many, size_t *lds);
 TreeKernel tree_kernel_192(int type, int q_type, int tiles, int many, size_t *lds);

@@ -12,20 +12,22 @@ namespace {
 
 constexpr int TREE_MAX_SPLITS = 128;
 
-// A row's slices joined: weights exp2(max_s - max).  A thread takes four values of every (1024 / hs)-th slice, eight
-// slices' loads at once.
-template <int QT>
+// A row's slices joined: weights exp2(max_s - max).  W waves a row (the block has four): a thread takes four values of
+// every (64 W / (hs / 4))-th slice, eight slices' loads at once.
+template <int QT, int W>
 __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
-    __shared__ float sm_f[TREE_MAX_SPLITS + 64]; // (a group's last loads may be past the last slice: weight 0)
+    __shared__ float sm_f[4 / W][TREE_MAX_SPLITS + 64]; // (a group's last loads may be past the last slice: weight 0)
     __shared__ float4 sm_o[256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    constexpr int T = 64 * W;
+    const int lane = threadIdx.x & 63, part = threadIdx.x / T, tid = threadIdx.x % T;
+    const int row = blockIdx.x * (4 / W) + part, h = blockIdx.y, b = blockIdx.z;
     const int len = min(max(a.lens[b], 0), a.ctx), nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n;
     int steps;
     const int slices = tree_slices((int)min((int64_t)len + nn, (int64_t)a.ctx), tp, a.splits, a.quantum, &steps);
-    if (slices == 1 || row >= nn * a.group) return;
+    if (slices == 1) return; // (every row of the sequence was finished by its block)
+    const bool there = row < nn * a.group;
     const int64_t stride = (int64_t)a.max_n * a.group, base = ((int64_t)b * a.n_kv + h) * a.splits * stride + row;
-    const int per = a.hs / 4, groups = 256 / per, g = threadIdx.x / per, d = 4 * (threadIdx.x - g * per);
+    const int per = a.hs / 4, groups = T / per, g = tid / per, d = 4 * (tid - g * per);
     constexpr int U = 8;
     float4 v[U];
     auto load = [&](int s0) {
@@ -33,7 +35,7 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
         for (int u = 0; u < U; u++) {
             const int s = s0 + u * groups;
             v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (g < groups && s < slices) v[u] = *(const float4 *)(a.acc + (base + s * stride) * a.hs + d);
+            if (there && g < groups && s < slices) v[u] = *(const float4 *)(a.acc + (base + s * stride) * a.hs + d);
         }
     };
     load(g); // (the first values do not wait for the weights)
@@ -41,8 +43,9 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
 #pragma unroll
     for (int i = 0; i < TREE_MAX_SPLITS / 64; i++) {
         const int s = lane + 64 * i;
-        m[i] = s < slices ? a.ml[2 * (base + s * stride)] : -INFINITY;
-        l[i] = s < slices ? a.ml[2 * (base + s * stride) + 1] : 0.0f;
+        const bool have = there && s < slices;
+        m[i] = have ? a.ml[2 * (base + s * stride)] : -INFINITY;
+        l[i] = have ? a.ml[2 * (base + s * stride) + 1] : 0.0f;
         mx = fmaxf(mx, m[i]);
     }
     mx = wave_max(mx);
@@ -52,25 +55,25 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
     for (int i = 0; i < TREE_MAX_SPLITS / 64; i++) {
         const float f = __builtin_amdgcn_exp2f(m[i] - mu);
         sum += l[i] * f;
-        if (wave == 0) sm_f[lane + 64 * i] = f;
+        if (tid < 64) sm_f[part][lane + 64 * i] = f;
     }
     sum = wave_sum(sum);
-    if (wave == 0) sm_f[lane + TREE_MAX_SPLITS] = 0.0f;
+    if (tid < 64) sm_f[part][lane + TREE_MAX_SPLITS] = 0.0f;
     __syncthreads();
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int s0 = g; s0 < slices; s0 += U * groups) {
         if (s0 != g) load(s0);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const float f = sm_f[min(s0 + u * groups, TREE_MAX_SPLITS)];
+            const float f = sm_f[part][min(s0 + u * groups, TREE_MAX_SPLITS)];
             o.x += v[u].x * f, o.y += v[u].y * f, o.z += v[u].z * f, o.w += v[u].w * f;
         }
     }
     sm_o[threadIdx.x] = o;
     __syncthreads();
-    if (g) return;
+    if (g || !there) return;
     for (int k = 1; k < groups; k++) {
-        const float4 x = sm_o[k * per + threadIdx.x];
+        const float4 x = sm_o[part * T + k * per + tid];
         o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
     }
     const int t = row / a.group, gr = row - t * a.group;
@@ -87,30 +90,34 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
 }
 
 struct TreePlan {
-    int hsp, tp, many, tiles, row_blocks, splits, quantum;
+    int hsp, tp, many, tiles, row_blocks, block_rows, splits, quantum;
     size_t bytes;
 };
 
-// How a call is cut.  Up to 32 rows a kv head: the block's waves share the positions, with one or two tiles of 16 rows
-// each.  More rows: the waves share the rows, and the cache's rows go through LDS.  (Not for fp32 caches, whose rows need
-// no conversion, and head sizes above 128, whose rows do not fit twice.)  Positions in slices, the same number of steps
-// for every sequence, until the grid has two blocks a CU; eight for several sequences, whose lengths the host does not
-// know.
-TreePlan tree_plan(const llm_kv *c, int n_heads, int max_n, int max_len) {
+// How a call is cut.  Up to 32 rows a kv head: the block's four waves share the positions, with one or two tiles of 16 rows
+// each.  More rows: the waves share the rows, 16 each (four waves up to 64 rows, else eight), and the cache's rows go
+// through LDS.  (Not for fp32 caches, whose rows need no conversion, nor head sizes above 128, whose rows do not fit twice.
+// fp32 queries over bf16 caches, three pieces, take two tiles in each of four waves: eight would spill.)  The rows are
+// spread evenly over their blocks.  Positions in slices, the same number of steps for every sequence, until the grid has a
+// block a CU (few rows) or two; four for several sequences, whose lengths the host does not know.
+TreePlan tree_plan(const llm_kv *c, int q_type, int n_heads, int max_n, int max_len) {
     TreePlan p;
     p.hsp = (c->hs + 63) / 64 * 64;
-    const int group = n_heads / c->n_kv, rows = group * max_n;
-    p.many = rows > 32 && p.hsp <= 128 && c->type != LLM_F32;
+    const int group = n_heads / c->n_kv, rows = group * max_n, tiles = (rows + 15) / 16;
+    const bool many = rows > 32 && p.hsp <= 128 && c->type != LLM_F32, pieces = c->type == LLM_BF16 && q_type == LLM_F32;
+    p.many = !many ? 0 : tiles <= 4 || pieces ? 4 : 8;
+    p.tiles = many ? (tiles > 4 && pieces ? 2 : 1) : tiles > 1 && p.hsp <= 128 ? 2 : 1;
+    const int per_block = p.tiles * (many ? p.many : 1); // tiles
+    p.row_blocks = (tiles + per_block - 1) / per_block;
+    p.block_rows = 16 * (many ? (tiles + p.row_blocks - 1) / p.row_blocks : per_block);
     p.tp = tree_positions(p.hsp, c->type, p.many);
-    p.tiles = rows > (p.many ? 64 : 16) && p.hsp <= 128 ? 2 : 1;
-    const int per_block = 16 * p.tiles * (p.many ? 4 : 1);
-    p.row_blocks = (rows + per_block - 1) / per_block;
     const int64_t end = std::min<int64_t>((int64_t)std::max(max_len, 0) + max_n, c->ctx);
     const int64_t steps = std::max<int64_t>((end + p.tp - 1) / p.tp, 1), blocks = (int64_t)c->n_seq * c->n_kv * p.row_blocks;
-    const int64_t least = p.many ? 2 : 4; // steps of a slice (few rows: one a wave)
-    const int64_t want = std::max<int64_t>(1, (c->n_seq > 1 ? 2048 : 512) / std::max<int64_t>(blocks, 1));
-    const int64_t cap = std::min({want, (steps + least - 1) / least, (int64_t)TREE_MAX_SPLITS});
-    p.quantum = (int)std::max<int64_t>((steps + cap - 1) / cap, 1);
+    const int64_t least = many ? 2 : 4; // steps of a slice (few rows: one a wave)
+    const int64_t grid = c->n_seq > 1 ? 1024 : many ? 512 : 256;
+    const int64_t cap = std::min({std::max<int64_t>(1, grid / std::max<int64_t>(blocks, 1)), (steps + least - 1) / least,
+                                  (int64_t)TREE_MAX_SPLITS});
+    p.quantum = (int)((steps + cap - 1) / cap);
     p.splits = (int)((steps + p.quantum - 1) / p.quantum);
     p.bytes = p.splits > 1 ? (size_t)c->n_seq * c->n_kv * p.splits * rows * (c->hs + 2) * 4 : 0;
     return p;
@@ -124,7 +131,8 @@ bool tree_shape_ok(const llm_kv *c, int n_heads, int max_n) {
 } // namespace
 
 extern "C" size_t llm_tree_attention_work(const llm_kv *c, int n_heads, int max_n, int max_len) {
-    return tree_shape_ok(c, n_heads, max_n) ? tree_plan(c, n_heads, max_n, max_len).bytes : 0;
+    return tree_shape_ok(c, n_heads, max_n) ? std::max(tree_plan(c, LLM_F32, n_heads, max_n, max_len).bytes,
+                                                       tree_plan(c, LLM_BF16, n_heads, max_n, max_len).bytes) : 0;
 }
 
 extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_rows *out, int n_heads, const int *lens,
@@ -151,12 +159,12 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
         fprintf(stderr, "%s: q and out of different types\n", who);
         return -1;
     }
-    const TreePlan p = tree_plan(c, n_heads, max_n, max_len);
+    const TreePlan p = tree_plan(c, q->type, n_heads, max_n, max_len);
     if (p.bytes && (work_bytes < p.bytes || ((uintptr_t)work & 15) || !dev.holds(work, "the work memory"))) {
         fprintf(stderr, "%s: %zu bytes of work memory are needed, 16-byte aligned\n", who, p.bytes);
         return -1;
     }
-    const int64_t blocks = (int64_t)c->n_seq * c->n_kv * p.splits;
+    const int64_t blocks = ((int64_t)c->n_seq * c->n_kv * p.splits + 7) / 8 * 8 * p.row_blocks;
     if (blocks > 0x7fffffff || c->n_seq > 65535 || c->n_kv > 65535) {
         fprintf(stderr, "%s: %d sequences of %d kv heads\n", who, c->n_seq, c->n_kv);
         return -1;
@@ -174,7 +182,7 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
     a.o_seq = out->seq * qs, a.o_tok = out->tok * qs, a.o_head = out->head * qs;
     a.lens = lens, a.n = n, a.mask = mask;
     a.n_seq = c->n_seq, a.n_kv = c->n_kv, a.hs = c->hs, a.ctx = c->ctx;
-    a.group = n_heads / c->n_kv, a.max_n = max_n, a.splits = p.splits, a.quantum = p.quantum;
+    a.group = n_heads / c->n_kv, a.max_n = max_n, a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.splits = p.splits, a.quantum = p.quantum;
     a.zero_rest = zero_rest;
     // (a scale of 0 as one so small that every weight is 1)
     a.c = std::max(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
@@ -188,12 +196,15 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
         fprintf(stderr, "%s: internal error: no kernel\n", who);
         return -1;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks, p.row_blocks), dim3(256), lds, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(p.many ? 64 * p.many : 256), lds, (hipStream_t)stream, a);
     HIP_OR_FAIL(who, hipGetLastError());
     if (p.splits > 1) {
-        const dim3 grid(max_n * a.group, c->n_kv, c->n_seq);
-        if (q->type == LLM_F32) hipLaunchKernelGGL(k_tree_join<LLM_F32>, grid, dim3(256), 0, (hipStream_t)stream, a, p.tp);
-        else hipLaunchKernelGGL(k_tree_join<LLM_BF16>, grid, dim3(256), 0, (hipStream_t)stream, a, p.tp);
+        // a wave a row up to 8 slices, the block's four above
+        const bool wide = p.splits > 8;
+        const dim3 grid(wide ? max_n * a.group : (max_n * a.group + 3) / 4, c->n_kv, c->n_seq);
+        auto *join = q->type == LLM_F32 ? wide ? k_tree_join<LLM_F32, 4> : k_tree_join<LLM_F32, 1>
+                                        : wide ? k_tree_join<LLM_BF16, 4> : k_tree_join<LLM_BF16, 1>;
+        hipLaunchKernelGGL(join, grid, dim3(256), 0, (hipStream_t)stream, a, p.tp);
         HIP_OR_FAIL(who, hipGetLastError());
     }
     return 0;

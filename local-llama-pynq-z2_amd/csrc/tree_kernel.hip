@@ -145,6 +145,13 @@ struct TreePieces {
     static constexpr int P = QT == LLM_BF16 ? (SCALED ? 1 : 2) : SCALED ? 2 : 3; // of a weight
 };
 
+template <int QT>
+__device__ __forceinline__ float4 load_query(const uint8_t *row, int d) {
+    if constexpr (QT == LLM_F32) return *(const float4 *)(row + (size_t)d * 4);
+    const uint2 u = *(const uint2 *)(row + (size_t)d * 2);
+    return make_float4(lo16(u.x), hi16(u.x), lo16(u.y), hi16(u.y));
+}
+
 // The dimension of value i = 4 q4 .. 4 q4 + 3 of lane group j in product s.  From memory, a lane's 16-byte pieces of a K row
 // are its own (piece j of every four); from LDS, rows are in order.
 template <int CT, bool LDS>
@@ -154,17 +161,23 @@ __device__ __forceinline__ int dim_of(int s, int j, int q4) {
     else return 64 * (s / 2) + 16 * j + 8 * (s % 2) + 4 * q4;
 }
 
-// Where a block works: sequence, kv head, slice, and how many positions and rows there are.
+// Where a block works: sequence, kv head, slice, first row, and how many positions and rows there are.
 struct Place {
-    int b, h, split, len, end, rows, slices, first, last;
+    int b, h, split, row0, len, end, rows, slices, first, last;
 };
+// Blocks go to the eight XCDs in turn.  The row blocks of a slice follow each other on one, whose L2 then holds the slice's
+// rows for all of them; the slices of a sequence go around, each head's from another XCD on, so that sequences with few
+// slices do not all use the same ones.
 template <int QT>
-__device__ __forceinline__ bool place(const TreeArgs &a, int tp, int row0, int block_rows, Place &p) {
-    int id = blockIdx.x;
-    p.split = id % a.splits;
-    id /= a.splits;
-    p.h = id % a.n_kv;
-    p.b = id / a.n_kv;
+__device__ __forceinline__ bool place(const TreeArgs &a, int tp, int block_rows, Place &p) {
+    const uint32_t k = blockIdx.x >> 3, kr = k / (uint32_t)a.row_blocks;
+    const uint32_t id = kr * 8 + (blockIdx.x & 7), bh = id / (uint32_t)a.splits;
+    if (bh >= (uint32_t)(a.n_seq * a.n_kv)) return false; // (the grid is rounded up to eight slices)
+    p.split = (int)((id + 3 * bh) % (uint32_t)a.splits);
+    p.b = (int)(bh / (uint32_t)a.n_kv);
+    p.h = (int)bh - p.b * a.n_kv;
+    const int row0 = (int)(k - kr * a.row_blocks) * block_rows;
+    p.row0 = row0;
     p.len = min(max(a.lens[p.b], 0), a.ctx);
     const int nn = a.n ? min(max(a.n[p.b], 0), a.max_n) : a.max_n;
     p.end = (int)min((int64_t)p.len + nn, (int64_t)a.ctx);
@@ -172,7 +185,7 @@ __device__ __forceinline__ bool place(const TreeArgs &a, int tp, int row0, int b
     int steps;
     p.slices = tree_slices(p.end, tp, a.splits, a.quantum, &steps);
     if (a.zero_rest && p.split == 0 && row0 + block_rows > p.rows) { // the rows behind the last token
-        for (int e = threadIdx.x * 4; e < block_rows * a.hs; e += 1024) {
+        for (int e = threadIdx.x * 4; e < block_rows * a.hs; e += 4 * blockDim.x) {
             const int row = row0 + e / a.hs, t = row / a.group, d = e - (row - row0) * a.hs;
             if (row < p.rows || row >= a.max_n * a.group) continue;
             uint8_t *op = a.o + p.b * a.o_seq + t * a.o_tok + (p.h * a.group + row - t * a.group) * a.o_head;
@@ -195,23 +208,30 @@ __device__ __forceinline__ float load_queries(const TreeArgs &a, const Place &p,
     const bool ok = row < p.rows;
     sees = 0;
     if (ok) sees = a.mask ? a.mask[(int64_t)p.b * a.max_n + t] : ~(uint64_t)0 >> (63 - t);
+    if (p.end - p.len < 64) sees &= ((uint64_t)1 << (p.end - p.len)) - 1; // (tokens that are there)
     const uint8_t *qp = a.q + p.b * a.q_seq + (ok ? t * a.q_tok + (p.h * a.group + g) * a.q_head : 0);
-    float x[HSP / 32][8], mx = 0.0f;
+    // every load goes out before the first is used (what is not there reads the row's start): behind conditions each would
+    // be waited for by itself
+    float4 v[HSP / 32][2];
 #pragma unroll
     for (int s = 0; s < HSP / 32; s++)
 #pragma unroll
         for (int q4 = 0; q4 < 2; q4++) {
             const int d = dim_of<CT, LDS>(s, j, q4);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (ok && d < a.hs) {
-                if constexpr (QT == LLM_F32) v = *(const float4 *)(qp + (size_t)d * 4);
-                else {
-                    const uint2 u = *(const uint2 *)(qp + (size_t)d * 2);
-                    v = make_float4(lo16(u.x), hi16(u.x), lo16(u.y), hi16(u.y));
-                }
+            v[s][q4] = load_query<QT>(qp, d < a.hs ? d : 0);
+        }
+    float x[HSP / 32][8], mx = 0.0f;
+#pragma unroll
+    for (int s = 0; s < HSP / 32; s++)
+#pragma unroll
+        for (int q4 = 0; q4 < 2; q4++) {
+            const bool there = ok && dim_of<CT, LDS>(s, j, q4) < a.hs;
+            const float y[4] = {v[s][q4].x, v[s][q4].y, v[s][q4].z, v[s][q4].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[s][4 * q4 + i] = there ? y[i] : 0.0f;
+                mx = fmaxf(mx, fabsf(x[s][4 * q4 + i]));
             }
-            x[s][4 * q4] = v.x, x[s][4 * q4 + 1] = v.y, x[s][4 * q4 + 2] = v.z, x[s][4 * q4 + 3] = v.w;
-            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
         }
     float to = 1.0f, from = 1.0f;
     if constexpr (TreePieces<CT, QT>::SCALED) {
@@ -229,16 +249,16 @@ __device__ __forceinline__ float load_queries(const TreeArgs &a, const Place &p,
     return fmaxf(a.c * from, 1e-37f);
 }
 
-// What row `sees` of a step's positions at its edge: bit 4 t + i.
+// What the row sees of a step's positions where new tokens or the end are among them: bit 4 t + i.
 template <int N>
 __device__ __forceinline__ uint32_t seen_bits(const Place &p, int p0, uint64_t sees) {
     const int j = (threadIdx.x & 63) >> 4;
     uint32_t vis = 0;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int at = p0 + 16 * (i / 4) + 4 * j + i % 4;
-        const bool v = at < p.len || (at < p.end && ((sees >> (at - p.len)) & 1));
-        vis |= (uint32_t)v << i;
+        const int at = p0 + 16 * (i / 4) + 4 * j + i % 4 - p.len;
+        const uint32_t bit = (uint32_t)(sees >> (at & 63)) & 1;
+        vis |= (at < 0 ? 1u : at < 64 ? bit : 0u) << i;
     }
     return vis;
 }
@@ -254,8 +274,7 @@ __device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *s
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (!((vis >> (4 * t + i)) & 1)) x[t][i] = -INFINITY;
+            for (int i = 0; i < 4; i++) x[t][i] = (vis >> (4 * t + i)) & 1 ? x[t][i] : -INFINITY;
     float mx = x[0][0];
 #pragma unroll
     for (int t = 0; t < NT; t++)
@@ -284,8 +303,11 @@ __device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *s
             if constexpr (SCALED) {
                 if (i % 4 == 0) s4 = *(const f32x4 *)(sv + 16 * t);
                 w[i] *= s4[i % 4];
-                if (edge && !((vis >> (8 * u + i)) & 1)) w[i] = 0.0f; // (0 * a scale that is not finite)
             }
+        }
+        if (SCALED && edge) { // (0 * a scale that is not finite)
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = (vis >> (8 * u + i)) & 1 ? w[i] : 0.0f;
         }
         fill(pf[u], w);
     }
@@ -352,9 +374,9 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && R == 1 && HSP <= 128 ? 2
 
     const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row0 = blockIdx.y * 16 * R;
     Place p;
-    if (!place<QT>(a, TP, row0, 16 * R, p)) return;
+    if (!place<QT>(a, TP, 16 * R, p)) return;
+    const int row0 = p.row0;
 
     const uint8_t *const kb = a.k + p.b * a.seq + p.h * a.head, *const vb = a.v + p.b * a.seq + p.h * a.head;
     const float *ksb = nullptr, *vsb = nullptr;
@@ -618,96 +640,129 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && R == 1 && HSP <= 128 ? 2
 // ---- many rows: the waves share the rows
 
 #if TREE_HSP <= 128
-// A step in LDS, 16-bit values: K rows in order, V transposed, its positions in the order of the weights' lanes (unit u, j
-// of eight: positions 4 j + i of tiles 2 u and 2 u + 1).  Rows are padded by 16 bytes, so that the sixteen rows of a read
-// start in different banks.
+// A step in LDS, 16-bit values in units of eight: K rows in order, V transposed, its positions in the order of the weights'
+// lanes: unit 4 u + j of a V row's eight holds positions 4 j + i of tiles 2 u and 2 u + 1.  Sixteen units are all banks
+// once; the units of a row change places by its number, so that the sixteen rows of a read are in different ones, and
+// the runs of a write in half of them.
 struct __align__(16) TreeStep {
-    static constexpr int KP = HSP * 2 + 16, VP = 128 + 16; // bytes of a row
-    uint8_t k[64 * KP], v[HSP * VP];
-    float s[2][64]; // K scales, V scales times a power of two
+    static constexpr int KU = HSP / 8; // units of a K row
+    uint4 k[64 * KU], v[HSP * 8];
+    float s[2][64];     // K scales, V scales times a power of two
     uint32_t e, pad[3]; // that power's exponent field (power_to)
+    __device__ __forceinline__ static int k_at(int row, int unit) {
+        return row * KU + (unit ^ (KU == 16 ? row & 15 : (row >> 1) & 7));
+    }
+    __device__ __forceinline__ static int v_at(int dim, int unit) { return dim * 8 + (unit ^ ((dim >> 1) & 7)); }
 };
 
-template <int CT, int QT, int R>
-__global__ void __launch_bounds__(256, 2) k_tree_rows(TreeArgs a) {
+// A wave has 16 rows and takes them through scores, softmax and values 32 positions at a time: few enough registers for
+// four waves a SIMD, which hide each other's LDS and product latencies (two rows tiles a wave, or 32 x 32 tiles, read less
+// LDS but leave two: a 37-token tree over 12k int8 positions 51 us a launch, a batch of 64-token trees over bf16 202).  A
+// step of 64 positions is in LDS while the next one's loads are under way: one barrier a step.
+template <int CT, int QT, int NW, int R>
+__global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs a) {
     using Pc = TreePieces<CT, QT>;
     constexpr int ES = Pc::ES, KS = HSP / 32, DT = HSP / 16;
+    constexpr bool APART = NW == 8; // waves 4 to 7 fetch K, 0 to 3 V; four waves fetch both
     constexpr int KN = HSP * ES / 16, KL = 64 * KN / 256; // 16-byte pieces of a K row, of a thread
     constexpr int VN = HSP / 4;                           // runs of four dimensions: a thread takes one, at eight positions
+    constexpr int VAT = APART ? 0 : 4 * KL, NR = APART ? (4 * KL > 8 * ES ? 4 * KL : 8 * ES) : 4 * KL + 8 * ES;
     constexpr bool SCALED = Pc::SCALED;
     __shared__ TreeStep sm[2];
     __shared__ uint32_t sm_bad[2]; // new tokens whose V row is not finite
 
     const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row0 = blockIdx.y * 64 * R, my_row0 = row0 + wave * 16 * R;
     Place p;
-    if (!place<QT>(a, 64, row0, 64 * R, p)) return;
+    if (!place<QT>(a, 64, a.block_rows, p)) return;
 
-    const uint8_t *const kb = a.k + p.b * a.seq + p.h * a.head, *const vb = a.v + p.b * a.seq + p.h * a.head;
-    const float *ksb = nullptr, *vsb = nullptr;
-    if constexpr (SCALED) {
-        ksb = a.ks + p.b * a.s_seq + p.h * a.s_head;
-        vsb = a.vs + p.b * a.s_seq + p.h * a.s_head;
-    }
-    const uint32_t ps = (uint32_t)a.pos, hb = (uint32_t)(a.hs * ES);
-    const int vu = threadIdx.x / VN, vc = threadIdx.x % VN; // V: unit (u = vu / 4, j = vu % 4) and run
-    const bool has_v = VN == 32 || threadIdx.x < 8 * VN;
-    u32x4 kr[KL];
-    uint32_t vr[8][ES], sr = 0, next_e = 20; // (the largest V scale's exponent field, at least 2^-107; wave 1 keeps it)
-    auto load = [&](int step) {
-        const auto rk = step_rsrc(kb, a.pos, step, 64, p);
+    const int row0 = p.row0 + wave * 16 * R;
+    const bool works = wave * 16 * R < a.block_rows && row0 < p.rows; // (a wave without rows still fetches)
+    const bool does_k = !APART || wave >= 4, does_v = (!APART || wave < 4) && (VN == 32 || (threadIdx.x & 255) < 8 * VN);
+    const uint32_t hb = (uint32_t)(a.hs * ES);
+    const int64_t p00 = (int64_t)p.first * 64;
+    const uint8_t *kp = a.k + p.b * a.seq + p.h * a.head + p00 * a.pos, *vp = a.v + p.b * a.seq + p.h * a.head + p00 * a.pos;
+    const float *sp = nullptr; // wave 0: K's scales, wave 1: V's
+    if constexpr (SCALED) sp = (wave == 1 ? a.vs : a.ks) + p.b * a.s_seq + p.h * a.s_head + p00 * a.s_pos;
+    int left = min(p.end, p.last * 64) - p.first * 64; // positions not fetched yet
+    uint32_t raw[NR], sr = 0, next_e = 20; // (the largest V scale's exponent field, at least 2^-107; wave 1 keeps it)
+    // Addresses are formed again at every use, from values that the compiler cannot see through: kept across the loop they
+    // would cost the registers that keep it free of spills (a reload waits for the loads under way).
+    auto again = [](uint32_t x) {
+        asm volatile("" : "+v"(x));
+        return x;
+    };
+    auto load = [&] {
+        const uint32_t tid = again(threadIdx.x & 255), ps = a.pos;
+        const int here = max(min(left, 64), 0);
+        if (does_k) {
+            const auto rk = __builtin_amdgcn_make_buffer_rsrc((void *)kp, 0, (int)(here * a.pos), 0x00020000);
 #pragma unroll
-        for (int i = 0; i < KL; i++) {
-            const uint32_t piece = threadIdx.x + 256 * i, at = piece % KN * 16;
-            const auto x = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(at < hb ? piece / KN * ps + at : OUT_OF_RANGE), 0, 0);
-            kr[i] = (u32x4){x[0], x[1], x[2], x[3]};
-        }
-        const auto rv = step_rsrc(vb, a.pos, step, 64, p);
+            for (int i = 0; i < KL; i++) {
+                const uint32_t piece = tid + 256 * i, at = piece % KN * 16;
+                const auto x = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(at < hb ? piece / KN * ps + at : OUT_OF_RANGE), 0, 0);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t pos = 32 * (vu / 4) + 16 * (i / 4) + 4 * (vu % 4) + i % 4;
-            const int off = (int)(has_v && 4 * ES * vc < hb ? pos * ps + 4 * ES * vc : OUT_OF_RANGE);
-            if constexpr (ES == 1) vr[i][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, off, 0, 0);
-            else {
-                const auto x = __builtin_amdgcn_raw_buffer_load_b64(rv, off, 0, 0);
-                vr[i][0] = x[0], vr[i][1] = x[1];
+                for (int k = 0; k < 4; k++) raw[4 * i + k] = x[k];
             }
         }
-        if constexpr (SCALED) // (waves 0 and 1: K's, V's)
-            if (wave < 2)
-                sr = __builtin_amdgcn_raw_buffer_load_b32(step_rsrc(wave ? vsb : ksb, a.s_pos * 4, step, 64, p),
-                                                          (int)(lane * (uint32_t)a.s_pos * 4), 0, 0);
-    };
-    auto store = [&](int step, TreeStep &st) {
+        if (does_v) {
+            const auto rv = __builtin_amdgcn_make_buffer_rsrc((void *)vp, 0, (int)(here * a.pos), 0x00020000);
+            const uint32_t vu = tid / VN, vc = tid % VN; // unit and run
+            const uint32_t vo = 4 * ES * vc < hb ? (32 * (vu / 4) + 4 * (vu % 4)) * ps + 4 * ES * vc : OUT_OF_RANGE;
 #pragma unroll
-        for (int i = 0; i < KL; i++) {
-            const uint32_t piece = threadIdx.x + 256 * i;
-            uint8_t *to = st.k + piece / KN * TreeStep::KP + piece % KN * (32 / ES);
-            if constexpr (CT == LLM_BF16) *(u32x4 *)to = kr[i];
-            else {
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const uint32_t u0 = flip_sign<CT>(kr[i][2 * k]), u1 = flip_sign<CT>(kr[i][2 * k + 1]);
-                    *(u32x4 *)(to + 16 * k) = (u32x4){codes2<CT, 0>(u0), codes2<CT, 1>(u0), codes2<CT, 0>(u1), codes2<CT, 1>(u1)};
+            for (int i = 0; i < 8; i++) {
+                const int off = (int)(vo + (16 * (i / 4) + i % 4) * ps); // (stays out of range)
+                if constexpr (ES == 1) raw[VAT + i] = __builtin_amdgcn_raw_buffer_load_b32(rv, off, 0, 0);
+                else {
+                    const auto x = __builtin_amdgcn_raw_buffer_load_b64(rv, off, 0, 0);
+                    raw[VAT + 2 * i] = x[0], raw[VAT + 2 * i + 1] = x[1];
                 }
             }
         }
-        if (has_v) {
+        if constexpr (SCALED)
+            if (wave < 2) {
+                const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)sp, 0, (int)(here * a.s_pos * 4), 0x00020000);
+                sr = __builtin_amdgcn_raw_buffer_load_b32(rs, (int)(lane * (uint32_t)a.s_pos * 4), 0, 0);
+                sp += 64 * a.s_pos;
+            }
+        kp += 64 * a.pos;
+        vp += 64 * a.pos;
+        left -= 64;
+    };
+    auto store = [&](int step, TreeStep &st) {
+        const uint32_t tid = again(threadIdx.x & 255), vu = tid / VN, vc = tid % VN;
+        if (does_k)
+#pragma unroll
+            for (int i = 0; i < KL; i++) {
+                const uint32_t piece = tid + 256 * i;
+                const int row = piece / KN, unit = piece % KN * (2 / ES);
+                if constexpr (CT == LLM_BF16)
+                    st.k[st.k_at(row, unit)] = make_uint4(raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
+                else {
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const uint32_t u0 = flip_sign<CT>(raw[4 * i + 2 * k]), u1 = flip_sign<CT>(raw[4 * i + 2 * k + 1]);
+                        st.k[st.k_at(row, unit + k)] =
+                            make_uint4(codes2<CT, 0>(u0), codes2<CT, 1>(u0), codes2<CT, 0>(u1), codes2<CT, 1>(u1));
+                    }
+                }
+            }
+        if (does_v) {
+            uint32_t *vr = raw + VAT;
             if constexpr (CT == LLM_BF16) {
-                if (step * 64 + 64 > p.len && step < p.last) { // (see k_tree_attention)
+                if (step * 64 + 64 > p.len) { // values that are not finite among the new tokens: see k_tree_attention
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int at = step * 64 + 32 * (vu / 4) + 16 * (i / 4) + 4 * (vu % 4) + i % 4 - p.len;
+                        const int at = step * 64 + (int)(32 * (vu / 4) + 4 * (vu % 4)) + 16 * (i / 4) + i % 4 - p.len;
                         bool nf = false;
 #pragma unroll
-                        for (int k = 0; k < ES; k++)
-                            nf |= (vr[i][k] & 0x7f80u) == 0x7f80u || (vr[i][k] & 0x7f800000u) == 0x7f800000u;
-                        // (only the values that are not finite have to go; the row's others make its readers NaN too)
-                        if (nf && at >= 0) {
+                        for (int k = 0; k < 2; k++) {
+                            const uint32_t u = vr[2 * i + k];
+                            nf |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
+                        }
+                        if (nf && at >= 0) { // (the row's other values may stay: who sees them becomes NaN)
                             atomicOr(&sm_bad[at / 32], 1u << (at % 32));
-#pragma unroll
-                            for (int k = 0; k < ES; k++) vr[i][k] = 0;
+                            vr[2 * i] = vr[2 * i + 1] = 0;
                         }
                     }
                 }
@@ -718,17 +773,17 @@ __global__ void __launch_bounds__(256, 2) k_tree_rows(TreeArgs a) {
                 if constexpr (CT == LLM_BF16) {
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        w[e][i / 2] = __builtin_amdgcn_perm(vr[i + 1][e / 2], vr[i][e / 2], e % 2 ? 0x07060302 : 0x05040100);
+                        w[e][i / 2] = __builtin_amdgcn_perm(vr[2 * i + 2 + e / 2], vr[2 * i + e / 2], e % 2 ? 0x07060302 : 0x05040100);
                 } else {
                     uint32_t q[4];
-                    pairs2<CT, 0>(vr[i][0], vr[i + 1][0], q);
-                    pairs2<CT, 1>(vr[i][0], vr[i + 1][0], q + 2);
+                    pairs2<CT, 0>(vr[i], vr[i + 1], q);
+                    pairs2<CT, 1>(vr[i], vr[i + 1], q + 2);
 #pragma unroll
                     for (int e = 0; e < 4; e++) w[e][i / 2] = q[e];
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) *(u32x4 *)(st.v + (4 * vc + e) * TreeStep::VP + 16 * vu) = w[e];
+            for (int e = 0; e < 4; e++) st.v[st.v_at(4 * vc + e, vu)] = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
         }
         if constexpr (SCALED)
             if (wave < 2) {
@@ -742,7 +797,7 @@ __global__ void __launch_bounds__(256, 2) k_tree_rows(TreeArgs a) {
             }
     };
 
-    load(p.first);
+    load();
     if (threadIdx.x < 2) sm_bad[threadIdx.x] = 0;
     Frag<CT, Pc::Q> qf[R][KS];
     uint64_t sees[R];
@@ -750,86 +805,87 @@ __global__ void __launch_bounds__(256, 2) k_tree_rows(TreeArgs a) {
     f32x4 o[R][DT];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        cq[r] = load_queries<CT, QT, true>(a, p, my_row0 + 16 * r + n, qf[r], sees[r]);
+        cq[r] = load_queries<CT, QT, true>(a, p, row0 + 16 * r + n, qf[r], sees[r]);
         m[r] = -INFINITY;
         l[r] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++) o[r][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
     uint32_t ve = 20;
-    const bool works = my_row0 < p.rows; // (a wave without rows still loads and stores)
     __syncthreads();
     store(p.first, sm[0]);
-    load(p.first + 1);
+    load();
     __syncthreads();
 
     for (int step = p.first; step < p.last; step++) {
         const TreeStep &st = sm[(step - p.first) & 1];
         if (works) {
             const bool edge = step * 64 + 64 > p.len;
-            f32x4 x[R][4];
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-#pragma unroll
-                for (int r = 0; r < R; r++) x[r][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    Frag<CT, 1> kf;
-                    kf.v[0] = *(const u32x4 *)(st.k + (16 * t + n) * TreeStep::KP + 64 * s + 16 * j);
-#pragma unroll
-                    for (int r = 0; r < R; r++) x[r][t] = product(kf, qf[r][s], x[r][t]);
-                }
-            }
             float oe = 1.0f;
             if constexpr (SCALED) {
                 const uint32_t e1 = __builtin_amdgcn_readfirstlane(st.e);
                 if (ve != e1) oe = power_from(ve) * power_to(e1);
                 ve = e1;
+            }
+#pragma unroll 1
+            for (int u = 0; u < 2; u++) { // 32 positions
+                const int n = again(threadIdx.x & 15), j = again(threadIdx.x & 63) >> 4;
+                f32x4 x[R][2];
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const f32x4 sk = *(const f32x4 *)&st.s[0][16 * t + 4 * j];
+                for (int r = 0; r < R; r++)
 #pragma unroll
-                    for (int r = 0; r < R; r++)
+                    for (int t = 0; t < 2; t++) x[r][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int i = 0; i < 4; i++) x[r][t][i] *= sk[i];
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        Frag<CT, 1> kf;
+                        kf.v[0] = *(const u32x4 *)&st.k[st.k_at(32 * u + 16 * t + n, 4 * s + j)];
+#pragma unroll
+                        for (int r = 0; r < R; r++) x[r][t] = product(kf, qf[r][s], x[r][t]);
+                    }
+                if constexpr (SCALED)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const f32x4 sk = *(const f32x4 *)&st.s[0][32 * u + 16 * t + 4 * j];
+#pragma unroll
+                        for (int r = 0; r < R; r++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) x[r][t][i] *= sk[i];
+                    }
+                Frag<CT, Pc::P> pf[R][1];
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    uint32_t vis = 0;
+                    if (edge) vis = seen_bits<8>(p, step * 64 + 32 * u, sees[r]);
+                    weights(x[r], cq[r], &st.s[1][32 * u + 4 * j], edge, vis, u ? 1.0f : oe, m[r], l[r], o[r], pf[r]);
                 }
-            }
-            Frag<CT, Pc::P> pf[R][2];
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                uint32_t vis = 0;
-                if (edge) vis = seen_bits<16>(p, step * 64, sees[r]);
-                weights(x[r], cq[r], &st.s[1][4 * j], edge, vis, oe, m[r], l[r], o[r], pf[r]);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     Frag<CT, 1> vf;
-                    vf.v[0] = *(const u32x4 *)(st.v + (16 * d + n) * TreeStep::VP + 64 * u + 16 * j);
+                    vf.v[0] = *(const u32x4 *)&st.v[st.v_at(16 * d + n, 4 * u + j)];
 #pragma unroll
-                    for (int r = 0; r < R; r++) o[r][d] = product(vf, pf[r][u], o[r][d]);
+                    for (int r = 0; r < R; r++) o[r][d] = product(vf, pf[r][0], o[r][d]);
                 }
+            }
         }
         store(step + 1, sm[(step + 1 - p.first) & 1]);
-        load(step + 2);
+        load();
         __syncthreads();
     }
     if (!works) return;
-    const uint64_t bad = CT == LLM_BF16 ? (uint64_t)sm_bad[1] << 32 | sm_bad[0] : 0;
 #pragma unroll
     for (int r = 0; r < R; r++) {
+        const int row = row0 + 16 * r + n;
         l[r] = over_groups(l[r], fadd_);
-        if (sees[r] & bad) l[r] = NAN;
-        const int row = my_row0 + 16 * r + n;
+        if (CT == LLM_BF16 && (sees[r] & ((uint64_t)sm_bad[1] << 32 | sm_bad[0]))) l[r] = NAN;
         if (row >= p.rows) continue;
         const float il = to_output(p, l[r]) * (SCALED ? power_from(ve) : 1.0f);
         if (p.slices > 1 && j == 0) put_sums(a, p, row, m[r], l[r]);
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            const f32x4 y = o[r][d];
-            put_values<QT>(a, p, row, 16 * d + 4 * j, make_float4(y[0] * il, y[1] * il, y[2] * il, y[3] * il));
-        }
+        for (int d = 0; d < DT; d++)
+            put_values<QT>(a, p, row, 16 * d + 4 * j,
+                           make_float4(o[r][d][0] * il, o[r][d][1] * il, o[r][d][2] * il, o[r][d][3] * il));
     }
 }
 #endif
@@ -849,14 +905,14 @@ TreeKernel TREE_NAME(TREE_HSP)(int type, int q_type, int tiles, int many, size_t
     TREE_PICK_Q(LLM_F32, 1) TREE_PICK_Q(LLM_BF16, 1) TREE_PICK_Q(LLM_I8, 1) TREE_PICK_Q(LLM_E4M3, 1)
 #if TREE_HSP <= 128
     TREE_PICK_Q(LLM_F32, 2) TREE_PICK_Q(LLM_BF16, 2) TREE_PICK_Q(LLM_I8, 2) TREE_PICK_Q(LLM_E4M3, 2)
-#define TREE_PICK_M(C, Q, T)                             \
-    if (many && type == C && q_type == Q && tiles == T) { \
-        *lds = 0;                                        \
-        return k_tree_rows<C, Q, T>;                     \
+#define TREE_PICK_M(C, Q, W, T)                                          \
+    if (many == W && tiles == T && type == C && q_type == Q) {           \
+        *lds = 0;                                                        \
+        return k_tree_rows<C, Q, W, T>;                                  \
     }
-#define TREE_PICK_MQ(C, T) TREE_PICK_M(C, LLM_F32, T) TREE_PICK_M(C, LLM_BF16, T)
-    TREE_PICK_MQ(LLM_BF16, 1) TREE_PICK_MQ(LLM_I8, 1) TREE_PICK_MQ(LLM_E4M3, 1)
-    TREE_PICK_MQ(LLM_BF16, 2) TREE_PICK_MQ(LLM_I8, 2) TREE_PICK_MQ(LLM_E4M3, 2)
+#define TREE_PICK_MQ(C, W, T) TREE_PICK_M(C, LLM_F32, W, T) TREE_PICK_M(C, LLM_BF16, W, T)
+    TREE_PICK_MQ(LLM_BF16, 4, 1) TREE_PICK_MQ(LLM_I8, 4, 1) TREE_PICK_MQ(LLM_E4M3, 4, 1)
+    TREE_PICK_M(LLM_BF16, LLM_F32, 4, 2) TREE_PICK_M(LLM_BF16, LLM_BF16, 8, 1) TREE_PICK_MQ(LLM_I8, 8, 1) TREE_PICK_MQ(LLM_E4M3, 8, 1)
 #endif
     return nullptr;
 }
