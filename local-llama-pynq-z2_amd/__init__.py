@@ -229,7 +229,7 @@ def _stream(t):
     dev = t.get_device()
     if dev < 0:
         raise ValueError("device tensors are needed")
-    return _torch[0].cuda.current_stream(dev).cuda_stream
+    return _torch[0]._C._cuda_getCurrentRawStream(dev)  # (torch.cuda.current_stream(dev).cuda_stream, without its object)
 
 
 def _ints(name, t, count, dtype):

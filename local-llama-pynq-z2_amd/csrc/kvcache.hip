@@ -16,6 +16,7 @@ struct KvArgs {
     int64_t seq, head, pos, s_seq, s_head, s_pos; // cache
     int64_t r_seq[2], r_tok[2], r_head[2];        // rows, of K and V
     const int *at, *n;
+    int at0, by_pos; // at NULL: every sequence's position; the rows lie at their positions, not from 0
     int n_kv, hs, ctx, max_n, zero_rest;
     uint32_t rows; // n_seq * max_n * n_kv
 };
@@ -71,9 +72,9 @@ __global__ void __launch_bounds__(256) k_kv_write(KvArgs a) {
     const int side = blockIdx.y, l = threadIdx.x & 15;
     if (item >= a.rows) return; // (whole DPP rows leave)
     const uint32_t h = item % a.n_kv, bt = item / a.n_kv, t = bt % a.max_n, b = bt / a.max_n;
-    const int64_t p = (int64_t)a.at[b] + t;
+    const int64_t p = (int64_t)(a.at ? a.at[b] : a.at0) + t;
     if ((a.n && (int)t >= a.n[b]) || p < 0 || p >= a.ctx) return;
-    const uint8_t *src = a.side[side].r + b * a.r_seq[side] + t * a.r_tok[side] + h * a.r_head[side];
+    const uint8_t *src = a.side[side].r + b * a.r_seq[side] + (a.by_pos ? p : t) * a.r_tok[side] + h * a.r_head[side];
     uint8_t *dst = a.side[side].c + b * a.seq + h * a.head + p * a.pos;
     float4 x[4];
     uint32_t m = 0;
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(256) k_kv_read(KvArgs a) {
     const int side = blockIdx.y, l = threadIdx.x & 15;
     if (item >= a.rows) return;
     const uint32_t h = item % a.n_kv, bt = item / a.n_kv, t = bt % a.max_n, b = bt / a.max_n;
-    const int64_t p = (int64_t)a.at[b] + t;
+    const int64_t p = (int64_t)(a.at ? a.at[b] : a.at0) + t;
     uint8_t *dst = a.side[side].r + b * a.r_seq[side] + t * a.r_tok[side] + h * a.r_head[side];
     if ((a.n && (int)t >= a.n[b]) || p < 0 || p >= a.ctx) {
         if (a.zero_rest)
@@ -166,6 +167,28 @@ __global__ void __launch_bounds__(256) k_kv_read(KvArgs a) {
     }
 }
 
+struct KeepArgs {
+    uint8_t *side[2];
+    float *scale[2];
+    int64_t layer, head, pos, s_layer, s_head, s_pos; // strides: bytes, of the scales floats
+    int words, pos0, n;                               // 4-byte words of a row
+    uint8_t path[64];
+};
+// Rows pos0 + path[j] to pos0 + j, in the order of j (path rising: a row is read before it is written over): a thread has
+// the same word of every row.
+__global__ void __launch_bounds__(64) k_kv_keep(KeepArgs a) {
+    const int head = blockIdx.x, layer = blockIdx.y, side = blockIdx.z;
+    uint8_t *rows = a.side[side] + layer * a.layer + head * a.head + (int64_t)a.pos0 * a.pos;
+    float *s = a.scale[side] ? a.scale[side] + layer * a.s_layer + head * a.s_head + (int64_t)a.pos0 * a.s_pos : nullptr;
+    for (int j = 0; j < a.n; j++) {
+        const int from = a.path[j];
+        if (from == j) continue;
+        for (int w = threadIdx.x; w < a.words; w += 64)
+            ((uint32_t *)(rows + j * a.pos))[w] = ((const uint32_t *)(rows + from * a.pos))[w];
+        if (s && threadIdx.x == 0) s[j * a.s_pos] = s[from * a.s_pos];
+    }
+}
+
 int kv_rows(const char *who, bool write, const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos,
             const int *n, int max_n, int zero_rest, void *stream) {
     if (!c || !k || !v || max_n < 0) {
@@ -182,35 +205,18 @@ int kv_rows(const char *who, bool write, const llm_kv *c, const llm_rows *k, con
         fprintf(stderr, "%s: k and v rows of different types\n", who);
         return -1;
     }
-    const int64_t rows = (int64_t)c->n_seq * max_n * c->n_kv;
-    if (rows > 0x7fffffff) {
-        fprintf(stderr, "%s: %lld rows\n", who, (long long)rows);
+    if ((int64_t)c->n_seq * max_n * c->n_kv > 0x7fffffff) {
+        fprintf(stderr, "%s: %d sequences of %d rows\n", who, c->n_seq, max_n);
         return -1;
     }
     if (!dev.select()) return -1;
-    const int cs = op_type_bytes(c->type), rs = op_type_bytes(k->type);
-    KvArgs a;
-    memset(&a, 0, sizeof a);
-    a.side[0] = {(uint8_t *)c->k, (uint8_t *)k->p, c->k_scale};
-    a.side[1] = {(uint8_t *)c->v, (uint8_t *)v->p, c->v_scale};
-    a.seq = c->seq * cs, a.head = c->head * cs, a.pos = c->pos * cs;
-    a.s_seq = c->s_seq, a.s_head = c->s_head, a.s_pos = c->s_pos;
-    for (int i = 0; i < 2; i++) {
-        const llm_rows *r = i ? v : k;
-        a.r_seq[i] = r->seq * rs, a.r_tok[i] = r->tok * rs, a.r_head[i] = r->head * rs;
-    }
-    a.at = pos;
-    a.n = n;
-    a.n_kv = c->n_kv, a.hs = c->hs, a.ctx = c->ctx, a.max_n = max_n, a.zero_rest = zero_rest;
-    a.rows = (uint32_t)rows;
-    void (*kern)(KvArgs) = nullptr;
-#define KV_PICK(C, R)                                                                 \
-    if (c->type == C && k->type == R) kern = write ? k_kv_write<C, R> : k_kv_read<C, R>;
-    KV_PICK(LLM_F32, LLM_F32) KV_PICK(LLM_F32, LLM_BF16) KV_PICK(LLM_BF16, LLM_F32) KV_PICK(LLM_BF16, LLM_BF16)
-    KV_PICK(LLM_I8, LLM_F32) KV_PICK(LLM_I8, LLM_BF16) KV_PICK(LLM_E4M3, LLM_F32) KV_PICK(LLM_E4M3, LLM_BF16)
-#undef KV_PICK
-    hipLaunchKernelGGL(kern, dim3((a.rows + 15) / 16, 2), dim3(256), 0, (hipStream_t)stream, a);
-    HIP_OR_FAIL(who, hipGetLastError());
+    KvCall q;
+    memset(&q, 0, sizeof q);
+    q.pos = pos;
+    q.n = n;
+    q.max_n = max_n;
+    q.zero_rest = zero_rest;
+    HIP_OR_FAIL(who, launch_kv(write, *c, *k, *v, q, (hipStream_t)stream));
     return 0;
 }
 
@@ -259,6 +265,48 @@ bool op_check_rows(const llm_rows *r, const char *what, OpDevice *dev, const cha
         return false;
     }
     return dev->holds(r->p, what);
+}
+
+hipError_t launch_kv(bool write, const llm_kv &c, const llm_rows &k, const llm_rows &v, const KvCall &q, hipStream_t st) {
+    const int cs = op_type_bytes(c.type), rs = op_type_bytes(k.type);
+    KvArgs a;
+    memset(&a, 0, sizeof a);
+    a.side[0] = {(uint8_t *)c.k, (uint8_t *)k.p, c.k_scale};
+    a.side[1] = {(uint8_t *)c.v, (uint8_t *)v.p, c.v_scale};
+    a.seq = c.seq * cs, a.head = c.head * cs, a.pos = c.pos * cs;
+    a.s_seq = c.s_seq, a.s_head = c.s_head, a.s_pos = c.s_pos;
+    for (int i = 0; i < 2; i++) {
+        const llm_rows &r = i ? v : k;
+        a.r_seq[i] = r.seq * rs, a.r_tok[i] = r.tok * rs, a.r_head[i] = r.head * rs;
+    }
+    a.at = q.pos, a.at0 = q.pos0, a.by_pos = q.by_pos;
+    a.n = q.n;
+    a.n_kv = c.n_kv, a.hs = c.hs, a.ctx = c.ctx, a.max_n = q.max_n, a.zero_rest = q.zero_rest;
+    a.rows = (uint32_t)c.n_seq * q.max_n * c.n_kv;
+    void (*kern)(KvArgs) = nullptr;
+#define KV_PICK(C, R)                                                                 \
+    if (c.type == C && k.type == R) kern = write ? k_kv_write<C, R> : k_kv_read<C, R>;
+    KV_PICK(LLM_F32, LLM_F32) KV_PICK(LLM_F32, LLM_BF16) KV_PICK(LLM_BF16, LLM_F32) KV_PICK(LLM_BF16, LLM_BF16)
+    KV_PICK(LLM_I8, LLM_F32) KV_PICK(LLM_I8, LLM_BF16) KV_PICK(LLM_E4M3, LLM_F32) KV_PICK(LLM_E4M3, LLM_BF16)
+#undef KV_PICK
+    hipLaunchKernelGGL(kern, dim3((a.rows + 15) / 16, 2), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_keep(const llm_kv &c, int pos0, const uint8_t *path, int n, hipStream_t st) {
+    const int cs = op_type_bytes(c.type);
+    KeepArgs a;
+    memset(&a, 0, sizeof a);
+    a.side[0] = (uint8_t *)c.k, a.side[1] = (uint8_t *)c.v;
+    a.scale[0] = c.k_scale, a.scale[1] = c.v_scale;
+    a.layer = c.seq * cs, a.head = c.head * cs, a.pos = c.pos * cs;
+    a.s_layer = c.s_seq, a.s_head = c.s_head, a.s_pos = c.s_pos;
+    a.words = c.hs * cs / 4;
+    a.pos0 = pos0;
+    a.n = n;
+    memcpy(a.path, path, n);
+    hipLaunchKernelGGL(k_kv_keep, dim3(c.n_kv, c.n_seq, 2), dim3(64), 0, st, a);
+    return hipGetLastError();
 }
 
 extern "C" int llm_kv_write(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos, const int *n, int max_n,

@@ -18,7 +18,7 @@ namespace {
 constexpr int LP_T = 256, LP_E = 16, LP_STEP = LP_T * LP_E; // values a block takes at once
 constexpr int LP_TOP = 32;                                  // most alternatives
 constexpr int LP_KEEP = 256;                                // the list is cut when it holds more
-constexpr int LP_CAP = LP_KEEP + LP_STEP;
+constexpr int LP_CAP = LP_KEEP + LP_STEP;          // (a step adds no more than it has)
 constexpr int LP_MAX_SEG = 64;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -67,14 +67,13 @@ __device__ __forceinline__ Stat join(Stat a, Stat b, float c) {
     return r;
 }
 __device__ __forceinline__ Stat wave_join(Stat v, float c) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        Stat o;
-        o.m = __shfl_xor(v.m, off), o.s = __shfl_xor(v.s, off), o.t = __shfl_xor(v.t, off);
-        // the same order in both lanes: one result
-        v = (threadIdx.x & off) ? join(o, v, c) : join(v, o, c);
-    }
-    return v;
+    Stat r;
+    r.m = wave_max(v.m);
+    const float mu = r.m == -INFINITY ? 0.0f : r.m;
+    const float d = fmaxf((v.m - mu) * c, -300.0f), f = __builtin_amdgcn_exp2f(d);
+    r.s = wave_sum(v.s * f);
+    r.t = wave_sum((v.t + d * v.s) * f);
+    return r;
 }
 
 // The k-th largest (k >= 1) of the 64 lanes' keys: the largest key that at least k lanes reach, bit by bit.
@@ -95,8 +94,11 @@ __device__ void list_cut(uint64_t *list, int n, int top, uint64_t *scratch) {
     if (n <= 2 * LP_KEEP) { // an entry's place is the number of larger ones
         for (int i = threadIdx.x; i < n; i += LP_T) {
             const uint64_t e = list[i];
-            int r = 0;
-            for (int k = 0; k < n; k++) r += list[k] > e;
+            int r = 0, k = 0;
+            for (; k + 8 <= n; k += 8) // (eight reads under way at once)
+#pragma unroll
+                for (int u = 0; u < 8; u++) r += list[k + u] > e;
+            for (; k < n; k++) r += list[k] > e;
             if (r < keep) scratch[r] = e;
         }
         __syncthreads();
@@ -146,14 +148,20 @@ __device__ __forceinline__ float value_at(const uint8_t *row, int i) {
     return __uint_as_float((uint32_t)((const uint16_t *)row)[i] << 16);
 }
 
+// the logit of a row's i-th given token
 template <int TY>
-__device__ __forceinline__ void given(const LpArgs &a, int row, Stat st) {
+__device__ __forceinline__ float given_logit(const LpArgs &a, int row, int i) {
+    const int tok = a.tokens[(int64_t)row * a.n_tokens + i];
+    return tok >= 0 && tok < a.vocab ? value_at<TY>(a.x + row * a.stride, tok) : -INFINITY;
+}
+// their log probabilities; x the thread's first logit (an id out of range: -infinity whatever the row holds)
+template <int TY>
+__device__ __forceinline__ void given(const LpArgs &a, int row, Stat st, float x) {
     const float ls = logf(st.s);
     for (int i = threadIdx.x; i < a.n_tokens; i += LP_T) {
         const int tok = a.tokens[(int64_t)row * a.n_tokens + i];
-        float v = -INFINITY;
-        if (tok >= 0 && tok < a.vocab) v = (value_at<TY>(a.x + row * a.stride, tok) - st.m) * a.inv_t - ls;
-        a.logp[(int64_t)row * a.n_tokens + i] = v;
+        if (i >= LP_T) x = given_logit<TY>(a, row, i);
+        a.logp[(int64_t)row * a.n_tokens + i] = tok >= 0 && tok < a.vocab ? (x - st.m) * a.inv_t - ls : -INFINITY;
     }
 }
 
@@ -229,16 +237,29 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(LpArgs a) {
             }
             uint32_t lim = bound; // values below lim, or equal to it behind a full list, are not among the top
             if (__popcll(__ballot(km > lim)) >= a.top) lim = max(lim, kth_of_wave(km, a.top) - 1);
-            if (km > lim) {
+            if (__any(km > lim)) { // places by one addition a wave
+                uint64_t in[LP_E];
+                int total = 0;
 #pragma unroll
                 for (int e = 0; e < LP_E; e++) {
-                    const bool in = !edge || (uint32_t)idx(e) < (uint32_t)a.vocab;
-                    if (in && key_of(x[e]) > lim) list[atomicAdd(&count, 1)] = entry_of(x[e], idx(e));
+                    in[e] = __ballot((!edge || (uint32_t)idx(e) < (uint32_t)a.vocab) && key_of(x[e]) > lim);
+                    total += __popcll(in[e]);
+                }
+                int at = 0;
+                if (lane == 0 && total) at = atomicAdd(&count, total);
+                at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+                for (int e = 0; e < LP_E; e++) {
+                    if (in[e] == 0) continue;
+                    if ((in[e] >> lane) & 1)
+                        list[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], 0))] =
+                            entry_of(x[e], idx(e));
+                    at += __popcll(in[e]);
                 }
             }
             __syncthreads();
             const int have = count;
-            if (have > LP_KEEP || (!bound && have >= a.top)) {
+            if (step + 1 < last && (have > LP_KEEP || (!bound && have >= a.top))) {
                 list_cut(list, have, a.top, scratch);
                 if (threadIdx.x == 0) {
                     count = a.top;
@@ -261,7 +282,7 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(LpArgs a) {
     }
     if (a.seg == 1) {
         finish(a, row, st, list);
-        given<TY>(a, row, st);
+        given<TY>(a, row, st, (int)threadIdx.x < a.n_tokens ? given_logit<TY>(a, row, threadIdx.x) : 0.0f);
     } else {
         const int64_t part = (int64_t)row * a.seg + seg;
         if (threadIdx.x == 0) {
@@ -282,28 +303,32 @@ __global__ void __launch_bounds__(LP_T) k_logprobs_join(LpArgs a) {
     const int row = blockIdx.x, lane = threadIdx.x & 63;
     const float c = a.inv_t * 1.44269504088896340736f;
     const float *pt = a.part + 4 * (int64_t)row * a.seg;
+    // every load that depends on no other first: the statistics, the lists, the given tokens' logits
+    constexpr int NE = LP_MAX_SEG * LP_TOP / LP_T;
+    const uint64_t *from = a.list + (int64_t)row * a.seg * a.top;
     Stat st = {-INFINITY, 0.0f, 0.0f};
     if (lane < a.seg) st = {pt[4 * lane], pt[4 * lane + 1], pt[4 * lane + 2]};
+    uint64_t ent[NE], end = 0;
+#pragma unroll
+    for (int u = 0; u < NE; u++) ent[u] = (int)threadIdx.x + u * LP_T < a.seg * a.top ? from[threadIdx.x + u * LP_T] : 0;
+    if (a.top && lane < a.seg) end = from[lane * a.top + a.top - 1];
+    float x = 0.0f;
+    if ((int)threadIdx.x < a.n_tokens) x = given_logit<TY>(a, row, threadIdx.x);
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
     st = wave_join(st, c);
     if (a.top) {
         // the segments' last entries: `top` values reach the largest of them
-        const uint64_t *from = a.list + (int64_t)row * a.seg * a.top;
-        uint64_t lim = lane < a.seg ? from[lane * a.top + a.top - 1] : 0;
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint64_t o = __shfl_xor((unsigned long long)lim, off);
-            if (o > lim) lim = o;
-        }
-        if (threadIdx.x == 0) count = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.seg * a.top; i += LP_T) {
-            const uint64_t e = from[i];
-            if (e && e >= lim) list[atomicAdd(&count, 1)] = e;
-        }
+        uint32_t lim = (uint32_t)(end >> 32);
+        for (int off = 1; off < 64; off <<= 1) lim = max(lim, (uint32_t)__shfl_xor((int)lim, off));
+#pragma unroll
+        for (int u = 0; u < NE; u++)
+            if (ent[u] && (uint32_t)(ent[u] >> 32) >= lim) list[atomicAdd(&count, 1)] = ent[u];
         __syncthreads();
         list_cut(list, count, a.top, scratch);
     }
     finish(a, row, st, list);
-    given<TY>(a, row, st);
+    given<TY>(a, row, st, x);
 }
 
 struct LpPlan {
@@ -311,11 +336,11 @@ struct LpPlan {
     size_t bytes;
 };
 
-// Segments of a row: one where the rows alone fill the chip, else until the grid has four blocks a CU, of two steps at least.
+// Segments of a row: one where the rows alone fill the chip, else until the grid has four blocks a CU.
 LpPlan lp_plan(int rows, int vocab, int top) {
     LpPlan p;
     const int steps = (int)(((int64_t)vocab + 7 + LP_STEP - 1) / LP_STEP); // (with the longest lead)
-    int seg = rows >= 512 ? 1 : std::min({(1024 + rows - 1) / std::max(rows, 1), (steps + 1) / 2, LP_MAX_SEG});
+    int seg = rows >= 512 ? 1 : std::min({(1024 + rows - 1) / std::max(rows, 1), steps, LP_MAX_SEG});
     seg = std::max(seg, 1);
     p.per = (steps + seg - 1) / seg;
     p.seg = std::max(1, (steps + p.per - 1) / p.per);
@@ -327,6 +352,27 @@ LpPlan lp_plan(int rows, int vocab, int top) {
 
 extern "C" size_t llm_logprobs_work(int rows, int vocab, int top) {
     return rows > 0 && vocab > 0 && top >= 0 && top <= LP_TOP ? lp_plan(rows, vocab, top).bytes : 0;
+}
+
+hipError_t launch_logprobs(const LogprobsCall &q, hipStream_t st) {
+    const int es = op_type_bytes(q.type);
+    const LpPlan p = lp_plan(q.rows, q.vocab, q.top);
+    LpArgs a;
+    memset(&a, 0, sizeof a);
+    a.x = (const uint8_t *)q.logits;
+    a.stride = q.stride * es;
+    a.rows = q.rows, a.vocab = q.vocab, a.seg = p.seg, a.per = p.per;
+    a.inv_t = 1.0f / q.temperature;
+    a.tokens = q.tokens, a.n_tokens = q.n_tokens, a.top = q.top;
+    a.logp = q.logp, a.entropy = q.entropy, a.lse = q.lse, a.top_ids = q.top_ids, a.top_logp = q.top_logp;
+    a.part = (float *)q.work;
+    a.list = (uint64_t *)((float *)q.work + (size_t)q.rows * p.seg * 4);
+    const bool f32 = q.type == LLM_F32;
+    hipLaunchKernelGGL(f32 ? k_logprobs<LLM_F32> : k_logprobs<LLM_BF16>, dim3(q.rows * p.seg), dim3(LP_T), 0, st, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.seg == 1) return e;
+    hipLaunchKernelGGL(f32 ? k_logprobs_join<LLM_F32> : k_logprobs_join<LLM_BF16>, dim3(q.rows), dim3(LP_T), 0, st, a);
+    return hipGetLastError();
 }
 
 extern "C" int llm_logprobs(const void *logits, int type, int rows, int vocab, int64_t stride, float temperature,
@@ -357,24 +403,8 @@ extern "C" int llm_logprobs(const void *logits, int type, int rows, int vocab, i
         return -1;
     }
     if (!dev.select()) return -1;
-    LpArgs a;
-    memset(&a, 0, sizeof a);
-    a.x = (const uint8_t *)logits;
-    a.stride = stride * es;
-    a.rows = rows, a.vocab = vocab, a.seg = p.seg, a.per = p.per;
-    a.inv_t = 1.0f / temperature;
-    a.tokens = tokens, a.n_tokens = n_tokens, a.top = top;
-    a.logp = logp, a.entropy = entropy, a.lse = lse, a.top_ids = top_ids, a.top_logp = top_logp;
-    a.part = (float *)work;
-    a.list = (uint64_t *)((float *)work + (size_t)rows * p.seg * 4);
-    const hipStream_t st = (hipStream_t)stream;
-    if (type == LLM_F32) hipLaunchKernelGGL(k_logprobs<LLM_F32>, dim3(rows * p.seg), dim3(LP_T), 0, st, a);
-    else hipLaunchKernelGGL(k_logprobs<LLM_BF16>, dim3(rows * p.seg), dim3(LP_T), 0, st, a);
-    HIP_OR_FAIL(who, hipGetLastError());
-    if (p.seg > 1) {
-        if (type == LLM_F32) hipLaunchKernelGGL(k_logprobs_join<LLM_F32>, dim3(rows), dim3(LP_T), 0, st, a);
-        else hipLaunchKernelGGL(k_logprobs_join<LLM_BF16>, dim3(rows), dim3(LP_T), 0, st, a);
-        HIP_OR_FAIL(who, hipGetLastError());
-    }
+    const LogprobsCall q = {logits, type, rows, vocab, stride, temperature, tokens, n_tokens,
+                            logp, entropy, lse, top, top_ids, top_logp, work};
+    HIP_OR_FAIL(who, launch_logprobs(q, (hipStream_t)stream));
     return 0;
 }

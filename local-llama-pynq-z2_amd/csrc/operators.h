@@ -59,3 +59,41 @@ class OpDevice {
 bool op_check_cache(const llm_kv *c, OpDevice *dev, const char *who);
 // Rows of activations beside it: fp32 or bf16, vectors of 4 values aligned.
 bool op_check_rows(const llm_rows *r, const char *what, OpDevice *dev, const char *who);
+
+// The launches behind the entry points, for callers that know their arguments to be right (the model).
+
+struct KvCall {
+    const int *pos; // NULL: pos0 for every sequence
+    int pos0;
+    int by_pos;     // writes: the row of position p is row p of the rows, not the t-th
+    const int *n;
+    int max_n, zero_rest;
+};
+hipError_t launch_kv(bool write, const llm_kv &c, const llm_rows &k, const llm_rows &v, const KvCall &q, hipStream_t st);
+// Of every sequence (the model: layer), rows pos0 + path[j] to pos0 + j; path rises, path[j] < 64.
+hipError_t launch_kv_keep(const llm_kv &c, int pos0, const uint8_t *path, int n, hipStream_t st);
+
+struct TreeCall {
+    int n_heads;
+    const int *lens, *n;
+    const uint64_t *mask;
+    int max_n, max_len;
+    float scale;
+    int zero_rest;
+    void *work; // llm_tree_attention_work()
+};
+hipError_t launch_tree_attention(const llm_kv &c, const llm_rows &q, const llm_rows &out, const TreeCall &t, hipStream_t st);
+
+struct LogprobsCall {
+    const void *logits;
+    int type, rows, vocab;
+    int64_t stride;
+    float temperature;
+    const int *tokens;
+    int n_tokens;
+    float *logp, *entropy, *lse;
+    int top, *top_ids;
+    float *top_logp;
+    void *work; // llm_logprobs_work()
+};
+hipError_t launch_logprobs(const LogprobsCall &q, hipStream_t st);

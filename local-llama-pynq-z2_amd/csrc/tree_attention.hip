@@ -117,10 +117,15 @@ TreePlan tree_plan(const llm_kv *c, int q_type, int n_heads, int max_n, int max_
     const int64_t grid = c->n_seq > 1 ? 1024 : many ? 512 : 256;
     const int64_t cap = std::min({std::max<int64_t>(1, grid / std::max<int64_t>(blocks, 1)), (steps + least - 1) / least,
                                   (int64_t)TREE_MAX_SPLITS});
-    p.quantum = (int)((steps + cap - 1) / cap);
-    p.splits = (int)((steps + p.quantum - 1) / p.quantum);
+    // one sequence: as many slices as its length, known to the kernel, gives of the least size, up to that number
+    p.quantum = (int)(c->n_seq > 1 ? (steps + cap - 1) / cap : least);
+    p.splits = (int)(c->n_seq > 1 ? (steps + p.quantum - 1) / p.quantum : cap);
     p.bytes = p.splits > 1 ? (size_t)c->n_seq * c->n_kv * p.splits * rows * (c->hs + 2) * 4 : 0;
     return p;
+}
+
+int64_t tree_blocks(const llm_kv &c, const TreePlan &p) { // (rounded up to a slice for each XCD)
+    return ((int64_t)c.n_seq * c.n_kv * p.splits + 7) / 8 * 8 * p.row_blocks;
 }
 
 bool tree_shape_ok(const llm_kv *c, int n_heads, int max_n) {
@@ -133,6 +138,44 @@ bool tree_shape_ok(const llm_kv *c, int n_heads, int max_n) {
 extern "C" size_t llm_tree_attention_work(const llm_kv *c, int n_heads, int max_n, int max_len) {
     return tree_shape_ok(c, n_heads, max_n) ? std::max(tree_plan(c, LLM_F32, n_heads, max_n, max_len).bytes,
                                                        tree_plan(c, LLM_BF16, n_heads, max_n, max_len).bytes) : 0;
+}
+
+hipError_t launch_tree_attention(const llm_kv &c, const llm_rows &q, const llm_rows &out, const TreeCall &t, hipStream_t st) {
+    const TreePlan p = tree_plan(&c, q.type, t.n_heads, t.max_n, t.max_len);
+    const int64_t blocks = tree_blocks(c, p);
+    const int cs = op_type_bytes(c.type), qs = op_type_bytes(q.type);
+    TreeArgs a;
+    memset(&a, 0, sizeof a);
+    a.k = (const uint8_t *)c.k, a.v = (const uint8_t *)c.v;
+    a.ks = c.k_scale, a.vs = c.v_scale;
+    a.seq = c.seq * cs, a.head = c.head * cs, a.pos = c.pos * cs;
+    a.s_seq = c.s_seq, a.s_head = c.s_head, a.s_pos = c.s_pos;
+    a.q = (const uint8_t *)q.p, a.o = (uint8_t *)out.p;
+    a.q_seq = q.seq * qs, a.q_tok = q.tok * qs, a.q_head = q.head * qs;
+    a.o_seq = out.seq * qs, a.o_tok = out.tok * qs, a.o_head = out.head * qs;
+    a.lens = t.lens, a.n = t.n, a.mask = t.mask;
+    a.n_seq = c.n_seq, a.n_kv = c.n_kv, a.hs = c.hs, a.ctx = c.ctx;
+    a.group = t.n_heads / c.n_kv, a.max_n = t.max_n, a.row_blocks = p.row_blocks, a.block_rows = p.block_rows;
+    a.splits = p.splits, a.quantum = p.quantum, a.zero_rest = t.zero_rest;
+    // (a scale of 0 as one so small that every weight is 1)
+    a.c = std::max(std::fabs(t.scale) * 1.44269504088896340736f, 1e-30f);
+    a.negate = t.scale < 0.0f;
+    a.acc = (float *)t.work; // (rows of hs values, hs a multiple of 16: 16-byte aligned)
+    a.ml = (float *)t.work + (p.bytes / 4 / (c.hs + 2)) * c.hs;
+    size_t lds = 0;
+    auto *pick = p.hsp == 64 ? tree_kernel_64 : p.hsp == 128 ? tree_kernel_128 : p.hsp == 192 ? tree_kernel_192 : tree_kernel_256;
+    TreeKernel kern = pick(c.type, q.type, p.tiles, p.many, &lds);
+    if (!kern) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(p.many ? 64 * p.many : 256), lds, st, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits == 1) return e;
+    // a wave a row up to 8 slices, the block's four above
+    const bool wide = p.splits > 8;
+    const dim3 grid(wide ? t.max_n * a.group : (t.max_n * a.group + 3) / 4, c.n_kv, c.n_seq);
+    auto *join = q.type == LLM_F32 ? wide ? k_tree_join<LLM_F32, 4> : k_tree_join<LLM_F32, 1>
+                                   : wide ? k_tree_join<LLM_BF16, 4> : k_tree_join<LLM_BF16, 1>;
+    hipLaunchKernelGGL(join, grid, dim3(256), 0, st, a, p.tp);
+    return hipGetLastError();
 }
 
 extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_rows *out, int n_heads, const int *lens,
@@ -164,48 +207,12 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
         fprintf(stderr, "%s: %zu bytes of work memory are needed, 16-byte aligned\n", who, p.bytes);
         return -1;
     }
-    const int64_t blocks = ((int64_t)c->n_seq * c->n_kv * p.splits + 7) / 8 * 8 * p.row_blocks;
-    if (blocks > 0x7fffffff || c->n_seq > 65535 || c->n_kv > 65535) {
+    if (tree_blocks(*c, p) > 0x7fffffff || c->n_seq > 65535 || c->n_kv > 65535) {
         fprintf(stderr, "%s: %d sequences of %d kv heads\n", who, c->n_seq, c->n_kv);
         return -1;
     }
     if (!dev.select()) return -1;
-    const int cs = op_type_bytes(c->type), qs = op_type_bytes(q->type);
-    TreeArgs a;
-    memset(&a, 0, sizeof a);
-    a.k = (const uint8_t *)c->k, a.v = (const uint8_t *)c->v;
-    a.ks = c->k_scale, a.vs = c->v_scale;
-    a.seq = c->seq * cs, a.head = c->head * cs, a.pos = c->pos * cs;
-    a.s_seq = c->s_seq, a.s_head = c->s_head, a.s_pos = c->s_pos;
-    a.q = (const uint8_t *)q->p, a.o = (uint8_t *)out->p;
-    a.q_seq = q->seq * qs, a.q_tok = q->tok * qs, a.q_head = q->head * qs;
-    a.o_seq = out->seq * qs, a.o_tok = out->tok * qs, a.o_head = out->head * qs;
-    a.lens = lens, a.n = n, a.mask = mask;
-    a.n_seq = c->n_seq, a.n_kv = c->n_kv, a.hs = c->hs, a.ctx = c->ctx;
-    a.group = n_heads / c->n_kv, a.max_n = max_n, a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.splits = p.splits, a.quantum = p.quantum;
-    a.zero_rest = zero_rest;
-    // (a scale of 0 as one so small that every weight is 1)
-    a.c = std::max(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);
-    a.negate = scale < 0.0f;
-    a.acc = (float *)work; // (rows of hs values, hs a multiple of 16: 16-byte aligned)
-    a.ml = (float *)work + (p.bytes / 4 / (c->hs + 2)) * c->hs;
-    size_t lds = 0;
-    auto *pick = p.hsp == 64 ? tree_kernel_64 : p.hsp == 128 ? tree_kernel_128 : p.hsp == 192 ? tree_kernel_192 : tree_kernel_256;
-    TreeKernel kern = pick(c->type, q->type, p.tiles, p.many, &lds);
-    if (!kern) {
-        fprintf(stderr, "%s: internal error: no kernel\n", who);
-        return -1;
-    }
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(p.many ? 64 * p.many : 256), lds, (hipStream_t)stream, a);
-    HIP_OR_FAIL(who, hipGetLastError());
-    if (p.splits > 1) {
-        // a wave a row up to 8 slices, the block's four above
-        const bool wide = p.splits > 8;
-        const dim3 grid(wide ? max_n * a.group : (max_n * a.group + 3) / 4, c->n_kv, c->n_seq);
-        auto *join = q->type == LLM_F32 ? wide ? k_tree_join<LLM_F32, 4> : k_tree_join<LLM_F32, 1>
-                                        : wide ? k_tree_join<LLM_BF16, 4> : k_tree_join<LLM_BF16, 1>;
-        hipLaunchKernelGGL(join, grid, dim3(256), 0, (hipStream_t)stream, a, p.tp);
-        HIP_OR_FAIL(who, hipGetLastError());
-    }
+    const TreeCall t = {n_heads, lens, n, mask, max_n, max_len, scale, zero_rest, work};
+    HIP_OR_FAIL(who, launch_tree_attention(*c, *q, *out, t, (hipStream_t)stream));
     return 0;
 }
