@@ -28,6 +28,9 @@ extern "C" {
 
 typedef struct llm_model llm_model;
 
+/* types of cache rows, activations and logits */
+enum { LLM_F32 = 0, LLM_BF16 = 1, LLM_I8 = 2, LLM_E4M3 = 3 };
+
 typedef struct {
     int kind;                  /* 0: .qwb Qwen2 (qwen.c), 1: llama2.c v2 .bin (runq.c) */
     int dim, hidden_dim, n_layers, n_heads, n_kv_heads, vocab_size;
@@ -134,6 +137,33 @@ int llm_set_sampler(llm_model *m, float temperature, float topp, unsigned long l
 /* the sampler's current RNG state (0 before llm_set_sampler) */
 int llm_sampler_state(llm_model *m, unsigned long long *rng);
 
+/* The type of the K/V cache: LLM_F32 (the reference's, as llm_open leaves it), LLM_BF16, LLM_I8 or LLM_E4M3.  The 8-bit types
+ * hold a row of each position and kv head as codes with one fp32 scale (a quarter of the memory and of a step's cache reads,
+ * plus 4 bytes a row): decode steps quantize the new row and attend over the codes, prompts attend over the values that the
+ * codes stand for.  The cache is empty afterwards: prompts start at position 0 again.  Not in the strict mode; head sizes
+ * that are multiples of 16.  Returns 0, or -1 with the old cache kept.  llm_get_kv: the type, -1 for a NULL model. */
+int llm_set_kv(llm_model *m, int type);
+int llm_get_kv(const llm_model *m);
+
+/* One pass over a tree of n <= 64 drafted tokens (speculative decoding; no counterpart in the reference): token i hangs on
+ * token parents[i] < i, or on the cache (-1: position pos0 - 1 is its predecessor); parents NULL: a chain.  Its K and V rows
+ * go to slot pos0 + i of the cache, its position is pos0 plus its depth, and it sees the cache below pos0, its ancestors and
+ * itself.  next[i]: the token that is most likely after token i (through head_ids); logp[i]: the log probability of token i
+ * after its parent (0 without one, -infinity outside the trimmed head); logits: n rows of n_logits floats.  Any of the three
+ * may be NULL.  Then llm_keep moves the rows of the accepted path together: path[j] rises, and the row of token path[j] goes
+ * to position pos0 + j, from where llm_verify, llm_continue or llm_forward go on.  Not in the strict mode; head sizes that
+ * are multiples of 16.  Return 0 or -1. */
+int llm_verify(llm_model *m, int pos0, const int *tokens, const int *parents, int n, int *next, float *logp, float *logits);
+int llm_keep(llm_model *m, int pos0, const int *path, int n);
+
+/* The log probabilities of a text of n tokens from position 0, in one batched pass where the prompt of a generation that
+ * keeps its logits takes one (llm_set_prefill): logp[i], i < n - 1, of token i + 1 after tokens 0 .. i (-infinity outside
+ * the trimmed head); entropy[i], i < n, of the distribution after token i; top_ids and top_logp, n x top, its `top` <= 32
+ * most likely tokens and their log probabilities, descending.  Logits are divided by temperature.  The arrays may be NULL.
+ * Returns 0 or -1. */
+int llm_score(llm_model *m, const int *ids, int n, float temperature, float *logp, float *entropy, int top, int *top_ids,
+              float *top_logp);
+
 void llm_close(llm_model *m);
 
 /* ---- operators on device memory -----------------------------------------------------------------------------
@@ -146,7 +176,6 @@ void llm_close(llm_model *m);
  * `stream` (a hipStream_t of that device; NULL: its default stream) and nothing is synchronized, allocated or kept, so a
  * call can be captured into a graph.  Scratch memory is the caller's: calls that may overlap need one each.
  * Returns 0, or -1 with a message on stderr; nothing is launched then. */
-enum { LLM_F32 = 0, LLM_BF16 = 1, LLM_I8 = 2, LLM_E4M3 = 3 };
 
 /* The K and V rows of n_seq sequences, ctx positions and n_kv heads of hs values (a multiple of 16, at most 256).  fp32
  * and bf16 rows hold the values.  int8 and e4m3 rows hold codes, and k_scale / v_scale a float per row: value = code *

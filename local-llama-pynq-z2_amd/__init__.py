@@ -103,6 +103,11 @@ def lib():
     L.mvh_read_floor.argtypes = [C.c_size_t, i32, i32, i32, i32, C.POINTER(C.c_float)]
     L.mvh_ref_expf_host.argtypes = [vp, i32, vp]
     L.mvh_seq_sum.argtypes = [vp, i32, i32, i32, vp]
+    L.llm_set_kv.argtypes = [vp, i32]
+    L.llm_get_kv.argtypes = [vp]
+    L.llm_verify.argtypes = [vp, i32, vp, vp, i32, vp, vp, vp]
+    L.llm_keep.argtypes = [vp, i32, vp, i32]
+    L.llm_score.argtypes = [vp, vp, i32, C.c_float, vp, vp, i32, vp, vp]
     L.llm_set_strict.argtypes = [vp, i32]
     L.llm_get_strict.argtypes = [vp]
     L.llm_kv_write.argtypes = [vp, vp, vp, vp, vp, i32, vp]
@@ -506,6 +511,47 @@ class Model:
         if self.L.llm_prefill(self.h, _ptr(p), len(p), _ptr(lg)) != 0:
             raise RuntimeError("llm_prefill failed")
         return lg
+
+    KV_TYPES = ["fp32", "bf16", "int8", "e4m3"]
+
+    def set_kv(self, kind):
+        """the cache's type ("fp32", "bf16", "int8", "e4m3"); the cache is empty afterwards (llm_set_kv)"""
+        if self.L.llm_set_kv(self.h, self.KV_TYPES.index(kind)) != 0:
+            raise RuntimeError("llm_set_kv failed")
+
+    @property
+    def kv(self):
+        return self.KV_TYPES[self.L.llm_get_kv(self.h)]
+
+    def verify(self, pos0, tokens, parents=None, logits=False):
+        """one pass over a drafted tree from position pos0 (llm_verify): (the most likely next token after each, the log
+        probability of each after its parent), and the logits of each where asked"""
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        p = None if parents is None else np.ascontiguousarray(parents, dtype=np.int32)
+        if p is not None and p.size != t.size:
+            raise ValueError("a parent for every token is needed")
+        nxt, lp = np.empty(t.size, np.int32), np.empty(t.size, np.float32)
+        lg = np.empty((t.size, self.info.n_logits), np.float32) if logits else None
+        if self.L.llm_verify(self.h, pos0, _ptr(t), None if p is None else _ptr(p), t.size, _ptr(nxt), _ptr(lp),
+                             _ptr(lg) if logits else None) != 0:
+            raise RuntimeError("llm_verify failed")
+        return (nxt, lp, lg) if logits else (nxt, lp)
+
+    def keep(self, pos0, path):
+        """the cache rows of the accepted tokens of a verified tree moved to positions pos0, pos0 + 1, ... (llm_keep)"""
+        p = np.ascontiguousarray(path, dtype=np.int32)
+        if self.L.llm_keep(self.h, pos0, _ptr(p), p.size) != 0:
+            raise RuntimeError("llm_keep failed")
+
+    def score(self, ids, top=0, temperature=1.0):
+        """log probabilities of a text (llm_score): (of every token after the first, the entropy after every token, the top
+        alternatives' ids and their log probabilities)"""
+        p = np.ascontiguousarray(ids, dtype=np.int32)
+        lp, ent = np.empty(max(p.size - 1, 0), np.float32), np.empty(p.size, np.float32)
+        ti, tl = np.empty((p.size, top), np.int32), np.empty((p.size, top), np.float32)
+        if self.L.llm_score(self.h, _ptr(p), p.size, temperature, _ptr(lp), _ptr(ent), top, _ptr(ti), _ptr(tl)) != 0:
+            raise RuntimeError("llm_score failed")
+        return lp, ent, ti, tl
 
     def close(self):
         if self.h:

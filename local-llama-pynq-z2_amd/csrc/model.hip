@@ -27,6 +27,7 @@
 
 #include "../../include/llm_hip.h"
 #include "host_common.h"
+#include "operators.h"
 #include "prefill.h"
 
 namespace {
@@ -78,6 +79,20 @@ struct llm_model {
     int32_t *head_ids_d = nullptr;
     std::vector<int32_t> head_ids_h;
     float *kc = nullptr, *vc = nullptr, *x = nullptr, *q = nullptr, *att_ml = nullptr, *att_acc = nullptr;
+    // The type of the K/V cache (llm_set_kv).  fp32: kc and vc hold [layer][ctx][kv_dim].  Others: kq and vq hold
+    // [layer][kv head][ctx][hs] values or codes, ks and vs (8-bit types) the scales [layer][kv head][ctx], and kc and vc one
+    // layer's rows, where the QKV kernels leave the new ones and the prefill reads back the old ones.
+    int kv_type = LLM_F32;
+    uint8_t *kq = nullptr, *vq = nullptr;
+    float *ks = nullptr, *vs = nullptr;
+    void *tree_work = nullptr; // the tree attention's partials, for steps and drafted trees alike
+    // llm_verify and llm_score: a tree's masks and depths, logits, and the log probabilities' inputs, results and scratch
+    uint64_t *ver_mask = nullptr;
+    int *ver_len = nullptr, *ver_depth = nullptr;
+    float *ver_logits = nullptr;
+    void *lp_buf = nullptr;
+    size_t lp_bytes = 0;
+    std::vector<int> head_row; // row of the head by token id (-1: none), made when first needed
     float *att_sc = nullptr;  // strict mode: scores [n_heads][ctx]
     float *att_one = nullptr; // fast mode, long contexts: merged attention, then (0, 1) per head
     float *logits = nullptr, *hist = nullptr, *part_v = nullptr, *hsc = nullptr;
@@ -139,6 +154,45 @@ int dalloc(llm_model *m, T **p, size_t bytes) {
     return 0;
 }
 
+template <typename T>
+void dfree(llm_model *m, T *&p) {
+    if (!p) return;
+    m->allocs.erase(std::remove(m->allocs.begin(), m->allocs.end(), (void *)p), m->allocs.end());
+    hipFree(p);
+    p = nullptr;
+}
+
+// ---- the K/V cache
+
+float *layer_k(const llm_model *m, int l) { return m->kc + (m->kv_type == LLM_F32 ? (size_t)l * m->ctx * m->kv_dim : 0); }
+float *layer_v(const llm_model *m, int l) { return m->vc + (m->kv_type == LLM_F32 ? (size_t)l * m->ctx * m->kv_dim : 0); }
+// the cache of layers l .. l + n - 1 as n sequences
+llm_kv layer_cache(const llm_model *m, int l, int n = 1) {
+    llm_kv c;
+    memset(&c, 0, sizeof c);
+    c.type = m->kv_type;
+    c.n_seq = n, c.n_kv = m->info.n_kv_heads, c.hs = m->hs, c.ctx = m->ctx;
+    const int64_t rows = (int64_t)c.n_kv * m->ctx;
+    if (m->kv_type == LLM_F32) {
+        c.k = layer_k(m, l), c.v = layer_v(m, l);
+        c.seq = (int64_t)m->ctx * m->kv_dim, c.head = m->hs, c.pos = m->kv_dim;
+        return c;
+    }
+    const int es = op_type_bytes(m->kv_type);
+    c.k = m->kq + l * rows * m->hs * es, c.v = m->vq + l * rows * m->hs * es;
+    c.seq = rows * m->hs, c.head = (int64_t)m->ctx * m->hs, c.pos = m->hs;
+    if (op_scaled(m->kv_type)) {
+        c.k_scale = m->ks + l * rows, c.v_scale = m->vs + l * rows;
+        c.s_seq = rows, c.s_head = m->ctx, c.s_pos = 1;
+    }
+    return c;
+}
+// one layer's fp32 rows [position][kv head][hs], as the rows of one sequence
+llm_rows cache_rows(const llm_model *m, float *p) {
+    return {p, LLM_F32, 0, m->kv_dim, m->hs};
+}
+llm_rows head_rows(const llm_model *m, float *p) { return {p, LLM_F32, 0, m->info.dim, m->hs}; }
+
 // ---- GEMV argument blocks of one step
 
 GemvArgs base_args(const llm_model *m, const TiledMat &T, const GemvShape &s) {
@@ -161,8 +215,11 @@ const float *attn_norm(const llm_model *m, int l) { return m->norms + (size_t)l 
 const float *ffn_norm(const llm_model *m, int l) { return m->norms + (size_t)(m->info.n_layers + l) * m->info.dim; }
 const float *out_norm(const llm_model *m) { return m->norms + (size_t)2 * m->info.n_layers * m->info.dim; }
 
+float att_scale(const llm_model *m) { return 1.0f / sqrtf((float)m->hs); }
+
 double attn_bytes(const llm_model *m, int pos) { // K and V rows read, q read, partials written
-    return 2.0 * (pos + 1) * m->kv_dim * 4.0 + m->info.dim * 4.0 + m->info.n_heads * 4.0 * (m->hs + 2);
+    const double row = m->kv_dim * op_type_bytes(m->kv_type) + (op_scaled(m->kv_type) ? m->info.n_kv_heads * 4.0 : 0.0);
+    return 2.0 * (pos + 1) * row + m->info.dim * 4.0 + m->info.n_heads * 4.0 * (m->hs + 2);
 }
 
 hipError_t launch_finalize(llm_model *m) {
@@ -282,7 +339,7 @@ int enqueue_step(llm_model *m, bool hist, Prof *prof, int pos_hint, bool finaliz
 
     for (int l = 0; l < I.n_layers; l++) {
         const Layer &Ly = m->L[l];
-        float *kc = m->kc + (size_t)l * m->ctx * kv, *vc = m->vc + (size_t)l * m->ctx * kv;
+        float *kc = layer_k(m, l), *vc = layer_v(m, l);
 
         GemvArgs a = base_args(m, Ly.qkv, Ly.s_qkv);
         a.x = m->x;
@@ -325,7 +382,17 @@ int enqueue_step(llm_model *m, bool hist, Prof *prof, int pos_hint, bool finaliz
         t.one = m->att_one;
         if (on(K_ATTN)) {
             mark(K_ATTN, kind_bytes(m, K_ATTN, pos_hint));
-            if (m->strict) {
+            if (m->kv_type != LLM_F32) { // the new row into the cache, then attention over it
+                const llm_kv c = layer_cache(m, l);
+                KvCall w;
+                memset(&w, 0, sizeof w);
+                w.pos = &m->ctrl->pos;
+                w.by_pos = 1;
+                w.max_n = 1;
+                HIP_OR_FAIL("llm", launch_kv(true, c, cache_rows(m, kc), cache_rows(m, vc), w, m->st));
+                const TreeCall tc = {I.n_heads, &m->ctrl->pos, nullptr, nullptr, 1, m->ctx, att_scale(m), 0, m->tree_work};
+                HIP_OR_FAIL("llm", launch_tree_attention(c, head_rows(m, m->q), head_rows(m, m->att_one), tc, m->st));
+            } else if (m->strict) {
                 t.splits = 1;
                 HIP_OR_FAIL("llm", launch_attention_strict(t, m->st));
             } else {
@@ -340,7 +407,7 @@ int enqueue_step(llm_model *m, bool hist, Prof *prof, int pos_hint, bool finaliz
         a.n_heads = I.n_heads;
         a.head_size = m->hs;
         a.att_splits = m->strict ? 1 : m->att_splits; // strict: one slice, merged as the identity
-        if (!m->strict && lng) { // merged already
+        if (m->kv_type != LLM_F32 || (!m->strict && lng)) { // merged already
             a.att_acc = m->att_one;
             a.att_ml = m->att_one + dim;
             a.att_splits = 1;
@@ -979,7 +1046,8 @@ int prefill_alloc(llm_model *m, int M, size_t score_floats) {
 
 // positions p0 .. p0 + M - 1 (token ids in host memory) through every layer; the residual stream of the chunk
 // is left in pf_x and its K/V rows in the caches
-int prefill_chunk(llm_model *m, const int *ids, int p0, int M) {
+// (tree: the tokens are a drafted tree at slots p0 .. p0 + M - 1, its depths, masks and length on the device)
+int prefill_chunk(llm_model *m, const int *ids, int p0, int M, bool tree = false) {
     const llm_info &I = m->info;
     const int dim = I.dim, kv = m->kv_dim, wb = m->kind == 0 ? 4 : 8, sf = m->kind == 0 ? 0 : 1;
     HIP_OR_FAIL("llm_prefill", hipMemcpyAsync(m->pf_ids, ids, (size_t)M * 4, hipMemcpyHostToDevice, m->st));
@@ -1015,7 +1083,8 @@ int prefill_chunk(llm_model *m, const int *ids, int p0, int M) {
     pa.simds = 4 * hip_cu_count(m->device);
     pa.flash_bf = m->pf_flash_bf;
     if (prefill_strict_scratch_floats(M, I.n_heads, I.n_kv_heads, p0 + M) <= m->pf_sc_n) pa.att_sc = m->pf_sc;
-    pa.xb = m->pf_y; // strict attention rows: the QKV GEMM output is consumed by then
+    pa.xb = m->pf_y; // attention rows (strict, trees): the QKV GEMM output is consumed by then
+    pa.depth = tree ? m->ver_depth : nullptr;
     HIP_OR_FAIL("llm_prefill", launch_p_embed(pa, m->st));
     PgemmArgs g;
     memset(&g, 0, sizeof g);
@@ -1038,7 +1107,7 @@ int prefill_chunk(llm_model *m, const int *ids, int p0, int M) {
     // and k_pgemm32
     const bool fuse_swiglu = sw && (gu_shape == 11 || gu_shape == 22 || gu_shape == PGEMM_SHAPE_32);
     // the QKV epilogue takes the 16 x 16 and 32 x 32 tiles and k_pgemm32
-    const bool fuse_qkv = m->pf_qkv && (qkv_shape == 11 || qkv_shape == 22 || qkv_shape == PGEMM_SHAPE_32);
+    const bool fuse_qkv = m->pf_qkv && !tree && (qkv_shape == 11 || qkv_shape == 22 || qkv_shape == PGEMM_SHAPE_32);
     g.hlay = down_shape == PGEMM_SHAPE_32;
     PgemmArgs gq = g;
     gq.qkv = 1;
@@ -1052,8 +1121,8 @@ int prefill_chunk(llm_model *m, const int *ids, int p0, int M) {
     gq.rope_kind = pa.rope_kind;
     for (int l = 0; l < I.n_layers; l++) {
         const Layer &Ly = m->L[l];
-        pa.kc = m->kc + (size_t)l * m->ctx * kv;
-        pa.vc = m->vc + (size_t)l * m->ctx * kv;
+        pa.kc = layer_k(m, l);
+        pa.vc = layer_v(m, l);
         pa.bias = m->biases ? m->biases + (size_t)l * (dim + 2 * kv) : nullptr;
         pa.norm_w = attn_norm(m, l);
         pa.lay = qkv_shape == PGEMM_SHAPE_32;
@@ -1073,7 +1142,26 @@ int prefill_chunk(llm_model *m, const int *ids, int p0, int M) {
             HIP_OR_FAIL("llm_prefill", launch_p_qkv(pa, m->st));
         }
         pa.lay = o_shape == PGEMM_SHAPE_32;
-        HIP_OR_FAIL("llm_prefill", launch_p_attention(pa, m->st)); // the o projection's int8 input
+        if (m->kv_type != LLM_F32) { // the new rows into the cache, and back with the old ones where the attention reads fp32
+            const llm_kv c = layer_cache(m, l);
+            const llm_rows kr = cache_rows(m, pa.kc), vr = cache_rows(m, pa.vc);
+            KvCall w;
+            memset(&w, 0, sizeof w);
+            w.pos0 = p0;
+            w.by_pos = 1;
+            w.max_n = M;
+            HIP_OR_FAIL("llm_prefill", launch_kv(true, c, kr, vr, w, m->st));
+            w.pos0 = w.by_pos = 0;
+            w.max_n = p0 + M;
+            if (!tree) HIP_OR_FAIL("llm_prefill", launch_kv(false, c, kr, vr, w, m->st));
+        }
+        if (tree) {
+            const TreeCall tc = {I.n_heads, m->ver_len, nullptr, m->ver_mask, M, m->ctx, att_scale(m), 0, m->tree_work};
+            HIP_OR_FAIL("llm_verify", launch_tree_attention(layer_cache(m, l), head_rows(m, pa.q), head_rows(m, pa.xb), tc, m->st));
+            HIP_OR_FAIL("llm_verify", launch_p_quant_rows(pa, m->st));
+        } else {
+            HIP_OR_FAIL("llm_prefill", launch_p_attention(pa, m->st)); // the o projection's int8 input
+        }
         g.W = Ly.o;
         g.shape = o_shape;
         HIP_OR_FAIL("llm_prefill", launch_pgemm(wb, m->gs, sf, g, m->st));
@@ -1108,12 +1196,12 @@ int prefill_chunk(llm_model *m, const int *ids, int p0, int M) {
 // not take the model's shape, a generation that keeps every position's logits runs its prompt position by position.
 bool head_gemm_ok(const llm_model *m) { return m->head.rows % 4 == 0 && m->head.bytes < ((size_t)1 << 31); }
 
-// The logits of a chunk's M positions (their residual streams in pf_x) into hist rows p0 .. p0 + M - 1: the final norm
+// The logits of a chunk's M positions (their residual streams in pf_x) into the rows from y on: the final norm
 // per token, then the head as one GEMM.  The prompt's steps one by one read every weight once per position: 97 tokens
 // through two layers of the 0.5B shape and a 16,384-row head 6587 us, this way 649.  Strict: bitwise the steps' logits.
 // Fast: the sums are taken in another order; the logits' distance from float64 by steps / this way, mean over 124 prompts
 // of 24 tokens 0.00360 / 0.00350, over 124 of 97 tokens 0.00690 / 0.00688.
-int prefill_logits(llm_model *m, int p0, int M) {
+int prefill_logits(llm_model *m, float *y, int M) {
     const llm_info &I = m->info;
     ProwArgs pa;
     memset(&pa, 0, sizeof pa);
@@ -1133,7 +1221,7 @@ int prefill_logits(llm_model *m, int p0, int M) {
     g.W = m->head;
     g.xq = m->pf_a;
     g.xs = m->pf_s;
-    g.y = m->hist + (size_t)p0 * I.n_logits;
+    g.y = y;
     g.M = M;
     g.simds = 4 * hip_cu_count(m->device);
     HIP_OR_FAIL("llm_generate", launch_pgemm(8, m->gs, m->head.sf32, g, m->st));
@@ -1160,7 +1248,7 @@ int prefill_all(llm_model *m, const int *ids, int n, bool sampled = false, int p
     for (int i = 0; i < n; i += chunk) {
         const int M = std::min(chunk, n - i);
         if (prefill_chunk(m, ids + i, pos0 + i, M)) return -1;
-        if (hist && prefill_logits(m, pos0 + i, M)) return -1;
+        if (hist && prefill_logits(m, m->hist + (size_t)(pos0 + i) * m->info.n_logits, M)) return -1;
         if (i + M == n)
             HIP_OR_FAIL("llm_prefill", hipMemcpyAsync(m->x, m->pf_x + (size_t)(M - 1) * m->info.dim,
                                                       (size_t)m->info.dim * 4, hipMemcpyDeviceToDevice, m->st));
@@ -1539,7 +1627,15 @@ extern "C" int llm_read_state(llm_model *m, int which, int layer, float *dst, si
     size_t avail;
     if (which == 0) { src = m->x; avail = (size_t)m->info.dim; }
     else if ((which == 1 || which == 2) && layer >= 0 && layer < m->info.n_layers) {
-        src = (which == 1 ? m->kc : m->vc) + (size_t)layer * m->ctx * m->kv_dim;
+        if (m->kv_type != LLM_F32) { // read back into the one layer's rows
+            KvCall r;
+            memset(&r, 0, sizeof r);
+            r.max_n = m->ctx;
+            HIP_OR_FAIL("llm_read_state", launch_kv(false, layer_cache(m, layer), cache_rows(m, m->kc), cache_rows(m, m->vc), r,
+                                                    m->st));
+            HIP_OR_FAIL("llm_read_state", hipStreamSynchronize(m->st));
+        }
+        src = which == 1 ? layer_k(m, layer) : layer_v(m, layer);
         avail = (size_t)m->ctx * m->kv_dim;
     } else return -1;
     if (count > avail) count = avail;
@@ -1605,6 +1701,10 @@ extern "C" int llm_set_strict(llm_model *m, int on) {
     hipSetDevice(m->device);
     HIP_OR_FAIL("llm_set_strict", hipStreamSynchronize(m->st));
     if ((on != 0) == (m->strict != 0)) return 0;
+    if (on && m->kv_type != LLM_F32) {
+        fprintf(stderr, "llm_set_strict: the reference's order needs the fp32 cache (llm_set_kv)\n");
+        return -1;
+    }
     m->strict = on != 0;
     if (pick_shapes(m)) {
         m->strict = !m->strict;
@@ -1621,6 +1721,249 @@ extern "C" int llm_get_strict(const llm_model *m) { return m ? m->strict : -1; }
 extern "C" int llm_set_prefill(llm_model *m, int on) {
     if (!m) return -1;
     m->prefill_on = on != 0;
+    return 0;
+}
+
+// ---- the cache's type, drafted trees, scores
+
+extern "C" int llm_set_kv(llm_model *m, int type) {
+    if (!m) return -1;
+    hipSetDevice(m->device);
+    HIP_OR_FAIL("llm_set_kv", hipStreamSynchronize(m->st));
+    if (!op_type_bytes(type)) {
+        fprintf(stderr, "llm_set_kv: no cache of type %d\n", type);
+        return -1;
+    }
+    if (type == m->kv_type) return 0;
+    if (type != LLM_F32 && (m->strict || m->hs % 16)) {
+        fprintf(stderr, m->strict ? "llm_set_kv: the strict mode keeps the reference's fp32 cache\n"
+                                  : "llm_set_kv: head size %d (multiples of 16)\n", m->hs);
+        return -1;
+    }
+    drop_graphs(m, false);
+    // the new cache beside the old one: without room for it the old one stays
+    const size_t layer = (size_t)m->ctx * m->kv_dim, all = layer * m->info.n_layers, es = op_type_bytes(type);
+    const size_t scales = op_scaled(type) ? all / m->hs * 4 : 0, rows = type == LLM_F32 ? all : layer;
+    float *kc = nullptr, *vc = nullptr, *ks = nullptr, *vs = nullptr;
+    uint8_t *kq = nullptr, *vq = nullptr;
+    void *work = nullptr;
+    const int old = m->kv_type;
+    m->kv_type = type;
+    const llm_kv c = layer_cache(m, 0);
+    const size_t work_b = llm_tree_attention_work(&c, m->info.n_heads, 1, m->ctx);
+    if (dalloc(m, &kc, rows * 4) || dalloc(m, &vc, rows * 4) ||
+        (type != LLM_F32 && (dalloc(m, &kq, all * es) || dalloc(m, &vq, all * es) || dalloc(m, (uint8_t **)&work, work_b))) ||
+        (scales && (dalloc(m, &ks, scales) || dalloc(m, &vs, scales)))) {
+        m->kv_type = old;
+        dfree(m, kc), dfree(m, vc), dfree(m, kq), dfree(m, vq), dfree(m, ks), dfree(m, vs), dfree(m, work);
+        return -1;
+    }
+    dfree(m, m->kc), dfree(m, m->vc), dfree(m, m->kq), dfree(m, m->vq), dfree(m, m->ks), dfree(m, m->vs);
+    dfree(m, m->tree_work), dfree(m, m->ver_logits), dfree(m, m->ver_mask), dfree(m, m->ver_len), dfree(m, m->ver_depth);
+    m->kc = kc, m->vc = vc, m->kq = kq, m->vq = vq, m->ks = ks, m->vs = vs, m->tree_work = work;
+    // the o projection takes the attention as one merged slice: (0, 1) for every head behind its output
+    std::vector<float> one((size_t)2 * m->info.n_heads);
+    for (int h = 0; h < m->info.n_heads; h++) one[2 * h] = 0.0f, one[2 * h + 1] = 1.0f;
+    HIP_OR_FAIL("llm_set_kv", hipMemcpy(m->att_one + m->info.dim, one.data(), one.size() * 4, hipMemcpyHostToDevice));
+    return 0;
+}
+
+extern "C" int llm_get_kv(const llm_model *m) { return m ? m->kv_type : -1; }
+
+namespace {
+
+// the head's row of every token id
+const std::vector<int> &head_rows_by_id(llm_model *m) {
+    if (m->head_row.empty()) {
+        m->head_row.assign(m->info.vocab_size, -1);
+        for (int i = m->info.n_logits - 1; i >= 0; i--) m->head_row[m->kind == 0 ? m->head_ids_h[i] : i] = i;
+    }
+    return m->head_row;
+}
+int head_id(const llm_model *m, int row) { return m->kind == 0 ? m->head_ids_h[row] : row; }
+
+// Log probabilities over `rows` rows of head logits on the device: the given head rows (`count` a row, -1: none), and the
+// top alternatives, into host arrays (NULL: not asked for).
+int score_rows(llm_model *m, const char *who, const float *logits, int rows, float temperature, const std::vector<int> &given,
+               int count, float *logp, float *entropy, int top, int *top_ids, float *top_logp) {
+    const int V = m->info.n_logits;
+    auto pad = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const size_t tok = pad((size_t)rows * count * 4), ent = pad((size_t)rows * 4), tops = pad((size_t)rows * top * 4);
+    const size_t need = 2 * tok + ent + 2 * tops + llm_logprobs_work(rows, V, top);
+    if (need > m->lp_bytes) {
+        dfree(m, m->lp_buf);
+        m->lp_bytes = 0;
+        if (dalloc(m, (uint8_t **)&m->lp_buf, need)) return -1;
+        m->lp_bytes = need;
+    }
+    uint8_t *p = (uint8_t *)m->lp_buf;
+    LogprobsCall q;
+    memset(&q, 0, sizeof q);
+    q.logits = logits;
+    q.type = LLM_F32;
+    q.rows = rows, q.vocab = V, q.stride = V;
+    q.temperature = temperature;
+    q.tokens = (int *)p, q.n_tokens = count;
+    q.logp = (float *)(p + tok);
+    q.entropy = (float *)(p + 2 * tok);
+    q.top = top;
+    q.top_ids = (int *)(p + 2 * tok + ent);
+    q.top_logp = (float *)(p + 2 * tok + ent + tops);
+    q.work = p + 2 * tok + ent + 2 * tops;
+    if (count) HIP_OR_FAIL(who, hipMemcpyAsync((void *)q.tokens, given.data(), (size_t)rows * count * 4, hipMemcpyHostToDevice, m->st));
+    HIP_OR_FAIL(who, launch_logprobs(q, m->st));
+    auto get = [&](void *dst, const void *src, size_t b) -> int {
+        if (dst && b) HIP_OR_FAIL(who, hipMemcpyAsync(dst, src, b, hipMemcpyDeviceToHost, m->st));
+        return 0;
+    };
+    if (get(logp, q.logp, (size_t)rows * count * 4) || get(entropy, q.entropy, (size_t)rows * 4) ||
+        get(top_ids, q.top_ids, (size_t)rows * top * 4) || get(top_logp, q.top_logp, (size_t)rows * top * 4))
+        return -1;
+    HIP_OR_FAIL(who, hipStreamSynchronize(m->st));
+    if (top_ids)
+        for (size_t i = 0; i < (size_t)rows * top; i++) top_ids[i] = head_id(m, top_ids[i]);
+    return 0;
+}
+
+int check_ids(const llm_model *m, const char *who, const int *ids, int n) {
+    for (int i = 0; i < n; i++)
+        if (ids[i] < 0 || ids[i] >= m->info.vocab_size) {
+            fprintf(stderr, "%s: token id %d out of range\n", who, ids[i]);
+            return -1;
+        }
+    return 0;
+}
+
+} // namespace
+
+extern "C" int llm_verify(llm_model *m, int pos0, const int *tokens, const int *parents, int n, int *next, float *logp,
+                          float *logits) {
+    const char *who = "llm_verify";
+    if (!m || !tokens || n < 1 || n > 64 || pos0 < 0) {
+        fprintf(stderr, "%s: bad arguments (1 to 64 tokens)\n", who);
+        return -1;
+    }
+    if (pos0 + n > m->ctx) {
+        fprintf(stderr, "%s: %d tokens from position %d do not fit the context %d\n", who, n, pos0, m->ctx);
+        return -1;
+    }
+    if (check_ids(m, who, tokens, n)) return -1;
+    if (m->strict || m->hs % 16) {
+        fprintf(stderr, m->strict ? "%s: not in the strict mode, whose sums follow one position at a time\n"
+                                  : "%s: the head size has to be a multiple of 16\n", who);
+        return -1;
+    }
+    uint64_t mask[64];
+    int depth[64], kids[64] = {0}, most = 0;
+    for (int i = 0; i < n; i++) {
+        const int p = parents ? parents[i] : i - 1;
+        if (p < -1 || p >= i) {
+            fprintf(stderr, "%s: the parent of token %d is %d (an earlier one, or -1)\n", who, i, p);
+            return -1;
+        }
+        mask[i] = (p < 0 ? 0 : mask[p]) | (uint64_t)1 << i;
+        depth[i] = p < 0 ? 0 : depth[p] + 1;
+        if (p >= 0) most = std::max(most, ++kids[p]);
+    }
+    hipSetDevice(m->device);
+    const size_t V = m->info.n_logits;
+    const llm_kv c = layer_cache(m, 0);
+    if (!m->ver_logits) {
+        size_t work_b = 0; // (a step's attention uses it too)
+        for (int t = 1; t <= 64; t++) work_b = std::max(work_b, llm_tree_attention_work(&c, m->info.n_heads, t, m->ctx));
+        void *work = nullptr;
+        if (dalloc(m, (uint8_t **)&work, work_b) || dalloc(m, &m->ver_mask, 64 * 8) || dalloc(m, &m->ver_len, 4) ||
+            dalloc(m, &m->ver_depth, 64 * 4) || dalloc(m, &m->ver_logits, 64 * V * 4)) {
+            dfree(m, work), dfree(m, m->ver_mask), dfree(m, m->ver_len), dfree(m, m->ver_depth), dfree(m, m->ver_logits);
+            return -1;
+        }
+        HIP_OR_FAIL(who, hipStreamSynchronize(m->st));
+        drop_graphs(m, false); // (they hold the old memory)
+        dfree(m, m->tree_work);
+        m->tree_work = work;
+    }
+    if (prefill_alloc(m, n, 0)) {
+        fprintf(stderr, "%s: cannot allocate the activations of %d tokens\n", who, n);
+        return -1;
+    }
+    HIP_OR_FAIL(who, hipMemcpyAsync(m->ver_mask, mask, (size_t)n * 8, hipMemcpyHostToDevice, m->st));
+    HIP_OR_FAIL(who, hipMemcpyAsync(m->ver_depth, depth, (size_t)n * 4, hipMemcpyHostToDevice, m->st));
+    HIP_OR_FAIL(who, hipMemcpyAsync(m->ver_len, &pos0, 4, hipMemcpyHostToDevice, m->st));
+    HIP_OR_FAIL(who, hipStreamSynchronize(m->st));
+    if (prefill_chunk(m, tokens, pos0, n, true)) return -1;
+    if (head_gemm_ok(m)) {
+        if (prefill_logits(m, m->ver_logits, n)) return -1;
+    } else { // the step's head, token by token
+        for (int i = 0; i < n; i++) {
+            HIP_OR_FAIL(who, hipMemcpyAsync(m->x, m->pf_x + (size_t)i * m->info.dim, (size_t)m->info.dim * 4,
+                                            hipMemcpyDeviceToDevice, m->st));
+            HIP_OR_FAIL(who, launch_head(m, false));
+            HIP_OR_FAIL(who, hipMemcpyAsync(m->ver_logits + i * V, m->logits, V * 4, hipMemcpyDeviceToDevice, m->st));
+        }
+    }
+    // a token's children are the given tokens of its row
+    const std::vector<int> &row = head_rows_by_id(m);
+    std::vector<int> given((size_t)n * most, -1), at(n, 0), of(n, -1);
+    for (int i = 0; i < n; i++) {
+        const int p = parents ? parents[i] : i - 1;
+        if (p >= 0) of[i] = p * most + at[p], given[(size_t)p * most + at[p]++] = row[tokens[i]];
+    }
+    std::vector<float> lp((size_t)n * most);
+    if (score_rows(m, who, m->ver_logits, n, 1.0f, given, most, lp.data(), nullptr, 1, next, nullptr)) return -1;
+    if (logp)
+        for (int i = 0; i < n; i++) logp[i] = of[i] < 0 ? 0.0f : lp[of[i]];
+    if (logits) HIP_OR_FAIL(who, hipMemcpy(logits, m->ver_logits, (size_t)n * V * 4, hipMemcpyDeviceToHost));
+    return 0;
+}
+
+extern "C" int llm_keep(llm_model *m, int pos0, const int *path, int n) {
+    if (!m || !path || n < 1 || n > 64 || pos0 < 0 || pos0 + path[n - 1] >= m->ctx) {
+        fprintf(stderr, "llm_keep: bad arguments\n");
+        return -1;
+    }
+    uint8_t p[64];
+    for (int i = 0; i < n; i++) {
+        if (path[i] < 0 || path[i] > 63 || (i && path[i] <= path[i - 1])) {
+            fprintf(stderr, "llm_keep: the path has to rise, within 64 tokens\n");
+            return -1;
+        }
+        p[i] = (uint8_t)path[i];
+    }
+    hipSetDevice(m->device);
+    HIP_OR_FAIL("llm_keep", launch_kv_keep(layer_cache(m, 0, m->info.n_layers), pos0, p, n, m->st));
+    HIP_OR_FAIL("llm_keep", hipStreamSynchronize(m->st));
+    return 0;
+}
+
+extern "C" int llm_score(llm_model *m, const int *ids, int n, float temperature, float *logp, float *entropy, int top,
+                         int *top_ids, float *top_logp) {
+    const char *who = "llm_score";
+    if (!m || !ids || n < 1 || n > m->ctx || !(temperature >= 1e-30f && temperature <= 1e30f) || top < 0 || top > 32 ||
+        top > m->info.n_logits) {
+        fprintf(stderr, "%s: bad arguments (1 to %d tokens, a positive temperature, at most 32 alternatives)\n", who,
+                m ? m->ctx : 0);
+        return -1;
+    }
+    if (check_ids(m, who, ids, n)) return -1;
+    hipSetDevice(m->device);
+    if (!m->hist && hipMalloc(&m->hist, (size_t)m->ctx * m->info.n_logits * 4) != hipSuccess) {
+        fprintf(stderr, "%s: no room for the logits history\n", who);
+        (void)hipGetLastError();
+        m->hist = nullptr;
+        return -1;
+    }
+    // as a generation that keeps its logits takes its prompt: batched, or position by position
+    if (n == 1 || !m->prefill_on || !head_gemm_ok(m) || prefill_all(m, ids, n, false, 0, true)) {
+        HIP_OR_FAIL(who, hipStreamSynchronize(m->st));
+        for (int p = 0; p < n; p++)
+            if (set_ctrl(m, p, ids[p], 0, 0) || enqueue_step(m, true, nullptr, p, true)) return -1;
+    }
+    const std::vector<int> &row = head_rows_by_id(m);
+    std::vector<int> given(n, -1);
+    for (int i = 0; i + 1 < n; i++) given[i] = row[ids[i + 1]];
+    std::vector<float> lp(n);
+    if (score_rows(m, who, m->hist, n, temperature, given, 1, lp.data(), entropy, top, top_ids, top_logp)) return -1;
+    if (logp) memcpy(logp, lp.data(), (size_t)(n - 1) * 4);
     return 0;
 }
 

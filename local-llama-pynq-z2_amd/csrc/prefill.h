@@ -104,6 +104,7 @@ static inline int pgemm_shape(const TiledMat &W, int M, int simds, bool swiglu) 
 
 struct ProwArgs {           // per-token elementwise kernels
     int M, p0;              // tokens, position of the first one
+    const int *depth;       // NULL, or a drafted tree's: token m's RoPE position is p0 + depth[m] (k_p_qkv)
     int dim, kv_dim, head_size, hidden, gs, qflavor, rope_kind, gu_rb;
     float eps;
     const int *ids;         // [M] token ids (embedding)
@@ -157,3 +158,4 @@ hipError_t launch_p_qkv(const ProwArgs &a, hipStream_t st);
 hipError_t launch_p_resid(const ProwArgs &a, hipStream_t st);
 hipError_t launch_p_swiglu_quant(const ProwArgs &a, hipStream_t st);
 hipError_t launch_p_attention(const ProwArgs &a, hipStream_t st); // slices, merge; int8 output in oq/os
+hipError_t launch_p_quant_rows(const ProwArgs &a, hipStream_t st); // the rows xb; int8 output in oq/os

@@ -1041,7 +1041,7 @@ __global__ void __launch_bounds__(1024) k_p_norm_quant(ProwArgs a) {
 // QKV rows of token m: bias (qwen.c:521-522), RoPE at position p0 + m (qwen.c:478-488 NeoX pairs; runq.c:506-521
 // interleaved pairs), q to q[m], k and v into the caches.  Logical rows follow the fused matrix's order.
 __global__ void __launch_bounds__(256) k_p_qkv(ProwArgs a) {
-    const int m = blockIdx.x, pos = a.p0 + m, dim = a.dim, kvd = a.kv_dim, hs = a.head_size, half = hs / 2;
+    const int m = blockIdx.x, pos = a.p0 + m, rp = a.depth ? a.p0 + a.depth[m] : pos, dim = a.dim, kvd = a.kv_dim, hs = a.head_size, half = hs / 2;
     const int rows = dim + 2 * kvd;
     const float *y = a.y + (size_t)m * rows;
     for (int R = threadIdx.x; R < rows; R += blockDim.x) {
@@ -1051,7 +1051,7 @@ __global__ void __launch_bounds__(256) k_p_qkv(ProwArgs a) {
                 const int blk = R / 16, r = R & 15, per = half / 8, hh = blk / per, i = (blk - hh * per) * 8 + (r & 7);
                 const bool first = r < 8;
                 const int e = hh * hs + (first ? i : half + i), ep = hh * hs + (first ? half + i : i);
-                const float c = a.rope_cos[(size_t)pos * half + i], sn = a.rope_sin[(size_t)pos * half + i];
+                const float c = a.rope_cos[(size_t)rp * half + i], sn = a.rope_sin[(size_t)rp * half + i];
                 const float self = v + a.bias[e], partner = y[R ^ 8] + a.bias[ep];
                 float o;
                 if (first) { float t1 = self * c, t2 = partner * sn; o = t1 - t2; }
@@ -1064,7 +1064,7 @@ __global__ void __launch_bounds__(256) k_p_qkv(ProwArgs a) {
         } else {
             if (R < dim + kvd) {
                 const int e = R < dim ? R : R - dim, i = (e % hs) / 2;
-                const float c = a.rope_cos[(size_t)pos * half + i], sn = a.rope_sin[(size_t)pos * half + i];
+                const float c = a.rope_cos[(size_t)rp * half + i], sn = a.rope_sin[(size_t)rp * half + i];
                 const float partner = y[R ^ 1];
                 float o;
                 if ((e & 1) == 0) { float t1 = v * c, t2 = partner * sn; o = t1 - t2; }
@@ -1774,6 +1774,11 @@ __global__ void __launch_bounds__(256) k_p_quant_rows(ProwArgs a) {
     block_quantize_tiles(sv, n, a.gs, a.qflavor, a.oq, a.os, m, a.M, a.lay);
 }
 
+hipError_t launch_p_quant_rows(const ProwArgs &a, hipStream_t st) {
+    if (a.dim % 4 || a.dim % a.gs || !a.xb || ((uintptr_t)a.oq & 3) || (size_t)a.dim * 4 > 65536) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(k_p_quant_rows, dim3(a.M), dim3(256), (size_t)a.dim * 4, st, a);
+    return hipGetLastError();
+}
 hipError_t launch_p_embed(const ProwArgs &a, hipStream_t st) {
     hipLaunchKernelGGL(k_p_embed, dim3(a.M), dim3(row_threads(a.dim, a.M)), 0, st, a);
     return hipGetLastError();

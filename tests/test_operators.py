@@ -99,3 +99,13 @@ def test_tensors_refused():
         P.tree_attention(torch.zeros(1, 1, 4, 64), k, k, i)
     with pytest.raises(ValueError):
         P.logprobs(torch.zeros(2, 10))
+
+
+def test_models_refused():
+    """a NULL model and bad arguments, before any device is touched"""
+    L = pkg().lib()
+    ids = (C.c_int * 2)(1, 2)
+    assert L.llm_set_kv(None, 0) == -1 and L.llm_get_kv(None) == -1
+    assert L.llm_verify(None, 0, ids, None, 2, None, None, None) == -1
+    assert L.llm_keep(None, 0, ids, 2) == -1
+    assert L.llm_score(None, ids, 2, 1.0, None, None, 0, None, None) == -1
