@@ -1,4 +1,4 @@
-/* Shared piece of the C host programs qwen_hip and runq_hip: prompt-id parsing.
+/* Shared pieces of the C host programs qwen_hip and runq_hip: prompt-id parsing, the cache's type.
  * Decoding (argmax or the sampler) runs on the device inside the step graph. */
 #pragma once
 #include <stdio.h>
@@ -16,4 +16,13 @@ static int *parse_ids(const char *arg, int *n) { /* qwen.c:771-777 */
         c = *end ? end + 1 : end;
     }
     return ids;
+}
+
+/* --kv: the type of the K/V cache (llm_set_kv) */
+static int parse_kv(const char *arg) {
+    static const char *names[] = {"fp32", "bf16", "int8", "e4m3"};
+    for (int i = 0; i < 4; i++)
+        if (!strcmp(arg, names[i])) return i;
+    fprintf(stderr, "bad --kv %s (fp32, bf16, int8 or e4m3)\n", arg);
+    exit(EXIT_FAILURE);
 }

@@ -1,7 +1,7 @@
 /* qwen_hip: the Qwen2 .qwb token loop of qwen/qwen.c (generate + CLI, qwen.c:669-817) on one MI355X through
  * libmatvec_hip.so's device-resident API.  Same options and output as qwen.c:
  *   qwen_hip model.qwb [-i text] [-m chat|raw] [-z tokenizer] [--ids a,b,c] [-t temp] [-p topp] [-s seed]
- *            [-n new] [-c ctx] [--logits file]
+ *            [-n new] [-c ctx] [--logits file] [--kv fp32|bf16|int8|e4m3]
  * A text prompt goes through the Qwen tokenizer (qwen_tokenizer.c; by default qwen_tokenizer.bin next to the
  * model), inside the Qwen chat template unless -m raw (qwen.c:778-797); the generated tokens are printed as
  * their bytes.  With --ids the prompt is token ids and the output the generated ids, comma separated
@@ -17,7 +17,7 @@
 
 static void usage(void) {
     fprintf(stderr, "Usage: qwen_hip <model.qwb> [-i text] [-m chat|raw] [-z tokenizer] [--ids a,b,c] [-t temp] [-p topp]\n"
-                    "                [-s seed] [-n new] [-c ctx] [--logits file]\n");
+                    "                [-s seed] [-n new] [-c ctx] [--logits file] [--kv fp32|bf16|int8|e4m3]\n");
     exit(EXIT_FAILURE);
 }
 
@@ -42,13 +42,14 @@ static int *text_prompt(Tokenizer *tok, const char *prompt, const char *mode, in
 int main(int argc, char **argv) {
     char *ids_arg = NULL, *logits_path = NULL, *prompt = "", *mode = "chat", *tokenizer_path = NULL;
     float temperature = 0.7f, topp = 0.8f;
-    int steps = 256, ctx = 1024;
+    int steps = 256, ctx = 1024, kv = LLM_F32;
     unsigned long long seed = 0;
     if (argc < 2) usage();
     for (int i = 2; i < argc; i += 2) { /* qwen.c:743-760 */
         if (i + 1 >= argc || argv[i][0] != '-') usage();
         if (!strcmp(argv[i], "--ids")) { ids_arg = argv[i + 1]; continue; }
         if (!strcmp(argv[i], "--logits")) { logits_path = argv[i + 1]; continue; }
+        if (!strcmp(argv[i], "--kv")) { kv = parse_kv(argv[i + 1]); continue; }
         if (strlen(argv[i]) != 2) usage();
         switch (argv[i][1]) {
         case 't': temperature = atof(argv[i + 1]); break;
@@ -87,6 +88,7 @@ int main(int argc, char **argv) {
     llm_info info;
     llm_get_info(m, &info);
     if (info.kind != 0) { fprintf(stderr, "%s: not a .qwb model\n", argv[1]); return 1; }
+    if (llm_set_kv(m, kv)) return 1;
     for (int i = 0; i < n_ids; i++)
         if (ids[i] >= info.vocab_size) { fprintf(stderr, "token id %d out of range\n", ids[i]); return 1; }
     if (n_ids >= info.ctx) { fprintf(stderr, "prompt (%d tokens) does not fit -c %d\n", n_ids, info.ctx); return 1; }

@@ -103,17 +103,18 @@ static int chat(llm_model *m, LlamaTokenizer *tok, const char *cli_user, const c
 
 int main(int argc, char **argv) {
     if (argc < 2) {
-        fprintf(stderr, "usage: runq_hip model.bin [-i text] [-z tokenizer.bin] [--ids a,b,c] [-n N] [-t T] [-p P] [-s S] [--logits f]\n");
+        fprintf(stderr, "usage: runq_hip model.bin [-i text] [-z tokenizer.bin] [--ids a,b,c] [-n N] [-t T] [-p P] [-s S] [--logits f] [--kv fp32|bf16|int8|e4m3]\n");
         return 1;
     }
     char *ids_arg = NULL, *logits_path = NULL, *prompt = NULL, *tokenizer_path = "tokenizer.bin", *mode = "generate";
     char *system_prompt = NULL;
     float temperature = 1.0f, topp = 0.9f;
-    int steps = 256;
+    int steps = 256, kv = LLM_F32;
     unsigned long long seed = 0;
     for (int i = 2; i + 1 < argc; i += 2) {
         if (!strcmp(argv[i], "--ids")) ids_arg = argv[i + 1];
         else if (!strcmp(argv[i], "--logits")) logits_path = argv[i + 1];
+        else if (!strcmp(argv[i], "--kv")) kv = parse_kv(argv[i + 1]);
         else if (!strcmp(argv[i], "-n")) steps = atoi(argv[i + 1]);
         else if (!strcmp(argv[i], "-t")) temperature = atof(argv[i + 1]);
         else if (!strcmp(argv[i], "-p")) topp = atof(argv[i + 1]);
@@ -132,6 +133,7 @@ int main(int argc, char **argv) {
     llm_info info;
     llm_get_info(m, &info);
     if (info.kind != 1) { fprintf(stderr, "%s: not a llama2.c .bin model\n", argv[1]); return 1; }
+    if (llm_set_kv(m, kv)) return 1;
     if (strcmp(mode, "generate") && strcmp(mode, "chat")) { fprintf(stderr, "unknown mode: %s\n", mode); return 1; }
     if (!strcmp(mode, "chat")) {
         if (steps <= 0 || steps > info.ctx) steps = info.ctx;

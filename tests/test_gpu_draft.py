@@ -6,10 +6,13 @@ positions, as for the batched prefill (test_gpu_prefill.py).  The first layer's 
 the fp32 model's, quantized by the definition, exactly.  A wiring mistake moves logits by their own size: the distance to the
 fp32 cache is held to a quarter of it.  Log probabilities: those of the logits in float64, within 1e-5 (sums of at most a few
 hundred terms in fp32)."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
-from helpers import GOLDEN, pkg, rel_err, synth
+from helpers import GOLDEN, PKG_DIR, pkg, rel_err, synth
 from test_gpu_operators import quantized
 
 torch = pytest.importorskip("torch")
@@ -226,3 +229,20 @@ def test_speculative_greedy_decoding_is_greedy_decoding():
         turns += 1
     assert out[:len(want)] == want and turns < len(want)
     m.close()
+
+
+@pytest.mark.parametrize("exe,name", [("qwen_hip", "tiny.qwb"), ("runq_hip", "tiny.bin")])
+def test_the_hosts_take_the_caches_type(exe, name):
+    path = os.path.join(GOLDEN, name)
+    m = pkg().Model(path, 64)
+    m.set_kv("int8")
+    ids = [1, 5, 77, 30]
+    n = 12 if name.endswith("qwb") else m.info.ctx
+    want = list(m.generate(ids, 12 if name.endswith("qwb") else n - len(ids) + 1)["ids"])
+    m.close()
+    run = [os.path.join(PKG_DIR, "host", exe), path, "--ids", ",".join(map(str, ids)), "-t", "0", "-n", str(n), "--kv", "int8"]
+    r = subprocess.run(run + (["-c", "64"] if exe == "qwen_hip" else []), capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    assert [int(x) for x in r.stdout.strip().split(",") if x] == want
+    bad = subprocess.run(run[:-1] + ["int4"], capture_output=True, text=True, timeout=60)
+    assert bad.returncode != 0 and "--kv int4" in bad.stderr
