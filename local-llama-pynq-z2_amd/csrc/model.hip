@@ -148,7 +148,8 @@ int dalloc(llm_model *m, T **p, size_t bytes) {
         (void)hipGetLastError();
         return -1;
     }
-    if (hipMemset(v, 0, bytes ? bytes : 16) != hipSuccess) return -1;
+    // the zeros are there before a copy or kernel of the model's own stream, which does not wait for the null stream
+    if (hipMemset(v, 0, bytes ? bytes : 16) != hipSuccess || hipStreamSynchronize(nullptr) != hipSuccess) return -1;
     m->allocs.push_back(v);
     *p = (T *)v;
     return 0;

@@ -170,6 +170,19 @@ def test_drafts_at_the_end_of_the_context_and_refusals(capfd):
     m.close()
 
 
+def test_first_scores_of_a_model():
+    """a model's first call allocates the buffers (zeroed, on another stream than the tokens come by): it scores as the next"""
+    for _ in range(60):
+        m = pkg().Model(TINY[0], 64)
+        ids = prompt(m, 31, 8)
+        for a, b in zip(m.score(ids, top=32), m.score(ids, top=32)):
+            assert np.array_equal(a, b)
+        v = [m.verify(len(ids), ids[:8], [-1, 0, 0, 1, 2, 3, 4, 5], logits=True) for _ in range(2)]
+        for a, b in zip(*v):
+            assert np.array_equal(a, b, equal_nan=a.dtype == np.float32)
+        m.close()
+
+
 @pytest.mark.parametrize("path", TINY)
 @pytest.mark.parametrize("strict", [False, True])
 @pytest.mark.parametrize("n", [1, 2, 31])
