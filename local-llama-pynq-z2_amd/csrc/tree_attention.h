@@ -19,21 +19,30 @@ struct TreeArgs {
     const uint64_t *mask;
     int n_seq, n_kv, hs, ctx, group, max_n, zero_rest;
     int row_blocks, block_rows;    // blocks that share a kv head's rows, rows of each
-    int splits, quantum;           // slices of a sequence's positions: at most, and their steps
+    int cap, each, least, tp;      // slices of positions: at most in all (0: none) and of a head, their steps at least, a
+                                   // step's positions
     float c;                       // |softmax scale| * log2(e), positive
     int negate;                    // the scale is negative: the queries change their sign
-    float *ml, *acc;               // slices: [seq][kv head][slice][row] (max, sum), the same with hs sums of values
+    float *ml, *acc;               // slices: [slice][row] (max, sum), the same with hs sums of values
+    int2 *plan;                    // [seq][kv head]: first slice, slices
 };
 
 // Positions of a step.  Few rows: a wave's step, its rows held in registers; many rows: the block's, in LDS.
-__host__ __device__ constexpr int tree_positions(int hsp, int type, int many) {
-    return many || hsp * (type == LLM_F32 ? 4 : type == LLM_BF16 ? 2 : 1) <= 128 ? 64 : 32;
+__host__ __device__ constexpr int tree_positions(int hsp, int type, int many, int tiles) {
+    return many || hsp * tiles * (type == LLM_F32 ? 4 : type == LLM_BF16 ? 2 : 1) <= 128 ? 64 : 32;
 }
-// Slices of `end` positions in steps of tp: of `quantum` steps, more where that gives more than `splits`; none is empty.
-__host__ __device__ inline int tree_slices(int end, int tp, int splits, int quantum, int *steps) {
-    const int all = max((end + tp - 1) / tp, 1);
-    *steps = max(quantum, (all + splits - 1) / splits);
-    return (all + *steps - 1) / *steps;
+constexpr int TREE_MAX_SLICES = 128; // of a sequence's kv head
+constexpr int TREE_MAX_SEQS = 512;   // of a call whose positions are cut
+
+// Steps of a sequence: of its positions in the cache and its new tokens (at least one: its block writes the empty rows).
+__device__ __forceinline__ int tree_steps(const TreeArgs &a, int seq) {
+    const int len = min(max(a.lens[seq], 0), a.ctx), nn = a.n ? min(max(a.n[seq], 0), a.max_n) : a.max_n;
+    return max(((int)min((int64_t)len + nn, (int64_t)a.ctx) + a.tp - 1) / a.tp, 1);
+}
+// Slices of the only sequence of a call, of `all` steps: head h has numbers h * each and on.
+__device__ __forceinline__ int tree_one(const TreeArgs &a, int all, int &steps) {
+    steps = max(a.least, (all + a.each - 1) / a.each);
+    return (all + steps - 1) / steps;
 }
 
 typedef void (*TreeKernel)(TreeArgs);

@@ -10,23 +10,29 @@
 
 namespace {
 
-constexpr int TREE_MAX_SPLITS = 128;
-
 // A row's slices joined: weights exp2(max_s - max).  W waves a row (the block has four): a thread takes four values of
 // every (64 W / (hs / 4))-th slice, eight slices' loads at once.
 template <int QT, int W>
-__global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
-    __shared__ float sm_f[4 / W][TREE_MAX_SPLITS + 64]; // (a group's last loads may be past the last slice: weight 0)
+__global__ void __launch_bounds__(256) k_tree_join(TreeArgs a) {
+    __shared__ float sm_f[4 / W][TREE_MAX_SLICES + 64]; // (a group's last loads may be past the last slice: weight 0)
     __shared__ float4 sm_o[256];
     constexpr int T = 64 * W;
     const int lane = threadIdx.x & 63, part = threadIdx.x / T, tid = threadIdx.x % T;
     const int row = blockIdx.x * (4 / W) + part, h = blockIdx.y, b = blockIdx.z;
-    const int len = min(max(a.lens[b], 0), a.ctx), nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n;
-    int steps;
-    const int slices = tree_slices((int)min((int64_t)len + nn, (int64_t)a.ctx), tp, a.splits, a.quantum, &steps);
+    const int nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n;
+    int slices, first;
+    if (a.n_seq == 1) {
+        int steps;
+        slices = tree_one(a, tree_steps(a, 0), steps);
+        first = h * a.each;
+    } else {
+        const int2 plan = a.plan[b * a.n_kv + h];
+        first = plan.x;
+        slices = plan.y;
+    }
     if (slices == 1) return; // (every row of the sequence was finished by its block)
     const bool there = row < nn * a.group;
-    const int64_t stride = (int64_t)a.max_n * a.group, base = ((int64_t)b * a.n_kv + h) * a.splits * stride + row;
+    const int64_t stride = (int64_t)a.max_n * a.group, base = first * stride + row;
     const int per = a.hs / 4, groups = T / per, g = tid / per, d = 4 * (tid - g * per);
     constexpr int U = 8;
     float4 v[U];
@@ -39,9 +45,9 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
         }
     };
     load(g); // (the first values do not wait for the weights)
-    float m[TREE_MAX_SPLITS / 64], l[TREE_MAX_SPLITS / 64], mx = -INFINITY;
+    float m[TREE_MAX_SLICES / 64], l[TREE_MAX_SLICES / 64], mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < TREE_MAX_SPLITS / 64; i++) {
+    for (int i = 0; i < TREE_MAX_SLICES / 64; i++) {
         const int s = lane + 64 * i;
         const bool have = there && s < slices;
         m[i] = have ? a.ml[2 * (base + s * stride)] : -INFINITY;
@@ -52,20 +58,20 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
     const float mu = mx == -INFINITY ? 0.0f : mx;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < TREE_MAX_SPLITS / 64; i++) {
+    for (int i = 0; i < TREE_MAX_SLICES / 64; i++) {
         const float f = __builtin_amdgcn_exp2f(m[i] - mu);
         sum += l[i] * f;
         if (tid < 64) sm_f[part][lane + 64 * i] = f;
     }
     sum = wave_sum(sum);
-    if (tid < 64) sm_f[part][lane + TREE_MAX_SPLITS] = 0.0f;
+    if (tid < 64) sm_f[part][lane + TREE_MAX_SLICES] = 0.0f;
     __syncthreads();
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int s0 = g; s0 < slices; s0 += U * groups) {
         if (s0 != g) load(s0);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const float f = sm_f[part][min(s0 + u * groups, TREE_MAX_SPLITS)];
+            const float f = sm_f[part][min(s0 + u * groups, TREE_MAX_SLICES)];
             o.x += v[u].x * f, o.y += v[u].y * f, o.z += v[u].z * f, o.w += v[u].w * f;
         }
     }
@@ -90,42 +96,57 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a, int tp) {
 }
 
 struct TreePlan {
-    int hsp, tp, many, tiles, row_blocks, block_rows, splits, quantum;
+    int hsp, tp, many, tiles, row_blocks, block_rows, cap, each, least;
     size_t bytes;
 };
 
-// How a call is cut.  Up to 32 rows a kv head: the block's four waves share the positions, with one or two tiles of 16 rows
-// each.  More rows: the waves share the rows, 16 each (four waves up to 64 rows, else eight), and the cache's rows go
-// through LDS.  (Not for fp32 caches, whose rows need no conversion, nor head sizes above 128, whose rows do not fit twice.
-// fp32 queries over bf16 caches, three pieces, take two tiles in each of four waves: eight would spill.)  The rows are
-// spread evenly over their blocks.  Positions in slices, the same number of steps for every sequence, until the grid has a
-// block a CU (few rows) or two; four for several sequences, whose lengths the host does not know.
+// How a call is cut.  Times: one call, heads of 128.
+// Rows.  The block's four waves share the positions, with one tile of 16 rows, or two where that is work enough: two read
+// and convert half as often, one gives twice the blocks (112 rows over 32k bf16 positions, 4 kv heads: 44 us with one tile, 31
+// with two; over 700: 10.8 and 13.7.  448 rows over 8 x 4000 int8 positions: 113 and 91; 63 rows over 32 x 2000: 39 and 41).
+// Not for fp32 caches, nor fp32 queries over bf16 ones (three pieces), whose registers leave one wave a SIMD.  Many rows over
+// a bf16 cache, whose L2 traffic then bounds: the waves share the rows, and the cache's rows go through LDS (eight
+// sequences of up to 16k positions, 448 rows: 186 us this way or with two tiles, 144 with LDS; one of 700: 14 and 18).  fp32
+// queries take two tiles in each of four waves there (eight waves of one would spill), bf16 ones one in each of eight.  The
+// rows are spread evenly over these blocks.
+// Positions.  One sequence: as many slices as give a block a CU, or two a CU where whole row blocks would leave much of the
+// chip idle (192 rows over 32k int8 positions: 70 us with 192 blocks, 55 with 480; 7 rows: 16 with 256, 18 with 512).
+// Several: two blocks a CU over all sequences, of equal steps (a decode step of 32 sequences, 0 to 8190 e4m3 positions: 31 us,
+// 37 with four a CU; with the same number of slices for each sequence, 37).
 TreePlan tree_plan(const llm_kv *c, int q_type, int n_heads, int max_n, int max_len) {
     TreePlan p;
     p.hsp = (c->hs + 63) / 64 * 64;
     const int group = n_heads / c->n_kv, rows = group * max_n, tiles = (rows + 15) / 16;
-    const bool many = rows > 32 && p.hsp <= 128 && c->type != LLM_F32, pieces = c->type == LLM_BF16 && q_type == LLM_F32;
-    p.many = !many ? 0 : tiles <= 4 || pieces ? 4 : 8;
-    p.tiles = many ? (tiles > 4 && pieces ? 2 : 1) : tiles > 1 && p.hsp <= 128 ? 2 : 1;
+    const int64_t end = std::min<int64_t>((int64_t)std::max(max_len, 0) + max_n, c->ctx), heads = (int64_t)c->n_seq * c->n_kv;
+    const bool bf16 = c->type == LLM_BF16, pieces = bf16 && q_type == LLM_F32, small = p.hsp <= 128;
+    const int64_t work = tiles * heads * end;
+    const bool many = bf16 && p.hsp == 128 && tiles > 8 && work >= (pieces ? 800000 : 2000000);
+    p.many = !many ? 0 : pieces ? 4 : 8;
+    const bool two = small && c->type != LLM_F32 && !pieces &&
+                     (bf16 ? tiles > 2 && work >= 250000 : tiles > 5 && work * p.hsp >= 100000000);
+    p.tiles = many ? (pieces ? 2 : 1) : two ? 2 : 1;
     const int per_block = p.tiles * (many ? p.many : 1); // tiles
     p.row_blocks = (tiles + per_block - 1) / per_block;
     p.block_rows = 16 * (many ? (tiles + p.row_blocks - 1) / p.row_blocks : per_block);
-    p.tp = tree_positions(p.hsp, c->type, p.many);
-    const int64_t end = std::min<int64_t>((int64_t)std::max(max_len, 0) + max_n, c->ctx);
-    const int64_t steps = std::max<int64_t>((end + p.tp - 1) / p.tp, 1), blocks = (int64_t)c->n_seq * c->n_kv * p.row_blocks;
-    const int64_t least = many ? 2 : 4; // steps of a slice (few rows: one a wave)
-    const int64_t grid = c->n_seq > 1 ? 1024 : many ? 512 : 256;
-    const int64_t cap = std::min({std::max<int64_t>(1, grid / std::max<int64_t>(blocks, 1)), (steps + least - 1) / least,
-                                  (int64_t)TREE_MAX_SPLITS});
-    // one sequence: as many slices as its length, known to the kernel, gives of the least size, up to that number
-    p.quantum = (int)(c->n_seq > 1 ? (steps + cap - 1) / cap : least);
-    p.splits = (int)(c->n_seq > 1 ? (steps + p.quantum - 1) / p.quantum : cap);
-    p.bytes = p.splits > 1 ? (size_t)c->n_seq * c->n_kv * p.splits * rows * (c->hs + 2) * 4 : 0;
+    p.tp = tree_positions(p.hsp, c->type, p.many, p.tiles);
+    const int64_t steps = std::max<int64_t>((end + p.tp - 1) / p.tp, 1);
+    p.least = many ? 2 : 4; // steps of a slice (few rows: one a wave)
+    // per XCD; a single sequence: one block a CU, two where whole blocks would leave much of the chip idle
+    const int64_t one = 32 / p.row_blocks * 8, both = 64 / p.row_blocks * 8;
+    int64_t cap = both, each = TREE_MAX_SLICES;
+    if (c->n_seq == 1) {
+        cap = both / c->n_kv * 5 > one / c->n_kv * 11 ? both : one;
+        each = std::min({cap / c->n_kv, (steps + p.least - 1) / p.least, each});
+        cap = each * c->n_kv;
+    }
+    p.cap = cap <= heads || c->n_seq > TREE_MAX_SEQS || steps <= p.least ? 0 : (int)cap;
+    p.each = (int)each;
+    p.bytes = p.cap ? (size_t)p.cap * rows * (c->hs + 2) * 4 + heads * sizeof(int2) : 0;
     return p;
 }
 
 int64_t tree_blocks(const llm_kv &c, const TreePlan &p) { // (rounded up to a slice for each XCD)
-    return ((int64_t)c.n_seq * c.n_kv * p.splits + 7) / 8 * 8 * p.row_blocks;
+    return ((p.cap ? p.cap : (int64_t)c.n_seq * c.n_kv) + 7) / 8 * 8 * p.row_blocks;
 }
 
 bool tree_shape_ok(const llm_kv *c, int n_heads, int max_n) {
@@ -156,25 +177,28 @@ hipError_t launch_tree_attention(const llm_kv &c, const llm_rows &q, const llm_r
     a.lens = t.lens, a.n = t.n, a.mask = t.mask;
     a.n_seq = c.n_seq, a.n_kv = c.n_kv, a.hs = c.hs, a.ctx = c.ctx;
     a.group = t.n_heads / c.n_kv, a.max_n = t.max_n, a.row_blocks = p.row_blocks, a.block_rows = p.block_rows;
-    a.splits = p.splits, a.quantum = p.quantum, a.zero_rest = t.zero_rest;
+    a.cap = p.cap, a.each = p.each, a.least = p.least, a.tp = p.tp, a.zero_rest = t.zero_rest;
     // (a scale of 0 as one so small that every weight is 1)
     a.c = std::max(std::fabs(t.scale) * 1.44269504088896340736f, 1e-30f);
     a.negate = t.scale < 0.0f;
     a.acc = (float *)t.work; // (rows of hs values, hs a multiple of 16: 16-byte aligned)
-    a.ml = (float *)t.work + (p.bytes / 4 / (c.hs + 2)) * c.hs;
+    const size_t parts = (size_t)p.cap * a.group * t.max_n;
+    a.ml = a.acc + parts * c.hs;
+    a.plan = (int2 *)(a.ml + 2 * parts);
     size_t lds = 0;
     auto *pick = p.hsp == 64 ? tree_kernel_64 : p.hsp == 128 ? tree_kernel_128 : p.hsp == 192 ? tree_kernel_192 : tree_kernel_256;
     TreeKernel kern = pick(c.type, q.type, p.tiles, p.many, &lds);
     if (!kern) return hipErrorInvalidValue;
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(p.many ? 64 * p.many : 256), lds, st, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return e;
-    // a wave a row up to 8 slices, the block's four above
-    const bool wide = p.splits > 8;
+    if (e != hipSuccess || !p.cap) return e;
+    // a wave a row up to 16 slices a head, the block's four above (7 rows of 64 slices over 32k positions: 18.9 us a call
+    // with one, 16.7 with four; 448 rows of up to 4, eight sequences: 124 and 135)
+    const bool wide = p.cap > 16 * c.n_seq * c.n_kv;
     const dim3 grid(wide ? t.max_n * a.group : (t.max_n * a.group + 3) / 4, c.n_kv, c.n_seq);
     auto *join = q.type == LLM_F32 ? wide ? k_tree_join<LLM_F32, 4> : k_tree_join<LLM_F32, 1>
                                    : wide ? k_tree_join<LLM_BF16, 4> : k_tree_join<LLM_BF16, 1>;
-    hipLaunchKernelGGL(join, grid, dim3(256), 0, st, a, p.tp);
+    hipLaunchKernelGGL(join, grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

@@ -6,15 +6,17 @@
 //           positions 4 j + i of every 16.
 //   values  O^T += V^T P^T: its own probabilities are the B operand as they are (eight positions: 4 j + i of two tiles of
 //           16); V, A, has those positions of one dimension in a lane.
-// Few rows (k_tree_attention): the block's four waves share the positions; K and V go from memory to the registers where
-// they are used.  Many rows (k_tree_rows): the waves share the rows; each step's K and V are converted once and read by
-// all four from LDS.
+// k_tree_attention: the block's four waves share the positions; K and V go from memory to the registers where they are used,
+// and blocks with other rows of the same heads find them in the L2.  k_tree_rows, for many rows over bf16 caches: the waves
+// share the rows; each step's K and V are read by all from LDS.
 //
 // Operands.  int8 and e4m3 codes are exact in fp16, and the fp32 side is held in two fp16 pieces (22 bits): a query row is
 // scaled by a power of two to the top of fp16's range first, and so are the weights p * V scale, by the largest V scale met
 // (a running exponent, as the maximum is running).  bf16 caches: three bf16 pieces.  16-bit queries are one piece; their
 // weights one in fp16 (half a step 2^-11, against the output's 2^-8) and two in bf16.  fp32 caches: v_mfma_f32_16x16x4_f32.
 // Maxima, sums and outputs are fp32.
+#include <limits.h>
+
 #include <type_traits>
 
 #include "device.h"
@@ -152,38 +154,108 @@ __device__ __forceinline__ float4 load_query(const uint8_t *row, int d) {
     return make_float4(lo16(u.x), hi16(u.x), lo16(u.y), hi16(u.y));
 }
 
-// The dimension of value i = 4 q4 .. 4 q4 + 3 of lane group j in product s.  From memory, a lane's 16-byte pieces of a K row
-// are its own (piece j of every four); from LDS, rows are in order.
-template <int CT, bool LDS>
+// The dimension of value i = 4 q4 .. 4 q4 + 3 of lane group j in product s: a lane has 16-byte pieces of a K row, piece j of
+// every four (for bf16 that is the rows' order, which k_tree_rows' LDS keeps).
+template <int CT>
 __device__ __forceinline__ int dim_of(int s, int j, int q4) {
-    if constexpr (LDS || CT == LLM_BF16) return 32 * s + 8 * j + 4 * q4;
+    if constexpr (CT == LLM_BF16) return 32 * s + 8 * j + 4 * q4;
     else if constexpr (CT == LLM_F32) return 32 * s + 16 * q4 + 4 * j;
     else return 64 * (s / 2) + 16 * j + 8 * (s % 2) + 4 * q4;
 }
 
-// Where a block works: sequence, kv head, slice, first row, and how many positions and rows there are.
+// Where a block works: sequence, kv head, slice (`id` of all), first row, and how many positions and rows there are.
 struct Place {
-    int b, h, split, row0, len, end, rows, slices, first, last;
+    int b, h, split, id, row0, len, end, rows, slices, first, last;
 };
+
+// The slice `id`: its sequence, kv head and number there, the slices of that head and their steps.  A sequence of n steps
+// has ceil(n / q) slices a head, the same q for all, so that long sequences do not outlast the others; q is about the least
+// at which there are no more than a.cap in all.  Every block finds it from the lengths.
+__device__ __forceinline__ bool find_slice(const TreeArgs &a, uint32_t id, Place &p, int &steps) {
+    if (a.n_seq == 1) {
+        p.b = 0;
+        p.h = (int)id / a.each;
+        p.split = (int)id - p.h * a.each;
+        p.slices = tree_one(a, tree_steps(a, 0), steps);
+        return p.split < p.slices;
+    }
+    const int lane = threadIdx.x & 63;
+    constexpr int GROUPS = TREE_MAX_SEQS / 64;
+    int all[GROUPS];
+    float sum = 0.0f, most = 0.0f; // (a guess to begin with: rounded sums of steps do)
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++) {
+        all[i] = 0;
+        if (64 * i < a.n_seq) {
+            if (64 * i + lane < a.n_seq) all[i] = tree_steps(a, 64 * i + lane);
+            sum += (float)all[i];
+            most = fmaxf(most, (float)all[i]);
+        }
+    }
+    const float kv = (float)a.n_kv;
+    const int guess = __builtin_amdgcn_readfirstlane((int)(wave_sum(sum) * kv / (float)a.cap));
+    steps = max(max(a.least, guess), __builtin_amdgcn_readfirstlane((int)wave_max(most)) / a.each + 1);
+    int n[GROUPS];
+    for (;; steps += (steps + 15) / 16) { // (ends: at the longest sequence's steps there is a slice a head)
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; i++) {
+            n[i] = 0;
+            if (64 * i < a.n_seq) {
+                n[i] = (all[i] + steps - 1) / steps;
+                total += (float)n[i];
+            }
+        }
+        if (__builtin_amdgcn_readfirstlane((int)wave_sum(total)) * kv <= (float)a.cap) break; // (exact up to 2^24)
+    }
+    int before = 0; // slices of a head of the sequences before
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++)
+        if (64 * i < a.n_seq) {
+            int upto = n[i];
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int x = __shfl_up(upto, off);
+                upto += lane >= off ? x : 0;
+            }
+            const int passed = __popcll(__ballot((before + upto) * a.n_kv <= (int)id));
+            if (passed < 64) { // (a lane without a sequence has passed none that its neighbours have not)
+                const int at = __builtin_amdgcn_readfirstlane(passed);
+                p.b = 64 * i + at;
+                p.slices = __builtin_amdgcn_readlane(n[i], at);
+                const int rest = (int)id - (before + __builtin_amdgcn_readlane(upto, at) - p.slices) * a.n_kv;
+                p.h = rest / p.slices;
+                p.split = rest - p.h * p.slices;
+                return true;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
+    return false;
+}
+
 // Blocks go to the eight XCDs in turn.  The row blocks of a slice follow each other on one, whose L2 then holds the slice's
-// rows for all of them; the slices of a sequence go around, each head's from another XCD on, so that sequences with few
-// slices do not all use the same ones.
+// rows for all of them.
 template <int QT>
-__device__ __forceinline__ bool place(const TreeArgs &a, int tp, int block_rows, Place &p) {
-    const uint32_t k = blockIdx.x >> 3, kr = k / (uint32_t)a.row_blocks;
-    const uint32_t id = kr * 8 + (blockIdx.x & 7), bh = id / (uint32_t)a.splits;
-    if (bh >= (uint32_t)(a.n_seq * a.n_kv)) return false; // (the grid is rounded up to eight slices)
-    p.split = (int)((id + 3 * bh) % (uint32_t)a.splits);
-    p.b = (int)(bh / (uint32_t)a.n_kv);
-    p.h = (int)bh - p.b * a.n_kv;
+__device__ __forceinline__ bool place(const TreeArgs &a, int block_rows, Place &p) {
+    const uint32_t k = blockIdx.x >> 3, kr = k / (uint32_t)a.row_blocks, id = kr * 8 + (blockIdx.x & 7);
+    int steps = INT_MAX;
+    if (a.cap) {
+        if (id >= (uint32_t)a.cap || !find_slice(a, id, p, steps)) return false;
+    } else {
+        if (id >= (uint32_t)(a.n_seq * a.n_kv)) return false; // (the grid is rounded up to eight slices)
+        p.b = (int)(id / (uint32_t)a.n_kv);
+        p.h = (int)id - p.b * a.n_kv;
+        p.split = 0;
+        p.slices = 1;
+    }
+    p.id = (int)id;
     const int row0 = (int)(k - kr * a.row_blocks) * block_rows;
+    if (a.cap && a.n_seq > 1 && p.split == 0 && row0 == 0 && threadIdx.x == 0) a.plan[p.b * a.n_kv + p.h] = make_int2((int)id, p.slices);
     p.row0 = row0;
     p.len = min(max(a.lens[p.b], 0), a.ctx);
     const int nn = a.n ? min(max(a.n[p.b], 0), a.max_n) : a.max_n;
     p.end = (int)min((int64_t)p.len + nn, (int64_t)a.ctx);
     p.rows = nn * a.group;
-    int steps;
-    p.slices = tree_slices(p.end, tp, a.splits, a.quantum, &steps);
     if (a.zero_rest && p.split == 0 && row0 + block_rows > p.rows) { // the rows behind the last token
         for (int e = threadIdx.x * 4; e < block_rows * a.hs; e += 4 * blockDim.x) {
             const int row = row0 + e / a.hs, t = row / a.group, d = e - (row - row0) * a.hs;
@@ -193,15 +265,15 @@ __device__ __forceinline__ bool place(const TreeArgs &a, int tp, int block_rows,
             else *(uint2 *)(op + (size_t)d * 2) = make_uint2(0, 0);
         }
     }
-    const int all = (p.end + tp - 1) / tp;
-    p.first = p.split * steps;
-    p.last = min(p.first + steps, all);
-    return row0 < p.rows && p.split < p.slices;
+    const int all = (p.end + a.tp - 1) / a.tp;
+    p.first = p.split ? p.split * steps : 0;
+    p.last = (int)min((int64_t)p.first + steps, (int64_t)all);
+    return row0 < p.rows;
 }
 
 // The queries of row `row` (none from p.rows on: zeros, nothing seen) as the operand of its scores.  Returns what takes a
 // score to the exponent of 2.
-template <int CT, int QT, bool LDS, int NP>
+template <int CT, int QT, int NP>
 __device__ __forceinline__ float load_queries(const TreeArgs &a, const Place &p, int row, Frag<CT, NP> (&qf)[HSP / 32],
                                               uint64_t &sees) {
     const int j = (threadIdx.x & 63) >> 4, t = row / a.group, g = row - t * a.group;
@@ -217,7 +289,7 @@ __device__ __forceinline__ float load_queries(const TreeArgs &a, const Place &p,
     for (int s = 0; s < HSP / 32; s++)
 #pragma unroll
         for (int q4 = 0; q4 < 2; q4++) {
-            const int d = dim_of<CT, LDS>(s, j, q4);
+            const int d = dim_of<CT>(s, j, q4);
             v[s][q4] = load_query<QT>(qp, d < a.hs ? d : 0);
         }
     float x[HSP / 32][8], mx = 0.0f;
@@ -225,7 +297,7 @@ __device__ __forceinline__ float load_queries(const TreeArgs &a, const Place &p,
     for (int s = 0; s < HSP / 32; s++)
 #pragma unroll
         for (int q4 = 0; q4 < 2; q4++) {
-            const bool there = ok && dim_of<CT, LDS>(s, j, q4) < a.hs;
+            const bool there = ok && dim_of<CT>(s, j, q4) < a.hs;
             const float y[4] = {v[s][q4].x, v[s][q4].y, v[s][q4].z, v[s][q4].w};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -318,7 +390,7 @@ template <int QT>
 __device__ __forceinline__ void put_values(const TreeArgs &a, const Place &p, int row, int d, float4 y) {
     if (d >= a.hs) return;
     if (p.slices > 1) {
-        const int64_t part = (((int64_t)p.b * a.n_kv + p.h) * a.splits + p.split) * a.max_n * a.group + row;
+        const int64_t part = (int64_t)p.id * a.max_n * a.group + row;
         *(float4 *)(a.acc + part * a.hs + d) = y;
         return;
     }
@@ -328,7 +400,7 @@ __device__ __forceinline__ void put_values(const TreeArgs &a, const Place &p, in
     else *(uint2 *)(op + (size_t)d * 2) = make_uint2(bf2(y.x, y.y), bf2(y.z, y.w));
 }
 __device__ __forceinline__ void put_sums(const TreeArgs &a, const Place &p, int row, float m, float l) {
-    const int64_t part = (((int64_t)p.b * a.n_kv + p.h) * a.splits + p.split) * a.max_n * a.group + row;
+    const int64_t part = (int64_t)p.id * a.max_n * a.group + row;
     a.ml[2 * part] = m;
     a.ml[2 * part + 1] = l;
 }
@@ -345,12 +417,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t step_rsrc(const void *base, in
                                              (int)(left * stride), 0x00020000);
 }
 
-// ---- few rows: the waves share the positions
+// ---- the waves share the positions
 
 template <int CT, int QT, int R>
 struct TreeShape {
     static constexpr int ES = TreePieces<CT, QT>::ES;
-    static constexpr int TP = tree_positions(HSP, CT, false), NT = TP / 16; // positions a step, their tiles of 16
+    static constexpr int TP = tree_positions(HSP, CT, 0, R), NT = TP / 16; // positions a step, their tiles of 16
     static constexpr int KL = HSP * ES / 64;                                // 16-byte pieces of a K row a lane
     static constexpr int KS = HSP / 32;                                     // products of a score
     static constexpr int VW = HSP % 128 ? 4 : 8;                            // neighbouring dimensions a lane of V
@@ -360,9 +432,14 @@ struct TreeShape {
 
 // K's lane 16 j + n has 16-byte pieces of position n (piece j of every four), so a row's bytes are read whole and once.  V's
 // lane n reads 4 or 8 neighbouring dimensions of its eight positions and pairs the registers of two positions, which
-// transposes for nothing.  The next step's loads go out as soon as a step's registers are used.
+// transposes for nothing.  The next step's loads go out as soon as a step's registers are used.  No wave waits for
+// another before the end.
+// What bounds it: for one token, memory (32 sequences of 0 to 8190 e4m3 positions, 4 kv heads of 128: 27 us, 5.0 TB/s), or
+// where few steps are left for each block, the latency of a step (32.7k int8 positions of one sequence: 12.6 us, 2.7 TB/s).
+// For trees the vector instructions: for each 64 positions and 16 rows about 360 convert codes and 240 make weights, beside 64
+// products of 17 cycles (a 37-token tree, 259 rows, over 12k int8 positions: 36 us, 177 TFLOP/s, 354 of issued products).
 template <int CT, int QT, int R>
-__global__ void __launch_bounds__(256, CT != LLM_F32 && R == 1 && HSP <= 128 ? 2 : 1) k_tree_attention(TreeArgs a) {
+__global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tree_attention(TreeArgs a) {
     using Sh = TreeShape<CT, QT, R>;
     using Pc = TreePieces<CT, QT>;
     constexpr int ES = Sh::ES, TP = Sh::TP, NT = Sh::NT, KL = Sh::KL, KS = Sh::KS, VW = Sh::VW, VC = Sh::VC, VR = Sh::VR;
@@ -375,7 +452,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && R == 1 && HSP <= 128 ? 2
     const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
-    if (!place<QT>(a, TP, 16 * R, p)) return;
+    if (!place<QT>(a, 16 * R, p)) return;
     const int row0 = p.row0;
 
     const uint8_t *const kb = a.k + p.b * a.seq + p.h * a.head, *const vb = a.v + p.b * a.seq + p.h * a.head;
@@ -438,7 +515,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && R == 1 && HSP <= 128 ? 2
     f32x4 o[R][VC * VW];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        cq[r] = load_queries<CT, QT, false>(a, p, row0 + 16 * r + n, qf[r], sees[r]);
+        cq[r] = load_queries<CT, QT>(a, p, row0 + 16 * r + n, qf[r], sees[r]);
         m[r] = -INFINITY;
         l[r] = 0.0f;
 #pragma unroll
@@ -637,9 +714,9 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && R == 1 && HSP <= 128 ? 2
     }
 }
 
-// ---- many rows: the waves share the rows
+// ---- many rows over bf16 caches: the waves share the rows
 
-#if TREE_HSP <= 128
+#if TREE_HSP == 128
 // A step in LDS, 16-bit values in units of eight: K rows in order, V transposed, its positions in the order of the weights'
 // lanes: unit 4 u + j of a V row's eight holds positions 4 j + i of tiles 2 u and 2 u + 1.  Sixteen units are all banks
 // once; the units of a row change places by its number, so that the sixteen rows of a read are in different ones, and
@@ -647,45 +724,42 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && R == 1 && HSP <= 128 ? 2
 struct __align__(16) TreeStep {
     static constexpr int KU = HSP / 8; // units of a K row
     uint4 k[64 * KU], v[HSP * 8];
-    float s[2][64];     // K scales, V scales times a power of two
-    uint32_t e, pad[3]; // that power's exponent field (power_to)
     __device__ __forceinline__ static int k_at(int row, int unit) {
         return row * KU + (unit ^ (KU == 16 ? row & 15 : (row >> 1) & 7));
     }
     __device__ __forceinline__ static int v_at(int dim, int unit) { return dim * 8 + (unit ^ ((dim >> 1) & 7)); }
 };
 
-// A wave has 16 rows and takes them through scores, softmax and values 32 positions at a time: few enough registers for
-// four waves a SIMD, which hide each other's LDS and product latencies (two rows tiles a wave, or 32 x 32 tiles, read less
-// LDS but leave two: a 37-token tree over 12k int8 positions 51 us a launch, a batch of 64-token trees over bf16 202).  A
-// step of 64 positions is in LDS while the next one's loads are under way: one barrier a step.
-template <int CT, int QT, int NW, int R>
+// A wave has R tiles of 16 rows and takes them through scores, softmax and values 32 positions at a time: few enough
+// registers for four waves a SIMD at R = 1, which hide each other's LDS and product latencies.  A step of 64 positions is
+// in LDS while the next one's loads are under way: one barrier a step.  LDS bounds it: 16 waves a CU read each step's 32 KB,
+// 4096 cycles at 128 bytes a cycle, of about 5500 (448 rows over eight sequences of 0 to 16k positions, 4 kv heads of 128: 113
+// us, 383 TFLOP/s, 574 of issued products.  Two tiles in each of four waves read half, with two waves a SIMD: 143).
+template <int QT, int NW, int R>
 __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs a) {
+    constexpr int CT = LLM_BF16;
     using Pc = TreePieces<CT, QT>;
-    constexpr int ES = Pc::ES, KS = HSP / 32, DT = HSP / 16;
+    constexpr int KS = HSP / 32, DT = HSP / 16;
     constexpr bool APART = NW == 8; // waves 4 to 7 fetch K, 0 to 3 V; four waves fetch both
-    constexpr int KN = HSP * ES / 16, KL = 64 * KN / 256; // 16-byte pieces of a K row, of a thread
-    constexpr int VN = HSP / 4;                           // runs of four dimensions: a thread takes one, at eight positions
-    constexpr int VAT = APART ? 0 : 4 * KL, NR = APART ? (4 * KL > 8 * ES ? 4 * KL : 8 * ES) : 4 * KL + 8 * ES;
-    constexpr bool SCALED = Pc::SCALED;
+    constexpr int KN = HSP / 8, KL = 64 * KN / 256; // 16-byte pieces of a K row, of a thread
+    constexpr int VN = HSP / 4;                     // runs of four dimensions: a thread takes one, at eight positions
+    constexpr int VAT = APART ? 0 : 4 * KL, NR = APART ? (KL > 4 ? 4 * KL : 16) : 4 * KL + 16;
     __shared__ TreeStep sm[2];
     __shared__ uint32_t sm_bad[2]; // new tokens whose V row is not finite
 
     const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
-    if (!place<QT>(a, 64, a.block_rows, p)) return;
+    if (!place<QT>(a, a.block_rows, p)) return;
 
     const int row0 = p.row0 + wave * 16 * R;
     const bool works = wave * 16 * R < a.block_rows && row0 < p.rows; // (a wave without rows still fetches)
     const bool does_k = !APART || wave >= 4, does_v = (!APART || wave < 4) && (VN == 32 || (threadIdx.x & 255) < 8 * VN);
-    const uint32_t hb = (uint32_t)(a.hs * ES);
-    const int64_t p00 = (int64_t)p.first * 64;
-    const uint8_t *kp = a.k + p.b * a.seq + p.h * a.head + p00 * a.pos, *vp = a.v + p.b * a.seq + p.h * a.head + p00 * a.pos;
-    const float *sp = nullptr; // wave 0: K's scales, wave 1: V's
-    if constexpr (SCALED) sp = (wave == 1 ? a.vs : a.ks) + p.b * a.s_seq + p.h * a.s_head + p00 * a.s_pos;
+    const uint32_t hb = (uint32_t)(a.hs * 2);
+    const int64_t at0 = p.b * a.seq + p.h * a.head + (int64_t)p.first * 64 * a.pos;
+    const uint8_t *kp = a.k + at0, *vp = a.v + at0;
     int left = min(p.end, p.last * 64) - p.first * 64; // positions not fetched yet
-    uint32_t raw[NR], sr = 0, next_e = 20; // (the largest V scale's exponent field, at least 2^-107; wave 1 keeps it)
+    uint32_t raw[NR];
     // Addresses are formed again at every use, from values that the compiler cannot see through: kept across the loop they
     // would cost the registers that keep it free of spills (a reload waits for the loads under way).
     auto again = [](uint32_t x) {
@@ -708,23 +782,13 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
         if (does_v) {
             const auto rv = __builtin_amdgcn_make_buffer_rsrc((void *)vp, 0, (int)(here * a.pos), 0x00020000);
             const uint32_t vu = tid / VN, vc = tid % VN; // unit and run
-            const uint32_t vo = 4 * ES * vc < hb ? (32 * (vu / 4) + 4 * (vu % 4)) * ps + 4 * ES * vc : OUT_OF_RANGE;
+            const uint32_t vo = 8 * vc < hb ? (32 * (vu / 4) + 4 * (vu % 4)) * ps + 8 * vc : OUT_OF_RANGE;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int off = (int)(vo + (16 * (i / 4) + i % 4) * ps); // (stays out of range)
-                if constexpr (ES == 1) raw[VAT + i] = __builtin_amdgcn_raw_buffer_load_b32(rv, off, 0, 0);
-                else {
-                    const auto x = __builtin_amdgcn_raw_buffer_load_b64(rv, off, 0, 0);
-                    raw[VAT + 2 * i] = x[0], raw[VAT + 2 * i + 1] = x[1];
-                }
+            for (int i = 0; i < 8; i++) { // (out of range stays so)
+                const auto x = __builtin_amdgcn_raw_buffer_load_b64(rv, (int)(vo + (16 * (i / 4) + i % 4) * ps), 0, 0);
+                raw[VAT + 2 * i] = x[0], raw[VAT + 2 * i + 1] = x[1];
             }
         }
-        if constexpr (SCALED)
-            if (wave < 2) {
-                const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)sp, 0, (int)(here * a.s_pos * 4), 0x00020000);
-                sr = __builtin_amdgcn_raw_buffer_load_b32(rs, (int)(lane * (uint32_t)a.s_pos * 4), 0, 0);
-                sp += 64 * a.s_pos;
-            }
         kp += 64 * a.pos;
         vp += 64 * a.pos;
         left -= 64;
@@ -735,66 +799,35 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
 #pragma unroll
             for (int i = 0; i < KL; i++) {
                 const uint32_t piece = tid + 256 * i;
-                const int row = piece / KN, unit = piece % KN * (2 / ES);
-                if constexpr (CT == LLM_BF16)
-                    st.k[st.k_at(row, unit)] = make_uint4(raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
-                else {
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const uint32_t u0 = flip_sign<CT>(raw[4 * i + 2 * k]), u1 = flip_sign<CT>(raw[4 * i + 2 * k + 1]);
-                        st.k[st.k_at(row, unit + k)] =
-                            make_uint4(codes2<CT, 0>(u0), codes2<CT, 1>(u0), codes2<CT, 0>(u1), codes2<CT, 1>(u1));
-                    }
-                }
+                st.k[st.k_at(piece / KN, piece % KN)] = make_uint4(raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
             }
         if (does_v) {
             uint32_t *vr = raw + VAT;
-            if constexpr (CT == LLM_BF16) {
-                if (step * 64 + 64 > p.len) { // values that are not finite among the new tokens: see k_tree_attention
+            if (step * 64 + 64 > p.len) { // values that are not finite among the new tokens: see k_tree_attention
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int at = step * 64 + (int)(32 * (vu / 4) + 4 * (vu % 4)) + 16 * (i / 4) + i % 4 - p.len;
-                        bool nf = false;
+                for (int i = 0; i < 8; i++) {
+                    const int at = step * 64 + (int)(32 * (vu / 4) + 4 * (vu % 4)) + 16 * (i / 4) + i % 4 - p.len;
+                    bool nf = false;
 #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const uint32_t u = vr[2 * i + k];
-                            nf |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
-                        }
-                        if (nf && at >= 0) { // (the row's other values may stay: who sees them becomes NaN)
-                            atomicOr(&sm_bad[at / 32], 1u << (at % 32));
-                            vr[2 * i] = vr[2 * i + 1] = 0;
-                        }
+                    for (int k = 0; k < 2; k++) {
+                        const uint32_t u = vr[2 * i + k];
+                        nf |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
+                    }
+                    if (nf && at >= 0) { // (the row's other values may stay: who sees them becomes NaN)
+                        atomicOr(&sm_bad[at / 32], 1u << (at % 32));
+                        vr[2 * i] = vr[2 * i + 1] = 0;
                     }
                 }
             }
             u32x4 w[4];
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                if constexpr (CT == LLM_BF16) {
+            for (int i = 0; i < 8; i += 2)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        w[e][i / 2] = __builtin_amdgcn_perm(vr[2 * i + 2 + e / 2], vr[2 * i + e / 2], e % 2 ? 0x07060302 : 0x05040100);
-                } else {
-                    uint32_t q[4];
-                    pairs2<CT, 0>(vr[i], vr[i + 1], q);
-                    pairs2<CT, 1>(vr[i], vr[i + 1], q + 2);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w[e][i / 2] = q[e];
-                }
-            }
+                for (int e = 0; e < 4; e++)
+                    w[e][i / 2] = __builtin_amdgcn_perm(vr[2 * i + 2 + e / 2], vr[2 * i + e / 2], e % 2 ? 0x07060302 : 0x05040100);
 #pragma unroll
             for (int e = 0; e < 4; e++) st.v[st.v_at(4 * vc + e, vu)] = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
         }
-        if constexpr (SCALED)
-            if (wave < 2) {
-                float s = __uint_as_float(sr);
-                if (wave) {
-                    next_e = max(next_e, exponent(wave_max(s < INFINITY ? s : 0.0f)));
-                    s *= power_to(next_e);
-                    if (lane == 0) st.e = next_e;
-                }
-                st.s[wave][lane] = s;
-            }
     };
 
     load();
@@ -805,13 +838,12 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
     f32x4 o[R][DT];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        cq[r] = load_queries<CT, QT, true>(a, p, row0 + 16 * r + n, qf[r], sees[r]);
+        cq[r] = load_queries<CT, QT>(a, p, row0 + 16 * r + n, qf[r], sees[r]);
         m[r] = -INFINITY;
         l[r] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++) o[r][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    uint32_t ve = 20;
     __syncthreads();
     store(p.first, sm[0]);
     load();
@@ -821,12 +853,6 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
         const TreeStep &st = sm[(step - p.first) & 1];
         if (works) {
             const bool edge = step * 64 + 64 > p.len;
-            float oe = 1.0f;
-            if constexpr (SCALED) {
-                const uint32_t e1 = __builtin_amdgcn_readfirstlane(st.e);
-                if (ve != e1) oe = power_from(ve) * power_to(e1);
-                ve = e1;
-            }
 #pragma unroll 1
             for (int u = 0; u < 2; u++) { // 32 positions
                 const int n = again(threadIdx.x & 15), j = again(threadIdx.x & 63) >> 4;
@@ -844,21 +870,12 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
 #pragma unroll
                         for (int r = 0; r < R; r++) x[r][t] = product(kf, qf[r][s], x[r][t]);
                     }
-                if constexpr (SCALED)
-#pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        const f32x4 sk = *(const f32x4 *)&st.s[0][32 * u + 16 * t + 4 * j];
-#pragma unroll
-                        for (int r = 0; r < R; r++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) x[r][t][i] *= sk[i];
-                    }
                 Frag<CT, Pc::P> pf[R][1];
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     uint32_t vis = 0;
                     if (edge) vis = seen_bits<8>(p, step * 64 + 32 * u, sees[r]);
-                    weights(x[r], cq[r], &st.s[1][32 * u + 4 * j], edge, vis, u ? 1.0f : oe, m[r], l[r], o[r], pf[r]);
+                    weights(x[r], cq[r], nullptr, edge, vis, 1.0f, m[r], l[r], o[r], pf[r]);
                 }
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
@@ -878,9 +895,9 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
     for (int r = 0; r < R; r++) {
         const int row = row0 + 16 * r + n;
         l[r] = over_groups(l[r], fadd_);
-        if (CT == LLM_BF16 && (sees[r] & ((uint64_t)sm_bad[1] << 32 | sm_bad[0]))) l[r] = NAN;
+        if (sees[r] & ((uint64_t)sm_bad[1] << 32 | sm_bad[0])) l[r] = NAN;
         if (row >= p.rows) continue;
-        const float il = to_output(p, l[r]) * (SCALED ? power_from(ve) : 1.0f);
+        const float il = to_output(p, l[r]);
         if (p.slices > 1 && j == 0) put_sums(a, p, row, m[r], l[r]);
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -896,23 +913,20 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
 #define TREE_NAME(n) TREE_NAME2(n)
 
 TreeKernel TREE_NAME(TREE_HSP)(int type, int q_type, int tiles, int many, size_t *lds) {
-#define TREE_PICK(C, Q, T)                                \
+#define TREE_PICK(C, Q, T)                                 \
     if (!many && type == C && q_type == Q && tiles == T) { \
-        *lds = TreeShape<C, Q, T>::LDS;                   \
-        return k_tree_attention<C, Q, T>;                 \
+        *lds = TreeShape<C, Q, T>::LDS;                    \
+        return k_tree_attention<C, Q, T>;                  \
     }
 #define TREE_PICK_Q(C, T) TREE_PICK(C, LLM_F32, T) TREE_PICK(C, LLM_BF16, T)
     TREE_PICK_Q(LLM_F32, 1) TREE_PICK_Q(LLM_BF16, 1) TREE_PICK_Q(LLM_I8, 1) TREE_PICK_Q(LLM_E4M3, 1)
 #if TREE_HSP <= 128
-    TREE_PICK_Q(LLM_F32, 2) TREE_PICK_Q(LLM_BF16, 2) TREE_PICK_Q(LLM_I8, 2) TREE_PICK_Q(LLM_E4M3, 2)
-#define TREE_PICK_M(C, Q, W, T)                                          \
-    if (many == W && tiles == T && type == C && q_type == Q) {           \
-        *lds = 0;                                                        \
-        return k_tree_rows<C, Q, W, T>;                                  \
-    }
-#define TREE_PICK_MQ(C, W, T) TREE_PICK_M(C, LLM_F32, W, T) TREE_PICK_M(C, LLM_BF16, W, T)
-    TREE_PICK_MQ(LLM_BF16, 4, 1) TREE_PICK_MQ(LLM_I8, 4, 1) TREE_PICK_MQ(LLM_E4M3, 4, 1)
-    TREE_PICK_M(LLM_BF16, LLM_F32, 4, 2) TREE_PICK_M(LLM_BF16, LLM_BF16, 8, 1) TREE_PICK_MQ(LLM_I8, 8, 1) TREE_PICK_MQ(LLM_E4M3, 8, 1)
+    TREE_PICK_Q(LLM_I8, 2) TREE_PICK_Q(LLM_E4M3, 2) TREE_PICK(LLM_BF16, LLM_BF16, 2)
+#endif
+#if TREE_HSP == 128
+    *lds = 0;
+    if (many == 8 && tiles == 1 && type == LLM_BF16 && q_type == LLM_BF16) return k_tree_rows<LLM_BF16, 8, 1>;
+    if (many == 4 && tiles == 2 && type == LLM_BF16 && q_type == LLM_F32) return k_tree_rows<LLM_F32, 4, 2>;
 #endif
     return nullptr;
 }
