@@ -33,6 +33,9 @@ __host__ __device__ constexpr int tree_positions(int hsp, int type, int many, in
 }
 constexpr int TREE_MAX_SLICES = 128; // of a sequence's kv head
 constexpr int TREE_MAX_SEQS = 512;   // of a call whose positions are cut
+// A sequence of so many times the least steps stays whole: cutting it costs the join (7 rows over 300 int8 positions: 11.0 us
+// whole, 12.4 in two slices; over 800, four times the least: 14.8 and 12.4).
+constexpr int TREE_WHOLE = 3;
 
 // Steps of a sequence: of its positions in the cache and its new tokens (at least one: its block writes the empty rows).
 __device__ __forceinline__ int tree_steps(const TreeArgs &a, int seq) {
@@ -41,7 +44,7 @@ __device__ __forceinline__ int tree_steps(const TreeArgs &a, int seq) {
 }
 // Slices of the only sequence of a call, of `all` steps: head h has numbers h * each and on.
 __device__ __forceinline__ int tree_one(const TreeArgs &a, int all, int &steps) {
-    steps = max(a.least, (all + a.each - 1) / a.each);
+    steps = all <= TREE_WHOLE * a.least ? all : max(a.least, (all + a.each - 1) / a.each);
     return (all + steps - 1) / steps;
 }
 

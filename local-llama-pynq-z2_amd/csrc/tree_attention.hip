@@ -139,7 +139,7 @@ TreePlan tree_plan(const llm_kv *c, int q_type, int n_heads, int max_n, int max_
         each = std::min({cap / c->n_kv, (steps + p.least - 1) / p.least, each});
         cap = each * c->n_kv;
     }
-    p.cap = cap <= heads || c->n_seq > TREE_MAX_SEQS || steps <= p.least ? 0 : (int)cap;
+    p.cap = cap <= heads || c->n_seq > TREE_MAX_SEQS || steps <= TREE_WHOLE * p.least ? 0 : (int)cap;
     p.each = (int)each;
     p.bytes = p.cap ? (size_t)p.cap * rows * (c->hs + 2) * 4 + heads * sizeof(int2) : 0;
     return p;

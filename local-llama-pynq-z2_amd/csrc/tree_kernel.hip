@@ -194,7 +194,8 @@ __device__ __forceinline__ bool find_slice(const TreeArgs &a, uint32_t id, Place
     }
     const float kv = (float)a.n_kv;
     const int guess = __builtin_amdgcn_readfirstlane((int)(wave_sum(sum) * kv / (float)a.cap));
-    steps = max(max(a.least, guess), __builtin_amdgcn_readfirstlane((int)wave_max(most)) / a.each + 1);
+    const int longest = __builtin_amdgcn_readfirstlane((int)wave_max(most));
+    steps = longest <= TREE_WHOLE * a.least ? longest : max(max(a.least, guess), longest / a.each + 1);
     int n[GROUPS];
     for (;; steps += (steps + 15) / 16) { // (ends: at the longest sequence's steps there is a slice a head)
         float total = 0.0f;
