@@ -3,7 +3,8 @@
 The library is C (include/matvec_fpga.h: the reference's six-function driver API; include/llm_hip.h: the
 device-resident token loop).  These bindings are what the Python tests and bench.py call; the C hosts in
 host/ and the reference's own hosts link the library directly.  Nothing here computes: every call goes
-through the C ABI, and loading fails loudly when the built library is missing.
+through the C ABI, and loading fails loudly when the built library is missing.  The operators on device memory
+(kv_write, kv_read, tree_attention, logprobs) take torch tensors; torch is imported by their first call.
 
 The directory name is not a Python identifier, so callers load this file by path, e.g.
     spec = importlib.util.spec_from_file_location("llm_hip", ".../local-llama-pynq-z2_amd/__init__.py")

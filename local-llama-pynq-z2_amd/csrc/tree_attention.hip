@@ -106,7 +106,7 @@ struct TreePlan {
 // with two; over 700: 10.8 and 13.7.  448 rows over 8 x 4000 int8 positions: 113 and 91; 63 rows over 32 x 2000: 39 and 41).
 // Not for fp32 caches, nor fp32 queries over bf16 ones (three pieces), whose registers leave one wave a SIMD.  Many rows over
 // a bf16 cache, whose L2 traffic then bounds: the waves share the rows, and the cache's rows go through LDS (eight
-// sequences of up to 16k positions, 448 rows: 186 us this way or with two tiles, 144 with LDS; one of 700: 14 and 18).  fp32
+// sequences of up to 16k positions, 448 rows: 186 us with two tiles, 144 with LDS; one sequence of 700: 14 and 18).  fp32
 // queries take two tiles in each of four waves there (eight waves of one would spill), bf16 ones one in each of eight.  The
 // rows are spread evenly over these blocks.
 // Positions.  One sequence: as many slices as give a block a CU, or two a CU where whole row blocks would leave much of the
