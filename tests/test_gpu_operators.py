@@ -275,6 +275,61 @@ def test_attention_over_many_slices(cache, heads, h, hs):
     assert float((a - b).abs().max()) < 1e-4
 
 
+def roomy_case(cache, rows, b, heads, h, hs, ctx, lens, t, n=None, max_len=None, seed=0):
+    """a cache of ctx positions whose bound the lengths stay far below (max_len None: the cache's): rows as of a long
+    context, checked over the positions that hold something; all others hold infinities and NaN"""
+    g = gen(hs + t + seed)
+    top = max(lens) + t
+    k, v, ks, vs = cache_tensors(cache, b, h, ctx, hs, "heads", math.nan)
+    vals = []
+    for store, sc in ((k, ks), (v, vs)):
+        x = torch.randn(b, h, top, hs, generator=g) * torch.exp(torch.randn(b, h, top, 1, generator=g))
+        val, code, s = quantized(x.double(), cache)
+        nn = [t] * b if n is None else n
+        for i in range(b):
+            end = lens[i] + nn[i]
+            store[i, :, :end] = code[i, :, :end].float().to(CACHES[cache]).to(DEV)
+            if s is not None:
+                sc[i, :, :end] = s[i, :, :end].to(DEV)
+        vals.append(val)
+    q = torch.randn(b, t, heads, hs, generator=g).to(ROWS[rows])
+    mask = tree_masks(g, b, t)
+    it = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    got = pkg().tree_attention(q.to(DEV), k, v, it(lens), None if n is None else it(n),
+                               torch.from_numpy(mask.view(np.int64)).to(DEV), k_scale=ks, v_scale=vs, max_len=max_len)
+    attention_check(q, vals[0], vals[1], lens, nn, mask, hs ** -0.5, got, ctx, cache)
+
+
+@pytest.mark.parametrize("cache,rows,b,heads,h,hs,ctx,t", [
+    ("bf16", "bf16", 1, 28, 4, 128, 30000, 37), ("bf16", "fp32", 1, 28, 4, 128, 12000, 37),
+    ("bf16", "bf16", 2, 12, 1, 96, 21000, 64), ("bf16", "fp32", 3, 20, 2, 112, 7000, 19),
+    ("bf16", "bf16", 1, 28, 4, 128, 16000, 8), ("bf16", "bf16", 1, 14, 2, 64, 32000, 7),
+    ("int8", "fp32", 1, 28, 4, 128, 12000, 37), ("int8", "bf16", 2, 28, 4, 128, 9000, 15),
+    ("e4m3", "fp32", 3, 28, 4, 112, 4500, 37), ("e4m3", "bf16", 1, 28, 4, 128, 12000, 64),
+    ("int8", "fp32", 3, 14, 2, 64, 16000, 37), ("fp32", "fp32", 1, 28, 4, 128, 9000, 37)])
+@pytest.mark.parametrize("length", [0, 95, 1500])
+def test_attention_of_many_rows(cache, rows, b, heads, h, hs, ctx, t, length):
+    """the cuts of calls with many rows and a large bound, over empty, short and sliced contexts"""
+    roomy_case(cache, rows, b, heads, h, hs, ctx, [length, 64, 7][:b], t, None if b == 1 else [t, t - 3, 1][:b])
+
+
+@pytest.mark.parametrize("cache,rows", [("int8", "fp32"), ("e4m3", "bf16"), ("bf16", "bf16"), ("fp32", "fp32")])
+@pytest.mark.parametrize("b,h,longest", [(2, 1, 40000), (3, 2, 9000), (63, 1, 2500), (64, 3, 1700), (65, 1, 2500),
+                                         (130, 1, 900), (300, 1, 700), (511, 1, 300), (512, 1, 300), (513, 1, 300)])
+def test_attention_of_uneven_batches(cache, rows, b, h, longest):
+    """one long sequence, one of every other length down to none: slices of equal steps over all of them"""
+    lens = [longest if i == b // 2 else (i * 37) % 301 for i in range(b)]
+    roomy_case(cache, rows, b, 2 * h, h, 16, longest + 70, lens, 2, [1 + i % 2 for i in range(b)])
+
+
+def test_attention_of_a_batch_above_its_bound():
+    """a bound of the lengths that is too low costs time, not results"""
+    for b, longest in ((3, 9000), (70, 3000)):
+        lens = [longest if i == 1 else 11 * (i % 9) for i in range(b)]
+        for max_len in (0, 13, 900):
+            roomy_case("int8", "fp32", b, 2, 1, 32, longest + 5, lens, 2, max_len=max_len)
+
+
 def test_attention_chain_is_the_default_mask():
     g = gen(5)
     b, t, heads, h, hs, ctx = 2, 9, 4, 2, 64, 100

@@ -80,7 +80,7 @@ def test_work_sizes():
     assert L.llm_tree_attention_work(C.byref(c), 3, 1, 100) == 0
     assert L.llm_tree_attention_work(C.byref(c), 4, 1, 100) == 0  # one slice
     b = L.llm_tree_attention_work(C.byref(c), 4, 1, 32767)
-    assert b and b % ((64 + 2) * 4 * 2 * 2) == 0
+    assert b >= 2 * 2 * (64 + 2) * 4 and b % 8 == 0  # at least a slice for each kv head
     assert L.llm_logprobs_work(1000, 151936, 20) == 0
     assert L.llm_logprobs_work(1, 65536, 20) > 0
 
