@@ -1844,7 +1844,7 @@ extern "C" int llm_verify(llm_model *m, int pos0, const int *tokens, const int *
         fprintf(stderr, "%s: bad arguments (1 to 64 tokens)\n", who);
         return -1;
     }
-    if (pos0 + n > m->ctx) {
+    if (pos0 > m->ctx - n) {
         fprintf(stderr, "%s: %d tokens from position %d do not fit the context %d\n", who, n, pos0, m->ctx);
         return -1;
     }
@@ -1918,7 +1918,7 @@ extern "C" int llm_verify(llm_model *m, int pos0, const int *tokens, const int *
 }
 
 extern "C" int llm_keep(llm_model *m, int pos0, const int *path, int n) {
-    if (!m || !path || n < 1 || n > 64 || pos0 < 0 || pos0 + path[n - 1] >= m->ctx) {
+    if (!m || !path || n < 1 || n > 64 || pos0 < 0) {
         fprintf(stderr, "llm_keep: bad arguments\n");
         return -1;
     }
@@ -1929,6 +1929,10 @@ extern "C" int llm_keep(llm_model *m, int pos0, const int *path, int n) {
             return -1;
         }
         p[i] = (uint8_t)path[i];
+    }
+    if (pos0 >= m->ctx - path[n - 1]) {
+        fprintf(stderr, "llm_keep: token %d from position %d is behind the context %d\n", path[n - 1], pos0, m->ctx);
+        return -1;
     }
     hipSetDevice(m->device);
     HIP_OR_FAIL("llm_keep", launch_kv_keep(layer_cache(m, 0, m->info.n_layers), pos0, p, n, m->st));

@@ -1041,7 +1041,8 @@ __global__ void __launch_bounds__(1024) k_p_norm_quant(ProwArgs a) {
 // QKV rows of token m: bias (qwen.c:521-522), RoPE at position p0 + m (qwen.c:478-488 NeoX pairs; runq.c:506-521
 // interleaved pairs), q to q[m], k and v into the caches.  Logical rows follow the fused matrix's order.
 __global__ void __launch_bounds__(256) k_p_qkv(ProwArgs a) {
-    const int m = blockIdx.x, pos = a.p0 + m, rp = a.depth ? a.p0 + a.depth[m] : pos, dim = a.dim, kvd = a.kv_dim, hs = a.head_size, half = hs / 2;
+    const int m = blockIdx.x, pos = a.p0 + m, dim = a.dim, kvd = a.kv_dim, hs = a.head_size, half = hs / 2;
+    const int rp = a.depth ? a.p0 + a.depth[m] : pos; // of RoPE
     const int rows = dim + 2 * kvd;
     const float *y = a.y + (size_t)m * rows;
     for (int R = threadIdx.x; R < rows; R += blockDim.x) {

@@ -119,15 +119,16 @@ TreePlan tree_plan(const llm_kv *c, int q_type, int n_heads, int max_n, int max_
     const int group = n_heads / c->n_kv, rows = group * max_n, tiles = (rows + 15) / 16;
     const int64_t end = std::min<int64_t>((int64_t)std::max(max_len, 0) + max_n, c->ctx), heads = (int64_t)c->n_seq * c->n_kv;
     const bool bf16 = c->type == LLM_BF16, pieces = bf16 && q_type == LLM_F32, small = p.hsp <= 128;
-    const int64_t work = tiles * heads * end;
-    const bool many = bf16 && p.hsp == 128 && tiles > 8 && work >= (pieces ? 800000 : 2000000);
+    const double work = (double)tiles * heads * end;
+    const bool many = bf16 && p.hsp == 128 && tiles > 8 && work >= (pieces ? 8e5 : 2e6);
     p.many = !many ? 0 : pieces ? 4 : 8;
     const bool two = small && c->type != LLM_F32 && !pieces &&
-                     (bf16 ? tiles > 2 && work >= 250000 : tiles > 5 && work * p.hsp >= 100000000);
+                     (bf16 ? tiles > 2 && work >= 2.5e5 : tiles > 5 && work * p.hsp >= 1e8);
     p.tiles = many ? (pieces ? 2 : 1) : two ? 2 : 1;
     const int per_block = p.tiles * (many ? p.many : 1); // tiles
     p.row_blocks = (tiles + per_block - 1) / per_block;
-    p.block_rows = 16 * (many ? (tiles + p.row_blocks - 1) / p.row_blocks : per_block);
+    const int waves = (tiles + p.row_blocks * p.tiles - 1) / (p.row_blocks * p.tiles); // that have rows
+    p.block_rows = 16 * (many ? waves * p.tiles : per_block);
     p.tp = tree_positions(p.hsp, c->type, p.many, p.tiles);
     const int64_t steps = std::max<int64_t>((end + p.tp - 1) / p.tp, 1);
     p.least = many ? 2 : 4; // steps of a slice (few rows: one a wave)

@@ -170,6 +170,20 @@ def test_drafts_at_the_end_of_the_context_and_refusals(capfd):
     m.close()
 
 
+def test_positions_far_outside_are_refused():
+    m = pkg().Model(TINY[0], 64)
+    far = 2 ** 31 - 1
+    for pos0, ids in ((far, [5, 6]), (far - 1, [5]), (64, [5]), (63, [5, 6])):
+        with pytest.raises(RuntimeError):
+            m.verify(pos0, ids)
+    for pos0, path in ((far, [0, 1]), (0, [0, far]), (64, [0]), (63, [0, 1]), (60, [0, 4]), (far - 2, [5, 63])):
+        with pytest.raises(RuntimeError):
+            m.keep(pos0, path)
+    m.verify(62, [5, 6])
+    m.keep(62, [1])
+    m.close()
+
+
 def test_first_scores_of_a_model():
     """a model's first call allocates the buffers (zeroed, on another stream than the tokens come by): it scores as the next"""
     for _ in range(60):

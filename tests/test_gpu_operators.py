@@ -303,6 +303,7 @@ def roomy_case(cache, rows, b, heads, h, hs, ctx, lens, t, n=None, max_len=None,
 @pytest.mark.parametrize("cache,rows,b,heads,h,hs,ctx,t", [
     ("bf16", "bf16", 1, 28, 4, 128, 30000, 37), ("bf16", "fp32", 1, 28, 4, 128, 12000, 37),
     ("bf16", "bf16", 2, 12, 1, 96, 21000, 64), ("bf16", "fp32", 3, 20, 2, 112, 7000, 19),
+    ("bf16", "fp32", 1, 28, 4, 128, 23000, 20), ("bf16", "bf16", 1, 28, 4, 128, 60000, 20),
     ("bf16", "bf16", 1, 28, 4, 128, 16000, 8), ("bf16", "bf16", 1, 14, 2, 64, 32000, 7),
     ("int8", "fp32", 1, 28, 4, 128, 12000, 37), ("int8", "bf16", 2, 28, 4, 128, 9000, 15),
     ("e4m3", "fp32", 3, 28, 4, 112, 4500, 37), ("e4m3", "bf16", 1, 28, 4, 128, 12000, 64),
