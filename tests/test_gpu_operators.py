@@ -323,6 +323,34 @@ def test_attention_of_uneven_batches(cache, rows, b, h, longest):
     roomy_case(cache, rows, b, 2 * h, h, 16, longest + 70, lens, 2, [1 + i % 2 for i in range(b)])
 
 
+@pytest.mark.parametrize("cache,rows", [("int8", "fp32"), ("fp32", "bf16")])
+def test_attention_of_the_most_rows(cache, rows):
+    roomy_case(cache, rows, 2, 64, 1, 16, 700, [130, 3], 64, [64, 2])
+
+
+@pytest.mark.parametrize("seq,head,pos", [(1 << 32, 64 * 300, 64), (64 * 400, 1 << 32, 64), (64, 128, 1 << 24)])
+def test_offsets_past_32_bits(seq, head, pos):
+    """sequences, heads or positions more than 4 GiB apart: the same as a small cache"""
+    P, g = pkg(), gen(8)
+    b, h, ctx, hs, t = (2, 2, 300, 64, 3) if pos == 64 else (1, 2, 300, 64, 3)
+    big = torch.zeros(((b - 1) * seq + (h - 1) * head + ctx * pos) + (1 << 20), dtype=torch.int8, device=DEV)
+    far = [big[o:].as_strided((b, h, ctx, hs), (seq, head, pos, 1)) for o in (0, 1 << 19)]
+    near = [torch.zeros(b, h, ctx, hs, dtype=torch.int8, device=DEV) for _ in range(2)]
+    rows = [torch.randn(b, 290, h, hs, generator=g).to(DEV) for _ in range(2)]
+    q = torch.randn(b, t, 4 * h, hs, generator=g).to(DEV)
+    at = torch.tensor([5, 10][:b], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([292, 100][:b], dtype=torch.int32, device=DEV)
+    got = []
+    for k, v in (far, near):
+        ks, vs = (torch.zeros(b, h, ctx, device=DEV) for _ in range(2))
+        P.kv_write(rows[0], rows[1], k, v, at, k_scale=ks, v_scale=vs)
+        got.append((k.clone(), v.clone(), ks, vs) + P.kv_read(k, v, at, 280, k_scale=ks, v_scale=vs) +
+                   (P.tree_attention(q, k, v, lens, k_scale=ks, v_scale=vs),))
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    assert bool((got[0][0] != 0).any()) and bool((got[0][6] != 0).any())
+
+
 def test_attention_of_a_batch_above_its_bound():
     """a bound of the lengths that is too low costs time, not results"""
     for b, longest in ((3, 9000), (70, 3000)):
