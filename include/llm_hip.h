@@ -213,21 +213,22 @@ int llm_kv_read(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int
  * bit j is set in mask[b * max_n + i] (a drafted tree: its ancestors and itself; mask NULL: j <= i, a chain; max_n 1: the
  * decode step).  out[b][i][h] = sum_p softmax_p(scale q.k_p) v_p over the kv head h / (n_heads / n_kv), in fp32, rounded to
  * out's type (q's type).  A token that sees nothing gets zeros.  Rows behind n[b] are left as they were, or zeroed
- * (zero_rest); positions from ctx on are not seen.  What is not seen has no influence, infinities and NaN included; a new token whose V row holds one makes
- * the tokens that see it NaN.  n_heads / n_kv is at most 64.  max_len is the host's upper bound of lens[] (lens above it
- * are right too, slower); `work` has llm_tree_attention_work() bytes, 16-byte aligned. */
+ * (zero_rest); positions from ctx on are not seen.  What is not seen has no influence, infinities and NaN included; a new
+ * token whose V row holds one makes the tokens that see it NaN.  n_heads / n_kv is at most 64.  max_len is the host's upper
+ * bound of lens[] (lens above it are right too, slower); `work` has llm_tree_attention_work() bytes, 16-byte aligned, and is
+ * one call's until it has run. */
 size_t llm_tree_attention_work(const llm_kv *c, int n_heads, int max_n, int max_len);
 int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_rows *out, int n_heads, const int *lens, const int *n,
                        const uint64_t *mask, int max_n, int max_len, float scale, int zero_rest, void *work,
                        size_t work_bytes, void *stream);
 
 /* Log probabilities over `rows` rows of `vocab` logits (type LLM_F32 or LLM_BF16, `stride` values from row to row), of
- * y = logit / temperature (1e-30 to 1e30): lse = log sum exp y, entropy = -sum p log p (nats), logp[r][i] = y[tokens[r][i]] - lse for
- * n_tokens tokens a row (an id outside 0 .. vocab - 1: -infinity), and the `top` <= 32 largest logits of the row in
- * descending order (equal ones, and NaN, which count as the largest: lowest index first) with their log probabilities.
+ * y = logit / temperature (1e-30 to 1e30): lse = log sum exp y, entropy = -sum p log p (nats), logp[r][i] =
+ * y[tokens[r][i]] - lse for n_tokens tokens a row (an id outside 0 .. vocab - 1: -infinity), and the `top` <= 32 largest
+ * logits of the row in descending order (equal ones, and NaN, which count as the largest: lowest index first) with their log probabilities.
  * Masked logits of -infinity have probability 0.  A row with +infinity or NaN, or of -infinity alone, has NaN for its
- * results (lse of -infinity alone: -infinity).  entropy and lse may be NULL, logp with n_tokens 0 and the two top arrays with top 0.  `work` has
- * llm_logprobs_work() bytes, 16-byte aligned. */
+ * results (lse of -infinity alone: -infinity).  entropy and lse may be NULL, logp with n_tokens 0 and the two
+ * top arrays with top 0.  `work` has llm_logprobs_work() bytes, 16-byte aligned, and is one call's until it has run. */
 size_t llm_logprobs_work(int rows, int vocab, int top);
 int llm_logprobs(const void *logits, int type, int rows, int vocab, int64_t stride, float temperature, const int *tokens,
                  int n_tokens, float *logp, float *entropy, float *lse, int top, int *top_ids, float *top_logp, void *work,

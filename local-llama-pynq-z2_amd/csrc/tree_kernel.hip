@@ -207,7 +207,7 @@ __device__ __forceinline__ bool find_slice(const TreeArgs &a, uint32_t id, Place
                 total += (float)n[i];
             }
         }
-        if (__builtin_amdgcn_readfirstlane((int)wave_sum(total)) * kv <= (float)a.cap) break; // (exact up to 2^24)
+        if (wave_sum(total) * kv <= (float)a.cap) break; // (exact up to 2^24)
     }
     int before = 0; // slices of a head of the sequences before
 #pragma unroll
@@ -251,7 +251,8 @@ __device__ __forceinline__ bool place(const TreeArgs &a, int block_rows, Place &
     }
     p.id = (int)id;
     const int row0 = (int)(k - kr * a.row_blocks) * block_rows;
-    if (a.cap && a.n_seq > 1 && p.split == 0 && row0 == 0 && threadIdx.x == 0) a.plan[p.b * a.n_kv + p.h] = make_int2((int)id, p.slices);
+    if (a.cap && a.n_seq > 1 && p.split == 0 && row0 == 0 && threadIdx.x == 0) // (for the join)
+        a.plan[p.b * a.n_kv + p.h] = make_int2((int)id, p.slices);
     p.row0 = row0;
     p.len = min(max(a.lens[p.b], 0), a.ctx);
     const int nn = a.n ? min(max(a.n[p.b], 0), a.max_n) : a.max_n;
@@ -337,8 +338,8 @@ __device__ __forceinline__ uint32_t seen_bits(const Place &p, int p0, uint64_t s
 }
 
 // A step's scores x (with the K scales, if any) into the weights of its values: the running maximum m (exponents of 2) and
-// sum l of the row; `sv` (in LDS) the V scales times their common power, at 16 t + i; o and l are rescaled when the maximum or, by `oe`, that
-// power has moved.
+// sum l of the row; `sv` (in LDS) the V scales times their common power, at 16 t + i; o and l are rescaled when the maximum
+// or, by `oe`, that power has moved.
 template <int NT, int CT, int NPP, int DT>
 __device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *sv, bool edge, uint32_t vis, float oe,
                                         float &m, float &l, f32x4 (&o)[DT], Frag<CT, NPP> (&pf)[NT / 2]) {
@@ -542,7 +543,8 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
                 } else if constexpr (CT == LLM_BF16) {
                     kf.v[0] = kr[t][s];
                 } else {
-                    const uint32_t u0 = flip_sign<CT>(kr[t][s / 2][2 * (s % 2)]), u1 = flip_sign<CT>(kr[t][s / 2][2 * (s % 2) + 1]);
+                    const uint32_t u0 = flip_sign<CT>(kr[t][s / 2][2 * (s % 2)]);
+                    const uint32_t u1 = flip_sign<CT>(kr[t][s / 2][2 * (s % 2) + 1]);
                     kf.v[0] = (u32x4){codes2<CT, 0>(u0), codes2<CT, 1>(u0), codes2<CT, 0>(u1), codes2<CT, 1>(u1)};
                 }
 #pragma unroll
@@ -735,7 +737,8 @@ struct __align__(16) TreeStep {
 // registers for four waves a SIMD at R = 1, which hide each other's LDS and product latencies.  A step of 64 positions is
 // in LDS while the next one's loads are under way: one barrier a step.  LDS bounds it: 16 waves a CU read each step's 32 KB,
 // 4096 cycles at 128 bytes a cycle, of about 5500 (448 rows over eight sequences of 0 to 16k positions, 4 kv heads of 128: 125
-// us, 346 TFLOP/s, 520 of issued products.  Two tiles in each of four waves read half, with two waves a SIMD: 144 a call against 128).
+// us, 346 TFLOP/s, 520 of issued products.  Two tiles in each of four waves read half, with two waves a SIMD: 144 a call
+// against 128).
 template <int QT, int NW, int R>
 __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs a) {
     constexpr int CT = LLM_BF16;
