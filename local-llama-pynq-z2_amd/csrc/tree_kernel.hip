@@ -339,7 +339,9 @@ __device__ __forceinline__ uint32_t seen_bits(const Place &p, int p0, uint64_t s
 
 // A step's scores x (with the K scales, if any) into the weights of its values: the running maximum m (exponents of 2) and
 // sum l of the row; `sv` (in LDS) the V scales times their common power, at 16 t + i; o and l are rescaled when the maximum
-// or, by `oe`, that power has moved.
+// or, by `oe`, that power has moved.  fp32 and bf16 weights have the exponents to go on with an old maximum until it is
+// passed by a factor of 2^8 (a batch of 64-token trees over bf16: 144 us with every new maximum, 139 so); the fp16 pieces'
+// range is used up.
 template <int NT, int CT, int NPP, int DT>
 __device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *sv, bool edge, uint32_t vis, float oe,
                                         float &m, float &l, f32x4 (&o)[DT], Frag<CT, NPP> (&pf)[NT / 2]) {
@@ -355,8 +357,11 @@ __device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *s
 #pragma unroll
         for (int i = 0; i < 4; i++) mx = fmaxf(mx, x[t][i]);
     mx = over_groups(mx, fmax_);
-    const float mn = fmaxf(m, mx * cq), mu = mn == -INFINITY ? 0.0f : mn;
-    if (__any(mn > m || oe != 1.0f)) {
+    const float mn = fmaxf(m, mx * cq);
+    float mu = m == -INFINITY ? 0.0f : m;
+    constexpr float SLACK = SCALED ? 0.0f : 8.0f;
+    if (__any(mn > m + SLACK || oe != 1.0f)) {
+        mu = mn == -INFINITY ? 0.0f : mn;
         const float al = __builtin_amdgcn_exp2f(m - mu), ao = al * oe;
         l *= al;
 #pragma unroll
