@@ -323,6 +323,33 @@ def test_attention_of_uneven_batches(cache, rows, b, h, longest):
     roomy_case(cache, rows, b, 2 * h, h, 16, longest + 70, lens, 2, [1 + i % 2 for i in range(b)])
 
 
+@pytest.mark.parametrize("cache,rows", [("fp32", "fp32"), ("bf16", "fp32"), ("bf16", "bf16"), ("int8", "fp32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("slope", [-0.05, 0.002, 0.05, 0.4])
+@pytest.mark.parametrize("t,heads,ctx", [(1, 2, 800), (40, 28, 30000)])
+def test_attention_of_scores_that_rise(cache, rows, slope, t, heads, ctx):
+    """every position's score above (below) the one before: a new maximum at every step, by little or by much"""
+    g = gen(9)
+    h, hs, length = 1, 128, 700
+    top = length + t
+    p = torch.arange(top).double() * slope
+    x = [torch.randn(1, h, top, hs, generator=g).double() * 0.1 for _ in range(2)]
+    u = torch.randn(hs, generator=g).double()
+    x[0] += p.view(1, 1, top, 1) * u * hs ** 0.5 / (u @ u)  # score slope * position, and noise
+    q = (u + 0.02 * torch.randn(1, t, heads, hs, generator=g).double()).float().to(ROWS[rows])
+    k, v, ks, vs = cache_tensors(cache, 1, h, ctx, hs, "heads", math.nan)
+    vals = []
+    for y, store, sc in ((x[0], k, ks), (x[1], v, vs)):
+        val, code, s = quantized(y, cache)
+        store[:, :, :top] = code.float().to(CACHES[cache]).to(DEV)
+        if s is not None:
+            sc[:, :, :top] = s.to(DEV)
+        vals.append(val)
+    mask = tree_masks(g, 1, t)
+    got = pkg().tree_attention(q.to(DEV), k, v, torch.tensor([length], dtype=torch.int32, device=DEV), None,
+                               torch.from_numpy(mask.view(np.int64)).to(DEV), k_scale=ks, v_scale=vs)
+    attention_check(q, vals[0], vals[1], [length], [t], mask, hs ** -0.5, got, ctx, cache)
+
+
 @pytest.mark.parametrize("cache,rows", [("int8", "fp32"), ("fp32", "bf16")])
 def test_attention_of_the_most_rows(cache, rows):
     roomy_case(cache, rows, 2, 64, 1, 16, 700, [130, 3], 64, [64, 2])
