@@ -741,8 +741,8 @@ struct __align__(16) TreeStep {
 // A wave has R tiles of 16 rows and takes them through scores, softmax and values 32 positions at a time: few enough
 // registers for four waves a SIMD at R = 1, which hide each other's LDS and product latencies.  A step of 64 positions is
 // in LDS while the next one's loads are under way: one barrier a step.  LDS bounds it: 16 waves a CU read each step's 32 KB,
-// 4096 cycles at 128 bytes a cycle, of about 5500 (448 rows over eight sequences of 0 to 16k positions, 4 kv heads of 128: 125
-// us, 346 TFLOP/s, 520 of issued products.  Two tiles in each of four waves read half, with two waves a SIMD: 144 a call
+// 4096 cycles at 128 bytes a cycle, of about 5500 (448 rows over eight sequences of 0 to 16k positions, 4 kv heads of 128: 121
+// us, 358 TFLOP/s, 537 of issued products.  Two tiles in each of four waves read half, with two waves a SIMD: 144 a call
 // against 128).
 template <int QT, int NW, int R>
 __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs a) {
