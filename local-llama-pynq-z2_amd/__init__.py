@@ -250,30 +250,38 @@ def _ints(name, t, count, dtype):
 def _kv(k, v, k_scale, v_scale):
     """llm_kv of tensors [seqs, kv heads, positions, head size] (any strides, a row's values together) and, for int8 and
     e4m3, scales [seqs, kv heads, positions]; and its dimensions"""
-    shape, types = k.shape, _types()[1]
-    ty = types.get(k.dtype)
-    if ty is None or v.dtype is not k.dtype or v.shape != shape or len(shape) != 4:
+    torch, types = _torch or _types()
+    shape, dtype, st = k.shape, k.dtype, k.stride()
+    ty = types.get(dtype)
+    if ty is None or v.dtype is not dtype or v.shape != shape or len(shape) != 4:
         raise ValueError("k and v: tensors [seqs, kv heads, positions, head size] of one type (float32, bfloat16, int8, "
                          "float8_e4m3fn) are needed")
     b, h, ctx, hs = shape
     # (a dimension of one has no stride that counts)
-    def strides(s, inner):
-        return s[0] if b > 1 else 0, s[1] if h > 1 else 0, s[2] if ctx > 1 else inner
-    st, sv = k.stride(), v.stride()
-    if st[3] != 1 or sv[3] != 1 or (st != sv and strides(st, hs) != strides(sv, hs)):
+    seq, head, pos, s_seq, s_head, s_pos = st[0] if b > 1 else 0, st[1] if h > 1 else 0, st[2] if ctx > 1 else hs, 0, 0, 1
+    sv = v.stride()
+    if st[3] != 1 or (st != sv and (sv[3] != 1 or (b > 1 and sv[0] != seq) or (h > 1 and sv[1] != head) or
+                                    (ctx > 1 and sv[2] != pos))):
         raise ValueError("k and v: equal strides with a row's values together are needed")
     if ty < 2:
         if k_scale is not None or v_scale is not None:
             raise ValueError("scales belong to int8 and e4m3 caches")
-        return _PACK_KV(k.data_ptr(), v.data_ptr(), 0, 0, ty, b, h, hs, ctx, *strides(st, hs), 0, 0, 1), shape
-    if k_scale is None or v_scale is None or k_scale.shape != shape[:3] or v_scale.shape != shape[:3] or \
-            k_scale.dtype is not _torch[0].float32 or v_scale.dtype is not _torch[0].float32:
+        return _PACK_KV(k.data_ptr(), v.data_ptr(), 0, 0, ty, b, h, hs, ctx, seq, head, pos, s_seq, s_head, s_pos), shape
+    f32, rows = torch.float32, shape[:3]
+    if k_scale is None or v_scale is None or k_scale.shape != rows or v_scale.shape != rows or \
+            k_scale.dtype is not f32 or v_scale.dtype is not f32:
         raise ValueError("an int8 or e4m3 cache needs float32 scales [seqs, kv heads, positions]")
     ss, sv = k_scale.stride(), v_scale.stride()
-    if ss != sv and strides(ss, 1) != strides(sv, 1):
+    if ss != sv and ((b > 1 and ss[0] != sv[0]) or (h > 1 and ss[1] != sv[1]) or (ctx > 1 and ss[2] != sv[2])):
         raise ValueError("k_scale and v_scale: equal strides are needed")
-    return _PACK_KV(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, b, h, hs, ctx,
-                    *strides(st, hs), *strides(ss, 1)), shape
+    if b > 1:
+        s_seq = ss[0]
+    if h > 1:
+        s_head = ss[1]
+    if ctx > 1:
+        s_pos = ss[2]
+    return _PACK_KV(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, b, h, hs, ctx, seq, head, pos,
+                    s_seq, s_head, s_pos), shape
 
 
 def _rows(name, x, b, t, h, hs):
