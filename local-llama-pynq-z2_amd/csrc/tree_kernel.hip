@@ -12,9 +12,10 @@
 //
 // Operands.  int8 and e4m3 codes are exact in fp16, and the fp32 side is held in two fp16 pieces (22 bits): a query row is
 // scaled by a power of two to the top of fp16's range first, and so are the weights p * V scale, by the largest V scale met
-// (a running exponent, as the maximum is running).  bf16 caches: three bf16 pieces.  16-bit queries are one piece; their
-// weights one in fp16 (half a step 2^-11, against the output's 2^-8) and two in bf16.  fp32 caches: v_mfma_f32_16x16x4_f32.
-// Maxima, sums and outputs are fp32.
+// (a running exponent, as the maximum is running).  bf16 caches: three bf16 pieces.  16-bit queries are one piece, exactly; their
+// weights stay two pieces over 8-bit caches (one, 2^-12 off, changed the rounding of a tenth of a batch's outputs) and are two
+// over bf16 ones (2^-16 off, against the output's 2^-8: one output in five hundred rounds otherwise).  fp32 caches:
+// v_mfma_f32_16x16x4_f32.  Maxima, sums and outputs are fp32.
 #include <limits.h>
 
 #include <type_traits>
@@ -143,8 +144,8 @@ template <int CT, int QT>
 struct TreePieces {
     static constexpr int ES = CT == LLM_F32 ? 4 : CT == LLM_BF16 ? 2 : 1;
     static constexpr bool SCALED = ES == 1;
-    static constexpr int Q = QT == LLM_BF16 ? 1 : SCALED ? 2 : 3;                // of a query
-    static constexpr int P = QT == LLM_BF16 ? (SCALED ? 1 : 2) : SCALED ? 2 : 3; // of a weight
+    static constexpr int Q = QT == LLM_BF16 ? 1 : SCALED ? 2 : 3; // of a query
+    static constexpr int P = QT == LLM_BF16 || SCALED ? 2 : 3;    // of a weight
 };
 
 template <int QT>

@@ -1,0 +1,116 @@
+"""What llm_tree_attention promises of scales, signs and unseen tokens, against the definition in float64.
+
+Tolerances.  u = 2^-24, half a step of fp32; L the positions a row sees.
+  A score, a sum of hs products with the query held to 22 bits at least (4 u), is off by at most d = (hs + 8) u |scale| max
+  sum |q k|, a weight then by a factor of e^(2 d), everything else (exponential, scales, sums, joins) by (L + 64) u: all
+  relative to sum p |v|.
+  8-bit caches: a weight p sv is two fp16 pieces, the second a rounding of what the first leaves: 2^-12 2^-12 = u, and at most
+  2^-25 where it is subnormal, with the largest |sv| that the row sees in [2^14, 2^15): L 2^-39 max |code| max |sv|.
+  bf16 caches: a weight is three bf16 pieces for fp32 queries (2^-9 each: below u) and two for bf16 ones, 2^-16.
+  bf16 outputs: 2^-8 of the value."""
+import math
+
+import numpy as np
+import pytest
+
+from helpers import pkg
+from test_gpu_operators import CACHES, DEV, ROWS, U, cache_tensors, gen, quantized, same, tree_masks
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def put(x, cache, ctx=None, layout="heads"):
+    """K or V rows (float64 [b, h, positions, hs]) as cache tensors on the device: codes, scales, the values they stand for"""
+    b, h, n, hs = x.shape
+    val, code, s = quantized(x, cache)
+    store, _, sc, _ = cache_tensors(cache, b, h, ctx or n, hs, layout, 0.0)
+    store[:, :, :n] = code.float().to(CACHES[cache]).to(DEV)
+    if sc is not None:
+        sc[:, :, :n] = s.to(DEV)
+    return store, sc, val, code, s
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def bits(mask):
+    return torch.from_numpy(np.array(mask, np.uint64).view(np.int64)).to(DEV)
+
+
+def check(q, k, v, lens, mask, scale, got, cache):
+    """got against float64; k and v are (values, codes, scales) of `put` on the CPU"""
+    b, t, heads, hs = q.shape
+    h, end = k[0].shape[1:3]
+    group, at = heads // h, torch.arange(end)
+    for i in range(b):
+        node = at - lens[i]
+        sees = torch.stack([(node < 0) | (torch.tensor([0 <= m < t and bool((int(mask[i][j]) >> m) & 1) for m in node.tolist()]))
+                            for j in range(t)])
+        sees = sees.unsqueeze(1).expand(t, group, end).reshape(t * group, end)
+        count = sees.sum(-1, keepdim=True)
+        for x in range(h):
+            mine = slice(x * group, (x + 1) * group)
+            qd, y = q[i, :, mine].double().cpu().reshape(t * group, hs), got[i, :, mine].double().cpu().reshape(t * group, hs)
+            s = (qd @ k[0][i, x].T * scale).masked_fill(~sees, -math.inf)
+            p = torch.softmax(s.masked_fill(count == 0, 0.0), -1) * (count > 0)
+            want, size = p @ v[0][i, x], p @ v[0][i, x].abs()
+            far = (qd.abs() @ k[0][i, x].abs().T).masked_fill(~sees, 0.0).amax(-1, keepdim=True)
+            tol = (2 * (hs + 8) * U * abs(scale) * far + (count + 64) * U) * size
+            if v[2] is not None:
+                big = v[1][i, x].abs().amax(-1) * v[2][i, x].double().abs()
+                tol = tol + count * 2.0 ** -39 * big.expand_as(sees).masked_fill(~sees, 0.0).amax(-1, keepdim=True)
+            if cache == "bf16":
+                tol = tol + (2.0 ** -16 if q.dtype == torch.bfloat16 else U) * size
+            if q.dtype == torch.bfloat16:
+                tol = tol * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs()
+            err = (y - want).abs()
+            assert (err <= tol + 1e-37).all(), (i, x, float((err / (tol + 1e-37)).max()))
+
+
+@pytest.mark.parametrize("cache", ["int8", "e4m3"])
+@pytest.mark.parametrize("hs,heads,h,lens,t", [(64, 4, 2, [0, 30], 2), (128, 28, 4, [70, 6], 3), (128, 28, 4, [1800, 333], 1),
+                                               (256, 2, 1, [40, 8], 5), (64, 14, 2, [90, 41], 37)])
+def test_weights_of_16_bit_queries_keep_their_bits(cache, hs, heads, h, lens, t):
+    """pairs of positions whose values nearly cancel: what is left of them holds a weight's low bits"""
+    g = gen(hs + t)
+    b, n = 2, max(lens) + t + 1
+    n += n % 2
+    x = [torch.randn(b, h, n, hs, generator=g).double() for _ in range(2)]
+    # a pair: K alike within 2^-9, V the negative within 2^-10
+    x[0][:, :, 1::2] = x[0][:, :, ::2] * (1 + 2.0 ** -9 * torch.rand(b, h, n // 2, 1, generator=g).double())
+    x[1][:, :, 1::2] = -x[1][:, :, ::2] * (1 + 2.0 ** -10 * torch.rand(b, h, n // 2, 1, generator=g).double())
+    q = (torch.randn(b, t, heads, hs, generator=g) * 0.1).to(torch.bfloat16)
+    (k, ks, *kv), (v, vs, *vv) = (put(y, cache) for y in x)
+    # every row sees both of a pair: the committed ones, and of the new tokens whole pairs (where lens is even)
+    mask = [[sum(1 << m for m in range(j | 1) if m < t) | 1 << j for j in range(t)] for _ in range(b)]
+    got = pkg().tree_attention(q.to(DEV), k, v, ints(lens), mask=bits(mask), k_scale=ks, v_scale=vs)
+    check(q, kv, vv, lens, mask, hs ** -0.5, got, cache)
+
+
+# many rows and positions enough for two row tiles a wave (8-bit caches; bf16), and few of one
+SHAPES = [(64, 4, 2, 33, 6), (128, 28, 4, 70, 6), (128, 4, 2, 1500, 6), (128, 28, 4, 2000, 37), (48, 6, 6, 40, 20), (160, 3, 1, 61, 9),
+          (256, 4, 2, 90, 7)]
+
+
+def tree_case(cache, rows, hs, heads, h, length, t, seed=0):
+    """a random tree over a filled cache with room behind it; node 1 has children, others do not see it"""
+    g = gen(hs + length + t + seed)
+    ctx = 40000 if t > 30 else length + t + 80
+    x = [torch.randn(1, h, length + t, hs, generator=g).double() for _ in range(2)]
+    q = torch.randn(1, t, heads, hs, generator=g).to(ROWS[rows])
+    (k, ks, *kv), (v, vs, *vv) = (put(y, cache, ctx) for y in x)
+    mask = tree_masks(g, 1, t)
+    mask[0, 2] = 0b101  # (node 2 hangs on the root)
+    mask[0, t - 1] &= ~np.uint64(2)
+    return q, k, ks, kv, v, vs, vv, mask
+
+
+def attend(q, k, ks, v, vs, length, mask, **kw):
+    return pkg().tree_attention(q.to(DEV), k, v, ints([length]), mask=bits(mask), k_scale=ks, v_scale=vs, **kw)
+
+
+def blind(mask, node):
+    """the tokens that do not see the node"""
+    return [i for i in range(mask.shape[1]) if not (int(mask[0, i]) >> node) & 1]
