@@ -570,15 +570,15 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
         load_k(step + 4);
 
         uint32_t vis[R];
-        uint64_t bad = 0; // edge, fp32 and bf16: new tokens whose V row is not finite
+        uint64_t bad = 0; // edge: new tokens whose V row is not finite
 #pragma unroll
         for (int r = 0; r < R; r++) vis[r] = 0;
         if (edge) {
 #pragma unroll
             for (int r = 0; r < R; r++) vis[r] = seen_bits<TP / 4>(p, p0, sees[r]);
-            if constexpr (!SCALED) {
-                // a value that is not finite would reach the rows that do not see it as 0 * inf: taken out here, and
-                // the rows that do see it become NaN
+            if constexpr (CT != LLM_I8) {
+                // a value (8-bit caches: an e4m3 code that is NaN) that is not finite would reach the rows that do not see it
+                // as 0 * inf: taken out here, and the rows that do see it become NaN
 #pragma unroll
                 for (int i = 0; i < TP / 4; i++) {
                     const int q = p0 + 16 * (i / 4) + i % 4; // of lane group 0
@@ -589,6 +589,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
                         for (int k = 0; k < VR; k++) {
                             const uint32_t u = vr[i][c][k];
                             if constexpr (CT == LLM_F32) nf |= (u & 0x7f800000u) == 0x7f800000u;
+                            else if constexpr (CT == LLM_E4M3) nf |= (((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; // 0x7f
                             else nf |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
                         }
                     nf = nf && q + 4 * j >= p.len;
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
 #pragma unroll
         for (int r = 0; r < R; r++) {
             weights(x[r], cq[r], my_s + 64 + 4 * j, edge, vis[r], oe, m[r], l[r], o[r], pf[r]);
-            if (!SCALED && (sees[r] & bad)) l[r] = NAN;
+            if (CT != LLM_I8 && (sees[r] & bad)) l[r] = NAN;
         }
 
 #pragma unroll

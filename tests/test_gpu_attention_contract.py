@@ -114,3 +114,24 @@ def attend(q, k, ks, v, vs, length, mask, **kw):
 def blind(mask, node):
     """the tokens that do not see the node"""
     return [i for i in range(mask.shape[1]) if not (int(mask[0, i]) >> node) & 1]
+
+
+@pytest.mark.parametrize("rows", ["fp32", "bf16"])
+@pytest.mark.parametrize("hs,heads,h,length,t", SHAPES)
+def test_codes_that_are_nan_reach_their_descendants_only(rows, hs, heads, h, length, t):
+    """e4m3 codes 0x7f and 0xff in the V row, or the K row, of one new token"""
+    q, k, ks, kv, v, vs, vv, mask = tree_case("e4m3", rows, hs, heads, h, length, t)
+    clean = attend(q, k, ks, v, vs, length, mask)
+    check(q, kv, vv, [length], mask, hs ** -0.5, clean, "e4m3")
+    for store in (v, k):
+        for code, at in ((0x7f, hs - 1), (0xff, 5)):
+            raw = store.view(torch.uint8)
+            old = raw[0, :, length + 1, at].clone()
+            raw[0, :, length + 1, at] = code
+            dirty = attend(q, k, ks, v, vs, length, mask)
+            raw[0, :, length + 1, at] = old
+            for i in range(t):
+                if i in blind(mask, 1):
+                    assert torch.equal(dirty[0, i], clean[0, i])
+                else:
+                    assert dirty[0, i].isnan().all()
