@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
         for (int d = 0; d < VC * VW; d++) o[r][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
     float *const my_s = sm_s + wave * 128;
-    uint32_t ve = 20; // exponent field of the largest V scale (at least 2^-107)
+    uint32_t ve = 20; // exponent field of the largest V scale's magnitude (at least 2^-107)
 
     for (; step < p.last; step += 4) {
         const int p0 = step * TP;
@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
             my_s[lane] = __uint_as_float(skr);
             const float sv = __uint_as_float(svr);
             const uint32_t e0 = ve;
-            ve = max(ve, exponent(wave_max(sv < INFINITY ? sv : 0.0f)));
+            ve = max(ve, exponent(wave_max(fabsf(sv) < INFINITY ? fabsf(sv) : 0.0f)));
             if (ve != e0) oe = power_from(e0) * power_to(ve);
             my_s[64 + lane] = sv * power_to(ve);
             wave_lds_fence();

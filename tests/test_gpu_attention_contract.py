@@ -135,3 +135,20 @@ def test_codes_that_are_nan_reach_their_descendants_only(rows, hs, heads, h, len
                     assert torch.equal(dirty[0, i], clean[0, i])
                 else:
                     assert dirty[0, i].isnan().all()
+
+
+@pytest.mark.parametrize("rows", ["fp32", "bf16"])
+@pytest.mark.parametrize("cache", ["int8", "e4m3"])
+@pytest.mark.parametrize("hs,heads,h,length,t", SHAPES + [(64, 4, 2, 0, 1), (128, 28, 4, 9, 1)])
+def test_scales_below_zero(cache, rows, hs, heads, h, length, t):
+    """a value is its code times its scale, whatever the scale's sign: all below zero, and in turn"""
+    q, k, ks, kv, v, vs, vv, mask = tree_case(cache, rows, hs, heads, h, length, max(t, 3))
+    q, mask = q[:, :t], mask[:, :t]
+    for every in (1, 2):
+        signs = torch.ones(kv[2].shape[2])
+        signs[::every] = -1.0
+        sk, sv = kv[2] * signs, vv[2] * signs * 0.01
+        ks[:, :, :sk.shape[2]], vs[:, :, :sv.shape[2]] = sk.to(DEV), sv.to(DEV)
+        got = attend(q, k, ks, v, vs, length, mask)
+        check(q, (kv[1] * sk.double().unsqueeze(-1), kv[1], sk), (vv[1] * sv.double().unsqueeze(-1), vv[1], sv), [length],
+              mask, hs ** -0.5, got, cache)
