@@ -324,34 +324,64 @@ __device__ __forceinline__ float load_queries(const TreeArgs &a, const Place &p,
     return fmaxf(a.c * from, 1e-37f);
 }
 
-// What the row sees of a step's positions where new tokens or the end are among them: bit 4 t + i.
+// What the row sees of a step's positions where new tokens or the end are among them: bit 4 t + i.  A lane's four neighbours at
+// once: those of `sees` from the first one on, ones below the new tokens, zeros past 64 of them.
 template <int N>
 __device__ __forceinline__ uint32_t seen_bits(const Place &p, int p0, uint64_t sees) {
     const int j = (threadIdx.x & 63) >> 4;
     uint32_t vis = 0;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int at = p0 + 16 * (i / 4) + 4 * j + i % 4 - p.len;
-        const uint32_t bit = (uint32_t)(sees >> (at & 63)) & 1;
-        vis |= (at < 0 ? 1u : at < 64 ? bit : 0u) << i;
+    for (int t = 0; t < N / 4; t++) {
+        const int at = p0 + 16 * t + 4 * j - p.len;
+        const uint32_t below = ((uint32_t)sees << 4 | 15u) >> (max(at + 4, 0) & 31), from = at < 64 ? (uint32_t)(sees >> (at & 63)) : 0u;
+        vis |= ((at < 0 ? below : from) & 15u) << (4 * t);
     }
     return vis;
 }
 
+// x where the row sees position i, else `or_else`, through a word of ones or zeros: as conditions the masks of all positions would
+// take more scalar registers than there are.
+__device__ __forceinline__ float if_seen(uint32_t vis, int i, float x, float or_else) {
+    const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)vis, i, 1);
+    return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(or_else) & ~m));
+}
+
 // A step's scores x (with the K scales, if any) into the weights of its values: the running maximum m (exponents of 2) and
-// sum l of the row; `sv` (in LDS) the V scales times their common power, at 16 t + i; o and l are rescaled when the maximum
-// or, by `oe`, that power has moved.  fp32 and bf16 weights have the exponents to go on with an old maximum until it is
+// sum l of the row; o and l are rescaled when the maximum has moved.  8-bit caches: `sv` (in LDS) holds the V scales at
+// 16 t + i, and `ve` is the row's running exponent of the weights.  Before the edge every row sees every position: `step_e` is the
+// exponent for all, and the scales come times its power.  At the edge they come as they are, and a row takes the exponent of
+// those that it sees: what a row does not see changes no bit of it.  fp32 and bf16 weights have the exponents to go on with an old maximum until it is
 // passed by a factor of 2^8 (a batch of 64-token trees over bf16: 144 us with every new maximum, 139 so); the fp16 pieces'
 // range is used up.
 template <int NT, int CT, int NPP, int DT>
-__device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *sv, bool edge, uint32_t vis, float oe,
+__device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *sv, bool edge, uint32_t vis, uint32_t step_e, uint32_t &ve,
                                         float &m, float &l, f32x4 (&o)[DT], Frag<CT, NPP> (&pf)[NT / 2]) {
     constexpr bool SCALED = CT == LLM_I8 || CT == LLM_E4M3;
+    float oe = 1.0f, pw = 1.0f; // what takes the row's values so far to its new power, and the power at the edge
+    if constexpr (SCALED) {
+        uint32_t e = step_e;
+        if (edge) {
+            float big = 0.0f;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const f32x4 s4 = *(const f32x4 *)(sv + 16 * t);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float s = fabsf(if_seen(vis, 4 * t + i, s4[i], 0.0f));
+                    big = fmaxf(big, s < INFINITY ? s : 0.0f);
+                }
+            }
+            e = max(ve, exponent(over_groups(big, fmax_)));
+            pw = power_to(e);
+        }
+        if (e != ve) oe = power_from(ve) * power_to(e);
+        ve = e;
+    }
     if (edge)
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[t][i] = (vis >> (4 * t + i)) & 1 ? x[t][i] : -INFINITY;
+            for (int i = 0; i < 4; i++) x[t][i] = if_seen(vis, 4 * t + i, x[t][i], -INFINITY);
     float mx = x[0][0];
 #pragma unroll
     for (int t = 0; t < NT; t++)
@@ -387,7 +417,7 @@ __device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *s
         }
         if (SCALED && edge) { // (0 * a scale that is not finite)
 #pragma unroll
-            for (int i = 0; i < 8; i++) w[i] = (vis >> (8 * u + i)) & 1 ? w[i] : 0.0f;
+            for (int i = 0; i < 8; i++) w[i] = if_seen(vis, 8 * u + i, w[i] * pw, 0.0f);
         }
         fill(pf[u], w);
     }
@@ -459,6 +489,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
 
     const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float2 *const my_ml = (float2 *)sm_ml + wave * R * 16; // until the end: what the wave's rows see, needed in its last step only
     Place p;
     if (!place<QT>(a, 16 * R, p)) return;
     const int row0 = p.row0;
@@ -518,19 +549,28 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
     load_v(step);
 
     Frag<CT, Pc::Q> qf[R][KS];
-    uint64_t sees[R];
     float cq[R], m[R], l[R];
     f32x4 o[R][VC * VW];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        cq[r] = load_queries<CT, QT>(a, p, row0 + 16 * r + n, qf[r], sees[r]);
+        uint64_t sees;
+        cq[r] = load_queries<CT, QT>(a, p, row0 + 16 * r + n, qf[r], sees);
+        if (j == 0) my_ml[16 * r + n] = make_float2(__uint_as_float((uint32_t)sees), __uint_as_float((uint32_t)(sees >> 32)));
         m[r] = -INFINITY;
         l[r] = 0.0f;
 #pragma unroll
         for (int d = 0; d < VC * VW; d++) o[r][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
+    wave_lds_fence();
+    auto row_sees = [&](int r) {
+        const float2 x = my_ml[16 * r + n];
+        return (uint64_t)__float_as_uint(x.y) << 32 | __float_as_uint(x.x);
+    };
     float *const my_s = sm_s + wave * 128;
-    uint32_t ve = 20; // exponent field of the largest V scale's magnitude (at least 2^-107)
+    // exponent field of the largest V scale's magnitude (at least 2^-107): of all before the edge, and of what a row sees
+    uint32_t ve = 20, row_ve[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) row_ve[r] = ve;
 
     for (; step < p.last; step += 4) {
         const int p0 = step * TP;
@@ -557,25 +597,20 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
                 for (int r = 0; r < R; r++) x[r][t] = product(kf, qf[r][s], x[r][t]);
             }
         }
-        float oe = 1.0f;
         if constexpr (SCALED) {
             my_s[lane] = __uint_as_float(skr);
-            const float sv = __uint_as_float(svr);
-            const uint32_t e0 = ve;
-            ve = max(ve, exponent(wave_max(fabsf(sv) < INFINITY ? fabsf(sv) : 0.0f)));
-            if (ve != e0) oe = power_from(e0) * power_to(ve);
-            my_s[64 + lane] = sv * power_to(ve);
+            float sv = __uint_as_float(svr);
+            if (!edge) {
+                ve = max(ve, exponent(wave_max(fabsf(sv) < INFINITY ? fabsf(sv) : 0.0f)));
+                sv *= power_to(ve);
+            }
+            my_s[64 + lane] = sv;
             wave_lds_fence();
         }
         load_k(step + 4);
 
-        uint32_t vis[R];
         uint64_t bad = 0; // edge: new tokens whose V row is not finite
-#pragma unroll
-        for (int r = 0; r < R; r++) vis[r] = 0;
         if (edge) {
-#pragma unroll
-            for (int r = 0; r < R; r++) vis[r] = seen_bits<TP / 4>(p, p0, sees[r]);
             if constexpr (CT != LLM_I8) {
                 // a value (8-bit caches: an e4m3 code that is NaN) that is not finite would reach the rows that do not see it
                 // as 0 * inf: taken out here, and the rows that do see it become NaN
@@ -620,8 +655,14 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
         Frag<CT, Pc::P> pf[R][NT / 2];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            weights(x[r], cq[r], my_s + 64 + 4 * j, edge, vis[r], oe, m[r], l[r], o[r], pf[r]);
-            if (CT != LLM_I8 && (sees[r] & bad)) l[r] = NAN;
+            uint32_t vis = 0;
+            uint64_t sees = 0;
+            if (edge) {
+                sees = row_sees(r);
+                vis = seen_bits<TP / 4>(p, p0, sees);
+            }
+            weights(x[r], cq[r], my_s + 64 + 4 * j, edge, vis, ve, row_ve[r], m[r], l[r], o[r], pf[r]);
+            if (CT != LLM_I8 && (sees & bad)) l[r] = NAN;
         }
 
 #pragma unroll
@@ -678,7 +719,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
             lw[w] = sm_ml[((w * R + r) * 16 + n) * 2 + 1];
         }
         const float mn = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3])), mu = mn == -INFINITY ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m[r] - mu) * (SCALED ? power_from(ve) : 1.0f);
+        const float al = __builtin_amdgcn_exp2f(m[r] - mu) * (SCALED ? power_from(row_ve[r]) : 1.0f);
         l[r] = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; w++) l[r] += lw[w] * __builtin_amdgcn_exp2f(mw[w] - mu);
@@ -884,9 +925,9 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
                 Frag<CT, Pc::P> pf[R][1];
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    uint32_t vis = 0;
+                    uint32_t vis = 0, none = 0;
                     if (edge) vis = seen_bits<8>(p, step * 64 + 32 * u, sees[r]);
-                    weights(x[r], cq[r], nullptr, edge, vis, 1.0f, m[r], l[r], o[r], pf[r]);
+                    weights(x[r], cq[r], nullptr, edge, vis, 0, none, m[r], l[r], o[r], pf[r]);
                 }
 #pragma unroll
                 for (int d = 0; d < DT; d++) {

@@ -137,6 +137,25 @@ def test_codes_that_are_nan_reach_their_descendants_only(rows, hs, heads, h, len
                     assert dirty[0, i].isnan().all()
 
 
+@pytest.mark.parametrize("cache,rows", [("int8", "fp32"), ("e4m3", "fp32"), ("e4m3", "bf16"), ("bf16", "bf16"), ("fp32", "fp32")])
+@pytest.mark.parametrize("t,pad", [(3, 8), (5, 64)])
+def test_padded_trees_over_slots_that_were_never_written(cache, rows, t, pad):
+    """a tree padded to a fixed number of nodes without masks: every byte of the slots behind it is 0xff, or 0x7f"""
+    hs, heads, h, length = 128, 14, 2, 75
+    q, k, ks, kv, v, vs, vv, mask = tree_case(cache, rows, hs, heads, h, length, t)
+    wide = torch.zeros(1, pad, heads, hs, dtype=q.dtype)
+    wide[:, :t] = q
+    m = np.zeros((1, pad), np.uint64)
+    m[:, :t] = mask
+    clean = attend(wide, k, ks, v, vs, length, m)
+    check(q, kv, vv, [length], mask, hs ** -0.5, clean[:, :t], cache)
+    for byte in (0xff, 0x7f):
+        for store in (k, v, ks, vs):
+            if store is not None:
+                store.view(torch.uint8).view(1, h, k.shape[2], -1)[:, :, length + t:] = byte
+        assert torch.equal(attend(wide, k, ks, v, vs, length, m), clean)
+
+
 @pytest.mark.parametrize("rows", ["fp32", "bf16"])
 @pytest.mark.parametrize("cache", ["int8", "e4m3"])
 @pytest.mark.parametrize("hs,heads,h,length,t", SHAPES + [(64, 4, 2, 0, 1), (128, 28, 4, 9, 1)])
@@ -152,3 +171,28 @@ def test_scales_below_zero(cache, rows, hs, heads, h, length, t):
         got = attend(q, k, ks, v, vs, length, mask)
         check(q, (kv[1] * sk.double().unsqueeze(-1), kv[1], sk), (vv[1] * sv.double().unsqueeze(-1), vv[1], sv), [length],
               mask, hs ** -0.5, got, cache)
+
+
+@pytest.mark.parametrize("rows", ["fp32", "bf16"])
+@pytest.mark.parametrize("cache", ["int8", "e4m3"])
+@pytest.mark.parametrize("hs,heads,h,length,t", SHAPES)
+def test_scales_of_unseen_tokens_change_nothing(cache, rows, hs, heads, h, length, t):
+    """one new token's V (and K) scale far above the others': the tokens that do not see it are the same bit for bit, those that
+    do follow it"""
+    q, k, ks, kv, v, vs, vv, mask = tree_case(cache, rows, hs, heads, h, length, t)
+    clean = attend(q, k, ks, v, vs, length, mask)
+    check(q, kv, vv, [length], mask, hs ** -0.5, clean, cache)
+    for far in (2.0 ** 20, 2.0 ** 30, -2.0 ** 40, 2.0 ** 100, math.inf):
+        s = vv[2].clone()
+        s[:, :, length + 1] *= far
+        vs[:, :, :length + t] = s.to(DEV)
+        got = attend(q, k, ks, v, vs, length, mask)
+        for i in blind(mask, 1):
+            assert torch.equal(got[0, i], clean[0, i]), (far, i)
+        if math.isfinite(far):
+            check(q, kv, (vv[1] * s.double().unsqueeze(-1), vv[1], s), [length], mask, hs ** -0.5, got, cache)
+    vs[:, :, :length + t] = vv[2].to(DEV)
+    ks[:, :, length + 1] *= 2.0 ** 40
+    got = attend(q, k, ks, v, vs, length, mask)
+    for i in blind(mask, 1):
+        assert torch.equal(got[0, i], clean[0, i])
