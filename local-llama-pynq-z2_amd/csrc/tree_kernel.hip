@@ -350,12 +350,12 @@ __device__ __forceinline__ float if_seen(uint32_t vis, int i, float x, float or_
 // sum l of the row; o and l are rescaled when the maximum has moved.  8-bit caches: `sv` (in LDS) holds the V scales at
 // 16 t + i, and `ve` is the row's running exponent of the weights.  Before the edge every row sees every position: `step_e` is the
 // exponent for all, and the scales come times its power.  At the edge they come as they are, and a row takes the exponent of
-// those that it sees: what a row does not see changes no bit of it.  fp32 and bf16 weights have the exponents to go on with an old maximum until it is
-// passed by a factor of 2^8 (a batch of 64-token trees over bf16: 144 us with every new maximum, 139 so); the fp16 pieces'
-// range is used up.
+// those that it sees: what a row does not see changes no bit of it.  fp32 and bf16 weights have the exponents to go on with an
+// old maximum until it is passed by a factor of 2^8 (a batch of 64-token trees over bf16: 144 us with every new maximum, 139
+// so); the fp16 pieces' range is used up.
 template <int NT, int CT, int NPP, int DT>
-__device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *sv, bool edge, uint32_t vis, uint32_t step_e, uint32_t &ve,
-                                        float &m, float &l, f32x4 (&o)[DT], Frag<CT, NPP> (&pf)[NT / 2]) {
+__device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *sv, bool edge, uint32_t vis, uint32_t step_e,
+                                        uint32_t &ve, float &m, float &l, f32x4 (&o)[DT], Frag<CT, NPP> (&pf)[NT / 2]) {
     constexpr bool SCALED = CT == LLM_I8 || CT == LLM_E4M3;
     float oe = 1.0f, pw = 1.0f; // what takes the row's values so far to its new power, and the power at the edge
     if constexpr (SCALED) {
@@ -388,10 +388,11 @@ __device__ __forceinline__ void weights(f32x4 (&x)[NT], float cq, const float *s
 #pragma unroll
         for (int i = 0; i < 4; i++) mx = fmaxf(mx, x[t][i]);
     mx = over_groups(mx, fmax_);
-    const float mn = fmaxf(m, mx * cq);
-    float mu = m == -INFINITY ? 0.0f : m;
     constexpr float SLACK = SCALED ? 0.0f : 8.0f;
-    if (__any(mn > m + SLACK || oe != 1.0f)) {
+    float mn = fmaxf(m, mx * cq), mu = m == -INFINITY ? 0.0f : m;
+    const bool moved = mn > m + SLACK;
+    if (__any(moved || oe != 1.0f)) {
+        if (SLACK > 0.0f) mn = moved ? mn : m; // (a row's own: the wave's other rows change no bit of it)
         mu = mn == -INFINITY ? 0.0f : mn;
         const float al = __builtin_amdgcn_exp2f(m - mu), ao = al * oe;
         l *= al;

@@ -196,3 +196,24 @@ def test_scales_of_unseen_tokens_change_nothing(cache, rows, hs, heads, h, lengt
     got = attend(q, k, ks, v, vs, length, mask)
     for i in blind(mask, 1):
         assert torch.equal(got[0, i], clean[0, i])
+
+
+@pytest.mark.parametrize("cache,rows", [("fp32", "fp32"), ("fp32", "bf16"), ("bf16", "fp32"), ("bf16", "bf16"), ("int8", "fp32"),
+                                        ("e4m3", "bf16")])
+@pytest.mark.parametrize("hs,heads,h,length,t", SHAPES + [(128, 28, 4, 2500, 64)])
+def test_rows_of_unseen_tokens_change_nothing(cache, rows, hs, heads, h, length, t):
+    """other K and V rows of one new token, whose scores lie little or much above the others': the tokens that do not see it are
+    the same bit for bit"""
+    q, k, ks, kv, v, vs, vv, mask = tree_case(cache, rows, hs, heads, h, length, t)
+    clean = attend(q, k, ks, v, vs, length, mask)
+    for size in (0.1, 2.0, 9.0):
+        # (along the first query of its own: its score, and those of its descendants', are far from the rest)
+        row = q[0, 1, ::heads // h].double().view(1, h, 1, hs) * size
+        code, s = quantized(row, cache)[1:]
+        k[:, :, length + 1:length + 2] = code.float().to(CACHES[cache]).to(DEV)
+        v[:, :, length + 1:length + 2] = (-code).float().to(CACHES[cache]).to(DEV)
+        if s is not None:
+            ks[:, :, length + 1:length + 2] = s.to(DEV)
+        got = attend(q, k, ks, v, vs, length, mask)
+        for i in blind(mask, 1):
+            assert torch.equal(got[0, i], clean[0, i]), (size, i)
