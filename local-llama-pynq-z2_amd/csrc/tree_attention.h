@@ -22,7 +22,7 @@ struct TreeArgs {
     int cap, each, least, tp;      // slices of positions: at most in all (0: none) and of a head, their steps at least, a
                                    // step's positions
     float c;                       // |softmax scale| * log2(e), positive
-    int negate;                    // the scale is negative: the queries change their sign
+    float sign;                    // the queries' factor: the scale's sign, 0 where the scale is
     float *ml, *acc;               // slices: [slice][row] (max, sum), the same with hs sums of values
     int2 *plan;                    // [seq][kv head]: first slice, slices
 };

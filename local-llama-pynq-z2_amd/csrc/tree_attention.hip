@@ -95,6 +95,8 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs a) {
     }
 }
 
+constexpr float LOG2E = 1.44269504088896340736f;
+
 struct TreePlan {
     int hsp, tp, many, tiles, row_blocks, block_rows, cap, each, least;
     size_t bytes;
@@ -179,9 +181,8 @@ hipError_t launch_tree_attention(const llm_kv &c, const llm_rows &q, const llm_r
     a.n_seq = c.n_seq, a.n_kv = c.n_kv, a.hs = c.hs, a.ctx = c.ctx;
     a.group = t.n_heads / c.n_kv, a.max_n = t.max_n, a.row_blocks = p.row_blocks, a.block_rows = p.block_rows;
     a.cap = p.cap, a.each = p.each, a.least = p.least, a.tp = p.tp, a.zero_rest = t.zero_rest;
-    // (a scale of 0 as one so small that every weight is 1)
-    a.c = std::max(std::fabs(t.scale) * 1.44269504088896340736f, 1e-30f);
-    a.negate = t.scale < 0.0f;
+    a.c = t.scale == 0.0f ? 1.0f : std::max(std::fabs(t.scale) * LOG2E, 1e-37f);
+    a.sign = t.scale > 0.0f ? 1.0f : t.scale < 0.0f ? -1.0f : 0.0f;
     a.acc = (float *)t.work; // (rows of hs values, hs a multiple of 16: 16-byte aligned)
     const size_t parts = (size_t)p.cap * a.group * t.max_n;
     a.ml = a.acc + parts * c.hs;
@@ -213,16 +214,16 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
                 who);
         return -1;
     }
+    if (!std::isfinite(scale * LOG2E)) {
+        fprintf(stderr, "%s: scale %g\n", who, scale);
+        return -1;
+    }
     OpDevice dev(who);
     if (!op_check_cache(c, &dev, who)) return -1;
     if (!max_n || !c->n_seq) return 0;
     if (!op_check_rows(q, "q", &dev, who) || !op_check_rows(out, "out", &dev, who) || !dev.holds(lens, "lens") ||
         (n && !dev.holds(n, "n")) || (mask && !dev.holds(mask, "mask")))
         return -1;
-    if (!std::isfinite(scale)) {
-        fprintf(stderr, "%s: scale %g\n", who, scale);
-        return -1;
-    }
     if (q->type != out->type) {
         fprintf(stderr, "%s: q and out of different types\n", who);
         return -1;

@@ -314,14 +314,14 @@ __device__ __forceinline__ float load_queries(const TreeArgs &a, const Place &p,
         to = power_to(e);
         from = power_from(e);
     }
-    if (a.negate) to = -to;
+    to *= a.sign;
 #pragma unroll
     for (int s = 0; s < HSP / 32; s++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[s][i] *= to;
         fill(qf[s], x[s]);
     }
-    return fmaxf(a.c * from, 1e-37f);
+    return fmaxf(a.c * from, 1e-45f); // (never 0: the scores of what is not seen are -infinity times this)
 }
 
 // What the row sees of a step's positions where new tokens or the end are among them: bit 4 t + i.  A lane's four neighbours at

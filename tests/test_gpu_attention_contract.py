@@ -217,3 +217,28 @@ def test_rows_of_unseen_tokens_change_nothing(cache, rows, hs, heads, h, length,
         got = attend(q, k, ks, v, vs, length, mask)
         for i in blind(mask, 1):
             assert torch.equal(got[0, i], clean[0, i]), (size, i)
+
+
+@pytest.mark.parametrize("rows", ["fp32", "bf16"])
+@pytest.mark.parametrize("cache", list(CACHES))
+@pytest.mark.parametrize("hs,heads,h,length,t", [(64, 4, 2, 50, 5), (128, 28, 4, 3000, 2), (128, 28, 4, 2500, 37)])
+@pytest.mark.parametrize("scale", [0.03, 0.5, -0.2, 0.0])
+def test_scales_of_the_softmax(cache, rows, hs, heads, h, length, t, scale):
+    """other scales than hs ** -0.5, below zero, and zero (the mean of what is seen), whole and in slices"""
+    q, k, ks, kv, v, vs, vv, mask = tree_case(cache, rows, hs, heads, h, length, max(t, 3), 1)
+    q, mask = q[:, :t], mask[:, :t]
+    got = attend(q, k, ks, v, vs, length, mask, scale=scale)
+    check(q, kv, vv, [length], mask, scale, got, cache)
+
+
+@pytest.mark.parametrize("cache", list(CACHES))
+def test_a_scale_of_zero_over_large_scores(cache):
+    """0 times any score is 0: the mean, however large the products"""
+    g = gen(12)
+    b, h, hs, length, t, heads = 1, 2, 64, 45, 3, 4
+    x = [torch.randn(b, h, length + t, hs, generator=g).double() * f for f in (2.0 ** 55, 1.0)]
+    q = torch.randn(b, t, heads, hs, generator=g) * 2.0 ** 55
+    (k, ks, *kv), (v, vs, *vv) = (put(y, cache) for y in x)
+    mask = tree_masks(g, b, t)
+    got = pkg().tree_attention(q.to(DEV), k, v, ints([length]), mask=bits(mask), k_scale=ks, v_scale=vs, scale=0.0)
+    check(q, kv, vv, [length], mask, 0.0, got, cache)
