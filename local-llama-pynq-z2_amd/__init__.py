@@ -214,7 +214,8 @@ def ref_expf(x, host=False):
 
 # ---- operators on device memory (torch tensors) -----------------------------------------------------------
 # (a call's host time is most of a small call's: the C structs are packed in one step, and what the library checks by
-# itself, that every address is memory of one device, is not checked here again)
+# itself, that every address is memory of one device, is not checked here again.  There is no backward pass: tensors that
+# require a gradient are refused where gradients are on)
 
 _torch = None
 _PACK_KV = struct.Struct("4P5i4x6q").pack
@@ -245,6 +246,18 @@ def _ints(name, t, count, dtype):
     if t.dtype is not dtype or t.numel() != count or not t.is_contiguous():
         raise ValueError(f"{name}: {count} contiguous {dtype} are needed")
     return t.data_ptr()
+
+
+def _no_grad(*tensors):
+    """refuses tensors that a gradient is asked of: the operators have none"""
+    for t in tensors:
+        if t is not None and t.requires_grad and _types()[0].is_grad_enabled():
+            raise ValueError("the operators have no gradient: call them under torch.no_grad(), or with detached tensors")
+
+
+def _written(*tensors):
+    """tensors changed in place, as autograd counts it: a graph that saved one of them refuses its backward pass"""
+    _torch[0].autograd.graph.increment_version([t for t in tensors if t is not None])
 
 
 def _kv(k, v, k_scale, v_scale):
@@ -296,17 +309,20 @@ def kv_write(k_rows, v_rows, k, v, pos, n=None, k_scale=None, v_scale=None):
     """Rows [seqs, tokens, kv heads, head size] into the cache (llm_kv_write): token t < n[b] of sequence b at position
     pos[b] + t.  The cache: k and v [seqs, kv heads, positions, head size] of float32, bfloat16, int8 or float8_e4m3fn, the
     last two with float32 scales [seqs, kv heads, positions]."""
+    _no_grad(k_rows, v_rows, k, v, k_scale, v_scale)
     c, (b, h, _, hs) = _kv(k, v, k_scale, v_scale)
     t, i32 = k_rows.shape[1], _torch[0].int32
     if lib().llm_kv_write(c, _rows("k_rows", k_rows, b, t, h, hs), _rows("v_rows", v_rows, b, t, h, hs),
                           _ints("pos", pos, b, i32), _ints("n", n, b, i32), t, _stream(k)) != 0:
         raise RuntimeError("llm_kv_write failed")
+    _written(k, v, k_scale, v_scale)
 
 
 def kv_read(k, v, pos, tokens, n=None, k_scale=None, v_scale=None, out=None, dtype=None):
     """The values of positions pos[b] .. pos[b] + n[b] - 1 (n None: `tokens` each) as rows [seqs, tokens, kv heads, head
     size] of K and V (llm_kv_read), float32 or `dtype`; new tensors (rows that are not read: zero) or `out`, a pair (such
     rows left as they were)."""
+    _no_grad(k, v, k_scale, v_scale, *(out or ()))
     c, (b, h, _, hs) = _kv(k, v, k_scale, v_scale)
     torch, fresh = _torch[0], out is None
     if fresh:
@@ -314,6 +330,8 @@ def kv_read(k, v, pos, tokens, n=None, k_scale=None, v_scale=None, out=None, dty
     if lib().llm_kv_read(c, _rows("out", out[0], b, tokens, h, hs), _rows("out", out[1], b, tokens, h, hs),
                          _ints("pos", pos, b, torch.int32), _ints("n", n, b, torch.int32), tokens, fresh, _stream(k)) != 0:
         raise RuntimeError("llm_kv_read failed")
+    if not fresh:
+        _written(*out)
     return out[0], out[1]
 
 
@@ -323,6 +341,7 @@ def tree_attention(q, k, v, lens, n=None, mask=None, k_scale=None, v_scale=None,
     sees the positions before lens[b] and the new tokens of mask[b, i]'s bits (int64; None: a chain).  n[b] tokens count
     (None: all); scale None: head size ** -0.5; max_len: the host's bound of lens (None: the cache's positions).  Returns
     a new tensor (rows behind n[b]: zero), or `out` (such rows left as they were)."""
+    _no_grad(q, k, v, k_scale, v_scale, out)
     c, (b, _, ctx, hs) = _kv(k, v, k_scale, v_scale)
     torch, fresh = _torch[0], out is None
     t, heads = q.shape[1:3]
@@ -336,6 +355,8 @@ def tree_attention(q, k, v, lens, n=None, mask=None, k_scale=None, v_scale=None,
                             _ints("mask", mask, b * t, torch.int64), t, bound, hs ** -0.5 if scale is None else scale, fresh,
                             work.data_ptr() if need else None, need, _stream(k)) != 0:
         raise RuntimeError("llm_tree_attention failed")
+    if not fresh:
+        _written(out)
     return out
 
 
@@ -344,6 +365,7 @@ def logprobs(logits, tokens=None, top=0, temperature=1.0):
     tokens [rows, count] int32.  Returns (logp [rows, count] of the tokens, entropy [rows], top_ids [rows, top] and top_logp
     [rows, top] of the largest logits in descending order, lse [rows])."""
     torch, types = _types()
+    _no_grad(logits)
     rows, vocab = logits.shape
     ty, st = types.get(logits.dtype, 4), logits.stride()
     if ty > 1 or (vocab > 1 and st[1] != 1) or (tokens is not None and (tokens.dim() != 2 or tokens.shape[0] != rows)):
