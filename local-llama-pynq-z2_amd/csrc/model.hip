@@ -22,6 +22,7 @@
 #include <unistd.h>
 
 #include <algorithm>
+#include <functional>
 #include <string>
 #include <vector>
 
@@ -90,6 +91,8 @@ struct llm_model {
     uint64_t *ver_mask = nullptr;
     int *ver_len = nullptr, *ver_depth = nullptr;
     float *ver_logits = nullptr;
+    float *score_logits = nullptr; // llm_score: rows of logits, a chunk's or as many as there was room for
+    int score_rows = 0;
     void *lp_buf = nullptr;
     size_t lp_bytes = 0;
     std::vector<int> head_row; // row of the head by token id (-1: none), made when first needed
@@ -1197,12 +1200,12 @@ int prefill_chunk(llm_model *m, const int *ids, int p0, int M, bool tree = false
 // not take the model's shape, a generation that keeps every position's logits runs its prompt position by position.
 bool head_gemm_ok(const llm_model *m) { return m->head.rows % 4 == 0 && m->head.bytes < ((size_t)1 << 31); }
 
-// The logits of a chunk's M positions (their residual streams in pf_x) into the rows from y on: the final norm
+// The logits of M positions of a chunk, its from-th on (their residual streams in pf_x), into the rows from y on: the final norm
 // per token, then the head as one GEMM.  The prompt's steps one by one read every weight once per position: 97 tokens
 // through two layers of the 0.5B shape and a 16,384-row head 6587 us, this way 649.  Strict: bitwise the steps' logits.
 // Fast: the sums are taken in another order; the logits' distance from float64 by steps / this way, mean over 124 prompts
 // of 24 tokens 0.00360 / 0.00350, over 124 of 97 tokens 0.00690 / 0.00688.
-int prefill_logits(llm_model *m, float *y, int M) {
+int prefill_logits(llm_model *m, float *y, int M, int from = 0) {
     const llm_info &I = m->info;
     ProwArgs pa;
     memset(&pa, 0, sizeof pa);
@@ -1211,7 +1214,7 @@ int prefill_logits(llm_model *m, float *y, int M) {
     pa.gs = m->gs;
     pa.qflavor = m->qflavor;
     pa.eps = I.rms_eps;
-    pa.x = m->pf_x;
+    pa.x = m->pf_x + (size_t)from * I.dim;
     pa.norm_w = out_norm(m);
     pa.oq = m->pf_a;
     pa.os = m->pf_s;
@@ -1232,7 +1235,10 @@ int prefill_logits(llm_model *m, float *y, int M) {
 // Positions pos0 .. pos0 + n - 1 (the cache below pos0 kept), then the head of the last one: logits, argmax
 // partials, and (finalize) its argmax into gen[pos0 + n - 1].  Afterwards the step state is position
 // pos0 + n - 1, as after those forward() calls.
-int prefill_all(llm_model *m, const int *ids, int n, bool sampled = false, int pos0 = 0, bool hist = false) {
+// (each: what is done with every chunk, from its first token's number and its length, once m->logits holds the last token's
+// logits if it is the last.  With it, as with hist, the caller has another way where this fails)
+int prefill_all(llm_model *m, const int *ids, int n, bool sampled = false, int pos0 = 0, bool hist = false,
+                const std::function<int(int, int)> &each = nullptr) {
     // on a nearly full card: chunks down to 128 tokens, then the strict attention without score rows
     int chunk = std::min(n, PREFILL_CHUNK);
     const bool by_rows = m->strict && prefill_strict_rows(m->hs);
@@ -1241,7 +1247,7 @@ int prefill_all(llm_model *m, const int *ids, int n, bool sampled = false, int p
             by_rows ? prefill_strict_scratch_floats(chunk, m->info.n_heads, m->info.n_kv_heads, pos0 + n) : 0;
         if (!prefill_alloc(m, chunk, score) || (chunk <= 128 && score && !prefill_alloc(m, chunk, 0))) break;
         if (chunk <= 128) {
-            if (!hist) fprintf(stderr, "llm_prefill: cannot allocate the activations of %d tokens\n", chunk);
+            if (!hist && !each) fprintf(stderr, "llm_prefill: cannot allocate the activations of %d tokens\n", chunk);
             return -1;
         }
         chunk = (chunk + 1) / 2;
@@ -1250,6 +1256,7 @@ int prefill_all(llm_model *m, const int *ids, int n, bool sampled = false, int p
         const int M = std::min(chunk, n - i);
         if (prefill_chunk(m, ids + i, pos0 + i, M)) return -1;
         if (hist && prefill_logits(m, m->hist + (size_t)(pos0 + i) * m->info.n_logits, M)) return -1;
+        if (each && i + M < n && each(i, M)) return -1;
         if (i + M == n)
             HIP_OR_FAIL("llm_prefill", hipMemcpyAsync(m->x, m->pf_x + (size_t)(M - 1) * m->info.dim,
                                                       (size_t)m->info.dim * 4, hipMemcpyDeviceToDevice, m->st));
@@ -1259,7 +1266,8 @@ int prefill_all(llm_model *m, const int *ids, int n, bool sampled = false, int p
     HIP_OR_FAIL("llm_prefill", launch_head(m, hist));
     if (sampled) HIP_OR_FAIL("llm_prefill", launch_sampler(m));
     HIP_OR_FAIL("llm_prefill", launch_finalize(m));
-    return 0;
+    const int last = (n - 1) / chunk * chunk;
+    return each ? each(last, n - last) : 0;
 }
 
 void free_model(llm_model *m) {
@@ -1785,8 +1793,8 @@ int head_id(const llm_model *m, int row) { return m->kind == 0 ? m->head_ids_h[r
 
 // Log probabilities over `rows` rows of head logits on the device: the given head rows (`count` a row, -1: none), and the
 // top alternatives, into host arrays (NULL: not asked for).
-int score_rows(llm_model *m, const char *who, const float *logits, int rows, float temperature, const std::vector<int> &given,
-               int count, float *logp, float *entropy, int top, int *top_ids, float *top_logp) {
+int score_rows(llm_model *m, const char *who, const float *logits, int rows, float temperature, const int *given, int count,
+               float *logp, float *entropy, int top, int *top_ids, float *top_logp) {
     const int V = m->info.n_logits;
     auto pad = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const size_t tok = pad((size_t)rows * count * 4), ent = pad((size_t)rows * 4), tops = pad((size_t)rows * top * 4);
@@ -1811,7 +1819,7 @@ int score_rows(llm_model *m, const char *who, const float *logits, int rows, flo
     q.top_ids = (int *)(p + 2 * tok + ent);
     q.top_logp = (float *)(p + 2 * tok + ent + tops);
     q.work = p + 2 * tok + ent + 2 * tops;
-    if (count) HIP_OR_FAIL(who, hipMemcpyAsync((void *)q.tokens, given.data(), (size_t)rows * count * 4, hipMemcpyHostToDevice, m->st));
+    if (count) HIP_OR_FAIL(who, hipMemcpyAsync((void *)q.tokens, given, (size_t)rows * count * 4, hipMemcpyHostToDevice, m->st));
     HIP_OR_FAIL(who, launch_logprobs(q, m->st));
     auto get = [&](void *dst, const void *src, size_t b) -> int {
         if (dst && b) HIP_OR_FAIL(who, hipMemcpyAsync(dst, src, b, hipMemcpyDeviceToHost, m->st));
@@ -1910,7 +1918,7 @@ extern "C" int llm_verify(llm_model *m, int pos0, const int *tokens, const int *
         if (p >= 0) of[i] = p * most + at[p], given[(size_t)p * most + at[p]++] = row[tokens[i]];
     }
     std::vector<float> lp((size_t)n * most);
-    if (score_rows(m, who, m->ver_logits, n, 1.0f, given, most, lp.data(), nullptr, 1, next, nullptr)) return -1;
+    if (score_rows(m, who, m->ver_logits, n, 1.0f, given.data(), most, lp.data(), nullptr, 1, next, nullptr)) return -1;
     if (logp)
         for (int i = 0; i < n; i++) logp[i] = of[i] < 0 ? 0.0f : lp[of[i]];
     if (logits) HIP_OR_FAIL(who, hipMemcpy(logits, m->ver_logits, (size_t)n * V * 4, hipMemcpyDeviceToHost));
@@ -1951,23 +1959,48 @@ extern "C" int llm_score(llm_model *m, const int *ids, int n, float temperature,
     }
     if (check_ids(m, who, ids, n)) return -1;
     hipSetDevice(m->device);
-    if (!m->hist && hipMalloc(&m->hist, (size_t)m->ctx * m->info.n_logits * 4) != hipSuccess) {
-        fprintf(stderr, "%s: no room for the logits history\n", who);
-        (void)hipGetLastError();
-        m->hist = nullptr;
-        return -1;
-    }
-    // as a generation that keeps its logits takes its prompt: batched, or position by position
-    if (n == 1 || !m->prefill_on || !head_gemm_ok(m) || prefill_all(m, ids, n, false, 0, true)) {
-        HIP_OR_FAIL(who, hipStreamSynchronize(m->st));
-        for (int p = 0; p < n; p++)
-            if (set_ctrl(m, p, ids[p], 0, 0) || enqueue_step(m, true, nullptr, p, true)) return -1;
+    // a chunk's rows of logits at most, fewer where there is no room for them
+    const size_t V = m->info.n_logits;
+    if (m->score_rows < std::min(n, PREFILL_CHUNK)) {
+        dfree(m, m->score_logits);
+        m->score_rows = std::min(n, PREFILL_CHUNK);
+        while (m->score_rows && dalloc(m, &m->score_logits, m->score_rows * V * 4)) m->score_rows /= 2;
+        if (!m->score_rows) {
+            fprintf(stderr, "%s: no room for a row of logits\n", who);
+            return -1;
+        }
     }
     const std::vector<int> &row = head_rows_by_id(m);
     std::vector<int> given(n, -1);
     for (int i = 0; i + 1 < n; i++) given[i] = row[ids[i + 1]];
     std::vector<float> lp(n);
-    if (score_rows(m, who, m->hist, n, temperature, given, 1, lp.data(), entropy, top, top_ids, top_logp)) return -1;
+    auto score = [&](int first, int rows) { // of score_logits, from position `first` on
+        return score_rows(m, who, m->score_logits, rows, temperature, given.data() + first, 1, lp.data() + first,
+                          entropy ? entropy + first : nullptr, top, top_ids ? top_ids + (size_t)first * top : nullptr,
+                          top_logp ? top_logp + (size_t)first * top : nullptr);
+    };
+    auto chunk = [&](int i, int M) -> int {
+        for (int r = 0; r < M; r += m->score_rows) {
+            const int rows = std::min(m->score_rows, M - r);
+            if (prefill_logits(m, m->score_logits, rows, r)) return -1;
+            if (i + r + rows == n) // (the last position's as llm_prefill has them)
+                HIP_OR_FAIL(who, hipMemcpyAsync(m->score_logits + (rows - 1) * V, m->logits, V * 4, hipMemcpyDeviceToDevice, m->st));
+            if (score(i + r, rows)) return -1;
+        }
+        return 0;
+    };
+    // as a generation that keeps its logits takes its prompt: batched, or position by position
+    if (n == 1 || !m->prefill_on || !head_gemm_ok(m) || prefill_all(m, ids, n, false, 0, false, chunk)) {
+        HIP_OR_FAIL(who, hipStreamSynchronize(m->st));
+        for (int p = 0, r = 0; p < n; p++) {
+            if (set_ctrl(m, p, ids[p], 0, 0) || enqueue_step(m, false, nullptr, p, true)) return -1;
+            HIP_OR_FAIL(who, hipMemcpyAsync(m->score_logits + r * V, m->logits, V * 4, hipMemcpyDeviceToDevice, m->st));
+            if (++r < m->score_rows && p + 1 < n) continue;
+            if (score(p + 1 - r, r)) return -1;
+            r = 0;
+        }
+        HIP_OR_FAIL(who, hipStreamSynchronize(m->st));
+    }
     if (logp) memcpy(logp, lp.data(), (size_t)(n - 1) * 4);
     return 0;
 }

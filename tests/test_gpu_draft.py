@@ -273,3 +273,40 @@ def test_the_hosts_take_the_caches_type(exe, name):
     assert [int(x) for x in r.stdout.strip().split(",") if x] == want
     bad = subprocess.run(run[:-1] + ["int4"], capture_output=True, text=True, timeout=60)
     assert bad.returncode != 0 and "--kv int4" in bad.stderr
+
+
+def test_scores_of_a_text_hold_no_logits_of_the_whole_context(tmp_path):
+    """ten tokens scored in a context of 65536: the memory of their own rows (those of every position: 67 MB)"""
+    m = pkg().Model(synth("qwb", str(tmp_path / "m.qwb"), "tiny", 3, "max_seq=65536"), 65536)
+    assert m.info.n_logits * 65536 * 4 > 60 << 20
+    ids = prompt(m, 10, 4)
+    m.prefill(ids)
+    before = torch.cuda.mem_get_info()[0]
+    a = m.score(ids, top=3)
+    assert before - torch.cuda.mem_get_info()[0] < 16 << 20
+    lg = m.generate(ids, 1, logits=True)["logits"][:10].astype(np.float64)
+    z = lg - lg.max(1, keepdims=True)
+    z -= np.log(np.exp(z).sum(1, keepdims=True))
+    assert np.abs(a[3] - np.take_along_axis(z, np.argsort(-lg, 1, kind="stable")[:, :3], 1)).max() < 1e-5
+    m.close()
+
+
+def test_scores_over_several_chunks(tmp_path):
+    """a text longer than a chunk of 2048, its scores those of the logits that a generation keeps"""
+    m = pkg().Model(synth("qwb", str(tmp_path / "m.qwb"), "tiny", 3, "max_seq=4600"), 4600)
+    ids = prompt(m, 4500, 4)
+    lp, ent, ti, tl = m.score(ids, top=2)
+    lg = m.generate(ids, 1, logits=True)["logits"][:4500].astype(np.float64)
+    z = lg - lg.max(1, keepdims=True)
+    z -= np.log(np.exp(z).sum(1, keepdims=True))
+    row = {int(t): r for r, t in reversed(list(enumerate(m.head_ids)))}
+    want = np.array([z[i, row[int(t)]] if int(t) in row else -np.inf for i, t in enumerate(ids[1:])])
+    there = np.isfinite(want)
+    assert (lp[~there] == -np.inf).all() and np.abs(lp[there] - want[there]).max() < 1e-5
+    assert np.abs(ent + (np.exp(z) * z).sum(1)).max() < 1e-5
+    order = np.argsort(-lg, 1, kind="stable")[:, :2]
+    assert np.array_equal(ti, m.head_ids[order])
+    assert np.abs(tl - np.take_along_axis(z, order, 1)).max() < 1e-5
+    b = m.score(ids[:7], top=2)  # fewer rows than the memory held
+    assert np.array_equal(b[2], ti[:7]) and np.abs(b[0][there[:6]] - lp[:6][there[:6]]).max() < 1e-2
+    m.close()
