@@ -44,10 +44,13 @@ __device__ __forceinline__ uint32_t bf16_pair(float x, float y) { // rounded hal
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){x, y}, b2));
 }
+// (rows of a cache start at multiples of 4 bytes: a store of that alignment, still one instruction)
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(4)));
 template <int RT>
 __device__ __forceinline__ void put4(uint8_t *p, float4 v) {
-    if constexpr (RT == LLM_F32) *(float4 *)p = v;
-    else *(uint2 *)p = make_uint2(bf16_pair(v.x, v.y), bf16_pair(v.z, v.w));
+    if constexpr (RT == LLM_F32) *(f32x4u *)p = (f32x4u){v.x, v.y, v.z, v.w};
+    else *(u32x2u *)p = (u32x2u){bf16_pair(v.x, v.y), bf16_pair(v.z, v.w)};
 }
 
 // x / s (s > 0, both scaled so that no step underflows) rounded to odd: the fp32 quotient that lies towards zero, its last
@@ -147,15 +150,13 @@ __global__ void __launch_bounds__(256) k_kv_read(KvArgs a) {
         if (e >= a.hs) continue;
         float4 v;
         if constexpr (CS > 1) {
-            // (rows of a cache start at multiples of 4 bytes)
             if constexpr (CS == 4) {
-                const float *f = (const float *)(src + (size_t)e * 4);
+                const f32x4u f = *(const f32x4u *)(src + (size_t)e * 4);
                 v = make_float4(f[0], f[1], f[2], f[3]);
             } else {
-                const uint32_t *u = (const uint32_t *)(src + (size_t)e * 2);
-                const uint32_t u0 = u[0], u1 = u[1];
-                v = make_float4(__uint_as_float(u0 << 16), __uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 << 16),
-                                __uint_as_float(u1 & 0xffff0000u));
+                const u32x2u u = *(const u32x2u *)(src + (size_t)e * 2);
+                v = make_float4(__uint_as_float(u[0] << 16), __uint_as_float(u[0] & 0xffff0000u), __uint_as_float(u[1] << 16),
+                                __uint_as_float(u[1] & 0xffff0000u));
             }
         } else {
             const uint32_t w = *(const uint32_t *)(src + e);

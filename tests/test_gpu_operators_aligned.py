@@ -1,0 +1,41 @@
+"""Cache rows that start at any multiple of 4 bytes, which is all that the operators ask of them."""
+import pytest
+
+from helpers import pkg
+from test_gpu_operators import CACHES, DEV, ROWS, attention_check, gen, quantized, same, tree_masks
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", ["fp32", "bf16"])
+@pytest.mark.parametrize("cache", list(CACHES))
+@pytest.mark.parametrize("hs,off,pad", [(64, 1, 1), (64, 3, 2), (128, 1, 3), (48, 2, 1), (256, 1, 0)])
+def test_rows_at_multiples_of_4_bytes(cache, rows, hs, off, pad):
+    """off and pad: 4-byte words before the first row, and between a row and the next"""
+    g, b, h, ctx, t, heads = gen(hs + off), 2, 2, 70, 5, 4
+    dt = CACHES[cache]
+    word = 4 // torch.empty(0, dtype=dt).element_size()
+    step = hs + pad * word
+    mem = [torch.zeros(off * word + b * h * ctx * step, dtype=torch.float32).to(dt).to(DEV) for _ in range(2)]
+    k, v = (m[off * word:].as_strided((b, h, ctx, hs), (h * ctx * step, ctx * step, step, 1)) for m in mem)
+    assert k.data_ptr() % 16 == 4 * off % 16
+    ks, vs = (torch.zeros(b, h, ctx, device=DEV) for _ in range(2)) if cache in ("int8", "e4m3") else (None, None)
+    x = [torch.randn(b, ctx, h, hs, generator=g).to(ROWS[rows]) for _ in range(2)]
+    zero = torch.zeros(b, dtype=torch.int32, device=DEV)
+    pkg().kv_write(x[0].to(DEV), x[1].to(DEV), k, v, zero, k_scale=ks, v_scale=vs)
+    back = pkg().kv_read(k, v, zero, ctx, k_scale=ks, v_scale=vs)
+    vals = []
+    for y, store, s, got in zip(x, (k, v), (ks, vs), back):
+        val, code, scale = quantized(y.double(), cache)
+        assert same(store.float(), code.transpose(1, 2)) and same(got, val.float())
+        assert s is None or same(s, scale.transpose(1, 2))
+        vals.append(val.transpose(1, 2))
+    for m, n in zip(mem, (step, step)):  # what lies between the rows stays
+        rest = m[off * word:].view(-1, n)[:, hs:]
+        assert (m[:off * word].float() == 0).all() and (rest.float() == 0).all()
+    q = torch.randn(b, t, heads, hs, generator=g).to(ROWS[rows])
+    mask, lens = tree_masks(g, b, t), [64, 7]
+    got = pkg().tree_attention(q.to(DEV), k, v, torch.tensor(lens, dtype=torch.int32, device=DEV),
+                               mask=torch.from_numpy(mask.view("int64")).to(DEV), k_scale=ks, v_scale=vs)
+    attention_check(q, vals[0], vals[1], lens, [t] * b, mask, hs ** -0.5, got, ctx, cache)
