@@ -47,7 +47,6 @@ class OpDevice {
         back_ = cur;
         return true;
     }
-    int device() const { return dev_; }
 
   private:
     const char *who_;

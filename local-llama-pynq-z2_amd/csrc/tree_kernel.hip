@@ -774,10 +774,11 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
 // once; the units of a row change places by its number, so that the sixteen rows of a read are in different ones, and
 // the runs of a write in half of them.
 struct __align__(16) TreeStep {
-    static constexpr int KU = HSP / 8; // units of a K row
+    static constexpr int KU = 16; // units of a K row
+    static_assert(HSP == 8 * KU, "rows of 128 values");
     uint4 k[64 * KU], v[HSP * 8];
     __device__ __forceinline__ static int k_at(int row, int unit) {
-        return row * KU + (unit ^ (KU == 16 ? row & 15 : (row >> 1) & 7));
+        return row * KU + (unit ^ (row & 15));
     }
     __device__ __forceinline__ static int v_at(int dim, int unit) { return dim * 8 + (unit ^ ((dim >> 1) & 7)); }
 };
@@ -796,7 +797,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
     constexpr bool APART = NW == 8; // waves 4 to 7 fetch K, 0 to 3 V; four waves fetch both
     constexpr int KN = HSP / 8, KL = 64 * KN / 256; // 16-byte pieces of a K row, of a thread
     constexpr int VN = HSP / 4;                     // runs of four dimensions: a thread takes one, at eight positions
-    constexpr int VAT = APART ? 0 : 4 * KL, NR = APART ? (KL > 4 ? 4 * KL : 16) : 4 * KL + 16;
+    constexpr int VAT = APART ? 0 : 4 * KL, NR = APART ? 16 : 4 * KL + 16;
     __shared__ TreeStep sm[2];
     __shared__ uint32_t sm_bad[2]; // new tokens whose V row is not finite
 
@@ -807,7 +808,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 4) k_tree_rows(TreeArgs
 
     const int row0 = p.row0 + wave * 16 * R;
     const bool works = wave * 16 * R < a.block_rows && row0 < p.rows; // (a wave without rows still fetches)
-    const bool does_k = !APART || wave >= 4, does_v = (!APART || wave < 4) && (VN == 32 || (threadIdx.x & 255) < 8 * VN);
+    const bool does_k = !APART || wave >= 4, does_v = !APART || wave < 4;
     const uint32_t hb = (uint32_t)(a.hs * 2);
     const int64_t at0 = p.b * a.seq + p.h * a.head + (int64_t)p.first * 64 * a.pos;
     const uint8_t *kp = a.k + at0, *vp = a.v + at0;
