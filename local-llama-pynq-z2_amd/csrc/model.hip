@@ -22,6 +22,7 @@
 #include <unistd.h>
 
 #include <algorithm>
+#include <exception>
 #include <functional>
 #include <string>
 #include <vector>
@@ -144,16 +145,24 @@ struct llm_model {
 namespace {
 
 template <typename T>
-int dalloc(llm_model *m, T **p, size_t bytes) {
+int dalloc(llm_model *m, T **p, size_t bytes, bool quiet = false) {
     void *v = nullptr;
     if (hipMalloc(&v, bytes ? bytes : 16) != hipSuccess) {
-        fprintf(stderr, "llm_open: cannot allocate %zu bytes of HBM\n", bytes);
+        if (!quiet) fprintf(stderr, "llm_open: cannot allocate %zu bytes of HBM\n", bytes);
         (void)hipGetLastError();
         return -1;
     }
     // the zeros are there before a copy or kernel of the model's own stream, which does not wait for the null stream
-    if (hipMemset(v, 0, bytes ? bytes : 16) != hipSuccess || hipStreamSynchronize(nullptr) != hipSuccess) return -1;
-    m->allocs.push_back(v);
+    bool ok = hipMemset(v, 0, bytes ? bytes : 16) == hipSuccess && hipStreamSynchronize(nullptr) == hipSuccess;
+    try {
+        if (ok) m->allocs.push_back(v);
+    } catch (const std::exception &) { // (no host memory: as without device memory)
+        ok = false;
+    }
+    if (!ok) {
+        hipFree(v);
+        return -1;
+    }
     *p = (T *)v;
     return 0;
 }
@@ -1735,7 +1744,20 @@ extern "C" int llm_set_prefill(llm_model *m, int on) {
 
 // ---- the cache's type, drafted trees, scores
 
-extern "C" int llm_set_kv(llm_model *m, int type) {
+namespace {
+
+// A C entry point's body: an exception (of host memory that is used up) becomes an error.
+template <typename F>
+int no_throw(const char *who, F &&body) {
+    try {
+        return body();
+    } catch (const std::exception &e) {
+        fprintf(stderr, "%s: %s\n", who, e.what());
+        return -1;
+    }
+}
+
+int set_kv(llm_model *m, int type) {
     if (!m) return -1;
     hipSetDevice(m->device);
     HIP_OR_FAIL("llm_set_kv", hipStreamSynchronize(m->st));
@@ -1749,6 +1771,10 @@ extern "C" int llm_set_kv(llm_model *m, int type) {
                                   : "llm_set_kv: head size %d (multiples of 16)\n", m->hs);
         return -1;
     }
+    // the o projection takes the attention as one merged slice: (0, 1) for every head behind its output
+    std::vector<float> one((size_t)2 * m->info.n_heads);
+    for (int h = 0; h < m->info.n_heads; h++) one[2 * h] = 0.0f, one[2 * h + 1] = 1.0f;
+    HIP_OR_FAIL("llm_set_kv", hipMemcpy(m->att_one + m->info.dim, one.data(), one.size() * 4, hipMemcpyHostToDevice));
     drop_graphs(m, false);
     // the new cache beside the old one: without room for it the old one stays
     const size_t layer = (size_t)m->ctx * m->kv_dim, all = layer * m->info.n_layers, es = op_type_bytes(type);
@@ -1770,11 +1796,13 @@ extern "C" int llm_set_kv(llm_model *m, int type) {
     dfree(m, m->kc), dfree(m, m->vc), dfree(m, m->kq), dfree(m, m->vq), dfree(m, m->ks), dfree(m, m->vs);
     dfree(m, m->tree_work), dfree(m, m->ver_logits), dfree(m, m->ver_mask), dfree(m, m->ver_len), dfree(m, m->ver_depth);
     m->kc = kc, m->vc = vc, m->kq = kq, m->vq = vq, m->ks = ks, m->vs = vs, m->tree_work = work;
-    // the o projection takes the attention as one merged slice: (0, 1) for every head behind its output
-    std::vector<float> one((size_t)2 * m->info.n_heads);
-    for (int h = 0; h < m->info.n_heads; h++) one[2 * h] = 0.0f, one[2 * h + 1] = 1.0f;
-    HIP_OR_FAIL("llm_set_kv", hipMemcpy(m->att_one + m->info.dim, one.data(), one.size() * 4, hipMemcpyHostToDevice));
     return 0;
+}
+
+} // namespace
+
+extern "C" int llm_set_kv(llm_model *m, int type) {
+    return no_throw("llm_set_kv", [&] { return set_kv(m, type); });
 }
 
 extern "C" int llm_get_kv(const llm_model *m) { return m ? m->kv_type : -1; }
@@ -1843,10 +1871,7 @@ int check_ids(const llm_model *m, const char *who, const int *ids, int n) {
     return 0;
 }
 
-} // namespace
-
-extern "C" int llm_verify(llm_model *m, int pos0, const int *tokens, const int *parents, int n, int *next, float *logp,
-                          float *logits) {
+int verify(llm_model *m, int pos0, const int *tokens, const int *parents, int n, int *next, float *logp, float *logits) {
     const char *who = "llm_verify";
     if (!m || !tokens || n < 1 || n > 64 || pos0 < 0) {
         fprintf(stderr, "%s: bad arguments (1 to 64 tokens)\n", who);
@@ -1925,6 +1950,13 @@ extern "C" int llm_verify(llm_model *m, int pos0, const int *tokens, const int *
     return 0;
 }
 
+} // namespace
+
+extern "C" int llm_verify(llm_model *m, int pos0, const int *tokens, const int *parents, int n, int *next, float *logp,
+                          float *logits) {
+    return no_throw("llm_verify", [&] { return verify(m, pos0, tokens, parents, n, next, logp, logits); });
+}
+
 extern "C" int llm_keep(llm_model *m, int pos0, const int *path, int n) {
     if (!m || !path || n < 1 || n > 64 || pos0 < 0) {
         fprintf(stderr, "llm_keep: bad arguments\n");
@@ -1948,8 +1980,10 @@ extern "C" int llm_keep(llm_model *m, int pos0, const int *path, int n) {
     return 0;
 }
 
-extern "C" int llm_score(llm_model *m, const int *ids, int n, float temperature, float *logp, float *entropy, int top,
-                         int *top_ids, float *top_logp) {
+namespace {
+
+int score(llm_model *m, const int *ids, int n, float temperature, float *logp, float *entropy, int top, int *top_ids,
+          float *top_logp) {
     const char *who = "llm_score";
     if (!m || !ids || n < 1 || n > m->ctx || !(temperature >= 1e-30f && temperature <= 1e30f) || top < 0 || top > 32 ||
         top > m->info.n_logits) {
@@ -1964,7 +1998,7 @@ extern "C" int llm_score(llm_model *m, const int *ids, int n, float temperature,
     if (m->score_rows < std::min(n, PREFILL_CHUNK)) {
         dfree(m, m->score_logits);
         m->score_rows = std::min(n, PREFILL_CHUNK);
-        while (m->score_rows && dalloc(m, &m->score_logits, m->score_rows * V * 4)) m->score_rows /= 2;
+        while (m->score_rows && dalloc(m, &m->score_logits, m->score_rows * V * 4, true)) m->score_rows /= 2;
         if (!m->score_rows) {
             fprintf(stderr, "%s: no room for a row of logits\n", who);
             return -1;
@@ -1974,7 +2008,7 @@ extern "C" int llm_score(llm_model *m, const int *ids, int n, float temperature,
     std::vector<int> given(n, -1);
     for (int i = 0; i + 1 < n; i++) given[i] = row[ids[i + 1]];
     std::vector<float> lp(n);
-    auto score = [&](int first, int rows) { // of score_logits, from position `first` on
+    auto score_from = [&](int first, int rows) { // of score_logits, from position `first` on
         return score_rows(m, who, m->score_logits, rows, temperature, given.data() + first, 1, lp.data() + first,
                           entropy ? entropy + first : nullptr, top, top_ids ? top_ids + (size_t)first * top : nullptr,
                           top_logp ? top_logp + (size_t)first * top : nullptr);
@@ -1985,7 +2019,7 @@ extern "C" int llm_score(llm_model *m, const int *ids, int n, float temperature,
             if (prefill_logits(m, m->score_logits, rows, r)) return -1;
             if (i + r + rows == n) // (the last position's as llm_prefill has them)
                 HIP_OR_FAIL(who, hipMemcpyAsync(m->score_logits + (rows - 1) * V, m->logits, V * 4, hipMemcpyDeviceToDevice, m->st));
-            if (score(i + r, rows)) return -1;
+            if (score_from(i + r, rows)) return -1;
         }
         return 0;
     };
@@ -1996,13 +2030,20 @@ extern "C" int llm_score(llm_model *m, const int *ids, int n, float temperature,
             if (set_ctrl(m, p, ids[p], 0, 0) || enqueue_step(m, false, nullptr, p, true)) return -1;
             HIP_OR_FAIL(who, hipMemcpyAsync(m->score_logits + r * V, m->logits, V * 4, hipMemcpyDeviceToDevice, m->st));
             if (++r < m->score_rows && p + 1 < n) continue;
-            if (score(p + 1 - r, r)) return -1;
+            if (score_from(p + 1 - r, r)) return -1;
             r = 0;
         }
         HIP_OR_FAIL(who, hipStreamSynchronize(m->st));
     }
     if (logp) memcpy(logp, lp.data(), (size_t)(n - 1) * 4);
     return 0;
+}
+
+} // namespace
+
+extern "C" int llm_score(llm_model *m, const int *ids, int n, float temperature, float *logp, float *entropy, int top,
+                         int *top_ids, float *top_logp) {
+    return no_throw("llm_score", [&] { return score(m, ids, n, temperature, logp, entropy, top, top_ids, top_logp); });
 }
 
 // Test hook: the bytes that one prefill activation buffer and the strict score rows may take before their allocation
