@@ -103,6 +103,25 @@ __device__ __forceinline__ f32x4 product(const Frag<CT, 1> &a, const Frag<CT, NP
     }
     return d;
 }
+// Scores of 16 positions and 16 rows.  fp32: an instruction adds its four products one after another, so one chain over all
+// dimensions would be off by up to twice as much as four do (and a score's error is the weight's).
+template <int CT, int NP>
+struct Scores {
+    static constexpr int N = CT == LLM_F32 ? 4 : 1;
+    f32x4 c[N] = {};
+    __device__ __forceinline__ void add(const Frag<CT, 1> &a, const Frag<CT, NP> &b) {
+        if constexpr (CT == LLM_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i % 4] = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c[i % 4], 0, 0, 0);
+        } else {
+            c[0] = product(a, b, c[0]);
+        }
+    }
+    __device__ __forceinline__ f32x4 sum() const {
+        if constexpr (CT == LLM_F32) return (c[0] + c[1]) + (c[2] + c[3]);
+        else return c[0];
+    }
+};
 template <int CT, int NP>
 __device__ __forceinline__ void fill(Frag<CT, NP> &f, const float (&x)[8]) {
 #pragma unroll
@@ -579,8 +598,7 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
         f32x4 x[R][NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-#pragma unroll
-            for (int r = 0; r < R; r++) x[r][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+Scores<CT, Pc::Q> sums[R];
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 Frag<CT, 1> kf;
@@ -595,8 +613,10 @@ __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tr
                     kf.v[0] = (u32x4){codes2<CT, 0>(u0), codes2<CT, 1>(u0), codes2<CT, 0>(u1), codes2<CT, 1>(u1)};
                 }
 #pragma unroll
-                for (int r = 0; r < R; r++) x[r][t] = product(kf, qf[r][s], x[r][t]);
+                for (int r = 0; r < R; r++) sums[r].add(kf, qf[r][s]);
             }
+#pragma unroll
+            for (int r = 0; r < R; r++) x[r][t] = sums[r].sum();
         }
         if constexpr (SCALED) {
             my_s[lane] = __uint_as_float(skr);

@@ -242,3 +242,31 @@ def test_a_scale_of_zero_over_large_scores(cache):
     mask = tree_masks(g, b, t)
     got = pkg().tree_attention(q.to(DEV), k, v, ints([length]), mask=bits(mask), k_scale=ks, v_scale=vs, scale=0.0)
     check(q, kv, vv, [length], mask, 0.0, got, cache)
+
+
+@pytest.mark.parametrize("hs", [64, 128, 256])
+def test_scores_over_fp32_caches_are_sums_of_short_chains(hs):
+    """two positions of about one score and values of +1 and -1 show a score difference as tanh(difference / 2).  A chain of n
+    additions is off by about u sqrt(n^2 / 2) of a term's size, four of n / 4 by half of that: the rms error is held to 3/4 of a
+    chain's"""
+    g = gen(hs)
+    b, h = 256, 4
+    k = torch.randn(b, h, 2, hs, generator=g) * 4
+    q = torch.randn(b, 1, h, hs, generator=g) * 4
+    qd = q[:, 0].double()  # [b, h, hs]
+    # the largest element of each query evens the scores out
+    at = qd.abs().argmax(-1, keepdim=True)
+    diff = ((k[:, :, 0] - k[:, :, 1]).double() * qd).sum(-1, keepdim=True) / qd.gather(-1, at)
+    k[:, :, 1] = k[:, :, 1].scatter_add(-1, at, diff.float())
+    v = torch.ones(b, h, 2, hs)
+    v[:, :, 1] = -1
+    want = ((k[:, :, 0].double() - k[:, :, 1].double()) * qd).sum(-1)
+    assert float(want.abs().max()) < 1e-3
+    lens = torch.ones(b, dtype=torch.int32, device=DEV)
+    got = pkg().tree_attention(q.to(DEV), k.to(DEV), v.to(DEV), lens, scale=1.0)[:, 0, :, 0].double().cpu()
+    own = 2 * torch.atanh(got) - want
+    chain = torch.zeros(b, h, 2, dtype=torch.float64)
+    for i in range(hs):
+        chain = (chain + k[..., i].double() * qd[:, :, None, i]).float().double()
+    one = chain[..., 0] - chain[..., 1] - want
+    assert float(own.square().mean().sqrt()) < 0.75 * float(one.square().mean().sqrt())
