@@ -345,6 +345,8 @@ def tree_attention(q, k, v, lens, n=None, mask=None, k_scale=None, v_scale=None,
     c, (b, _, ctx, hs) = _kv(k, v, k_scale, v_scale)
     torch, fresh = _torch[0], out is None
     t, heads = q.shape[1:3]
+    if mask is not None and mask.dim() > 1 and mask.shape != (b, t):
+        raise ValueError(f"mask: int64 {(b, t)} are needed")
     if fresh:
         out = torch.empty(b, t, heads, hs, dtype=q.dtype, device=k.device)
     L, bound = lib(), ctx if max_len is None else max_len

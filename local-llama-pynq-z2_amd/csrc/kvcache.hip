@@ -200,12 +200,28 @@ int kv_rows(const char *who, bool write, const llm_kv *c, const llm_rows *k, con
         fprintf(stderr, "%s: bad arguments\n", who);
         return -1;
     }
+    if (!op_check_cache(c, nullptr, who)) return -1;
+    if (write) {
+        const int count[] = {c->n_seq, c->n_kv, c->n_seq, c->n_kv};
+        const int64_t stride[] = {c->seq, c->head, c->s_seq, c->s_head};
+        if (!op_check_apart(who, "the cache", op_scaled(c->type) ? 4 : 2, count, stride)) return -1;
+    } else {
+        for (const llm_rows *r : {k, v}) {
+            const int count[] = {c->n_seq, max_n, c->n_kv};
+            const int64_t stride[] = {r->seq, r->tok, r->head};
+            if (!op_check_apart(who, "the rows", 3, count, stride)) return -1;
+        }
+    }
     OpDevice dev(who);
     if (!op_check_cache(c, &dev, who)) return -1;
     if (!max_n || !c->n_seq) return 0;
     if (!op_check_rows(k, "k", &dev, who) || !op_check_rows(v, "v", &dev, who) || !dev.holds(pos, "pos") ||
         (n && !dev.holds(n, "n")))
         return -1;
+    if (write && c->k == c->v) {
+        fprintf(stderr, "%s: k and v are the same memory\n", who);
+        return -1;
+    }
     if (k->type != v->type) {
         fprintf(stderr, "%s: k and v rows of different types\n", who);
         return -1;

@@ -59,6 +59,17 @@ bool op_check_cache(const llm_kv *c, OpDevice *dev, const char *who);
 // Rows of activations beside it: fp32 or bf16, vectors of 4 values aligned.
 bool op_check_rows(const llm_rows *r, const char *what, OpDevice *dev, const char *who);
 
+// Memory that a call writes: sequences, heads and tokens whose stride is zero lie on one another, and what is left there would
+// depend on timing.  Prints what is wrong.  dims, strides: of as many as there are.
+static inline bool op_check_apart(const char *who, const char *what, int dims, const int *count, const int64_t *stride) {
+    for (int i = 0; i < dims; i++)
+        if (count[i] > 1 && stride[i] == 0) {
+            fprintf(stderr, "%s: a stride of zero in %s, which is written\n", who, what);
+            return false;
+        }
+    return true;
+}
+
 // The launches behind the entry points, for callers that know their arguments to be right (the model).
 
 struct KvCall {

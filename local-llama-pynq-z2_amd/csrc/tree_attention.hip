@@ -218,6 +218,9 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
         fprintf(stderr, "%s: scale %g\n", who, scale);
         return -1;
     }
+    const int count[] = {c->n_seq, max_n, n_heads};
+    const int64_t stride[] = {out->seq, out->tok, out->head};
+    if (!op_check_apart(who, "out", 3, count, stride)) return -1;
     OpDevice dev(who);
     if (!op_check_cache(c, &dev, who)) return -1;
     if (!max_n || !c->n_seq) return 0;

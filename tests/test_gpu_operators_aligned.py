@@ -1,4 +1,4 @@
-"""Cache rows that start at any multiple of 4 bytes, which is all that the operators ask of them."""
+"""Cache rows that start at any multiple of 4 bytes, which is all that the operators ask of them, and memory that lies on itself."""
 import pytest
 
 from helpers import pkg
@@ -39,3 +39,26 @@ def test_rows_at_multiples_of_4_bytes(cache, rows, hs, off, pad):
     got = pkg().tree_attention(q.to(DEV), k, v, torch.tensor(lens, dtype=torch.int32, device=DEV),
                                mask=torch.from_numpy(mask.view("int64")).to(DEV), k_scale=ks, v_scale=vs)
     attention_check(q, vals[0], vals[1], lens, [t] * b, mask, hs ** -0.5, got, ctx, cache)
+
+
+def test_shared_memory_is_read_and_not_written(capfd):
+    """sequences that share one cache (a stride of zero), and K and V in one tensor: attention and reads take them, writes do not"""
+    g, b, h, ctx, hs = gen(3), 3, 2, 40, 64
+    one = torch.randn(1, h, ctx, hs, generator=g).to(DEV)
+    shared, apart = one.expand(b, h, ctx, hs), one.expand(b, h, ctx, hs).contiguous()
+    lens = torch.tensor([30, 7, 0], dtype=torch.int32, device=DEV)
+    q = torch.randn(b, 2, 4, hs, generator=g).to(DEV)
+    assert torch.equal(pkg().tree_attention(q, shared, shared, lens), pkg().tree_attention(q, apart, apart.clone(), lens))
+    for x, y in zip(pkg().kv_read(shared, shared, lens, 5), pkg().kv_read(apart, apart, lens, 5)):
+        assert torch.equal(x, y)
+    rows = torch.randn(b, 2, h, hs, generator=g).to(DEV)
+    for k, v, says in ((shared, one.clone().expand(b, h, ctx, hs), "a stride of zero"), (apart, apart, "the same memory")):
+        old = k.clone()
+        with pytest.raises(RuntimeError):
+            pkg().kv_write(rows, rows, k, v, lens)
+        assert says in capfd.readouterr().err
+        assert torch.equal(k, old)
+    for out in (torch.zeros(1, 2, 4, hs, device=DEV).expand(b, 2, 4, hs), torch.zeros(b, 1, 4, hs, device=DEV).expand(b, 2, 4, hs)):
+        with pytest.raises(RuntimeError):
+            pkg().tree_attention(q, apart, apart, lens, out=out)
+        assert "a stride of zero" in capfd.readouterr().err
