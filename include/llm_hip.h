@@ -140,8 +140,9 @@ int llm_sampler_state(llm_model *m, unsigned long long *rng);
 /* The type of the K/V cache: LLM_F32 (the reference's, as llm_open leaves it), LLM_BF16, LLM_I8 or LLM_E4M3.  The 8-bit types
  * hold a row of each position and kv head as codes with one fp32 scale (a quarter of the memory and of a step's cache reads,
  * plus 4 bytes a row): decode steps quantize the new row and attend over the codes, prompts attend over the values that the
- * codes stand for.  The cache is empty afterwards: prompts start at position 0 again.  Not in the strict mode; head sizes
- * that are multiples of 16.  Returns 0, or -1 with the old cache kept.  llm_get_kv: the type, -1 for a NULL model. */
+ * codes stand for.  The cache is empty afterwards: prompts start at position 0 again (of the type it has already, it stays as it
+ * is).  Not in the strict mode; head sizes that are multiples of 16.  Returns 0, or -1 with the old cache kept.  llm_get_kv:
+ * the type, -1 for a NULL model. */
 int llm_set_kv(llm_model *m, int type);
 int llm_get_kv(const llm_model *m);
 
@@ -160,7 +161,7 @@ int llm_keep(llm_model *m, int pos0, const int *path, int n);
  * keeps its logits takes one (llm_set_prefill): logp[i], i < n - 1, of token i + 1 after tokens 0 .. i (-infinity outside
  * the trimmed head); entropy[i], i < n, of the distribution after token i; top_ids and top_logp, n x top, its `top` <= 32
  * most likely tokens and their log probabilities, descending.  Logits are divided by temperature.  The arrays may be NULL.
- * Returns 0 or -1. */
+ * It holds the logits of at most 2048 tokens at once, of fewer where there is no room.  Returns 0 or -1. */
 int llm_score(llm_model *m, const int *ids, int n, float temperature, float *logp, float *entropy, int top, int *top_ids,
               float *top_logp);
 
@@ -174,12 +175,13 @@ void llm_close(llm_model *m);
  *
  * Every address is device memory (checked), all on one device, which need not be the current one.  The launches go to
  * `stream` (a hipStream_t of that device; NULL: its default stream) and nothing is synchronized, allocated or kept, so a
- * call can be captured into a graph.  Scratch memory is the caller's: calls that may overlap need one each.
+ * call can be captured into a graph.  Scratch memory is the caller's: calls that may overlap need one each.  There is no
+ * backward pass.  What a call reads may lie on itself (strides of zero: sequences that share a cache), what it writes may not.
  * Returns 0, or -1 with a message on stderr; nothing is launched then. */
 
 /* The K and V rows of n_seq sequences, ctx positions and n_kv heads of hs values (a multiple of 16, at most 256).  fp32
- * and bf16 rows hold the values.  int8 and e4m3 rows hold codes, and k_scale / v_scale a float per row: value = code *
- * scale.  Strides are in values (of K and V alike) and in floats (of the scales); the values of a row lie together, rows
+ * and bf16 rows hold the values.  int8 and e4m3 rows hold codes, and k_scale / v_scale a float per row, of either sign: value =
+ * code * scale.  Strides are in values (of K and V alike) and in floats (of the scales); the values of a row lie together, rows
  * start at multiples of 4 bytes, and a position's stride is at most 16 MiB. */
 typedef struct {
     void *k, *v;
@@ -199,7 +201,8 @@ typedef struct {
 
 /* Rows of K and V into the cache: token t < n[b] (n NULL: max_n, else at most max_n) of sequence b at position pos[b] + t.
  * Positions outside 0 .. ctx - 1 are not written.  int8: scale = amax / 127 rounded to fp32, code = the quotient value /
- * scale, exact, rounded half to even; e4m3: amax / 448, the quotient rounded to e4m3 half to even.  A row of zeros has
+ * scale, exact, rounded half to even; e4m3: amax / 448, the quotient rounded to e4m3 half to even (neither past 127 or 448, where
+ * the smallest scales, rounded, would lead).  A row of zeros has
  * scale 0; a row that holds an infinity or a NaN gets scale NaN and reads back as NaN.  pos and n: n_seq ints each. */
 int llm_kv_write(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int *pos, const int *n, int max_n,
                  void *stream);
@@ -212,9 +215,14 @@ int llm_kv_read(const llm_kv *c, const llm_rows *k, const llm_rows *v, const int
  * sequence b has its K and V rows at position lens[b] + i; it sees positions 0 .. lens[b] - 1 and the new tokens j whose
  * bit j is set in mask[b * max_n + i] (a drafted tree: its ancestors and itself; mask NULL: j <= i, a chain; max_n 1: the
  * decode step).  out[b][i][h] = sum_p softmax_p(scale q.k_p) v_p over the kv head h / (n_heads / n_kv), in fp32, rounded to
- * out's type (q's type).  A token that sees nothing gets zeros.  Rows behind n[b] are left as they were, or zeroed
- * (zero_rest); positions from ctx on are not seen.  What is not seen has no influence, infinities and NaN included; a new
- * token whose V row holds one makes the tokens that see it NaN.  n_heads / n_kv is at most 64.  max_len is the host's upper
+ * out's type (q's type); the scale is finite, of either sign, and 0 gives the mean.  A token that sees nothing gets zeros.  Rows
+ * behind n[b] are left as they were, or zeroed (zero_rest); positions from ctx on are not seen, and lens below 0 count as 0.
+ * What is not seen changes no bit, infinities and NaN included; a new token whose V row holds one (a value, a code, a scale)
+ * makes the tokens that see it NaN.
+ * Products of matrices hold less than fp32 where the cache does: over 8-bit caches queries and weights (times V scale) have 22
+ * bits, a weight no finer step than 2^-39 of the largest V scale that the token sees; over bf16 caches fp32 queries and their
+ * weights have 24, the weights of bf16 queries 16.
+ * n_heads / n_kv is at most 64.  max_len is the host's upper
  * bound of lens[] (lens above it are right too, slower); `work` has llm_tree_attention_work() bytes, 16-byte aligned, and is
  * one call's until it has run. */
 size_t llm_tree_attention_work(const llm_kv *c, int n_heads, int max_n, int max_len);
@@ -225,7 +233,8 @@ int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_rows *out, 
 /* Log probabilities over `rows` rows of `vocab` logits (type LLM_F32 or LLM_BF16, `stride` values from row to row), of
  * y = logit / temperature (1e-30 to 1e30): lse = log sum exp y, entropy = -sum p log p (nats), logp[r][i] =
  * y[tokens[r][i]] - lse for n_tokens tokens a row (an id outside 0 .. vocab - 1: -infinity), and the `top` <= 32 largest
- * logits of the row in descending order (equal ones, and NaN, which count as the largest: lowest index first) with their log probabilities.
+ * logits of the row in descending order (equal ones, and NaN, which count as the largest: lowest index first) with their log
+ * probabilities.
  * Masked logits of -infinity have probability 0.  A row with +infinity or NaN, or of -infinity alone, has NaN for its
  * results (lse of -infinity alone: -infinity).  entropy and lse may be NULL, logp with n_tokens 0 and the two
  * top arrays with top 0.  `work` has llm_logprobs_work() bytes, 16-byte aligned, and is one call's until it has run. */

@@ -336,9 +336,9 @@ def kv_read(k, v, pos, tokens, n=None, k_scale=None, v_scale=None, out=None, dty
 
 
 def tree_attention(q, k, v, lens, n=None, mask=None, k_scale=None, v_scale=None, scale=None, max_len=None, out=None):
-    """Attention of the newest tokens of every sequence over its cache (llm_tree_attention).  q [seqs, tokens <= 64, heads,
-    head size] float32 or bfloat16; the cache as in kv_write; token i of sequence b has its rows at position lens[b] + i and
-    sees the positions before lens[b] and the new tokens of mask[b, i]'s bits (int64; None: a chain).  n[b] tokens count
+    """Attention of the newest tokens of every sequence over its cache (llm_tree_attention; no gradient).  q [seqs, tokens <= 64,
+    heads, head size] float32 or bfloat16; the cache as in kv_write; token i of sequence b has its rows at position lens[b] + i
+    and sees the positions before lens[b] and the new tokens of mask[b, i]'s bits (int64; None: a chain).  n[b] tokens count
     (None: all); scale None: head size ** -0.5; max_len: the host's bound of lens (None: the cache's positions).  Returns
     a new tensor (rows behind n[b]: zero), or `out` (such rows left as they were)."""
     _no_grad(q, k, v, k_scale, v_scale, out)

@@ -68,8 +68,9 @@ __device__ __forceinline__ float div_to_odd(float x, float s) {
 
 // A row: scale = largest magnitude / 127 (448), codes = value / scale.  Bytes in, bytes out: a DPP row of 16 lanes takes one
 // row of a head, lane l its values 4 l .. 4 l + 3 and every 64th from there; the largest magnitude is four DPP steps, the scale
-// and the codes follow from registers, so the row is read once.  Memory bounds it, and for few rows a launch's latency: 2048
-// fp32 tokens of 4 heads of 128 into int8 6.4 us, 1.7 TB/s; one token 2.6.
+// and the codes follow from registers, so the row is read once.  Few rows are bound by a launch's latency (one token 2.7 us), many
+// by vector instructions, a wave's 402 with the exact quotients: 2048 fp32 tokens of 4 heads of 128 into int8 6.4 us (1.7 TB/s),
+// and they are issued in 6.4k of the 10k cycles that a SIMD's waves live.
 template <int CT, int RT>
 __global__ void __launch_bounds__(256) k_kv_write(KvArgs a) {
     constexpr int RS = RT == LLM_F32 ? 4 : 2;

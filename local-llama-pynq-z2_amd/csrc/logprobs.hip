@@ -5,8 +5,10 @@
 // The largest logits: a value goes into the block's list in LDS only if it is above a bound that at least `top` values
 // reach.  The bound starts as the top-th largest of a wave's 64 lane maxima (at least `top` values reach that), and becomes
 // the list's own top-th value when the list is cut, so that after the first steps almost nothing is listed and the
-// logits are read at the rate of memory: 1021 rows of 151936 fp32 logits 140 us, 4.4 TB/s.  Few rows are bound by latency: one
-// of 65536 logits, top 20, 7.5 us and the segments' join 6.4; 37 of 151936 bf16 logits, top 5, 11.6 and 3.9.
+// logits are read at the rate of memory: 1021 rows of 151936 fp32 logits 132 us, 4.7 TB/s.  Few rows are bound by what every
+// segment begins with, the first bound's 32 dependent ballots and the first cut of the list, and by a second launch: one row of
+// 65536 logits, top 20, 7.8 us and the segments' join 6.0; 37 of 151936 bf16 logits, top 5, 12.0 and 3.9 (vector instructions in
+// 11k of the 20k cycles that a SIMD's waves live, with two steps a segment).
 #include <string.h>
 
 #include <algorithm>

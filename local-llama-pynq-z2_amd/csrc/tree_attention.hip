@@ -111,6 +111,10 @@ struct TreePlan {
 // sequences of up to 16k positions, 448 rows: 186 us with two tiles, 144 with LDS; one sequence of 700: 14 and 18).  fp32
 // queries take two tiles in each of four waves there (eight waves of one would spill), bf16 ones one in each of eight.  The
 // rows are spread evenly over these blocks.
+// The thresholds were measured at heads of 128 and hold at 64 for one sequence (448 rows over 32k int8 positions: 50 us with one
+// tile, 43 with two, which it takes; 259 over 12k: 17.9 with one, which it takes, 20.4; bf16: 49 and 32, 21 and 18, two); for
+// batches there it can be a third off (448 rows over 8 x 4000 int8 positions: 28 us with one, 34 with two, which it takes; over
+// 8 x 700 bf16 ones: 13.6 and 18.9, two).
 // Positions.  One sequence: as many slices as give a block a CU, or two a CU where whole row blocks would leave much of the
 // chip idle (192 rows over 32k int8 positions: 70 us with 192 blocks, 55 with 480; 7 rows: 16 with 256, 18 with 512).
 // Several: two blocks a CU over all sequences, of equal steps (a decode step of 32 sequences, 0 to 8190 e4m3 positions: 31 us,

@@ -352,7 +352,8 @@ __device__ __forceinline__ uint32_t seen_bits(const Place &p, int p0, uint64_t s
 #pragma unroll
     for (int t = 0; t < N / 4; t++) {
         const int at = p0 + 16 * t + 4 * j - p.len;
-        const uint32_t below = ((uint32_t)sees << 4 | 15u) >> (max(at + 4, 0) & 31), from = at < 64 ? (uint32_t)(sees >> (at & 63)) : 0u;
+        const uint32_t below = ((uint32_t)sees << 4 | 15u) >> (max(at + 4, 0) & 31);
+        const uint32_t from = at < 64 ? (uint32_t)(sees >> (at & 63)) : 0u;
         vis |= ((at < 0 ? below : from) & 15u) << (4 * t);
     }
     return vis;
@@ -492,10 +493,12 @@ struct TreeShape {
 // lane n reads 4 or 8 neighbouring dimensions of its eight positions and pairs the registers of two positions, which
 // transposes for nothing.  The next step's loads go out as soon as a step's registers are used.  No wave waits for
 // another before the end.
-// What bounds it: for one token, memory (32 sequences of 0 to 8190 e4m3 positions, 4 kv heads of 128: 27 us, 5.0 TB/s), or
-// where few steps are left for each block, the latency of a step (32.7k int8 positions of one sequence: 12.6 us, 2.7 TB/s).
-// For trees the vector instructions: for each 64 positions and 16 rows about 360 convert codes and 240 make weights, beside 64
-// products of 17 cycles (a 37-token tree, 259 rows, over 12k int8 positions: 36 us, 177 TFLOP/s, 354 of issued products).
+// What bounds it: for one token, memory (32 sequences of 0 to 8190 e4m3 positions, 4 kv heads of 128: 28 us, 4.8 TB/s), or
+// where few steps are left for each block, the latency of a step (32.7k int8 positions of one sequence: 13 us, 2.7 TB/s).
+// For trees over 8-bit caches the vector instructions (codes into fp16, weights) and each step's chain of products, maximum,
+// exponentials and products again, which two waves a SIMD hide in part: a 37-token tree, 259 rows, over 12k int8 positions takes
+// 37 us (171 TFLOP/s, 342 of issued products), and of the 60k cycles that a SIMD's waves live, vector instructions are issued
+// in 34k and the matrix unit is busy in 14k.
 template <int CT, int QT, int R>
 __global__ void __launch_bounds__(256, CT != LLM_F32 && HSP <= 128 ? 2 : 1) k_tree_attention(TreeArgs a) {
     using Sh = TreeShape<CT, QT, R>;
