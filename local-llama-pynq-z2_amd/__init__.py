@@ -322,7 +322,7 @@ def kv_read(k, v, pos, tokens, n=None, k_scale=None, v_scale=None, out=None, dty
     """The values of positions pos[b] .. pos[b] + n[b] - 1 (n None: `tokens` each) as rows [seqs, tokens, kv heads, head
     size] of K and V (llm_kv_read), float32 or `dtype`; new tensors (rows that are not read: zero) or `out`, a pair (such
     rows left as they were)."""
-    _no_grad(k, v, k_scale, v_scale, *(out or ()))
+    _no_grad(k, v, k_scale, v_scale, *(() if out is None else (out[0], out[1])))
     c, (b, h, _, hs) = _kv(k, v, k_scale, v_scale)
     torch, fresh = _torch[0], out is None
     if fresh:
@@ -331,7 +331,7 @@ def kv_read(k, v, pos, tokens, n=None, k_scale=None, v_scale=None, out=None, dty
                          _ints("pos", pos, b, torch.int32), _ints("n", n, b, torch.int32), tokens, fresh, _stream(k)) != 0:
         raise RuntimeError("llm_kv_read failed")
     if not fresh:
-        _written(*out)
+        _written(out[0], out[1])
     return out[0], out[1]
 
 

@@ -62,3 +62,14 @@ def test_shared_memory_is_read_and_not_written(capfd):
         with pytest.raises(RuntimeError):
             pkg().tree_attention(q, apart, apart, lens, out=out)
         assert "a stride of zero" in capfd.readouterr().err
+
+
+def test_rows_read_into_one_tensor():
+    """`out` as a tensor of two, K's rows and V's"""
+    g = gen(4)
+    k, v = (torch.randn(2, 2, 20, 64, generator=g).to(DEV) for _ in range(2))
+    pos = torch.tensor([3, 11], dtype=torch.int32, device=DEV)
+    out = torch.zeros(2, 2, 6, 2, 64, device=DEV)
+    got = pkg().kv_read(k, v, pos, 6, out=out)
+    for x, y, z in zip(got, pkg().kv_read(k, v, pos, 6), out):
+        assert torch.equal(x, y) and torch.equal(z, y)
