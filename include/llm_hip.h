@@ -243,6 +243,109 @@ int llm_logprobs(const void *logits, int type, int rows, int vocab, int64_t stri
                  int n_tokens, float *logp, float *entropy, float *lse, int top, int *top_ids, float *top_logp, void *work,
                  size_t work_bytes, void *stream);
 
+/* ---- a cache in pages -------------------------------------------------------------------------------------------
+ *
+ * A pool of pages that the sequences of a batch take as they grow, share and give back.  A page holds `page` positions (64, 128
+ * or 256) of every kv head, as int8 or e4m3 codes in blocks of 64 positions: K as 64 rows of hs codes, V turned, as hs rows of 64
+ * (both are then operands of the matrix instructions as they lie), with an fp32 scale for each block of either; value = code *
+ * scale.  Page i, head h of K: page * hs codes at k + i * id + h * head, of V the same, its scales page / 64 floats at k_scale +
+ * i * s_id + h * s_head.  Layers lie `layer` codes and `s_layer` floats apart; llm_page_write, llm_page_read and
+ * llm_page_attention take the first one (a later one: its addresses).  Addresses and strides of k and v are multiples of 16.
+ * hs is a multiple of 16, at most 256.
+ *
+ * table: n_seq rows of `per` page numbers (contiguous ints); entry j of a row is the page of positions j * page and on, and a number
+ * outside 0 .. n_pages - 1 is none.  refs: for each page in how many places the tables have it; 0: free.  The calls that change
+ * tables keep refs right; what refs and tables that contradict each other lead to is not said, but that no memory outside the
+ * arrays is touched. */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int type;                      /* LLM_I8 or LLM_E4M3 */
+    int n_layers, n_pages, n_kv, hs, page;
+    int64_t layer, id, head;       /* strides of k and v, in codes */
+    int64_t s_layer, s_id, s_head; /* of the scales, in floats */
+} llm_pages;
+
+/* Rows of K and V of n[b] <= max_n tokens (n NULL: max_n) of each sequence to positions pos[b] and on: position pos[b] + i gets
+ * row path[b * max_n + i] of the sequence's rows (a token of a drafted tree that was kept; path NULL: row i; outside 0 .. max_n
+ * - 1: zeros).  Positions outside 0 .. per * page - 1, of no page, or (refs not NULL) of a page whose count is not 1 are not
+ * written.  The rows of a call that fall into one block of a kv head have a = amax / top, rounded to fp32, top 127 (int8) or 448
+ * (e4m3).  Where the first of them stands at the block's start, or the block's scale is 0, the scale becomes a; else the positions
+ * before them keep theirs if it is at least a, and if not it is doubled until it is, and their codes are divided by the same
+ * power of two, rounded half to even.  New codes are the exact quotients value / scale, rounded half to even and kept within top.
+ * What the block holds at and behind the last row is the caller's no longer.  An infinity or a NaN among the rows makes
+ * the block's scale NaN, which it stays until it is begun again. */
+int llm_page_write(const llm_pages *c, const llm_rows *k, const llm_rows *v, int n_seq, const int *table, int per,
+                   const int *refs, const int *pos, const int *n, const int *path, int max_n, void *stream);
+/* The values of positions pos[b] .. pos[b] + n[b] - 1 into rows 0 .. n[b] - 1 of k and v, rounded to their type.  The rows
+ * behind n[b], and those of positions without a page, are left as they were, or zeroed (zero_rest). */
+int llm_page_read(const llm_pages *c, const llm_rows *k, const llm_rows *v, int n_seq, const int *table, int per, const int *pos,
+                  const int *n, int max_n, int zero_rest, void *stream);
+
+/* Attention of the n[b] <= max_n <= 64 newest tokens of every sequence over the lens[b] positions of its pages and over their own
+ * K and V rows, which are not in the pages yet (k and v, of q's type; NULL: none, and mask is not looked at).  Token i sees all
+ * positions below lens[b] that have a page, and the new tokens j whose bit j is set in mask[b * max_n + i] (mask NULL: j <= i; a
+ * decode step has max_n 1).  out[b][i][h] = sum_p softmax_p(scale q.k_p) v_p over the kv head h / (n_heads / n_kv), rounded to out's
+ * type (q's type); scale is finite, of either sign.  A token that sees nothing gets zeros.  Rows behind n[b] are left as
+ * they were, or zeroed (zero_rest).  lens outside 0 .. per * page count as the nearer end.
+ * What is not seen changes no bit, infinities and NaN included; a new token whose V row holds one makes the tokens that see it
+ * NaN, a block whose scale is one of them makes those NaN that see any of its positions.
+ * Sums are fp32.  Over pages a query holds 22 bits of its largest value (bf16 queries: all their bits down to 2^-39 of it), a
+ * weight 22 bits, and no finer step than 2^-39 of the row's largest weight in the block; over the new rows both hold fp32.
+ * n_heads / n_kv is at most 64.  max_len is the host's upper bound of lens[] (lens above it are right too, slower); `work`
+ * has llm_page_attention_work() bytes, 16-byte aligned, and is one call's until it has run. */
+size_t llm_page_attention_work(const llm_pages *c, int n_seq, int n_heads, int max_n, int max_len);
+int llm_page_attention(const llm_pages *c, const llm_rows *q, const llm_rows *k, const llm_rows *v, const llm_rows *out,
+                       int n_heads, int n_seq, const int *table, int per, const int *lens, const int *n, const uint64_t *mask,
+                       int max_n, int max_len, float scale, int zero_rest, void *work, size_t work_bytes, void *stream);
+
+/* All at once: sequence to[i] becomes what sequence from[i] was before the call, sharing the pages of its lens[] positions;
+ * from[i] outside 0 .. n_seq - 1: it becomes empty.  Pages that no table has any more are free.  to[i] outside 0 .. n_seq - 1, or
+ * named again by a later entry, does nothing.  Beams that follow their parents, a prompt shared by new dialogs, dialogs that
+ * end.  count <= 65535; `work`: llm_page_fork_work() bytes, 4-byte aligned. */
+size_t llm_page_fork_work(int per, int count);
+int llm_page_fork(int n_pages, int page, int n_seq, int *table, int per, int *lens, int *refs, const int *to, const int *from,
+                  int count, void *work, size_t work_bytes, void *stream);
+/* Room for n[b] <= max_n more tokens of every sequence, at positions lens[b] and on, in pages that are its own.  Where there
+ * is none it gets a free page: the lowest numbers, in the order of sequences and positions.  A shared page is left to the others
+ * and replaced by a free one, into which the blocks that hold positions below lens[b] are copied, of all layers; only where all
+ * that share a page ask for it in this call, the last of them (by number) keeps it.  Everything or nothing: result[0] = 1, and
+ * result[1] the pages taken; or result[0] = 0, the tables as they were and result[1] the pages wanted, where so many are not
+ * free, a sequence does not fit its row of the table (which wants none then) or n[b] is above max_n.  Work: llm_page_reserve_work() bytes, 16-byte aligned. */
+size_t llm_page_reserve_work(const llm_pages *c, int n_seq, int per, int max_n);
+int llm_page_reserve(const llm_pages *c, int n_seq, int *table, int per, int *refs, const int *lens, const int *n, int max_n,
+                     int *result, void *work, size_t work_bytes, void *stream);
+/* The used pages to the front of the pool: with u of them, those numbered u and above move, in order, to the free numbers below
+ * u (codes and scales of all layers), and tables and refs follow; entries from u on that refs calls free become -1.  result[0] = u,
+ * result[1] = pages moved.  Work: llm_page_compact_work() bytes, 4-byte aligned. */
+size_t llm_page_compact_work(const llm_pages *c);
+int llm_page_compact(const llm_pages *c, int n_seq, int *table, int per, int *refs, int *result, void *work, size_t work_bytes,
+                     void *stream);
+
+/* Drafted tokens kept or turned down so that what is kept, and the token drawn behind it, are distributed as if the target had
+ * drawn them one by one (speculative sampling).  Sequence b has n[b] <= max_n <= 64 nodes (n NULL: max_n): node 0 is its newest
+ * token, node i > 0 the drafted token tokens[b * max_n + i] behind node parents[b * max_n + i] < i (parents NULL: i - 1; any other
+ * number: the node is not reached).  Logits: row (b, r) of `vocab` logits at logits + b * seq + r * row (values of
+ * type), the target's after node r; p_r = softmax(logits / temperature), temperature 0: all on the largest (the first of equal
+ * ones), else 1e-30 to 1e30.  probs: rows of the draft's probabilities alike (p_type, p_seq, p_row), row r those that the children of
+ * node r were drawn from, each by itself, used as they are; NULL: drafts that were not drawn (looked up, the likeliest).
+ * From node 0, the children of a node are tried in order.  With probs, the target left is w = max(0, p_r - a q_r), at first a = 0 and
+ * its sum z = 1: a child with token x is kept if coins[child] q_r(x) z < w(x), and its children are next; if not, a grows by z
+ * and z becomes the sum of the new w.  Without, w is p_r without the tokens turned down, q_r(x) = 1.  Where no child is kept, the
+ * token next[b] is drawn from w (from p_r where w is zero throughout): the first whose inclusive running sum is above coins[0]
+ * times the whole.  A drafted token outside 0 .. vocab - 1 is turned down and changes nothing.  coins: n_seq x max_n floats in [0, 1).
+ * Probabilities, sums and comparisons are in 64 bits.
+ * kept[b]: the nodes kept, node 0 among them; path[b * max_n + j], j < kept[b]: their numbers, rising, -1 behind them (as
+ * llm_page_write takes them); next[b]; logp[b * max_n + i], 0 < i < n[b]: log p of node i's token after its parent (0 without a
+ * parent, -infinity outside the vocabulary), and in its place 0 the log p of next[b].  n[b] < 1: kept 0, next -1.  A row with
+ * a NaN or +infinity, or of -infinity alone, keeps nothing behind it and draws -1 (log probabilities NaN).
+ * `work`: llm_draft_accept_work() bytes, 16-byte aligned. */
+size_t llm_draft_accept_work(int n_seq, int max_n, int vocab);
+int llm_draft_accept(const void *logits, int type, int n_seq, int max_n, int vocab, int64_t seq, int64_t row, float temperature,
+                     const void *probs, int p_type, int64_t p_seq, int64_t p_row, const int *tokens, const int *parents,
+                     const int *n, const float *coins, int *kept, int *path, int *next, float *logp, void *work,
+                     size_t work_bytes, void *stream);
+
 /* ---- test hooks: no counterpart in the reference; they expose single device stages so the tests can
  * hold each one against the oracle (like the reference's FPGA_CHECK side-by-side check, qwen.c:464-472) --- */
 

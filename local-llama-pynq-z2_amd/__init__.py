@@ -4,7 +4,7 @@ The library is C (include/matvec_fpga.h: the reference's six-function driver API
 device-resident token loop).  These bindings are what the Python tests and bench.py call; the C hosts in
 host/ and the reference's own hosts link the library directly.  Nothing here computes: every call goes
 through the C ABI, and loading fails loudly when the built library is missing.  The operators on device memory
-(kv_write, kv_read, tree_attention, logprobs) take torch tensors; torch is imported by their first call.
+(kv_write, kv_read, tree_attention, logprobs, page_*, draft_accept) take torch tensors; torch is imported by their first call.
 
 The directory name is not a Python identifier, so callers load this file by path, e.g.
     spec = importlib.util.spec_from_file_location("llm_hip", ".../local-llama-pynq-z2_amd/__init__.py")
@@ -40,6 +40,13 @@ class LlmKv(C.Structure):
 
 class LlmRows(C.Structure):
     _fields_ = [("p", C.c_void_p), ("type", C.c_int), ("seq", C.c_int64), ("tok", C.c_int64), ("head", C.c_int64)]
+
+
+class LlmPages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("type", C.c_int), ("n_layers", C.c_int), ("n_pages", C.c_int), ("n_kv", C.c_int), ("hs", C.c_int),
+                ("page", C.c_int), ("layer", C.c_int64), ("id", C.c_int64), ("head", C.c_int64),
+                ("s_layer", C.c_int64), ("s_id", C.c_int64), ("s_head", C.c_int64)]
 
 
 class LlmTiming(C.Structure):
@@ -119,6 +126,24 @@ def lib():
     L.llm_logprobs_work.argtypes = [i32, i32, i32]
     L.llm_logprobs_work.restype = sz
     L.llm_logprobs.argtypes = [vp, i32, i32, i32, C.c_int64, C.c_float, vp, i32, vp, vp, vp, i32, vp, vp, vp, sz, vp]
+    L.llm_page_write.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, i32, vp]
+    L.llm_page_read.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, i32, i32, vp]
+    L.llm_page_attention_work.argtypes = [vp, i32, i32, i32, i32]
+    L.llm_page_attention_work.restype = sz
+    L.llm_page_attention.argtypes = [vp, vp, vp, vp, vp, i32, i32, vp, i32, vp, vp, vp, i32, i32, C.c_float, i32, vp, sz, vp]
+    L.llm_page_fork_work.argtypes = [i32, i32]
+    L.llm_page_fork_work.restype = sz
+    L.llm_page_fork.argtypes = [i32, i32, i32, vp, i32, vp, vp, vp, vp, i32, vp, sz, vp]
+    L.llm_page_reserve_work.argtypes = [vp, i32, i32, i32]
+    L.llm_page_reserve_work.restype = sz
+    L.llm_page_reserve.argtypes = [vp, i32, vp, i32, vp, vp, vp, i32, vp, vp, sz, vp]
+    L.llm_page_compact_work.argtypes = [vp]
+    L.llm_page_compact_work.restype = sz
+    L.llm_page_compact.argtypes = [vp, i32, vp, i32, vp, vp, vp, sz, vp]
+    L.llm_draft_accept_work.argtypes = [i32, i32, i32]
+    L.llm_draft_accept_work.restype = sz
+    L.llm_draft_accept.argtypes = [vp, i32, i32, i32, i32, C.c_int64, C.c_int64, C.c_float, vp, i32, C.c_int64, C.c_int64,
+                                   vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     _lib = L
     return L
 
@@ -220,6 +245,7 @@ def ref_expf(x, host=False):
 _torch = None
 _PACK_KV = struct.Struct("4P5i4x6q").pack
 _PACK_ROWS = struct.Struct("Pi4x3q").pack
+_PACK_PAGES = struct.Struct("4P6i6q").pack
 
 
 def _types():
@@ -389,6 +415,202 @@ def logprobs(logits, tokens=None, top=0, temperature=1.0):
                                p + 4 * at if need else None, need, _stream(logits)) != 0:
         raise RuntimeError("llm_logprobs failed")
     return logp.view(rows, count), entropy, ids.view(rows, top), top_logp.view(rows, top), lse
+
+
+# ---- a cache in pages (torch tensors)
+
+def _pages(k, v, k_scale, v_scale):
+    """llm_pages of K [pages, kv heads, page, head size], V [pages, kv heads, page / 64, head size, 64] (int8 or float8_e4m3fn) and
+    their scales [pages, kv heads, page / 64] (float32), with the layers before the pages or without; pages and heads may lie apart.
+    And its dimensions (layers, pages, kv heads, page, head size)"""
+    torch, types = _torch or _types()
+    ty, shape, many = types.get(k.dtype, 0), k.shape, k.dim() == 5
+    if ty < 2 or v.dtype is not k.dtype or len(shape) != 4 + many or (shape[-2] % 64 or not shape[-2]):
+        raise ValueError("k: int8 or float8_e4m3fn codes [pages, kv heads, page, head size] are needed, v of the same type")
+    page, hs = shape[-2:]
+    rows = shape[:-2] + (page // 64,)
+    if v.shape != rows + (hs, 64):
+        raise ValueError(f"v: codes {tuple(rows) + (hs, 64)} are needed")
+    f32 = torch.float32
+    if k_scale.shape != rows or v_scale.shape != rows or k_scale.dtype is not f32 or v_scale.dtype is not f32:
+        raise ValueError(f"k_scale, v_scale: float32 {tuple(rows)} are needed")
+    if not many:
+        k, v, k_scale, v_scale = k.unsqueeze(0), v.unsqueeze(0), k_scale.unsqueeze(0), v_scale.unsqueeze(0)
+    n = k.shape[:3]
+    sk, sv, ss, st = k.stride(), v.stride(), k_scale.stride(), v_scale.stride()
+    if (sk[4] != 1 and hs > 1) or sk[3] != hs or sv[5] != 1 or sv[4] != 64 or (page > 64 and (sv[3] != 64 * hs or ss[3] != 1 or
+                                                                                            st[3] != 1)):
+        raise ValueError("k, v and their scales: what a page holds of a head has to lie together")
+    if any(n[i] > 1 and (sk[i] != sv[i] or ss[i] != st[i]) for i in range(3)):
+        raise ValueError("k and v, and their scales: equal strides of layers, pages and heads are needed")
+    at = [(sk[i], ss[i]) if n[i] > 1 else (0, 0) for i in range(3)]
+    return _PACK_PAGES(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, *n, hs, page,
+                       *(x[0] for x in at), *(x[1] for x in at)), (*n, page, hs)
+
+
+def _table(table):
+    """the address of a table [seqs, pages of one], and its shape"""
+    if table.dim() != 2:
+        raise ValueError("table: contiguous int32 [seqs, pages] are needed")
+    return _ints("table", table, table.numel(), _torch[0].int32), table.shape
+
+
+def page_write(k_rows, v_rows, k, v, k_scale, v_scale, table, pos, n=None, path=None, refs=None):
+    """Rows [seqs, tokens, kv heads, head size] into the pages of one layer (llm_page_write): row i < n[b] of sequence b, or row
+    path[b, i] (int32 [seqs, tokens]), at position pos[b] + i, in codes with a scale for each 64 positions of a head.  The pages
+    as in page_attention; refs (int32 [pages]): pages that more than one table has are not written."""
+    _no_grad(k_rows, v_rows, k_scale, v_scale)
+    c, (_, pages, h, _, hs) = _pages(k, v, k_scale, v_scale)
+    (at, (b, per)), i32 = _table(table), _torch[0].int32
+    t = k_rows.shape[1]
+    if lib().llm_page_write(c, _rows("k_rows", k_rows, b, t, h, hs), _rows("v_rows", v_rows, b, t, h, hs), b, at, per,
+                            _ints("refs", refs, pages, i32), _ints("pos", pos, b, i32), _ints("n", n, b, i32),
+                            _ints("path", path, b * t, i32), t, _stream(k)) != 0:
+        raise RuntimeError("llm_page_write failed")
+    _written(k, v, k_scale, v_scale)
+
+
+def page_read(k, v, k_scale, v_scale, table, pos, tokens, n=None, out=None, dtype=None):
+    """The values of positions pos[b] .. pos[b] + n[b] - 1 (n None: `tokens` each) as rows [seqs, tokens, kv heads, head size] of
+    K and V (llm_page_read), float32 or `dtype`; new tensors (rows that are not read: zero) or `out`, a pair (such rows left as
+    they were)."""
+    _no_grad(k_scale, v_scale, *(() if out is None else (out[0], out[1])))
+    c, (_, _, h, _, hs) = _pages(k, v, k_scale, v_scale)
+    (at, (b, per)), torch, fresh = _table(table), _torch[0], out is None
+    if fresh:
+        out = torch.empty(2, b, tokens, h, hs, dtype=dtype or torch.float32, device=k.device).unbind()
+    if lib().llm_page_read(c, _rows("out", out[0], b, tokens, h, hs), _rows("out", out[1], b, tokens, h, hs), b, at, per,
+                           _ints("pos", pos, b, torch.int32), _ints("n", n, b, torch.int32), tokens, fresh, _stream(k)) != 0:
+        raise RuntimeError("llm_page_read failed")
+    if not fresh:
+        _written(out[0], out[1])
+    return out[0], out[1]
+
+
+def page_attention(q, k, v, k_scale, v_scale, table, lens, k_rows=None, v_rows=None, n=None, mask=None, scale=None, max_len=None,
+                   out=None):
+    """Attention of the newest tokens of every sequence over the pages of one layer and over their own rows (llm_page_attention;
+    no gradient).  q [seqs, tokens <= 64, heads, head size] float32 or bfloat16; k [pages, kv heads, page, head size] and v [pages,
+    kv heads, page / 64, head size, 64], codes of int8 or float8_e4m3fn, k_scale and v_scale [pages, kv heads, page / 64] float32;
+    table [seqs, pages of one] int32.  Token i of sequence b sees the lens[b] positions of its pages and, of k_rows and v_rows
+    [seqs, tokens, kv heads, head size] of q's type, the tokens of mask[b, i]'s bits (int64; None: those up to itself).  n[b] tokens
+    count (None: all); scale None: head size ** -0.5; max_len: the host's bound of lens (None: the table's positions).  Returns a
+    new tensor (rows behind n[b]: zero), or `out` (such rows left as they were)."""
+    _no_grad(q, k_scale, v_scale, k_rows, v_rows, out)
+    c, (_, _, h, page, hs) = _pages(k, v, k_scale, v_scale)
+    (at, (b, per)), torch, fresh = _table(table), _torch[0], out is None
+    t, heads = q.shape[1:3]
+    if (k_rows is None) != (v_rows is None):
+        raise ValueError("k_rows and v_rows: both or neither are needed")
+    if mask is not None and mask.dim() > 1 and mask.shape != (b, t):
+        raise ValueError(f"mask: int64 {(b, t)} are needed")
+    if fresh:
+        out = torch.empty(b, t, heads, hs, dtype=q.dtype, device=k.device)
+    L, bound = lib(), min(per * page if max_len is None else max_len, per * page)
+    need = L.llm_page_attention_work(c, b, heads, t, bound)
+    work = torch.empty(need, dtype=torch.uint8, device=k.device) if need else None
+    if L.llm_page_attention(c, _rows("q", q, b, t, heads, hs), None if k_rows is None else _rows("k_rows", k_rows, b, t, h, hs),
+                            None if v_rows is None else _rows("v_rows", v_rows, b, t, h, hs),
+                            _rows("out", out, b, t, heads, hs), heads, b, at, per, _ints("lens", lens, b, torch.int32),
+                            _ints("n", n, b, torch.int32), _ints("mask", mask, b * t, torch.int64), t, bound,
+                            hs ** -0.5 if scale is None else scale, fresh, work.data_ptr() if need else None, need,
+                            _stream(k)) != 0:
+        raise RuntimeError("llm_page_attention failed")
+    if not fresh:
+        _written(out)
+    return out
+
+
+def page_fork(table, lens, refs, to, source, page):
+    """Sequence to[i] becomes what sequence source[i] was before the call, all at once, sharing its pages of `page` positions;
+    source -1: it becomes empty (llm_page_fork).  table [seqs, pages of one], lens [seqs], refs [pages], to and source: int32."""
+    torch = _types()[0]
+    (at, (b, per)), i32, L = _table(table), torch.int32, lib()
+    count = to.numel()
+    need = L.llm_page_fork_work(per, count)
+    work = torch.empty(need, dtype=torch.uint8, device=table.device)
+    if L.llm_page_fork(refs.numel(), page, b, at, per, _ints("lens", lens, b, i32), _ints("refs", refs, refs.numel(), i32),
+                       _ints("to", to, count, i32), _ints("source", source, count, i32), count, work.data_ptr(), need,
+                       _stream(table)) != 0:
+        raise RuntimeError("llm_page_fork failed")
+    _written(table, lens, refs)
+
+
+def page_reserve(k, v, k_scale, v_scale, table, refs, lens, n, max_n=None):
+    """Room for n[b] (int32; at most max_n, None: a table's row) more tokens of every sequence in pages of its own, shared ones
+    copied in all layers (llm_page_reserve).  The pages as in page_attention, with the layers first where there are more.  Returns
+    int32 (1, pages taken), or (0, pages wanted) with nothing changed where there is no room."""
+    _no_grad(k_scale, v_scale)
+    c, (_, pages, _, page, _) = _pages(k, v, k_scale, v_scale)
+    (at, (b, per)), torch, L = _table(table), _torch[0], lib()
+    most = per * page if max_n is None else max_n
+    need = L.llm_page_reserve_work(c, b, per, most)
+    work = torch.empty(need, dtype=torch.uint8, device=k.device)
+    result = torch.empty(2, dtype=torch.int32, device=k.device)
+    i32 = torch.int32
+    if L.llm_page_reserve(c, b, at, per, _ints("refs", refs, pages, i32), _ints("lens", lens, b, i32), _ints("n", n, b, i32), most,
+                          result.data_ptr(), work.data_ptr(), need, _stream(k)) != 0:
+        raise RuntimeError("llm_page_reserve failed")
+    _written(k, v, k_scale, v_scale, table, refs)
+    return result
+
+
+def page_compact(k, v, k_scale, v_scale, table, refs):
+    """The used pages moved to the front of the pool, in all layers (llm_page_compact).  Returns int32 (pages used, pages
+    moved)."""
+    _no_grad(k_scale, v_scale)
+    c, (_, pages, _, _, _) = _pages(k, v, k_scale, v_scale)
+    (at, (b, per)), torch, L = _table(table), _torch[0], lib()
+    need = L.llm_page_compact_work(c)
+    work = torch.empty(need, dtype=torch.uint8, device=k.device)
+    result = torch.empty(2, dtype=torch.int32, device=k.device)
+    if L.llm_page_compact(c, b, at, per, _ints("refs", refs, pages, torch.int32), result.data_ptr(), work.data_ptr(), need,
+                          _stream(k)) != 0:
+        raise RuntimeError("llm_page_compact failed")
+    _written(k, v, k_scale, v_scale, table, refs)
+    return result
+
+
+def draft_accept(logits, tokens, coins, parents=None, n=None, probs=None, temperature=1.0):
+    """Drafted tokens kept or turned down so that the target's distribution stays (llm_draft_accept).  logits [seqs, nodes <= 64,
+    vocab] float32 or bfloat16, the target's after each node; tokens and parents (None: a chain) [seqs, nodes] int32, node 0 the
+    newest token; coins [seqs, nodes] float32 in [0, 1), the first for the token that is drawn; probs: the draft's probabilities
+    behind each node, laid out like logits (None: drafts that were not drawn).  Returns (kept [seqs]: nodes kept, path [seqs, nodes]:
+    their numbers and -1, next [seqs]: the token drawn behind them, logp [seqs, nodes]: the target's log probability of each drafted
+    token and, first, of the one drawn)."""
+    torch, types = _types()
+    _no_grad(logits, coins, probs)
+    b, t, vocab = logits.shape
+    i32 = torch.int32
+
+    def rows(name, x):
+        ty, st = types.get(x.dtype, 4), x.stride()
+        if ty > 1 or x.shape != (b, t, vocab) or (vocab > 1 and st[2] != 1):
+            raise ValueError(f"{name}: float32 or bfloat16 rows {(b, t, vocab)} are needed")
+        return x.data_ptr(), ty, st[0] if b > 1 else 0, st[1] if t > 1 else 0
+
+    x, ty, seq, row = rows("logits", logits)
+    q, qy, q_seq, q_row = (None, 0, 0, 0) if probs is None else rows("probs", probs)
+    for name, y in (("tokens", tokens), ("parents", parents), ("coins", coins)):
+        if y is not None and y.shape != (b, t):
+            raise ValueError(f"{name}: {(b, t)} are needed")
+    if t == 0:
+        return (torch.zeros(b, dtype=i32, device=logits.device), torch.empty(b, 0, dtype=i32, device=logits.device),
+                torch.full((b,), -1, dtype=i32, device=logits.device), torch.empty(b, 0, device=logits.device))
+    L = lib()
+    need = L.llm_draft_accept_work(b, t, vocab)
+    # one allocation: the results, and the scratch memory behind them
+    have = b * (2 + 2 * t)
+    have += -have % 4
+    mem = torch.empty(have + need // 4, dtype=i32, device=logits.device)
+    kept, drawn, path, logp, _ = mem.split_with_sizes((b, b, b * t, b * t, mem.numel() - b * (2 + 2 * t)))
+    p = mem.data_ptr()
+    if b and L.llm_draft_accept(x, ty, b, t, vocab, seq, row, temperature, q, qy, q_seq, q_row, _ints("tokens", tokens, b * t, i32),
+                                _ints("parents", parents, b * t, i32), _ints("n", n, b, i32),
+                                _ints("coins", coins, b * t, torch.float32), p, p + 8 * b, p + 4 * b, p + 8 * b + 4 * b * t,
+                                p + 4 * have, need, _stream(logits)) != 0:
+        raise RuntimeError("llm_draft_accept failed")
+    return kept, path.view(b, t), drawn, logp.view(torch.float32).view(b, t)
 
 
 # ---- drop-in driver API -----------------------------------------------------------------------------------

@@ -107,3 +107,12 @@ struct LogprobsCall {
     void *work; // llm_logprobs_work()
 };
 hipError_t launch_logprobs(const LogprobsCall &q, hipStream_t st);
+
+// ---- a cache in pages
+
+constexpr int PAGE_BLOCK = 64; // positions that share a scale
+
+// Prints what is wrong with a pool, or with the memory it names (dev not NULL).
+bool op_check_pages(const llm_pages *c, OpDevice *dev, const char *who);
+// The same of a table of n_seq rows of `per` entries.
+bool op_check_table(const int *table, int n_seq, int per, OpDevice *dev, const char *who);
