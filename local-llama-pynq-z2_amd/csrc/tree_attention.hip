@@ -10,91 +10,6 @@
 
 namespace {
 
-// A row's slices joined: weights exp2(max_s - max).  W waves a row (the block has four): a thread takes four values of
-// every (64 W / (hs / 4))-th slice, eight slices' loads at once.
-template <int QT, int W>
-__global__ void __launch_bounds__(256) k_tree_join(TreeArgs a) {
-    __shared__ float sm_f[4 / W][TREE_MAX_SLICES + 64]; // (a group's last loads may be past the last slice: weight 0)
-    __shared__ float4 sm_o[256];
-    constexpr int T = 64 * W;
-    const int lane = threadIdx.x & 63, part = threadIdx.x / T, tid = threadIdx.x % T;
-    const int row = blockIdx.x * (4 / W) + part, h = blockIdx.y, b = blockIdx.z;
-    const int nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n;
-    int slices, first;
-    if (a.n_seq == 1) {
-        int steps;
-        slices = tree_one(a, tree_steps(a, 0), steps);
-        first = h * a.each;
-    } else {
-        const int2 plan = a.plan[b * a.n_kv + h];
-        first = plan.x;
-        slices = plan.y;
-    }
-    if (slices == 1) return; // (every row of the sequence was finished by its block)
-    const bool there = row < nn * a.group;
-    const int64_t stride = (int64_t)a.max_n * a.group, base = first * stride + row;
-    const int per = a.hs / 4, groups = T / per, g = tid / per, d = 4 * (tid - g * per);
-    constexpr int U = 8;
-    float4 v[U];
-    auto load = [&](int s0) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int s = s0 + u * groups;
-            v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (there && g < groups && s < slices) v[u] = *(const float4 *)(a.acc + (base + s * stride) * a.hs + d);
-        }
-    };
-    load(g); // (the first values do not wait for the weights)
-    float m[TREE_MAX_SLICES / 64], l[TREE_MAX_SLICES / 64], mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < TREE_MAX_SLICES / 64; i++) {
-        const int s = lane + 64 * i;
-        const bool have = there && s < slices;
-        m[i] = have ? a.ml[2 * (base + s * stride)] : -INFINITY;
-        l[i] = have ? a.ml[2 * (base + s * stride) + 1] : 0.0f;
-        mx = fmaxf(mx, m[i]);
-    }
-    mx = wave_max(mx);
-    const float mu = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < TREE_MAX_SLICES / 64; i++) {
-        const float f = __builtin_amdgcn_exp2f(m[i] - mu);
-        sum += l[i] * f;
-        if (tid < 64) sm_f[part][lane + 64 * i] = f;
-    }
-    sum = wave_sum(sum);
-    if (tid < 64) sm_f[part][lane + TREE_MAX_SLICES] = 0.0f;
-    __syncthreads();
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = g; s0 < slices; s0 += U * groups) {
-        if (s0 != g) load(s0);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const float f = sm_f[part][min(s0 + u * groups, TREE_MAX_SLICES)];
-            o.x += v[u].x * f, o.y += v[u].y * f, o.z += v[u].z * f, o.w += v[u].w * f;
-        }
-    }
-    sm_o[threadIdx.x] = o;
-    __syncthreads();
-    if (g || !there) return;
-    for (int k = 1; k < groups; k++) {
-        const float4 x = sm_o[part * T + k * per + tid];
-        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
-    }
-    const int t = row / a.group, gr = row - t * a.group;
-    uint8_t *op = a.o + b * a.o_seq + t * a.o_tok + (h * a.group + gr) * a.o_head;
-    const float il = sum == 0.0f ? 0.0f : 1.0f / sum;
-    o = make_float4(o.x * il, o.y * il, o.z * il, o.w * il);
-    if constexpr (QT == LLM_F32) *(float4 *)(op + (size_t)d * 4) = o;
-    else {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        *(uint2 *)(op + (size_t)d * 2) = make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector((f2){o.x, o.y}, b2)),
-                                                    __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){o.z, o.w}, b2)));
-    }
-}
-
 constexpr float LOG2E = 1.44269504088896340736f;
 
 struct TreePlan {
@@ -140,13 +55,13 @@ TreePlan tree_plan(const llm_kv *c, int q_type, int n_heads, int max_n, int max_
     p.least = many ? 2 : 4; // steps of a slice (few rows: one a wave)
     // per XCD; a single sequence: one block a CU, two where whole blocks would leave much of the chip idle
     const int64_t one = 32 / p.row_blocks * 8, both = 64 / p.row_blocks * 8;
-    int64_t cap = both, each = TREE_MAX_SLICES;
+    int64_t cap = both, each = MAX_SLICES;
     if (c->n_seq == 1) {
         cap = both / c->n_kv * 5 > one / c->n_kv * 11 ? both : one;
         each = std::min({cap / c->n_kv, (steps + p.least - 1) / p.least, each});
         cap = each * c->n_kv;
     }
-    p.cap = cap <= heads || c->n_seq > TREE_MAX_SEQS || steps <= TREE_WHOLE * p.least ? 0 : (int)cap;
+    p.cap = cap <= heads || c->n_seq > MAX_CUT_SEQS || steps <= WHOLE_STEPS * p.least ? 0 : (int)cap;
     p.each = (int)each;
     p.bytes = p.cap ? (size_t)p.cap * rows * (c->hs + 2) * 4 + heads * sizeof(int2) : 0;
     return p;
@@ -202,8 +117,8 @@ hipError_t launch_tree_attention(const llm_kv &c, const llm_rows &q, const llm_r
     // with one, 16.7 with four; 448 rows of up to 4, eight sequences: 124 and 135)
     const bool wide = p.cap > 16 * c.n_seq * c.n_kv;
     const dim3 grid(wide ? t.max_n * a.group : (t.max_n * a.group + 3) / 4, c.n_kv, c.n_seq);
-    auto *join = q.type == LLM_F32 ? wide ? k_tree_join<LLM_F32, 4> : k_tree_join<LLM_F32, 1>
-                                   : wide ? k_tree_join<LLM_BF16, 4> : k_tree_join<LLM_BF16, 1>;
+    auto *join = q.type == LLM_F32 ? wide ? k_join_slices<TreeArgs, LLM_F32, 4> : k_join_slices<TreeArgs, LLM_F32, 1>
+                                   : wide ? k_join_slices<TreeArgs, LLM_BF16, 4> : k_join_slices<TreeArgs, LLM_BF16, 1>;
     hipLaunchKernelGGL(join, grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }

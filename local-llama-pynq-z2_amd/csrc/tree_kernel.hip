@@ -188,72 +188,6 @@ struct Place {
     int b, h, split, id, row0, len, end, rows, slices, first, last;
 };
 
-// The slice `id`: its sequence, kv head and number there, the slices of that head and their steps.  A sequence of n steps
-// has ceil(n / q) slices a head, the same q for all, so that long sequences do not outlast the others; q is about the least
-// at which there are no more than a.cap in all.  Every block finds it from the lengths.
-__device__ __forceinline__ bool find_slice(const TreeArgs &a, uint32_t id, Place &p, int &steps) {
-    if (a.n_seq == 1) {
-        p.b = 0;
-        p.h = (int)id / a.each;
-        p.split = (int)id - p.h * a.each;
-        p.slices = tree_one(a, tree_steps(a, 0), steps);
-        return p.split < p.slices;
-    }
-    const int lane = threadIdx.x & 63;
-    constexpr int GROUPS = TREE_MAX_SEQS / 64;
-    int all[GROUPS];
-    float sum = 0.0f, most = 0.0f; // (a guess to begin with: rounded sums of steps do)
-#pragma unroll
-    for (int i = 0; i < GROUPS; i++) {
-        all[i] = 0;
-        if (64 * i < a.n_seq) {
-            if (64 * i + lane < a.n_seq) all[i] = tree_steps(a, 64 * i + lane);
-            sum += (float)all[i];
-            most = fmaxf(most, (float)all[i]);
-        }
-    }
-    const float kv = (float)a.n_kv;
-    const int guess = __builtin_amdgcn_readfirstlane((int)(wave_sum(sum) * kv / (float)a.cap));
-    const int longest = __builtin_amdgcn_readfirstlane((int)wave_max(most));
-    steps = longest <= TREE_WHOLE * a.least ? longest : max(max(a.least, guess), longest / a.each + 1);
-    int n[GROUPS];
-    for (;; steps += (steps + 15) / 16) { // (ends: at the longest sequence's steps there is a slice a head)
-        float total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < GROUPS; i++) {
-            n[i] = 0;
-            if (64 * i < a.n_seq) {
-                n[i] = (all[i] + steps - 1) / steps;
-                total += (float)n[i];
-            }
-        }
-        if (wave_sum(total) * kv <= (float)a.cap) break; // (exact up to 2^24)
-    }
-    int before = 0; // slices of a head of the sequences before
-#pragma unroll
-    for (int i = 0; i < GROUPS; i++)
-        if (64 * i < a.n_seq) {
-            int upto = n[i];
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int x = __shfl_up(upto, off);
-                upto += lane >= off ? x : 0;
-            }
-            const int passed = __popcll(__ballot((before + upto) * a.n_kv <= (int)id));
-            if (passed < 64) { // (a lane without a sequence has passed none that its neighbours have not)
-                const int at = __builtin_amdgcn_readfirstlane(passed);
-                p.b = 64 * i + at;
-                p.slices = __builtin_amdgcn_readlane(n[i], at);
-                const int rest = (int)id - (before + __builtin_amdgcn_readlane(upto, at) - p.slices) * a.n_kv;
-                p.h = rest / p.slices;
-                p.split = rest - p.h * p.slices;
-                return true;
-            }
-            before += __builtin_amdgcn_readlane(upto, 63);
-        }
-    return false;
-}
-
 // Blocks go to the eight XCDs in turn.  The row blocks of a slice follow each other on one, whose L2 then holds the slice's
 // rows for all of them.
 template <int QT>
