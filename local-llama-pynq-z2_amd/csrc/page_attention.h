@@ -6,6 +6,7 @@
 
 #include "../../include/llm_hip.h"
 #include "operators.h"
+#include "slices.h"
 
 struct PageArgs {
     const uint8_t *k, *v;
@@ -21,13 +22,28 @@ struct PageArgs {
     const uint64_t *mask;
     int per, n_pages, page, n_seq, n_kv, hs, group, max_n, zero_rest;
     int row_blocks;                 // workgroups that share a kv head's rows
+    int new_tokens;                 // new tokens that count as a step
+    int cap, each, least;           // slices of positions: at most in all (0: none) and of a head, their steps at least
     float c;                        // |softmax scale| * log2(e)
     float sign;                     // the queries' factor: the scale's sign, 0 where the scale is
+    float *ml, *acc;                // slices: [slice][row] (exponent, sum), the same with hs sums of values
+    int2 *plan;                     // [seq][kv head]: first slice, slices
 };
 
+__device__ __forceinline__ int page_len(const PageArgs &a, int seq) {
+    return (int)min((int64_t)max(a.lens[seq], 0), (int64_t)a.per * a.page);
+}
+// Steps that a sequence's new tokens' own rows count as, and all of them: these and the blocks of its positions.
+__device__ __forceinline__ int new_steps(const PageArgs &a, int nn) { return a.kr ? (nn + a.new_tokens - 1) / a.new_tokens : 0; }
+__device__ __forceinline__ int steps_of(const PageArgs &a, int seq) {
+    const int nn = a.n ? min(max(a.n[seq], 0), a.max_n) : a.max_n;
+    return max((page_len(a, seq) + PAGE_BLOCK - 1) / PAGE_BLOCK + new_steps(a, nn), 1);
+}
+
 typedef void (*PageKernel)(PageArgs);
-// The kernel for pages of `type` and queries of `q_type`, and its LDS bytes.
-PageKernel page_kernel_64(int type, int q_type, size_t *lds);
-PageKernel page_kernel_128(int type, int q_type, size_t *lds);
-PageKernel page_kernel_192(int type, int q_type, size_t *lds);
-PageKernel page_kernel_256(int type, int q_type, size_t *lds);
+// The kernel for pages of `type` and queries of `q_type`, `tiles` tiles of 16 rows a wave, its waves taking positions or
+// rows, and its LDS bytes.
+PageKernel page_kernel_64(int type, int q_type, int tiles, int rows, size_t *lds);
+PageKernel page_kernel_128(int type, int q_type, int tiles, int rows, size_t *lds);
+PageKernel page_kernel_192(int type, int q_type, int tiles, int rows, size_t *lds);
+PageKernel page_kernel_256(int type, int q_type, int tiles, int rows, size_t *lds);

@@ -1,4 +1,4 @@
-// llm_page_attention: the entry point (the kernel is in page_kernel.hip).
+// llm_page_attention: how a call is cut, and the entry point (the kernel is in page_kernel.hip).
 #include <string.h>
 
 #include <algorithm>
@@ -12,6 +12,51 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
+struct PagePlan {
+    int hsp, tiles, rows, row_blocks, block_rows, new_tokens, cap, each, least;
+    size_t bytes;
+};
+
+// How a call is cut.  Times: one call, heads of 128, int8 pages.
+// Rows.  The four waves of a workgroup share the positions, with one tile of 16 rows, or two where that is work enough: two read
+// and convert the codes half as often, one gives twice the workgroups (448 rows of bf16 over 4 x 8000 positions, 4 kv heads: 72
+// us with one, 61 with two; 259 of fp32 over 12k: 38 and 46).  Many rows over long contexts: the waves have two other tiles each of
+// the same positions, which need no join of waves, and whose pages the L1 then holds for all four (448 rows over eight sequences
+// of up to 16k: 128 us and 117; fp32 over two of 16k: 108 and 85, over eight of 3000: 62 and 63).
+// Positions.  One sequence: as many slices as give a workgroup a CU, or two a CU where whole row blocks would leave much of the
+// chip idle.  Several: two workgroups a CU over all sequences, of equal steps (more of them cost more in find_slice and the join
+// than they even out: 32 decode steps over 0 to 8190 e4m3 positions 32 us, with four a CU 38).
+PagePlan page_plan(const llm_pages *c, int n_seq, int n_heads, int max_n, int max_len) {
+    PagePlan p;
+    p.hsp = (c->hs + 63) / 64 * 64;
+    const int group = n_heads / c->n_kv, rows = group * max_n, tiles = (rows + 15) / 16;
+    const int64_t heads = (int64_t)n_seq * c->n_kv, blocks = ((int64_t)std::max(max_len, 0) + PAGE_BLOCK - 1) / PAGE_BLOCK;
+    const double work = p.hsp <= 128 && tiles > 1 ? (double)tiles * heads * blocks * p.hsp : 0.0;
+    p.tiles = work >= 2e6 ? 2 : 1;
+    p.rows = work >= 6e6 && tiles > 8;
+    p.block_rows = 16 * p.tiles * (p.rows ? 4 : 1);
+    p.row_blocks = (rows + p.block_rows - 1) / p.block_rows;
+    p.least = p.rows ? 2 : 4; // steps of a slice (one a wave)
+    p.new_tokens = 16;        // (16 new tokens' rows take about as long as a block)
+    const int64_t steps = blocks + (max_n + p.new_tokens - 1) / p.new_tokens;
+    // per XCD; a single sequence: one workgroup a CU, two where whole row blocks would leave much of the chip idle
+    const int64_t one = std::max(32 / p.row_blocks, 1) * 8, both = std::max(64 / p.row_blocks, 1) * 8;
+    int64_t cap = both, each = MAX_SLICES;
+    if (n_seq == 1) {
+        cap = p.tiles > 1 || both / c->n_kv * 5 > one / c->n_kv * 11 ? both : one;
+        each = std::max<int64_t>(std::min({cap / c->n_kv, (steps + p.least - 1) / p.least, each}), 1);
+        cap = each * c->n_kv;
+    }
+    p.cap = cap <= heads || n_seq > MAX_CUT_SEQS || steps <= WHOLE_STEPS * p.least ? 0 : (int)cap;
+    p.each = (int)each;
+    p.bytes = p.cap ? (size_t)p.cap * rows * (c->hs + 2) * 4 + heads * sizeof(int2) : 0;
+    return p;
+}
+
+int64_t page_blocks(const llm_pages *c, int n_seq, const PagePlan &p) { // (rounded up to a slice for each XCD)
+    return ((p.cap ? p.cap : (int64_t)n_seq * c->n_kv) + 7) / 8 * 8 * p.row_blocks;
+}
+
 bool page_shape_ok(const llm_pages *c, int n_heads, int max_n) {
     return c && c->n_kv > 0 && max_n >= 0 && max_n <= 64 && n_heads > 0 && n_heads % c->n_kv == 0 &&
            n_heads / c->n_kv <= 64;
@@ -19,7 +64,10 @@ bool page_shape_ok(const llm_pages *c, int n_heads, int max_n) {
 
 } // namespace
 
-extern "C" size_t llm_page_attention_work(const llm_pages *, int, int, int, int) { return 0; }
+extern "C" size_t llm_page_attention_work(const llm_pages *c, int n_seq, int n_heads, int max_n, int max_len) {
+    return page_shape_ok(c, n_heads, max_n) && max_n > 0 && n_seq > 0 && c->hs >= 16 && c->hs <= 256
+               ? page_plan(c, n_seq, n_heads, max_n, max_len).bytes : 0;
+}
 
 extern "C" int llm_page_attention(const llm_pages *c, const llm_rows *q, const llm_rows *k, const llm_rows *v,
                                   const llm_rows *out, int n_heads, int n_seq, const int *table, int per, const int *lens,
@@ -52,7 +100,16 @@ extern "C" int llm_page_attention(const llm_pages *c, const llm_rows *q, const l
         fprintf(stderr, "%s: q, out and the new rows are of different types\n", who);
         return -1;
     }
-    if (n_seq > 65535 || c->n_kv > 65535) {
+    if (k && (k->tok > (16 << 20) / op_type_bytes(k->type) || v->tok > (16 << 20) / op_type_bytes(v->type))) {
+        fprintf(stderr, "%s: the new rows' tokens have to be at most 16 MiB from the next\n", who);
+        return -1;
+    }
+    const PagePlan p = page_plan(c, n_seq, n_heads, max_n, max_len);
+    if (p.bytes && (work_bytes < p.bytes || ((uintptr_t)work & 15) || !dev.holds(work, "the work memory"))) {
+        fprintf(stderr, "%s: %zu bytes of work memory are needed, 16-byte aligned\n", who, p.bytes);
+        return -1;
+    }
+    if (page_blocks(c, n_seq, p) > 0x7fffffff || n_seq > 65535 || c->n_kv > 65535) {
         fprintf(stderr, "%s: %d sequences of %d kv heads\n", who, n_seq, c->n_kv);
         return -1;
     }
@@ -73,14 +130,31 @@ extern "C" int llm_page_attention(const llm_pages *c, const llm_rows *q, const l
     a.table = table, a.lens = lens, a.n = n, a.mask = mask;
     a.per = per, a.n_pages = c->n_pages, a.page = c->page, a.n_seq = n_seq, a.n_kv = c->n_kv, a.hs = c->hs;
     a.group = n_heads / c->n_kv, a.max_n = max_n, a.zero_rest = zero_rest;
-    a.row_blocks = (a.group * max_n + 15) / 16;
+    a.row_blocks = p.row_blocks, a.cap = p.cap, a.each = p.each, a.least = p.least;
+    a.new_tokens = p.new_tokens;
     a.c = std::fabs(scale) * LOG2E;
     a.sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
-    const int hsp = (c->hs + 63) / 64 * 64;
-    auto *pick = hsp == 64 ? page_kernel_64 : hsp == 128 ? page_kernel_128 : hsp == 192 ? page_kernel_192 : page_kernel_256;
+    a.acc = (float *)work; // (rows of hs values, hs a multiple of 16: 16-byte aligned)
+    const size_t parts = (size_t)p.cap * a.group * max_n;
+    a.ml = a.acc + parts * c->hs;
+    a.plan = (int2 *)(a.ml + 2 * parts);
+    auto *pick = p.hsp == 64 ? page_kernel_64 : p.hsp == 128 ? page_kernel_128 : p.hsp == 192 ? page_kernel_192 : page_kernel_256;
     size_t lds = 0;
-    PageKernel kern = pick(c->type, q->type, &lds);
-    hipLaunchKernelGGL(kern, dim3(a.row_blocks, c->n_kv, n_seq), dim3(256), lds, (hipStream_t)stream, a);
+    PageKernel kern = pick(c->type, q->type, p.tiles, p.rows, &lds);
+    if (!kern) {
+        fprintf(stderr, "%s: no kernel\n", who);
+        return -1;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(kern, dim3((unsigned)page_blocks(c, n_seq, p)), dim3(256), lds, st, a);
+    HIP_OR_FAIL(who, hipGetLastError());
+    if (!p.cap) return 0;
+    // a wave a row up to 16 slices a head, the block's four above
+    const bool wide = p.cap > 16 * n_seq * c->n_kv;
+    const dim3 grid(wide ? max_n * a.group : (max_n * a.group + 3) / 4, c->n_kv, n_seq);
+    auto *join = q->type == LLM_F32 ? wide ? k_join_slices<PageArgs, LLM_F32, 4> : k_join_slices<PageArgs, LLM_F32, 1>
+                                    : wide ? k_join_slices<PageArgs, LLM_BF16, 4> : k_join_slices<PageArgs, LLM_BF16, 1>;
+    hipLaunchKernelGGL(join, grid, dim3(256), 0, st, a);
     HIP_OR_FAIL(who, hipGetLastError());
     return 0;
 }

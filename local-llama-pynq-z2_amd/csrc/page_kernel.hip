@@ -49,16 +49,19 @@ __device__ __forceinline__ void split(float x, float y, uint32_t *p) {
         if (i + 1 < NP) x = fmaf((float)h[0], -1.0f, x), y = fmaf((float)h[1], -1.0f, y);
     }
 }
-// Eight codes (two words) as fp16.  int8: 0x64 over the byte with its sign bit flipped is 1024 + code + 128.
-template <int CT>
+// Eight codes (two words) as fp16.  int8, its sign bit flipped, is code + 128 in a byte: 0x64 over it is 1024 + code + 128, from
+// which 1152 is taken; with BIASED it stays, a subnormal, as 2^-24 (code + 128).
+template <int CT, bool BIASED>
 __device__ __forceinline__ f16x8 codes8(uint32_t a, uint32_t b) {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t u = i < 2 ? a : b;
         if constexpr (CT == LLM_I8) {
-            const uint32_t h = __builtin_amdgcn_perm(0x64646464u, u ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u);
-            r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, h) - (f16x2){(_Float16)1152.0f, (_Float16)1152.0f});
+            const uint32_t h = __builtin_amdgcn_perm(BIASED ? 0u : 0x64646464u, u ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u);
+            r[i] = h;
+            if constexpr (!BIASED)
+                r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, h) - (f16x2){(_Float16)1152.0f, (_Float16)1152.0f});
         } else {
             r[i] = __builtin_bit_cast(uint32_t, i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u, 1.0f, 1)
                                                       : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u, 1.0f, 0));
@@ -68,6 +71,13 @@ __device__ __forceinline__ f16x8 codes8(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ f32x4 product(f16x8 a, u32x4 b, f32x4 d) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
+}
+
+// an operand of ones, or of -128 units of biased codes
+template <bool BIASED>
+__device__ __forceinline__ f16x8 all_of() {
+    const uint32_t u = BIASED ? 0x80808080u : 0x3c003c00u; // (-2^-17, 1)
+    return __builtin_bit_cast(f16x8, (u32x4){u, u, u, u});
 }
 
 // The power of two that takes a magnitude to [2^14, 2^15) (magnitudes below 2^-112 to less, infinities: 2^-127 and NaN), and
@@ -104,13 +114,16 @@ __device__ __forceinline__ void store4(uint8_t *row, int d, float4 y) {
     else *(uint2 *)(row + (size_t)d * 2) = make_uint2(bf2(y.x, y.y), bf2(y.z, y.w));
 }
 
-template <int QT>
-struct Pieces {
-    static constexpr int Q = QT == LLM_BF16 ? 1 : 2, P = 2; // of a query, of a weight
+// How 16-bit rows may hold less: their output is rounded to 8 bits.
+template <int CT, int QT>
+struct Form {
+    static constexpr int Q = QT == LLM_BF16 ? 1 : 2, P = QT == LLM_BF16 ? 1 : 2; // pieces of a query, of a weight
+    static constexpr bool BIASED = QT == LLM_BF16 && CT == LLM_I8;               // codes as 2^-24 (code + 128)
+    static constexpr float UNIT = BIASED ? 0x1p24f : 1.0f;                       // what a product is short of
 };
 
-// The running state of a row: the exponent of 2 that its weights are relative to, the lane's part of their sum, the sums of values
-// (dimension 16 d + 4 j + i).
+// The running state of a row: the exponent of 2 that its weights are relative to, their sum, the sums of values (dimension
+// 16 d + 4 j + i).
 struct State {
     float m, l;
     f32x4 o[DT];
@@ -129,238 +142,515 @@ __device__ __forceinline__ void join(State &s, float ms, float &f, float &g) {
             for (int i = 0; i < 4; i++) s.o[d][i] *= f;
 }
 
-template <int CT, int QT>
-__global__ void __launch_bounds__(256, HSP <= 128 ? 2 : 1) k_page_attention(PageArgs a) {
-    using Pc = Pieces<QT>;
-    extern __shared__ __align__(16) uint8_t lds[];
-    f32x4 *const sm_o = (f32x4 *)lds;                            // [2][DT][64]
-    float2 *const sm_ml = (float2 *)(lds + (size_t)2 * DT * 64 * 16); // [4][16]
-    const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row0 = blockIdx.x * 16, h = blockIdx.y, b = blockIdx.z;
-    const int nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n, rows = nn * a.group;
-    const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.per * a.page), steps = (len + PAGE_BLOCK - 1) / PAGE_BLOCK;
-    if (a.zero_rest && row0 + 16 > rows) // the rows behind the last token
-        for (int e = threadIdx.x * 4; e < 16 * a.hs; e += 1024) {
-            const int row = row0 + e / a.hs, t = row / a.group, d = e % a.hs;
-            if (row >= rows && row < a.max_n * a.group)
-                store4<QT>(a.o + b * a.o_seq + t * a.o_tok + (h * a.group + row - t * a.group) * a.o_head, d,
+// A value that the wave's lanes share and nothing writes while the kernel runs, through the scalar unit.
+template <typename T>
+__device__ __forceinline__ T uniform(const T *p) {
+    return *(const __attribute__((address_space(4))) T *)(uintptr_t)p;
+}
+
+// Where a workgroup works: sequence, kv head, slice (`id` of all), first row; the slice's blocks and whether the
+// new tokens' rows are its, the sequence's positions and rows.
+struct Place {
+    int b, h, split, id, row0, len, nn, rows, slices, first, last;
+    bool fresh;
+};
+
+// Blocks go to the eight XCDs in turn.  The row blocks of a slice follow each other on one, whose L2 then holds the slice's
+// pages for all of them.
+template <int QT>
+__device__ __forceinline__ bool place(const PageArgs &a, int block_rows, Place &p) {
+    const uint32_t k = blockIdx.x >> 3, kr = k / (uint32_t)a.row_blocks, id = kr * 8 + (blockIdx.x & 7);
+    int steps = 0x7fffffff;
+    if (a.cap) {
+        if (id >= (uint32_t)a.cap || !find_slice(a, id, p, steps)) return false;
+    } else {
+        if (id >= (uint32_t)(a.n_seq * a.n_kv)) return false; // (the grid is rounded up to eight slices)
+        p.b = (int)(id / (uint32_t)a.n_kv);
+        p.h = (int)id - p.b * a.n_kv;
+        p.split = 0;
+        p.slices = 1;
+    }
+    p.id = (int)id;
+    p.row0 = (int)(k - kr * a.row_blocks) * block_rows;
+    if (a.cap && a.n_seq > 1 && p.split == 0 && p.row0 == 0 && threadIdx.x == 0) // (for the join)
+        a.plan[p.b * a.n_kv + p.h] = make_int2((int)id, p.slices);
+    p.nn = a.n ? min(max(a.n[p.b], 0), a.max_n) : a.max_n;
+    p.rows = p.nn * a.group;
+    if (a.zero_rest && p.split == 0 && p.row0 + block_rows > p.rows) // the rows behind the last token
+        for (int e = threadIdx.x * 4; e < block_rows * a.hs; e += 1024) {
+            const int row = p.row0 + e / a.hs, t = row / a.group, d = e % a.hs;
+            if (row >= p.rows && row < a.max_n * a.group)
+                store4<QT>(a.o + p.b * a.o_seq + t * a.o_tok + (p.h * a.group + row - t * a.group) * a.o_head, d,
                            make_float4(0.0f, 0.0f, 0.0f, 0.0f));
         }
-    if (row0 >= rows) return;
+    p.len = page_len(a, p.b);
+    const int all = (p.len + PAGE_BLOCK - 1) / PAGE_BLOCK, end = (int)min((int64_t)(p.split + 1) * steps, (int64_t)0x7fffffff);
+    p.first = p.split ? min(p.split * steps, all) : 0;
+    p.last = min(end, all);
+    p.fresh = new_steps(a, p.nn) && p.split == p.slices - 1; // (the steps behind the blocks)
+    return p.row0 < p.rows;
+}
+
+// Sums of row `row` at dimensions d .. d + 3: the output where there is one slice, else this slice's partial sums.
+template <int QT>
+__device__ __forceinline__ void put_values(const PageArgs &a, const Place &p, int row, int d, float4 y) {
+    if (d >= a.hs) return;
+    if (p.slices > 1) {
+        const int64_t part = (int64_t)p.id * a.max_n * a.group + row;
+        *(float4 *)(a.acc + part * a.hs + d) = y;
+        return;
+    }
+    const int t = row / a.group;
+    store4<QT>(a.o + p.b * a.o_seq + t * a.o_tok + (p.h * a.group + row - t * a.group) * a.o_head, d, y);
+}
+template <int QT>
+__device__ __forceinline__ void put_row(const PageArgs &a, const Place &p, int row, int j, const State &s, float l) {
+    if (p.slices > 1 && j == 0) {
+        const int64_t part = (int64_t)p.id * a.max_n * a.group + row;
+        a.ml[2 * part] = s.m;
+        a.ml[2 * part + 1] = l;
+    }
+    const float il = p.slices > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l; // (a row that sees nothing has the sum 0)
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+        put_values<QT>(a, p, row, 16 * d + 4 * j,
+                       make_float4(s.o[d][0] * il, s.o[d][1] * il, s.o[d][2] * il, s.o[d][3] * il));
+}
+
+// The new tokens' own rows, all in fp32: tiles of 16 tokens, from `first` on every `stride`-th.  A tile's K and V values are
+// loaded while the one before is worked on; what is not there reads a row that is.
+template <int QT>
+__device__ __forceinline__ void new_rows(const PageArgs &a, const Place &p, int first, int stride, const uint8_t *qp, bool ok, int tok,
+                                         State &st) {
+    const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4, nn = p.nn, tiles = (nn + 15) / 16;
+    uint64_t sees = 0;
+    if (ok) sees = a.mask ? a.mask[(int64_t)p.b * a.max_n + tok] : ~(uint64_t)0 >> (63 - tok);
+    if (nn < 64) sees &= ((uint64_t)1 << nn) - 1;
+    const uint8_t *const kp = a.kr + p.b * a.k_seq + p.h * a.k_head, *const vp = a.vr + p.b * a.v_seq + p.h * a.v_head;
+    const int part = a.hs / 4; // dimension part * j + 4 s + i is term j of product 4 s + i
+    const float c = a.c * a.sign;
+    float4 kx[HSP / 16], qx[HSP / 16];
+    float v[4][DT];
+    auto load = [&](int t) {
+        const uint8_t *const krow = kp + min(16 * t + n, nn - 1) * a.k_tok;
+#pragma unroll
+        for (int s = 0; s < HSP / 16; s++) kx[s] = load4<QT>(krow, part * j + (4 * s < part ? 4 * s : 0));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint8_t *const vrow = vp + min(16 * t + 4 * j + i, nn - 1) * a.v_tok;
+#pragma unroll
+            for (int d = 0; d < DT; d++) v[i][d] = load1<QT>(vrow, (16 * d < a.hs ? 16 * d : 0) + n);
+        }
+    };
+    // (tiles of which no row sees a token are left out)
+    auto next = [&](int t) {
+        while (t < tiles && !__any((int)(sees >> 16 * t) & 0xffff)) t += stride;
+        return t;
+    };
+    int t = next(first);
+    if (t >= tiles) return;
+    load(t);
+#pragma unroll
+    for (int s = 0; s < HSP / 16; s++) {
+        qx[s] = load4<QT>(qp, part * j + (4 * s < part ? 4 * s : 0));
+        if (!ok || 4 * s >= part) qx[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (;;) {
+        f32x4 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < HSP / 16; s++) // (four chains: a score is off by half as much as one would be)
+            if (4 * s < part) {
+                y[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[s].x, qx[s].x, y[0], 0, 0, 0);
+                y[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[s].y, qx[s].y, y[1], 0, 0, 0);
+                y[2] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[s].z, qx[s].z, y[2], 0, 0, 0);
+                y[3] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[s].w, qx[s].w, y[3], 0, 0, 0);
+            }
+        const f32x4 sum = (y[0] + y[1]) + (y[2] + y[3]);
+        const uint32_t mine = (uint32_t)(sees >> (16 * t + 4 * j));
+        float x[4], ms = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; i++) { // token 16 t + 4 j + i
+            x[i] = mine & (1u << i) ? sum[i] * c : -INFINITY;
+            ms = fmaxf(ms, x[i]);
+        }
+        ms = over_groups(ms, fmax_);
+        const float mu = ms == -INFINITY ? 0.0f : ms;
+        float f, g, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[i] = __builtin_amdgcn_exp2f(x[i] - mu);
+            l += x[i];
+        }
+        l = over_groups(l, fadd_);
+        join(st, ms, f, g);
+        bool nf[4] = {false, false, false, false};
+        f32x4 z[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            z[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 4; i++) { // a value that is not finite is zero here
+                const bool bad = !(fabsf(v[i][d]) < INFINITY);
+                nf[i] |= bad;
+                z[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 0.0f : v[i][d], x[i], z[d], 0, 0, 0);
+            }
+        }
+        const int now = t;
+        t = next(t + stride);
+        if (t < tiles) load(t);
+        st.l = fmaf(l, g, st.l);
+        if (__any(nf[0] | nf[1] | nf[2] | nf[3])) { // and who sees its token becomes NaN
+            uint64_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint64_t any = __ballot(nf[i] && 16 * now + 4 * j + i < nn);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if ((any >> (16 * k)) & 0xffff) bad |= (uint64_t)1 << (16 * now + 4 * k + i);
+            }
+            if (sees & bad) st.l = NAN;
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) st.o[d][i] = fmaf(z[d][i], g, st.o[d][i]);
+        if (t >= tiles) return;
+    }
+}
+
+// LDS: 16-byte values a lane of a wave with two tiles (their queries, later a tile's sums), and bytes in all (later what joins the waves).
+template <int R, int Q>
+constexpr int page_wave_lds() {
+    const int q = R * 2 * KL * Q;
+    return R == 1 ? 0 : q > DT ? q : DT;
+}
+template <int R, bool ROWS, int Q>
+constexpr size_t page_lds() {
+    const size_t q = (size_t)4 * page_wave_lds<R, Q>() * 64 * 16, o = ROWS ? 0 : (size_t)2 * R * DT * 64 * 16 + 4 * R * 16 * 8;
+    return q > o ? q : o;
+}
+
+// A wave has R tiles of 16 rows.  ROWS: the workgroup's four waves have other rows of the same positions each; else they share the
+// rows and take every fourth step, and are joined at the end.  A step's codes are converted once for the R tiles; the next step's
+// loads go out as soon as a step's registers are used, its page's number a step before.
+template <int CT, int QT, int R, bool ROWS>
+__global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(PageArgs a) {
+    using Fm = Form<CT, QT>;
+    constexpr int WAVE_LDS = page_wave_lds<R, Fm::Q>();
+    constexpr int STRIDE = ROWS ? 1 : 4, BLOCK_ROWS = 16 * R * (ROWS ? 4 : 1);
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Place p;
+    if (!place<QT>(a, BLOCK_ROWS, p)) return;
+    const int row0 = p.row0 + (ROWS ? wave * 16 * R : 0);
+    if (ROWS && row0 >= p.rows) return; // (no wave waits for another)
+
+    const uint32_t bytes = PAGE_BLOCK * a.hs;
+    const int *const table = a.table + (int64_t)p.b * a.per;
+    const int shift = __builtin_ctz(a.page); // (a power of two)
+    auto page_of = [&](int step) { // -1: none
+        int page = -1;
+        if (step < p.last) page = uniform(table + (step * PAGE_BLOCK >> shift));
+        return (uint32_t)page < (uint32_t)a.n_pages ? page : -1;
+    };
+    // Offsets are formed again at every use, from values that the compiler cannot see through: all of them kept across the loop
+    // take registers that spill, and a reload waits for the loads under way.
+    auto again = [](uint32_t x) {
+        asm volatile("" : "+v"(x));
+        return x;
+    };
+    const uint32_t k_at = (16 * (n >> 2) + (n & 3)) * a.hs + 16 * j, k_last = 64 * (KL - 1) + 16 * j < a.hs ? k_at : OUT_OF_RANGE;
+    u32x4 kr[4][KL], vr[DT];
+    float ks = 0.0f, vs = 0.0f; // (no page: nothing of the step is seen, and zero scales keep it finite)
+    auto load_k = [&](int step, int page) {
+        const int blk = (step * PAGE_BLOCK & (a.page - 1)) / PAGE_BLOCK;
+        const uint8_t *base = a.k;
+        ks = 0.0f;
+        if (page >= 0) {
+            base += page * a.id + p.h * a.head + blk * (int64_t)bytes;
+            ks = uniform(a.ks + (page * a.s_id + p.h * a.s_head + blk));
+        }
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, page >= 0 ? (int)bytes : 0, 0x00020000);
+        const uint32_t at = again(k_at), last = again(k_last);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < KL; i++) {
+                const auto c = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)((i < KL - 1 ? at : last) + 4 * t * a.hs + 64 * i), 0, 0);
+                kr[t][i] = (u32x4){c[0], c[1], c[2], c[3]};
+            }
+    };
+    auto load_v = [&](int step, int page) {
+        const int blk = (step * PAGE_BLOCK & (a.page - 1)) / PAGE_BLOCK;
+        const uint8_t *base = a.v;
+        vs = 0.0f;
+        if (page >= 0) {
+            base += page * a.id + p.h * a.head + blk * (int64_t)bytes;
+            vs = uniform(a.vs + (page * a.s_id + p.h * a.s_head + blk));
+        }
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, page >= 0 ? (int)bytes : 0, 0x00020000);
+        const uint32_t at = again(n * PAGE_BLOCK + 16 * j);
+#pragma unroll
+        for (int d = 0; d < DT; d++) { // (dimensions from hs on lie past the block)
+            const auto c = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(at + 16 * d * PAGE_BLOCK), 0, 0);
+            vr[d] = (u32x4){c[0], c[1], c[2], c[3]};
+        }
+    };
+    u32x4 *const mine_ = (u32x4 *)lds + wave * WAVE_LDS * 64 + lane; // [WAVE_LDS][64], a lane's own
+    auto park = [&](State &s, bool out) {
+        f32x4 *const at = (f32x4 *)mine_;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            if (out) at[d * 64] = s.o[d];
+            else s.o[d] = at[d * 64];
+        }
+    };
+    int step = p.first + (ROWS ? 0 : wave);
+    int page = page_of(step), next = page_of(step + STRIDE);
+    if (R == 1) { // (with more rows their queries' values take the registers)
+        load_k(step, page);
+        load_v(step, page);
+    }
 
     // the queries: value e of product s is dimension 64 (s / 2) + 16 j + 8 (s % 2) + e
-    const int row = row0 + n, tok = row / a.group;
-    const bool ok = row < rows;
-    const uint8_t *const qp = a.q + b * a.q_seq + (ok ? tok * a.q_tok + (h * a.group + row - tok * a.group) * a.q_head : 0);
-    u32x4 qf[2 * KL][Pc::Q];
-    float cq;
-    {
+    // (two tiles' queries wait in LDS, a lane's own: in registers they would spill)
+    u32x4 qf[R > 1 ? 1 : R][2 * KL][Fm::Q];
+    u32x4 *const sm_q = mine_; // [R][2 KL][Q]
+    float cq[R];
+    State st[R];
+    float off[R], bias[R]; // what scores and values of biased codes have too much: 128 times a query's sum, and the weights'
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int row = row0 + 16 * r + n, tok = row / a.group;
+        const bool ok = row < p.rows;
+        const uint8_t *const qp = a.q + p.b * a.q_seq + (ok ? tok * a.q_tok + (p.h * a.group + row - tok * a.group) * a.q_head : 0);
         float x[2 * KL][8], mx = 0.0f;
 #pragma unroll
         for (int s = 0; s < 2 * KL; s++)
 #pragma unroll
-            for (int q4 = 0; q4 < 2; q4++) {
+            for (int q4 = 0; q4 < 2; q4++) { // (what is not there reads the row's start: no load waits behind a condition)
                 const int d = 64 * (s / 2) + 16 * j + 8 * (s % 2) + 4 * q4;
-                const float4 y = ok && d < a.hs ? load4<QT>(qp, d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 y = load4<QT>(qp, d < a.hs ? d : 0);
                 x[s][4 * q4] = y.x, x[s][4 * q4 + 1] = y.y, x[s][4 * q4 + 2] = y.z, x[s][4 * q4 + 3] = y.w;
-                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+            }
+#pragma unroll
+        for (int s = 0; s < 2 * KL; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (!ok || 64 * (s / 2) + 16 * j + 8 * (s % 2) >= a.hs) x[s][e] = 0.0f;
+                mx = fmaxf(mx, fabsf(x[s][e]));
             }
         const uint32_t e = exponent(over_groups(mx, fmax_));
         const float to = power_to(e) * a.sign;
-        cq = a.c * power_from(e);
+        cq[r] = a.c * power_from(e) * Fm::UNIT;
 #pragma unroll
         for (int s = 0; s < 2 * KL; s++)
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                uint32_t p[Pc::Q];
-                split<Pc::Q>(x[s][i] * to, x[s][i + 1] * to, p);
+                uint32_t w[Fm::Q];
+                split<Fm::Q>(x[s][i] * to, x[s][i + 1] * to, w);
 #pragma unroll
-                for (int k = 0; k < Pc::Q; k++) qf[s][k][i / 2] = p[k];
+                for (int k = 0; k < Fm::Q; k++) qf[R > 1 ? 0 : r][s][k][i / 2] = w[k];
             }
+        if (R > 1)
+#pragma unroll
+            for (int s = 0; s < 2 * KL; s++)
+#pragma unroll
+                for (int k = 0; k < Fm::Q; k++) sm_q[((r * 2 * KL + s) * Fm::Q + k) * 64] = qf[0][s][k];
+        st[r].m = -INFINITY, st[r].l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) st[r].o[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        off[r] = bias[r] = 0.0f;
+        if (Fm::BIASED) {
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < 2 * KL; s++) sum = product(all_of<true>(), qf[R > 1 ? 0 : r][s][0], sum);
+            off[r] = sum[0];
+        }
     }
-
-    State st;
-    st.m = -INFINITY, st.l = 0.0f;
+    if (R > 1) {
+        load_k(step, page);
+        load_v(step, page);
+    }
+    for (; step < p.last; step += STRIDE) {
+        const int left = page < 0 ? 0 : p.len - step * PAGE_BLOCK; // positions of the block that are seen
+        const int mine = left - (int)again(16 * j);                // of the lane's 16
+        f32x4 x[R][4];
 #pragma unroll
-    for (int d = 0; d < DT; d++) st.o[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t bytes = PAGE_BLOCK * a.hs;
-    for (int step = wave; step < steps; step += 4) {
-        const int at = step * PAGE_BLOCK;
-        const int page = __builtin_amdgcn_readfirstlane(a.table[(int64_t)b * a.per + at / a.page]), blk = at % a.page / PAGE_BLOCK;
-        if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
-        const int64_t base = page * a.id + h * a.head + blk * (int64_t)bytes, s_at = page * a.s_id + h * a.s_head + blk;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + base), 0, (int)bytes, 0x00020000);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc((void *)(a.v + base), 0, (int)bytes, 0x00020000);
-        const float ks = a.ks[s_at] * cq, vs = a.vs[s_at];
-        f32x4 x[4];
-        float ms = -INFINITY;
-        const int left = len - at; // positions of the block that are there
+        for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            x[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < 4; t++) x[r][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < KL; i++) {
-                const uint32_t d = 64 * i + 16 * j, off = (16 * (n >> 2) + 4 * t + (n & 3)) * a.hs + d;
-                const auto c = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(d < (uint32_t)a.hs ? off : OUT_OF_RANGE), 0, 0);
+        for (int s = 0; s < 2 * KL; s++) {
+            u32x4 q[R][Fm::Q];
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const f16x8 kf = codes8<CT>(c[2 * u], c[2 * u + 1]);
+            for (int r = 0; r < R; r++)
 #pragma unroll
-                    for (int p = Pc::Q - 1; p >= 0; p--) x[t] = product(kf, qf[2 * i + u][p], x[t]); // smallest pieces first
-                }
-            }
+                for (int k = 0; k < Fm::Q; k++) q[r][k] = R > 1 ? sm_q[((r * 2 * KL + s) * Fm::Q + k) * 64] : qf[r % (R > 1 ? 1 : R)][s][k];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x[t][i] = 16 * j + 4 * t + i < left ? x[t][i] * ks : -INFINITY;
-                ms = fmaxf(ms, x[t][i]);
+            for (int t = 0; t < 4; t++) {
+                const f16x8 kf = codes8<CT, Fm::BIASED>(kr[t][s / 2][2 * (s % 2)], kr[t][s / 2][2 * (s % 2) + 1]);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int k = Fm::Q - 1; k >= 0; k--) x[r][t] = product(kf, q[r][k], x[r][t]); // smallest pieces first
             }
         }
-        ms = over_groups(ms, fmax_);
-        // A step's largest weight is 2^15, the top of fp16's range.  Scores from 2^23 on have steps of 1 or more, and the
-        // difference could be 16: those weights are few and far apart, and their largest is 1.
-        ms -= fabsf(ms) < 0x1p23f ? 15.0f : 0.0f;
-        const float mu = ms == -INFINITY ? 0.0f : ms;
-        float f, g, l = 0.0f;
-        u32x4 pf[2][Pc::P];
+        // a scale below zero turns the scores round; one that is not finite makes every row NaN through its values
+        if (ks < 0.0f)
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+            for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float w0 = __builtin_amdgcn_exp2f(x[2 * u + e / 4][e % 4] - mu);
-                const float w1 = __builtin_amdgcn_exp2f(x[2 * u + e / 4][e % 4 + 1] - mu);
-                l += w0;
-                l += w1;
-                uint32_t p[Pc::P];
-                split<Pc::P>(w0, w1, p);
+                for (int t = 0; t < 4; t++) x[r][t] = -x[r][t];
+        const float size = fabsf(ks) < INFINITY ? fabsf(ks) : 0.0f, v_size = fabsf(ks) < INFINITY ? vs : NAN;
+        u32x4 pf[R][2][Fm::P];
+        float gv[R];
 #pragma unroll
-                for (int k = 0; k < Pc::P; k++) pf[u][k][e / 2] = p[k];
+        for (int r = 0; r < R; r++) {
+            float c = fmaxf(cq[r] * size, 1e-45f), ms = -INFINITY; // (never 0: what is not seen is -infinity times it)
+            if (left < PAGE_BLOCK)
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (4 * t + i >= mine) x[r][t][i] = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) ms = fmaxf(ms, x[r][t][i]);
+            float o = Fm::BIASED ? ks < 0.0f ? -off[r] : off[r] : 0.0f;
+            ms = (over_groups(ms, fmax_) + o) * c;
+            // A step's largest weight is 2^15, the top of fp16's range.  Scores from 2^23 on have steps of 1 or more, and the
+            // difference could be 16: those weights are few and far apart, their largest is 1, and it takes scores rounded alike.
+            if (__any(fabsf(ms) >= 0x1p23f && ms != -INFINITY)) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[r][t][i] = (x[r][t][i] + o) * c;
+                c = 1.0f, o = 0.0f;
             }
-        join(st, ms, f, g);
-        st.l += l * g;
-        const float gv = g * vs;
+            ms -= fabsf(ms) < 0x1p23f ? 15.0f : 0.0f;
+            const float mu = fmaf(o, c, ms == -INFINITY ? 0.0f : -ms);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    uint32_t w[Fm::P];
+                    split<Fm::P>(__builtin_amdgcn_exp2f(fmaf(x[r][2 * u + e / 4][e % 4], c, mu)),
+                                 __builtin_amdgcn_exp2f(fmaf(x[r][2 * u + e / 4][e % 4 + 1], c, mu)), w);
+#pragma unroll
+                    for (int k = 0; k < Fm::P; k++) pf[r][u][k][e / 2] = w[k];
+                }
+            // the sum of the weights as the products take them: 1 or, for biased codes, -128 of their units times each
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = Fm::P - 1; k >= 0; k--)
+#pragma unroll
+                for (int u = 0; u < 2; u++) sum = product(all_of<Fm::BIASED>(), pf[r][u][k], sum);
+            float f, g;
+            join(st[r], ms, f, g);
+            gv[r] = g * v_size * Fm::UNIT;
+            st[r].l = fmaf(Fm::BIASED ? sum[0] * -0x1p17f : sum[0], g, st[r].l);
+            if (Fm::BIASED) bias[r] = fmaf(bias[r], f, sum[0] * gv[r]);
+        }
+        load_k(step + STRIDE, next);
+        if (CT == LLM_E4M3 && left < PAGE_BLOCK) // codes past the end may be NaN: 0 * NaN
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int have = min(max(mine - 4 * k, 0), 4);
+                const uint32_t keep = have == 4 ? 0xffffffffu : (1u << (8 * have)) - 1;
+#pragma unroll
+                for (int d = 0; d < DT; d++) vr[d][k] &= keep;
+            }
 #pragma unroll
         for (int d = 0; d < DT; d++) {
-            if (16 * d >= a.hs) break;
-            const auto c = __builtin_amdgcn_raw_buffer_load_b128(rv, (16 * d + n) * PAGE_BLOCK + 16 * j, 0, 0);
-            uint32_t w[4] = {c[0], c[1], c[2], c[3]};
-            if (CT == LLM_E4M3 && left < PAGE_BLOCK) // codes past the end may be NaN: 0 * NaN
+            f16x8 vf[2];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int have = min(max(left - 16 * j - 4 * k, 0), 4);
-                    w[k] &= have == 4 ? 0xffffffffu : (1u << (8 * have)) - 1;
-                }
-            f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int u = 0; u < 2; u++) vf[u] = codes8<CT, Fm::BIASED>(vr[d][2 * u], vr[d][2 * u + 1]);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const f16x8 vf = codes8<CT>(w[2 * u], w[2 * u + 1]);
+            for (int r = 0; r < R; r++) {
+                f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int p = Pc::P - 1; p >= 0; p--) y = product(vf, pf[u][p], y);
+                for (int k = Fm::P - 1; k >= 0; k--)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) y = product(vf[u], pf[r][u][k], y);
+#pragma unroll
+                for (int i = 0; i < 4; i++) st[r].o[d][i] = fmaf(y[i], gv[r], st[r].o[d][i]);
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++) st.o[d][i] = fmaf(y[i], gv, st.o[d][i]);
         }
+        load_v(step + STRIDE, next);
+        page = next;
+        next = page_of(step + 2 * STRIDE);
     }
 
-    // the new tokens' own rows, by the wave with the fewest steps: tiles of 16 tokens, all in fp32
-    if (a.kr && wave == (steps & 3)) {
-        uint64_t sees = 0;
-        if (ok) sees = a.mask ? a.mask[(int64_t)b * a.max_n + tok] : ~(uint64_t)0 >> (63 - tok);
-        if (nn < 64) sees &= ((uint64_t)1 << nn) - 1;
-        const uint8_t *const kp = a.kr + b * a.k_seq + h * a.k_head, *const vp = a.vr + b * a.v_seq + h * a.v_head;
-        const int part = a.hs / 4; // dimension part * j + 4 s + i is term j of product 4 s + i
-        float c = a.c * a.sign;
-        for (int t = 0; t < (nn + 15) / 16; t++) {
-            f32x4 y[4];
+    if (Fm::BIASED)
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-            const bool there = 16 * t + n < nn;
-            for (int s = 0; s < part; s += 4) { // (four chains: a score is off by half as much as one would be)
-                const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const float4 kx = there ? load4<QT>(kp + (16 * t + n) * a.k_tok, part * j + s) : none;
-                const float4 qx = ok ? load4<QT>(qp, part * j + s) : none;
-                y[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx.x, qx.x, y[0], 0, 0, 0);
-                y[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx.y, qx.y, y[1], 0, 0, 0);
-                y[2] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx.z, qx.z, y[2], 0, 0, 0);
-                y[3] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx.w, qx.w, y[3], 0, 0, 0);
-            }
-            const f32x4 sum = (y[0] + y[1]) + (y[2] + y[3]);
-            float x[4], ms = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; i++) { // token 16 t + 4 j + i
-                x[i] = (sees >> (16 * t + 4 * j + i)) & 1 ? sum[i] * c : -INFINITY;
-                ms = fmaxf(ms, x[i]);
-            }
-            ms = over_groups(ms, fmax_);
-            const float mu = ms == -INFINITY ? 0.0f : ms;
-            float f, g, l = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x[i] = __builtin_amdgcn_exp2f(x[i] - mu);
-                l += x[i];
-            }
-            join(st, ms, f, g);
-            uint64_t bad = 0; // tokens whose V row is not finite: who sees them becomes NaN, to the others they are zero
-            f32x4 z[DT];
-#pragma unroll
-            for (int d = 0; d < DT; d++) z[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int at = 16 * t + 4 * j + i;
-                bool nf = false;
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    if (16 * d >= a.hs) break;
-                    float v = at < nn ? load1<QT>(vp + at * a.v_tok, 16 * d + n) : 0.0f;
-                    if (!(fabsf(v) < INFINITY)) nf = true, v = 0.0f;
-                    z[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[i], z[d], 0, 0, 0);
-                }
-                const uint64_t any = __ballot(nf);
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if ((any >> (16 * k)) & 0xffff) bad |= (uint64_t)1 << (16 * t + 4 * k + i);
-            }
-            st.l = sees & bad ? NAN : st.l + l * g;
+        for (int r = 0; r < R; r++)
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) st.o[d][i] = fmaf(z[d][i], g, st.o[d][i]);
+                for (int i = 0; i < 4; i++) st[r].o[d][i] += bias[r];
+    // the new tokens' rows; waves that share the rows take a tile each, from the one with the fewest steps on
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int row = row0 + 16 * r + n, tok = row / a.group;
+        const bool ok = row < p.rows;
+        const uint8_t *const qp = a.q + p.b * a.q_seq + (ok ? tok * a.q_tok + (p.h * a.group + row - tok * a.group) * a.q_head : 0);
+        if (!p.fresh || row0 + 16 * r >= p.rows) break;
+        if (R > 1) park(st[R - 1 - r], true); // (the other tile's sums out of the way, over the queries)
+        new_rows<QT>(a, p, ROWS ? 0 : (wave - (p.last - p.first)) & 3, ROWS ? 1 : 4, qp, ok, tok, st[r]);
+        if (R > 1) park(st[R - 1 - r], false);
+    }
+    if constexpr (!ROWS) { // the four waves' sums joined: each scaled to a common exponent, waves 2 and 3 into 0 and 1, then 1 into 0
+        f32x4 *const sm_o = (f32x4 *)lds;                                     // [2][R][DT][64]
+        float2 *const sm_ml = (float2 *)(lds + (size_t)2 * R * DT * 64 * 16); // [4][R][16]
+        __syncthreads(); // (their queries may lie there)
+        if (j == 0)
+#pragma unroll
+            for (int r = 0; r < R; r++) sm_ml[(wave * R + r) * 16 + n] = make_float2(st[r].m, st[r].l);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float mn = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) mn = fmaxf(mn, sm_ml[(w * R + r) * 16 + n].x);
+            const float mu = mn == -INFINITY ? 0.0f : mn, al = __builtin_amdgcn_exp2f(st[r].m - mu);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float2 ml = sm_ml[(w * R + r) * 16 + n];
+                l += ml.y * __builtin_amdgcn_exp2f(ml.x - mu);
+            }
+            st[r].m = mn, st[r].l = l;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) st[r].o[d][i] *= al;
         }
+#pragma unroll
+        for (int half = 2; half; half >>= 1) {
+            if (wave >= half && wave < 2 * half)
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) sm_o[(((wave - half) * R + r) * DT + d) * 64 + lane] = st[r].o[d];
+            __syncthreads();
+            if (wave < half)
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) st[r].o[d] += sm_o[((wave * R + r) * DT + d) * 64 + lane];
+            __syncthreads();
+        }
+        if (wave) return;
     }
-
-    // the four waves' sums joined: each scaled to the common maximum, waves 2 and 3 into 0 and 1, then 1 into 0
-    st.l = over_groups(st.l, fadd_);
-    if (j == 0) sm_ml[wave * 16 + n] = make_float2(st.m, st.l);
-    __syncthreads();
-    float mn = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) mn = fmaxf(mn, sm_ml[w * 16 + n].x);
-    const float mu = mn == -INFINITY ? 0.0f : mn;
-#pragma unroll
-    for (int w = 0; w < 4; w++) l += sm_ml[w * 16 + n].y * __builtin_amdgcn_exp2f(sm_ml[w * 16 + n].x - mu);
-    const float al = __builtin_amdgcn_exp2f(st.m - mu);
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) st.o[d][i] *= al;
-#pragma unroll
-    for (int half = 2; half; half >>= 1) {
-        if (wave >= half && wave < 2 * half)
-#pragma unroll
-            for (int d = 0; d < DT; d++) sm_o[((wave - half) * DT + d) * 64 + lane] = st.o[d];
-        __syncthreads();
-        if (wave < half)
-#pragma unroll
-            for (int d = 0; d < DT; d++) st.o[d] += sm_o[(wave * DT + d) * 64 + lane];
-        __syncthreads();
+    for (int r = 0; r < R; r++) {
+        const int row = row0 + 16 * r + n;
+        if (row < p.rows) put_row<QT>(a, p, row, j, st[r], st[r].l);
     }
-    if (wave || !ok) return;
-    const float il = l == 0.0f ? 0.0f : 1.0f / l;
-    uint8_t *const op = a.o + b * a.o_seq + tok * a.o_tok + (h * a.group + row - tok * a.group) * a.o_head;
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-        if (16 * d < a.hs)
-            store4<QT>(op, 16 * d + 4 * j, make_float4(st.o[d][0] * il, st.o[d][1] * il, st.o[d][2] * il, st.o[d][3] * il));
 }
 
 } // namespace
@@ -368,8 +658,18 @@ __global__ void __launch_bounds__(256, HSP <= 128 ? 2 : 1) k_page_attention(Page
 #define PAGE_NAME2(n) page_kernel_##n
 #define PAGE_NAME(n) PAGE_NAME2(n)
 
-PageKernel PAGE_NAME(PAGE_HSP)(int type, int q_type, size_t *lds) {
-    *lds = (size_t)2 * DT * 64 * 16 + 4 * 16 * 8;
-    if (type == LLM_I8) return q_type == LLM_F32 ? k_page_attention<LLM_I8, LLM_F32> : k_page_attention<LLM_I8, LLM_BF16>;
-    return q_type == LLM_F32 ? k_page_attention<LLM_E4M3, LLM_F32> : k_page_attention<LLM_E4M3, LLM_BF16>;
+PageKernel PAGE_NAME(PAGE_HSP)(int type, int q_type, int tiles, int rows, size_t *lds) {
+#define PAGE_PICK(C, QY, T, W)                                                   \
+    if (type == C && q_type == QY && tiles == T && (rows != 0) == W) {            \
+        *lds = page_lds<T, W, Form<C, QY>::Q>();                                 \
+        return k_page_attention<C, QY, T, W>;                                    \
+    }
+#define PAGE_PICK_T(T, W)                                                        \
+    PAGE_PICK(LLM_I8, LLM_F32, T, W) PAGE_PICK(LLM_I8, LLM_BF16, T, W)           \
+    PAGE_PICK(LLM_E4M3, LLM_F32, T, W) PAGE_PICK(LLM_E4M3, LLM_BF16, T, W)
+    PAGE_PICK_T(1, false)
+#if PAGE_HSP <= 128
+    PAGE_PICK_T(2, false) PAGE_PICK_T(2, true)
+#endif
+    return nullptr;
 }

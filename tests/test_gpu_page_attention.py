@@ -6,7 +6,10 @@ Tolerances.  u = 2^-24, half a step of fp32; L the positions a row sees, |q| its
   row, a weight is off by a factor of e^(2 d), and everything else (exponentials, a weight's second fp16 piece (2 u), sums, scales,
   joins) by (L + 64) u: all relative to sum p |v|.
   A weight far below the block's largest is held to 2^-39 of that, at most 1: L 2^-39 max |v|.
-  bf16 outputs: 2^-8 of the value."""
+  bf16 rows: the output's rounding, 2^-8 of the value; a weight over pages is one fp16 piece, off by 2^-11 at most, and so is its
+  share of the sum: 2^-10 sum p |v|.  int8 codes count as code + 128 on the way, with 128 times the query's and the weights' sums
+  taken off again: sums of up to 255 in the place of 127 |code|, (hs + 8) u |scale| 128 s sum |q| more for a score (s the block's
+  scale) and (L + 64) u 128 s sum p for a value."""
 import math
 import random
 
@@ -35,6 +38,8 @@ def tree_masks(r, b, t):
 
 
 def check(pool, table, q, kn, vn, lens, n, mask, scale, got, layer=0):
+    half = got.dtype == torch.bfloat16
+    biased = half and pool.cache == "int8"
     b, t, heads, hs = q.shape
     group, page = heads // pool.h, pool.page
     val = [pool.values(0, layer), pool.values(1, layer)]
@@ -48,6 +53,8 @@ def check(pool, table, q, kn, vn, lens, n, mask, scale, got, layer=0):
         for h in range(pool.h):
             k, v = val[0][pg, h, off].reshape(-1, hs), val[1][pg, h, off].reshape(-1, hs)
             old = k.shape[0]
+            size_k, size_v = ((pool.scale[side][layer][pg, h].abs().double()[range(old), [o // 64 for o in off]] if biased and old else
+                               torch.zeros(old, dtype=torch.float64)) for side in range(2))
             if kn is not None:
                 k, v = torch.cat((k, kn[i, :live, h].double())), torch.cat((v, vn[i, :live, h].double()))
             for j in range(live):
@@ -68,9 +75,13 @@ def check(pool, table, q, kn, vn, lens, n, mask, scale, got, layer=0):
                         assert y.isnan().all()
                         continue
                     d = abs(scale) * float(((hs + 8) * U * (ks.abs() @ qd.abs()) + 2.0 ** -39 * qd.abs().max() * ks.abs().sum(1)).max())
+                    if biased and old:
+                        d += abs(scale) * (hs + 8) * U * 128 * float(size_k.max()) * float(qd.abs().sum())
                     tol = (math.expm1(min(2 * d, 700.0)) + (len(ks) + 64) * U) * size + len(ks) * 2.0 ** -39 * float(vs.abs().max()) + 1e-37
-                    if got.dtype == torch.bfloat16:
-                        tol = tol + 2.0 ** -8 * want.abs()
+                    if half:
+                        tol = tol + 2.0 ** -8 * want.abs() + 2.0 ** -10 * size
+                    if biased and old:
+                        tol = tol + (len(ks) + 64) * U * 128 * float((p[:old] * size_v).sum())
                     worst = max(worst, float(((y - want).abs() / tol).max()))
                     assert ((y - want).abs() <= tol).all(), (i, j, x, worst)
         # rows behind the last token
