@@ -424,8 +424,9 @@ def _pages(k, v, k_scale, v_scale):
     their scales [pages, kv heads, page / 64] (float32), with the layers before the pages or without; pages and heads may lie apart.
     And its dimensions (layers, pages, kv heads, page, head size)"""
     torch, types = _torch or _types()
-    ty, shape, many = types.get(k.dtype, 0), k.shape, k.dim() == 5
-    if ty < 2 or v.dtype is not k.dtype or len(shape) != 4 + many or (shape[-2] % 64 or not shape[-2]):
+    ty, shape = types.get(k.dtype, 0), k.shape
+    many = len(shape) == 5
+    if ty < 2 or v.dtype is not k.dtype or len(shape) != 4 + many or shape[-2] % 64 or not shape[-2]:
         raise ValueError("k: int8 or float8_e4m3fn codes [pages, kv heads, page, head size] are needed, v of the same type")
     page, hs = shape[-2:]
     rows = shape[:-2] + (page // 64,)
@@ -434,18 +435,18 @@ def _pages(k, v, k_scale, v_scale):
     f32 = torch.float32
     if k_scale.shape != rows or v_scale.shape != rows or k_scale.dtype is not f32 or v_scale.dtype is not f32:
         raise ValueError(f"k_scale, v_scale: float32 {tuple(rows)} are needed")
-    if not many:
-        k, v, k_scale, v_scale = k.unsqueeze(0), v.unsqueeze(0), k_scale.unsqueeze(0), v_scale.unsqueeze(0)
-    n = k.shape[:3]
     sk, sv, ss, st = k.stride(), v.stride(), k_scale.stride(), v_scale.stride()
-    if (sk[4] != 1 and hs > 1) or sk[3] != hs or sv[5] != 1 or sv[4] != 64 or (page > 64 and (sv[3] != 64 * hs or ss[3] != 1 or
-                                                                                            st[3] != 1)):
+    if (sk[-1] != 1 and hs > 1) or sk[-2] != hs or sv[-1] != 1 or sv[-2] != 64 or \
+            (page > 64 and (sv[-3] != 64 * hs or ss[-1] != 1 or st[-1] != 1)):
         raise ValueError("k, v and their scales: what a page holds of a head has to lie together")
-    if any(n[i] > 1 and (sk[i] != sv[i] or ss[i] != st[i]) for i in range(3)):
-        raise ValueError("k and v, and their scales: equal strides of layers, pages and heads are needed")
-    at = [(sk[i], ss[i]) if n[i] > 1 else (0, 0) for i in range(3)]
-    return _PACK_PAGES(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, *n, hs, page,
-                       *(x[0] for x in at), *(x[1] for x in at)), (*n, page, hs)
+    n, at = (shape[:3] if many else (1, *shape[:2])), [0] * 6
+    for i in range(0 if many else 1, 3): # (a dimension of one has no stride that counts)
+        if n[i] > 1:
+            j = i if many else i - 1
+            if sk[j] != sv[j] or ss[j] != st[j]:
+                raise ValueError("k and v, and their scales: equal strides of layers, pages and heads are needed")
+            at[i], at[i + 3] = sk[j], ss[j]
+    return _PACK_PAGES(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, *n, hs, page, *at), (*n, page, hs)
 
 
 def _table(table):

@@ -53,39 +53,95 @@ __device__ __forceinline__ uint8_t code_of(float q) { // |q| within the type's r
     else return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
 }
 template <int CT>
+__device__ __forceinline__ uint32_t code4(const float (&q)[4]) {
+    if constexpr (CT == LLM_E4M3)
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false), true);
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) w |= (uint32_t)code_of<CT>(q[k]) << (8 * k);
+    return w;
+}
+template <int CT>
+__device__ __forceinline__ void value4(uint32_t w, float (&v)[4]) {
+    if constexpr (CT == LLM_I8) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = (float)(int8_t)(w >> (8 * k));
+    } else {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+        v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
+    }
+}
+template <int CT>
 __device__ __forceinline__ float value_of(uint8_t c) {
     if constexpr (CT == LLM_I8) return (float)(int8_t)c;
     else return __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
 }
 
-// The rows of a block: their largest magnitude decides the scale, then their codes; a workgroup a block and side.
+// Codes of values x / s (both scaled up as div_to_odd needs it; inv a rounded 1 / s): a product with the reciprocal is off by 2^-22
+// of itself at most (1 / s and the product are rounded, 2^-24 each), so it decides unless it falls that close to a border between two
+// codes; then the exact quotient does.  Borders: int8 the halves, 127 2^-22 = 3e-5; e4m3 the middles between two neighbours, the 20
+// bits below its three at 0x80000, and anywhere below its normal values, 2^-6.
+template <int CT>
+__device__ __forceinline__ uint32_t codes_of(float4 x, float s, float inv, float sign) {
+    constexpr float top = CT == LLM_I8 ? 127.0f : 448.0f;
+    float v[4] = {x.x * sign, x.y * sign, x.z * sign, x.w * sign}, q[4];
+    bool near = false;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        q[k] = v[k] * inv;
+        if constexpr (CT == LLM_I8) {
+            near |= fabsf(fabsf(q[k] - rintf(q[k])) - 0.5f) < 1e-4f;
+        } else {
+            near |= ((__float_as_uint(q[k]) + 16u - 0x80000u) & 0xfffffu) < 32u;
+            near |= fabsf(q[k]) < 0x1p-6f && q[k] != 0.0f;
+        }
+    }
+    if (__any(near))
+#pragma unroll
+        for (int k = 0; k < 4; k++) q[k] = div_to_odd(v[k], s);
+#pragma unroll
+    for (int k = 0; k < 4; k++) q[k] = fminf(fmaxf(q[k], -top), top);
+    return code4<CT>(q);
+}
+
+constexpr int WRITE_T = 512; // threads of a block's workgroup: few rows a thread, whose latencies count
+constexpr int TURN = 68; // bytes from row to row of a turned block in LDS: rows of a wave's stores fall into 16 banks
+
+// The rows of a block: their largest magnitude decides the scale, then their codes; a workgroup a block and side.  The rows are
+// read once, all loads at once, and wait in registers; V's codes are turned in LDS.
 template <int CT, int RT>
-__global__ void __launch_bounds__(256) k_page_write(RowArgs a) {
-    constexpr int RS = RT == LLM_F32 ? 4 : 2;
-    __shared__ uint32_t sm_max[4];
+__global__ void __launch_bounds__(WRITE_T) k_page_write(RowArgs a) {
+    constexpr int RS = RT == LLM_F32 ? 4 : 2, ITEMS = 64 * 256 / 4 / WRITE_T; // of four values a thread
+    __shared__ uint32_t sm_max[WRITE_T / 64];
+    __shared__ __align__(4) uint8_t sm_v[256 * TURN];
     Unit u;
     if (!find_unit(a, blockIdx.x, u) || u.page < 0 || (a.refs && a.refs[u.page] != 1)) return;
     const int side = blockIdx.y, per_row = a.hs / 4, items = (u.hi - u.lo) * per_row;
     uint8_t *const dst = a.c[side] + u.page * a.id + u.h * a.head + u.blk * (PAGE_BLOCK * a.hs);
     float *const scale = a.s[side] + u.page * a.s_id + u.h * a.s_head + u.blk;
     const uint8_t *const src = a.r[side] + u.b * a.r_seq[side] + u.h * a.r_head[side];
-    auto load = [&](int item) {
-        const int o = u.lo + item / per_row, d = item % per_row * 4;
-        int64_t t = u.first + o;
-        if (a.path) t = a.path[(int64_t)u.b * a.max_n + t];
-        return (uint64_t)t < (uint64_t)a.max_n ? row4<RT>(src + t * a.r_tok[side] + (size_t)d * RS)
-                                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    };
-    uint32_t m = 0;
-    for (int i = threadIdx.x; i < items; i += 256) {
-        const float4 x = load(i);
-        for (float v : {x.x, x.y, x.z, x.w}) m = max(m, __float_as_uint(v) & 0x7fffffffu);
-    }
-    for (int off = 1; off < 64; off <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off));
-    if ((threadIdx.x & 63) == 0) sm_max[threadIdx.x / 64] = m;
     const float old = u.lo ? *scale : 0.0f;
+    float4 x[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const int i = threadIdx.x + WRITE_T * k;
+        x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i < items) {
+            int64_t t = u.first + u.lo + i / per_row;
+            if (a.path) t = a.path[(int64_t)u.b * a.max_n + t];
+            if ((uint64_t)t < (uint64_t)a.max_n) x[k] = row4<RT>(src + t * a.r_tok[side] + (size_t)(i % per_row) * 4 * RS);
+        }
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++)
+        for (float v : {x[k].x, x[k].y, x[k].z, x[k].w}) m = max(m, __float_as_uint(v) & 0x7fffffffu);
+    m = umax16(m);
+    for (int off = 16; off < 64; off <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off));
+    if ((threadIdx.x & 63) == 0) sm_max[threadIdx.x / 64] = m;
     __syncthreads();
-    m = max(max(sm_max[0], sm_max[1]), max(sm_max[2], sm_max[3]));
+#pragma unroll
+    for (int i = 0; i < WRITE_T / 64; i++) m = max(m, sm_max[i]);
     const float top = CT == LLM_I8 ? 127.0f : 448.0f, want = __uint_as_float(m) / top;
     const bool bad = m >= 0x7f800000u || !(fabsf(old) < INFINITY);
     float s = fabsf(old), back = 1.0f; // the new scale's magnitude, and what takes the codes before lo to it
@@ -93,60 +149,88 @@ __global__ void __launch_bounds__(256) k_page_write(RowArgs a) {
     else if (!bad)
         while (s < want) s *= 2.0f, back *= 0.5f;
     if (u.lo && !bad && back != 1.0f)
-        for (int i = threadIdx.x; i < u.lo * a.hs; i += 256) {
+        for (int i = threadIdx.x; i < u.lo * a.hs; i += WRITE_T) {
             uint8_t *c = side ? dst + i / u.lo * PAGE_BLOCK + i % u.lo : dst + i;
             *c = back == 0.0f ? 0 : code_of<CT>(value_of<CT>(*c) * back);
         }
     const bool zero = bad || s == 0.0f;
-    const float up = s < 0x1p-60f ? 0x1p80f : 1.0f, su = s * up, sign = old < 0.0f ? -up : up;
-    for (int i = threadIdx.x; i < items; i += 256) {
-        const int o = u.lo + i / per_row, d = i % per_row * 4;
-        const float4 x = load(i);
-        float q[4] = {x.x, x.y, x.z, x.w};
-        uint32_t w = 0;
+    // (rows of tiny values: scaled by 2^80, their remainders would underflow; no code but 0 of a block without a scale)
+    const float up = s < 0x1p-60f ? 0x1p80f : 1.0f, su = zero ? 1.0f : s * up, sign = old < 0.0f ? -up : up, inv = 1.0f / su;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float v = zero ? 0.0f : fminf(fmaxf(div_to_odd(q[k] * sign, su), -top), top);
-            w |= (uint32_t)code_of<CT>(v) << (8 * k);
-        }
+    for (int k = 0; k < ITEMS; k++) {
+        if (WRITE_T * k >= items) break;
+        const int i = threadIdx.x + WRITE_T * k;
+        if (i >= items) continue;
+        const int o = u.lo + i / per_row, d = i % per_row * 4;
+        uint32_t w = 0;
+        if (!zero) w = codes_of<CT>(x[k], su, inv, sign); // (0 * infinity)
         if (side == 0) *(uint32_t *)(dst + o * a.hs + d) = w;
         else
 #pragma unroll
-            for (int k = 0; k < 4; k++) dst[(d + k) * PAGE_BLOCK + o] = (uint8_t)(w >> (8 * k));
+            for (int e = 0; e < 4; e++) sm_v[(d + e) * TURN + o] = (uint8_t)(w >> (8 * e));
     }
     if (threadIdx.x == 0) *scale = bad ? __uint_as_float(0x7fc00000u) : old < 0.0f ? -s : s;
+    if (side == 0) return;
+    __syncthreads();
+    // 16 positions of a dimension a thread: whole, or those of the call
+    for (int i = threadIdx.x; i < a.hs * 4; i += WRITE_T) {
+        const int d = i / 4, o = i % 4 * 16, lo = max(u.lo, o), hi = min(u.hi, o + 16);
+        const uint8_t *from = sm_v + d * TURN;
+        uint8_t *to = dst + d * PAGE_BLOCK;
+        if (hi - lo == 16) {
+            const uint32_t *w = (const uint32_t *)(from + o);
+            *(uint4 *)(to + o) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            for (int k = lo; k < hi; k++) to[k] = from[k];
+        }
+    }
 }
 
-// The same the other way.  blocks: of max_n tokens from the first one's block on; what lies behind a sequence's rows is zeroed by
-// the workgroups that its blocks would have.
+// The same the other way: a workgroup a block of the cache and side, its rows out of the block's codes.
 template <int CT, int RT>
 __global__ void __launch_bounds__(256) k_page_read(RowArgs a) {
     constexpr int RS = RT == LLM_F32 ? 4 : 2;
-    const uint32_t per_row = a.hs / 4;
-    const int side = blockIdx.y;
-    const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int d = (int)(item % per_row) * 4;
-    const int64_t row = item / per_row;
-    const int h = (int)(row % a.n_kv);
-    const int64_t bt = row / a.n_kv;
-    const int t = (int)(bt % a.max_n);
-    const int64_t b = bt / a.max_n;
-    if (b >= a.blocks) return; // (of a read: the sequences)
-    uint8_t *dst = a.r[side] + b * a.r_seq[side] + t * a.r_tok[side] + h * a.r_head[side] + (size_t)d * RS;
-    const int64_t p = (int64_t)a.pos[b] + t;
+    __shared__ __align__(4) uint8_t sm_v[PAGE_BLOCK * 260]; // V's codes by position
+    const int side = blockIdx.y, h = blockIdx.x % a.n_kv, x = blockIdx.x / a.n_kv, b = x / a.blocks;
+    const int64_t p0 = a.pos[b], at = ((p0 >> 6) + x % a.blocks) * PAGE_BLOCK; // (rounded down, below 0 too)
+    const int lo = (int)max((int64_t)0, p0 - at), hi = (int)min((int64_t)PAGE_BLOCK, p0 + a.max_n - at); // offsets that rows are for
+    if (lo >= hi) return;
+    const int nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n;
     int page = -1;
-    if ((!a.n || t < a.n[b]) && p >= 0 && p < (int64_t)a.per * a.page) page = a.table[b * a.per + p / a.page];
-    if ((uint32_t)page >= (uint32_t)a.n_pages) {
-        if (a.zero_rest) put4<RT>(dst, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-        return;
-    }
-    const int blk = (int)(p % a.page / PAGE_BLOCK), o = (int)(p % PAGE_BLOCK);
-    const uint8_t *src = a.c[side] + page * a.id + h * a.head + blk * (PAGE_BLOCK * a.hs);
+    if (at >= 0 && at < (int64_t)a.per * a.page) page = a.table[(int64_t)b * a.per + at / a.page];
+    const int have = (uint32_t)page < (uint32_t)a.n_pages ? (int)min((int64_t)hi, p0 + nn - at) : lo; // offsets up to which there are
+    uint8_t *const dst = a.r[side] + b * a.r_seq[side] + (at - p0) * a.r_tok[side] + h * a.r_head[side];
+    const int per_row = a.hs / 4;
+    if (a.zero_rest)
+        for (int i = threadIdx.x; i < (hi - max(lo, have)) * per_row; i += 256)
+            put4<RT>(dst + (max(lo, have) + i / per_row) * a.r_tok[side] + (size_t)(i % per_row) * 4 * RS, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+    if (lo >= have) return;
+    const int blk = (int)(at & (a.page - 1)) / PAGE_BLOCK;
+    const uint8_t *const src = a.c[side] + page * a.id + h * a.head + blk * (PAGE_BLOCK * a.hs);
     const float s = a.s[side][page * a.s_id + h * a.s_head + blk];
-    float v[4];
+    if (side) {
+        uint4 w[4]; // 16 positions of a dimension each
 #pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = value_of<CT>(side ? src[(d + k) * PAGE_BLOCK + o] : src[o * a.hs + d + k]) * s;
-    put4<RT>(dst, make_float4(v[0], v[1], v[2], v[3]));
+        for (int k = 0; k < 4; k++)
+            if ((int)threadIdx.x + 256 * k < a.hs * 4) w[k] = *(const uint4 *)(src + (threadIdx.x + 256 * k) * 16);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = threadIdx.x + 256 * k, d = i / 4, o = i % 4 * 16;
+            if (i >= a.hs * 4) break;
+            const uint32_t q[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+            for (int e = 0; e < 16; e++) sm_v[(o + e) * (a.hs + 4) + d] = (uint8_t)(q[e / 4] >> (8 * (e % 4)));
+        }
+        __syncthreads();
+    }
+#pragma unroll 4
+    for (int i = threadIdx.x; i < (have - lo) * per_row; i += 256) {
+        const int o = lo + i / per_row, d = i % per_row * 4;
+        const uint32_t w = side ? *(const uint32_t *)(sm_v + o * (a.hs + 4) + d) : *(const uint32_t *)(src + o * a.hs + d);
+        float v[4];
+        value4<CT>(w, v);
+        put4<RT>(dst + o * a.r_tok[side] + (size_t)d * RS, make_float4(v[0] * s, v[1] * s, v[2] * s, v[3] * s));
+    }
 }
 
 int page_rows(const char *who, bool write, const llm_pages *c, const llm_rows *k, const llm_rows *v, int n_seq, const int *table,
@@ -163,7 +247,7 @@ int page_rows(const char *who, bool write, const llm_pages *c, const llm_rows *k
             if (!op_check_apart(who, "the rows", 3, count, stride)) return -1;
         }
     const int blocks = blocks_of(max_n);
-    if ((int64_t)n_seq * (write ? blocks : max_n) * c->n_kv * (write ? 1 : c->hs / 4) > 0x7fffffffll) {
+    if ((int64_t)n_seq * blocks * c->n_kv > 0x7fffffffll) {
         fprintf(stderr, "%s: %d sequences of %d rows\n", who, n_seq, max_n);
         return -1;
     }
@@ -190,15 +274,14 @@ int page_rows(const char *who, bool write, const llm_pages *c, const llm_rows *k
     a.id = c->id, a.head = c->head, a.s_id = c->s_id, a.s_head = c->s_head;
     a.table = table, a.refs = refs, a.pos = pos, a.n = n, a.path = path;
     a.per = per, a.n_pages = c->n_pages, a.n_kv = c->n_kv, a.hs = c->hs, a.page = c->page, a.max_n = max_n;
-    a.blocks = write ? blocks : n_seq, a.zero_rest = zero_rest;
-    const unsigned grid = write ? (unsigned)(n_seq * blocks * c->n_kv)
-                                : (unsigned)(((int64_t)n_seq * max_n * c->n_kv * (c->hs / 4) + 255) / 256);
+    a.blocks = blocks, a.zero_rest = zero_rest;
+    const unsigned grid = (unsigned)(n_seq * blocks * c->n_kv);
     void (*kern)(RowArgs) = nullptr;
 #define PAGE_PICK(C, R)                                                                   \
     if (c->type == C && k->type == R) kern = write ? k_page_write<C, R> : k_page_read<C, R>;
     PAGE_PICK(LLM_I8, LLM_F32) PAGE_PICK(LLM_I8, LLM_BF16) PAGE_PICK(LLM_E4M3, LLM_F32) PAGE_PICK(LLM_E4M3, LLM_BF16)
 #undef PAGE_PICK
-    hipLaunchKernelGGL(kern, dim3(grid, 2), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kern, dim3(grid, 2), dim3(write ? WRITE_T : 256), 0, (hipStream_t)stream, a);
     HIP_OR_FAIL(who, hipGetLastError());
     return 0;
 }
@@ -275,13 +358,31 @@ struct ReserveArgs {
     int4 *copies;                    // of each sequence: from, to, blocks
 };
 
-// The pages that each sequence needs, in the order of sequences and positions, one workgroup.
+constexpr int BOOK_PAGES = 8; // neighbouring pages that a thread of the books looks at
+// Bits of the thread's pages from `first` on that are free (used: the others).
+__device__ __forceinline__ uint32_t free_pages(const int *refs, int n_pages, int first, bool used) {
+    typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+    uint32_t bits = 0;
+    if (first + BOOK_PAGES <= n_pages) {
+        const i32x4 a = *(const i32x4 *)(refs + first), b = *(const i32x4 *)(refs + first + 4);
+#pragma unroll
+        for (int k = 0; k < 4; k++) bits |= (uint32_t)((a[k] > 0) == used) << k | (uint32_t)((b[k] > 0) == used) << (k + 4);
+    } else {
+        for (int k = 0; first + k < n_pages; k++) bits |= (uint32_t)((refs[first + k] > 0) == used) << k;
+    }
+    return bits;
+}
+
+// The pages that each sequence needs, in the order of sequences and positions, one workgroup.  It is bound by the latency of
+// loads that depend on each other: what the free pages are is asked for first, an entry's own loads are kept for the end, and the
+// claims to shared pages are compared only where there are some.
 __global__ void __launch_bounds__(BOOK_T) k_reserve(ReserveArgs a) {
-    __shared__ int sm[BOOK_T / 64], misfit;
+    __shared__ int sm[BOOK_T / 64], misfit, any_shared;
+    __shared__ int2 claim[BOOK_T];
     const int items = a.n_seq * a.most;
     struct Item {
-        int b, e, len;
-        int64_t at; // of the table
+        int b, e, len, refs;
+        int64_t at;       // of the table
         bool fits, asked; // the sequence's tokens; a page that they are written to
     };
     auto item = [&](int i) {
@@ -294,73 +395,90 @@ __global__ void __launch_bounds__(BOOK_T) k_reserve(ReserveArgs a) {
         t.at = (int64_t)t.b * a.per + j;
         t.e = t.asked ? a.table[t.at] : -1;
         if ((uint32_t)t.e >= (uint32_t)a.n_pages) t.e = -1;
+        t.refs = t.e >= 0 ? a.refs[t.e] : 0;
         return t;
     };
-    if (threadIdx.x == 0) misfit = 0;
-    for (int i = threadIdx.x; i < items; i += BOOK_T) {
-        const Item t = item(i);
-        if (t.e >= 0 && a.refs[t.e] > 1) a.claims[t.e] = 0, a.last[t.e] = -1;
-    }
-    __threadfence();
+    if (threadIdx.x == 0) misfit = any_shared = 0;
+    uint32_t free = free_pages(a.refs, a.n_pages, BOOK_PAGES * (int)threadIdx.x, false);
     __syncthreads();
+    Item mine; // of entry threadIdx.x
+    int plan0 = 0, want = 0; // plan: 1 a page, 2 one in place of a shared one, 3 shared, not decided yet
+    mine.e = -1, mine.len = 0, mine.at = 0, mine.b = 0;
     for (int i = threadIdx.x; i < items; i += BOOK_T) {
         const Item t = item(i);
-        if (t.e >= 0 && a.refs[t.e] > 1) {
-            atomicAdd(&a.claims[t.e], 1);
-            atomicMax(&a.last[t.e], t.b);
-        }
+        const int plan = !t.asked ? 0 : t.refs <= 0 ? 1 : t.refs > 1 ? 3 : 0;
         if (!t.fits) misfit = 1;
+        if (plan == 3) any_shared = 1;
+        if (i < BOOK_T) mine = t, plan0 = plan;
+        else a.plan[i] = plan;
+        want += plan == 1;
     }
-    __threadfence();
     __syncthreads();
-    int want = 0;
-    for (int i = threadIdx.x; i < items; i += BOOK_T) {
-        const Item t = item(i);
-        int plan = 0; // 1 a page, 2 one in place of a shared one
-        if (t.asked) {
-            const int r = t.e >= 0 ? a.refs[t.e] : 0;
-            if (r <= 0) plan = 1;
-            else if (r > 1) {
+    if (any_shared && items <= BOOK_T) { // few: compared with each other in LDS
+        int all;
+        const int at = block_scan(plan0 == 3, sm, all) - 1;
+        if (plan0 == 3) claim[at] = make_int2(mine.e, mine.b);
+        __syncthreads();
+        if (plan0 == 3) {
+            int claims = 0;
+            bool later = false;
+            for (int k = 0; k < all; k++) {
+                const int2 c = claim[k];
+                claims += c.x == mine.e;
+                later |= c.x == mine.e && c.y > mine.b;
+            }
+            plan0 = claims != mine.refs || later ? 2 : 0; // (all who have it want it: the last one keeps it)
+            want += plan0 == 2;
+        }
+    } else if (any_shared) {
+        for (int i = threadIdx.x; i < items; i += BOOK_T)
+            if ((i < BOOK_T ? plan0 : a.plan[i]) == 3) {
+                const Item t = i < BOOK_T ? mine : item(i);
+                a.claims[t.e] = 0, a.last[t.e] = -1;
+            }
+        __threadfence();
+        __syncthreads();
+        for (int i = threadIdx.x; i < items; i += BOOK_T)
+            if ((i < BOOK_T ? plan0 : a.plan[i]) == 3) {
+                const Item t = i < BOOK_T ? mine : item(i);
+                atomicAdd(&a.claims[t.e], 1);
+                atomicMax(&a.last[t.e], t.b);
+            }
+        __threadfence();
+        __syncthreads();
+        for (int i = threadIdx.x; i < items; i += BOOK_T)
+            if ((i < BOOK_T ? plan0 : a.plan[i]) == 3) {
+                const Item t = i < BOOK_T ? mine : item(i);
                 const int claims = __hip_atomic_load(&a.claims[t.e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 const int last = __hip_atomic_load(&a.last[t.e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (claims != r || last != t.b) plan = 2;
+                const int plan = claims != t.refs || last != t.b ? 2 : 0;
+                if (i < BOOK_T) plan0 = plan;
+                else a.plan[i] = plan;
+                want += plan == 2;
             }
-        }
-        a.plan[i] = plan;
-        want += plan != 0;
     }
     int total, found = 0;
     block_scan(want, sm, total);
-    for (int base = 0; base < a.n_pages && found < total; base += 8 * BOOK_T) { // eight pages a thread
-        const int first = base + 8 * (int)threadIdx.x;
-        uint32_t free = 0;
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (first + k < a.n_pages && a.refs[first + k] <= 0) free |= 1u << k;
-        int all;
-        int at = found + block_scan(__popc(free), sm, all) - __popc(free);
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            if ((free >> k) & 1) {
-                if (at < total) a.ids[at] = first + k;
-                at++;
-            }
+    for (int base = 0; base < a.n_pages && found < total; base += BOOK_PAGES * BOOK_T) {
+        const int first = base + BOOK_PAGES * (int)threadIdx.x;
+        if (base) free = free_pages(a.refs, a.n_pages, first, false);
+        int all, at = found + block_scan(__popc(free), sm, all) - __popc(free);
+        for (uint32_t f = free; f && at < total; f &= f - 1) a.ids[at++] = first + __ffs(f) - 1;
         found += all;
     }
     const bool ok = found >= total && !misfit;
     if (threadIdx.x == 0) a.result[0] = ok, a.result[1] = total;
     for (int b = threadIdx.x; b < a.n_seq; b += BOOK_T) a.copies[b] = make_int4(-1, 0, 0, 0);
-    __threadfence();
+    if (!ok || !total) return;
     __syncthreads();
-    if (!ok) return;
     int before = 0;
     for (int base = 0; base < items; base += BOOK_T) {
-        const int i = base + threadIdx.x, plan = i < items ? a.plan[i] : 0;
+        const int i = base + threadIdx.x, plan = i >= items ? 0 : base ? a.plan[i] : plan0;
         int all;
         const int rank = before + block_scan(plan != 0, sm, all) - 1;
         before += all;
         if (!plan) continue;
-        const Item t = item(i);
+        const Item t = base ? item(i) : mine;
         const int page = a.ids[rank];
         a.table[t.at] = page;
         a.refs[page] = 1;
@@ -378,19 +496,31 @@ struct MoveArgs {
     int64_t layer, id, head, s_layer, s_id, s_head;
     int hs, n_kv, n_layers;
 };
-// `blocks` blocks of page `from` to page `to`, of one layer, head and side, by a workgroup.
-__device__ __forceinline__ void move_blocks(const MoveArgs &a, int layer, int h, int side, int from, int to, int blocks) {
+// `blocks` blocks of page `from` to page `to`, of one layer, head and side, by a wave: eight loads of 16 bytes a lane under way.
+__device__ __forceinline__ void move_blocks(const MoveArgs &a, uint32_t unit, int from, int to, int blocks) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63, side = unit & 1, h = unit / 2 % a.n_kv, layer = unit / 2 / a.n_kv;
     const int64_t at = layer * a.layer + h * a.head, s_at = layer * a.s_layer + h * a.s_head;
-    const uint4 *src = (const uint4 *)(a.c[side] + at + from * a.id);
-    uint4 *dst = (uint4 *)(a.c[side] + at + to * a.id);
-    for (int i = threadIdx.x; i < blocks * PAGE_BLOCK / 16 * a.hs; i += 256) dst[i] = src[i];
-    if ((int)threadIdx.x < blocks) a.s[side][s_at + to * a.s_id + threadIdx.x] = a.s[side][s_at + from * a.s_id + threadIdx.x];
+    const u32x4 *src = (const u32x4 *)(a.c[side] + at + from * a.id);
+    u32x4 *dst = (u32x4 *)(a.c[side] + at + to * a.id);
+    const int count = blocks * (PAGE_BLOCK / 16) * a.hs;
+    float s = 0.0f;
+    if (lane < blocks) s = a.s[side][s_at + from * a.s_id + lane];
+    for (int i = lane; i < count; i += 64 * 8) {
+        u32x4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (i + 64 * k < count) v[k] = src[i + 64 * k];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (i + 64 * k < count) dst[i + 64 * k] = v[k];
+    }
+    if (lane < blocks) a.s[side][s_at + to * a.s_id + lane] = s;
 }
-__global__ void __launch_bounds__(256) k_reserve_copy(MoveArgs a, const int4 *copies) {
+__global__ void __launch_bounds__(256) k_reserve_copy(MoveArgs a, const int4 *copies, uint32_t units) {
     const int4 c = copies[blockIdx.y];
-    if (c.x < 0) return;
-    const uint32_t u = blockIdx.x, side = u & 1, h = u / 2 % a.n_kv, layer = u / 2 / a.n_kv;
-    move_blocks(a, layer, h, side, c.x, c.y, c.z);
+    const uint32_t u = blockIdx.x * 4 + threadIdx.x / 64;
+    if (c.x >= 0 && u < units) move_blocks(a, u, c.x, c.y, c.z);
 }
 
 struct CompactArgs {
@@ -398,25 +528,33 @@ struct CompactArgs {
     int *table, *refs, *result;
     int *map, *hole, *far; // work: where pages from the u-th on went; the free numbers below, the used ones above
 };
+// Holes and what goes there, in order, by one workgroup.
 __global__ void __launch_bounds__(BOOK_T) k_compact(CompactArgs a) {
     __shared__ int sm[BOOK_T / 64];
-    int mine = 0, u, holes = 0, fars = 0;
-    for (int i = threadIdx.x; i < a.n_pages; i += BOOK_T) mine += a.refs[i] > 0;
-    block_scan(mine, sm, u);
-    for (int base = 0; base < a.n_pages; base += BOOK_T) {
-        const int i = base + threadIdx.x;
-        const bool used = i < a.n_pages && a.refs[i] > 0, hole = i < u && !used, far = i >= u && used;
-        int all;
-        const int rh = block_scan(hole, sm, all) - 1 + holes;
-        holes += all;
-        const int rf = block_scan(far, sm, all) - 1 + fars;
-        fars += all;
-        if (hole) a.hole[rh] = i;
-        if (far) a.far[rf] = i;
-        if (i >= u && i < a.n_pages) a.map[i] = far ? rf : -1;
+    constexpr int STEP = BOOK_PAGES * BOOK_T;
+    const int mine = BOOK_PAGES * (int)threadIdx.x;
+    const uint32_t first = free_pages(a.refs, a.n_pages, mine, true); // (of most pools these are all)
+    int sum = __popc(first), u, holes = 0, fars = 0;
+    for (int base = STEP; base < a.n_pages; base += STEP) sum += __popc(free_pages(a.refs, a.n_pages, base + mine, true));
+    block_scan(sum, sm, u);
+    for (int base = 0; base < a.n_pages; base += STEP) {
+        const int at = base + mine, have = min(max(a.n_pages - at, 0), BOOK_PAGES), below = min(max(u - at, 0), have);
+        const uint32_t used = base ? free_pages(a.refs, a.n_pages, at, true) : first;
+        const uint32_t low = (1u << below) - 1, there = (1u << have) - 1;
+        const uint32_t hole = ~used & low, far = used & there & ~low;
+        int all; // (both counts in one sum: a pass has no more than 8192 of either)
+        const int upto = block_scan(__popc(hole) | __popc(far) << 16, sm, all);
+        int h = holes + (upto & 0xffff) - __popc(hole), f = fars + (upto >> 16) - __popc(far);
+        holes += all & 0xffff;
+        fars += all >> 16;
+        for (uint32_t x = hole; x; x &= x - 1) a.hole[h++] = at + __ffs(x) - 1;
+        for (int k = below; k < have; k++) {
+            const bool moves = far >> k & 1;
+            a.map[at + k] = moves ? f : -1;
+            if (moves) a.far[f++] = at + k;
+        }
     }
     if (threadIdx.x == 0) a.result[0] = u, a.result[1] = fars;
-    __threadfence();
     __syncthreads();
     for (int k = threadIdx.x; k < fars; k += BOOK_T) {
         const int to = a.hole[k], from = a.far[k];
@@ -437,9 +575,9 @@ __global__ void __launch_bounds__(256) k_compact_move(MoveArgs a, CompactArgs t,
         return;
     }
     const int64_t per = (int64_t)2 * a.n_kv * a.n_layers;
-    for (int64_t i = blockIdx.x; i < moves * per; i += movers) {
-        const int k = (int)(i / per), x = (int)(i - k * per);
-        move_blocks(a, x / 2 / a.n_kv, x / 2 % a.n_kv, x & 1, t.far[k], t.hole[k], blocks);
+    for (int64_t i = blockIdx.x * 4 + threadIdx.x / 64; i < moves * per; i += 4 * movers) {
+        const int k = (int)(i / per);
+        move_blocks(a, (uint32_t)(i - k * per), t.far[k], t.hole[k], blocks);
     }
 }
 
@@ -580,8 +718,8 @@ extern "C" int llm_page_reserve(const llm_pages *c, int n_seq, int *table, int p
     hipLaunchKernelGGL(k_reserve, dim3(1), dim3(BOOK_T), 0, (hipStream_t)stream, a);
     HIP_OR_FAIL(who, hipGetLastError());
     if (!any) return 0;
-    hipLaunchKernelGGL(k_reserve_copy, dim3((unsigned)units, n_seq), dim3(256), 0, (hipStream_t)stream, move_args(c),
-                       (const int4 *)a.copies);
+    hipLaunchKernelGGL(k_reserve_copy, dim3((unsigned)((units + 3) / 4), n_seq), dim3(256), 0, (hipStream_t)stream, move_args(c),
+                       (const int4 *)a.copies, (uint32_t)units);
     HIP_OR_FAIL(who, hipGetLastError());
     return 0;
 }
