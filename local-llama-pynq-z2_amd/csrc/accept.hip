@@ -1,15 +1,21 @@
 // llm_draft_accept: drafted tokens kept or turned down against the target's probabilities.
 //
-// Three launches.  k_accept_rows reads every row of logits once: a workgroup takes a segment of a row into registers, finds its
-// largest value and the sum of e^((x - largest) / T).  k_accept_walk joins them, walks the tree and sums the weights of the last node's
-// row, a workgroup a segment: every workgroup of a sequence walks by itself, which needs no wait between them.  k_accept_draw
+// k_accept_rows reads every row of logits once: a workgroup takes a segment of a row into registers, finds its largest value and
+// the sum of e^((x - largest) / T).  k_accept_walk joins them, walks the tree and sums the weights of the last node's row, a
+// workgroup a segment: every workgroup of a sequence walks by itself, which needs no wait between them, and the last one to be done
 // finds the segment and the token that the drawn point falls into.
 //
 // What is left of p after a child was turned down: max(0, w / z - q) in proportion, w = max(0, p - a q), z the sum of w.  That is
 // max(0, p - (a + z) q) / z: one number, a, says all that the tokens turned down have changed.
 //
-// Sums and exponentials are in 64 bits: a token drawn in the tail of 150k stands between borders 1e-6 apart, which an error of
-// 2^-24 in the likeliest token's weight would all move by 6e-8.
+// Sums and exponentials that decide are in 64 bits: a token drawn in the tail of 150k stands between borders 1e-6 apart, which an
+// error of 2^-24 in the likeliest token's weight would all move by 6e-8.
+//
+// What bounds it: the rows' bytes, read once.  16 trees of 37 rows of 152064 bf16 logits, 180 MB: 26.5 us, 6.8 TB/s, for the rows (the
+// last call left a part of them in the caches) and 24.5 for the walk; a chain of 8 fp32 rows with draft probabilities: 4.3 and 16.8.
+// The walk is a chain of short steps: the parts' loads, the join, the tokens' probabilities, a segment's sum, the count, the sums of
+// the others, the drawn segment's sum again.  What is not spread is the row's pass where a child with a later sibling is turned down
+// against draft probabilities: each workgroup takes it by itself, 25 us a time, so that none waits for another.
 #include <string.h>
 
 #include <algorithm>
@@ -20,32 +26,32 @@
 namespace {
 
 constexpr int AC_T = 256, AC_E = 16, AC_SEG = AC_T * AC_E; // values of a segment
-constexpr int AC_N = 64;                                   // most nodes
+constexpr int AC_N = 64;                                   // most nodes: a lane each
 
-struct AcPart { // of a segment: largest value, its first place (temperature 0), sum relative to it
+struct AcPart { // of a part of a row: largest value, its first place (temperature 0), sum relative to it
     float m;
     int best;
     double s;
 };
-struct AcEnd { // of a sequence: the last node, its row's statistics, what is left of it
+struct AcEnd { // a sequence's last node, its row's statistics, what is left of it
     int node, turned;
     float m;
     int best;
-    double s, a;
+    double s, inv, a; // inv: 1 / s
     int out[AC_N]; // tokens turned down (no draft probabilities)
 };
 struct AcArgs {
     const uint8_t *x, *q;
     int64_t seq, row, p_seq, p_row; // bytes
-    int max_n, vocab, segs;
-    double inv_t; // 0: temperature 0
+    int max_n, vocab, segs, parts; // parts: workgroups of a row in k_accept_rows
+    double c; // log2(e) / T; 0: temperature 0
     const int *tokens, *parents, *n;
     const float *coins;
     int *kept, *path, *next;
     float *logp;
-    AcPart *part; // [seq][row][segment]
-    AcEnd *end;   // [seq]
+    AcPart *part; // [seq][row][part]
     double *sums; // [seq][segment]
+    int *done;    // [seq]: segments that are summed
 };
 
 template <int TY>
@@ -53,32 +59,101 @@ __device__ __forceinline__ float at(const uint8_t *row, int i) {
     if constexpr (TY == LLM_F32) return ((const float *)row)[i];
     return __uint_as_float((uint32_t)((const uint16_t *)row)[i] << 16);
 }
+// Neighbouring values from i on (16 bytes; a row starts anywhere), `none` behind the row's end.
+template <int TY>
+constexpr int AC_V = TY == LLM_F32 ? 4 : 8;
+template <int TY, bool ALL = false> // ALL: they are in the row, all of the wave's
+__device__ __forceinline__ void values(const uint8_t *row, int i, int vocab, float none, float *x) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+    constexpr int V = AC_V<TY>;
+    if (ALL || i + V <= vocab) {
+        const u32x4 u = *(const u32x4 *)(row + (size_t)i * (TY == LLM_F32 ? 4 : 2));
+#pragma unroll
+        for (int k = 0; k < V; k++)
+            x[k] = TY == LLM_F32 ? __uint_as_float(u[k % 4]) : __uint_as_float(k % 2 ? u[k / 2] & 0xffff0000u : u[k / 2] << 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; k++) x[k] = i + k < vocab ? at<TY>(row, i + k) : none;
+    }
+}
 __device__ __forceinline__ int nodes(const AcArgs &a, int b) { return a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n; }
 
-__device__ __forceinline__ double wave_add(double v) { // in a fixed order
-    for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
-    return v;
+// 2^y for y <= 0 (below -1020, and NaN: 2^-1020): y = n + f, f in [-1/2, 1/2], and 2^f = e^(f ln 2) by its series up to the tenth
+// power, whose next term is below (ln 2 / 2)^11 / 11! = 2.2e-13.  Adding 1.5 2^52 rounds to whole numbers and leaves n in the sum's
+// low bits, from where it goes into the exponent: no instruction of less than full rate.
+__device__ __forceinline__ double exp2_of(double y) {
+    constexpr double WHOLE = 6755399441055744.0, L = 0.693147180559945309417232121458;
+    y = fmax(y, -1020.0);
+    const double t = y + WHOLE, f = y - (t - WHOLE);
+    constexpr double L2 = L * L, L4 = L2 * L2, L8 = L4 * L4;
+    constexpr double k[] = {L8 * L / 362880.0, L8 / 40320.0, L4 * L2 * L / 5040.0, L4 * L2 / 720.0, L4 * L / 120.0, L4 / 24.0,
+                            L2 * L / 6.0, L2 / 2.0, L, 1.0};
+    double p = L8 * L2 / 3628800.0;
+#pragma unroll
+    for (double c : k) p = fma(p, f, c);
+    const uint64_t u = __builtin_bit_cast(uint64_t, p);
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
+    return __builtin_bit_cast(double, (uint64_t)((uint32_t)(u >> 32) + (n << 20)) << 32 | (uint32_t)u);
 }
-// e^(x / T) relative to the largest value m of a row; temperature 0: 1 at `best`
-__device__ __forceinline__ double weight(const AcArgs &a, float x, float m, int i, int best) {
-    if (a.inv_t == 0.0) return i == best ? 1.0 : 0.0;
-    return exp(((double)x - (double)m) * a.inv_t);
+// e^(x / T) relative to the largest value m of a row, c = log2(e) / T.  A masked logit's is 0, not nearly 0: by a product, since a
+// branch would keep the series of neighbouring values from being worked on together.
+__device__ __forceinline__ double weight(float x, double m, double c) {
+    const double y = ((double)x - m) * c; // (an exact difference: 1 / T may be large)
+    return exp2_of(y) * (y >= -1020.0 ? 1.0 : 0.0);
+}
+// The same of one value; temperature 0: 1 at `best`.
+__device__ __forceinline__ double weight_of(const AcArgs &a, float x, float m, int i, int best) {
+    return a.c == 0.0 ? i == best ? 1.0 : 0.0 : weight(x, (double)m, a.c);
 }
 
-template <int TY>
+template <int W> // over W neighbouring lanes, in a fixed order
+__device__ __forceinline__ double lanes_add(double v) {
+#pragma unroll
+    for (int off = 1; off < W; off <<= 1) v += __shfl_xor(v, off);
+    return v;
+}
+__device__ __forceinline__ double block_add(double v, double *sm) {
+    v = lanes_add<64>(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x / 64] = v;
+    __syncthreads();
+    return (sm[0] + sm[1]) + (sm[2] + sm[3]);
+}
+__device__ __forceinline__ double upto(double v) { // inclusive sum over a wave
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const double y = __shfl_up(v, off);
+        v += (int)(threadIdx.x & 63) >= off ? y : 0.0;
+    }
+    return v;
+}
+
+// PER segments of a row a workgroup: one where there are few rows, four else (the walk has a quarter to join).
+// EXACT: exponentials in 64 bits, for draft probabilities, which are held against p itself; without them a row's sum only decides
+// about its children and log probabilities, and it takes those of the hardware in 32 bits: off by 2^-18 of itself for rows up to
+// 2^22 (three roundings of the exponent, the instruction's, eight chains of additions); what is drawn from is summed in 64 bits by
+// the walk.  16 trees of 37 bf16 rows: 26.5 us, with the series in 64 bits 70.
+template <int TY, int PER, bool EXACT>
 __global__ void __launch_bounds__(AC_T) k_accept_rows(AcArgs a) {
+    constexpr int V = AC_V<TY>, E = AC_E * PER;
     __shared__ float sm_m[AC_T / 64];
     __shared__ int sm_i[AC_T / 64];
     __shared__ double sm_s[AC_T / 64];
     const int seg = blockIdx.x, r = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    if (seg == 0 && r == 0 && threadIdx.x == 0) a.done[b] = 0;
     if (r >= nodes(a, b)) return;
     const uint8_t *row = a.x + b * a.seq + r * a.row;
-    float x[AC_E], m = -INFINITY;
+    auto index = [&](int e) { return seg * (PER * AC_SEG) + (e / V * AC_T + (int)threadIdx.x) * V + e % V; };
+    float x[E], m = -INFINITY;
     bool nan = false;
+    if ((seg + 1) * (PER * AC_SEG) <= a.vocab)
 #pragma unroll
-    for (int e = 0; e < AC_E; e++) {
-        const int i = seg * AC_SEG + e * AC_T + threadIdx.x;
-        x[e] = i < a.vocab ? at<TY>(row, i) : -INFINITY;
+        for (int e = 0; e < E; e += V) values<TY, true>(row, index(e), a.vocab, -INFINITY, x + e);
+    else
+#pragma unroll
+        for (int e = 0; e < E; e += V) values<TY, false>(row, index(e), a.vocab, -INFINITY, x + e);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
         m = fmaxf(m, x[e]);
         nan |= x[e] != x[e];
     }
@@ -88,76 +163,159 @@ __global__ void __launch_bounds__(AC_T) k_accept_rows(AcArgs a) {
     m = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
     double s = 0.0;
     int best = 0x7fffffff;
-    if (a.inv_t == 0.0) {
+    if (a.c == 0.0) {
 #pragma unroll
-        for (int e = AC_E - 1; e >= 0; e--)
-            if (x[e] == m) best = seg * AC_SEG + e * AC_T + threadIdx.x;
-        s = nan || m == INFINITY ? __builtin_nan("") : 0.0;
-    } else if (m > -INFINITY) {
+        for (int e = 0; e < E; e++)
+            if (x[e] == m) best = min(best, index(e));
+        for (int off = 1; off < 64; off <<= 1) best = min(best, __shfl_xor(best, off));
+    } else if (m > -INFINITY && m < INFINITY) {
+        if constexpr (EXACT) {
 #pragma unroll
-        for (int e = 0; e < AC_E; e++) s += exp(((double)x[e] - (double)m) * a.inv_t);
-    } else if (nan) {
-        s = __builtin_nan("");
+            for (int e = 0; e < E; e++) s += exp2_of(((double)x[e] - (double)m) * a.c);
+        } else {
+            const float c = (float)a.c;
+            float f[8] = {}; // (eight chains: a sum is off by 2^-21 of itself at most)
+#pragma unroll
+            for (int e = 0; e < E; e++) f[e % 8] += __builtin_amdgcn_exp2f((x[e] - m) * c);
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += (double)f[k];
+        }
     }
-    s = wave_add(s);
-    for (int off = 1; off < 64; off <<= 1) best = min(best, __shfl_xor(best, off));
+    if (nan || m == INFINITY) s = __builtin_nan(""); // (the row has no probabilities)
+    s = lanes_add<64>(s);
     if (lane == 0) sm_s[wave] = s, sm_i[wave] = best;
     __syncthreads();
     if (threadIdx.x == 0) {
-        AcPart &p = a.part[((int64_t)b * a.max_n + r) * a.segs + seg];
+        AcPart &p = a.part[((int64_t)b * a.max_n + r) * a.parts + seg];
         p.m = m;
         p.best = min(min(sm_i[0], sm_i[1]), min(sm_i[2], sm_i[3]));
         p.s = (sm_s[0] + sm_s[1]) + (sm_s[2] + sm_s[3]);
     }
 }
 
-// A row's segments joined by a wave: largest value, its first place, the sum (NaN: the row has no probabilities).
-__device__ __forceinline__ void row_stats(const AcArgs &a, int b, int r, float &m, int &best, double &s) {
-    const AcPart *p = a.part + ((int64_t)b * a.max_n + r) * a.segs;
-    const int lane = threadIdx.x & 63;
-    m = -INFINITY;
-    for (int k = lane; k < a.segs; k += 64) m = fmaxf(m, p[k].m);
-    m = wave_max(m);
-    s = 0.0;
-    best = 0x7fffffff;
-    for (int k = lane; k < a.segs; k += 64) {
-        if (a.inv_t == 0.0) {
-            s += p[k].s; // (0 or NaN)
-            if (p[k].m == m) best = min(best, p[k].best);
-        } else if (p[k].m > -INFINITY || p[k].s != p[k].s) {
-            s += p[k].s * exp(((double)p[k].m - (double)m) * a.inv_t);
+// A row's parts joined by 16 neighbouring lanes: largest value, its first place, the sum (NaN: no probabilities).
+struct AcRow {
+    static constexpr int U = 4; // parts of a lane at once
+    AcPart p[U];
+    __device__ __forceinline__ void load(const AcArgs &a, int b, int r, int k0) {
+        const AcPart *from = a.part + ((int64_t)b * a.max_n + r) * a.parts;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = k0 + 16 * u + (threadIdx.x & 15);
+            p[u] = from[min(k, a.parts - 1)];
+            if (k >= a.parts) p[u].m = -INFINITY, p[u].s = 0.0, p[u].best = 0x7fffffff;
         }
     }
-    s = wave_add(s);
-    for (int off = 1; off < 64; off <<= 1) best = min(best, __shfl_xor(best, off));
-    if (a.inv_t == 0.0) s = s == 0.0 && m > -INFINITY ? 1.0 : __builtin_nan("");
-    else if (!(s > 0.0)) s = __builtin_nan("");
+    __device__ __forceinline__ void join(const AcArgs &a, int b, int r, float &m, int &best, double &s) {
+        m = -INFINITY, s = 0.0, best = 0x7fffffff;
+        for (int k0 = 0;;) {
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < U; u++) top = fmaxf(top, p[u].m);
+            top = max16(top);
+            auto scaled = [&](float mk, double sk) { // (0 and NaN stay what they are)
+                return a.c == 0.0 || !(mk > -INFINITY) ? sk : sk * exp2_of(((double)mk - (double)top) * a.c);
+            };
+            s = scaled(m, s);
+            if (top != m) best = 0x7fffffff;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                s += scaled(p[u].m, p[u].s);
+                if (p[u].m == top) best = min(best, p[u].best);
+            }
+            m = top;
+            k0 += 16 * U;
+            if (k0 >= a.parts) break;
+            load(a, b, r, k0);
+        }
+        s = lanes_add<16>(s);
+        if (a.c == 0.0) {
+#pragma unroll
+            for (int off = 1; off < 16; off <<= 1) best = min(best, __shfl_xor(best, off));
+            s = s == 0.0 && m > -INFINITY ? 1.0 : __builtin_nan("");
+        } else if (!(s > 0.0)) {
+            s = __builtin_nan("");
+        }
+    }
+};
+
+// log2(s) for s >= 1: the hardware's, and what it is short of.
+__device__ __forceinline__ double log2_of(double s) {
+    const double l = (double)__builtin_amdgcn_logf((float)s);
+    return l + (s * exp2_of(-l) - 1.0) * 1.44269504088896340736;
 }
 
-// The weights of the thread's AC_E neighbouring values of a segment, in order.
-template <int TY, int PT>
-__device__ __forceinline__ void left_of(const AcArgs &a, const uint8_t *row, const uint8_t *probs, const AcEnd &e, int first,
-                                        double (&w)[AC_E]) {
+// What is left of N neighbouring values from `first` on: x their logits (-infinity behind the row), q the draft's probabilities.
+template <int PT, int N>
+__device__ __forceinline__ void left_of(const AcArgs &a, const AcEnd &e, const float *x, const float *q, int first, double (&w)[N]) {
+    const double m = (double)e.m, inv = e.inv, aq = e.a;
+    if (a.c == 0.0) {
 #pragma unroll
-    for (int k = 0; k < AC_E; k++) {
-        const int i = first + k;
-        w[k] = 0.0;
-        if (i >= a.vocab) continue;
-        w[k] = weight(a, at<TY>(row, i), e.m, i, e.best) / e.s;
-        if (PT >= 0 && e.a != 0.0) w[k] = fmax(w[k] - e.a * (double)at<PT>(probs, i), 0.0);
-        if (PT < 0)
-            for (int t = 0; t < e.turned; t++)
-                if (e.out[t] == i) w[k] = 0.0;
+        for (int k = 0; k < N; k++) w[k] = first + k == e.best ? inv : inv - inv; // (NaN: no probabilities)
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) w[k] = weight(x[k], m, a.c) * inv;
     }
+    if (PT >= 0 && aq != 0.0)
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const double d = w[k] - aq * (double)q[k];
+            w[k] = d < 0.0 ? 0.0 : d; // (NaN stays)
+        }
+    if (PT < 0)
+        for (int t = 0; t < e.turned; t++) {
+            const int at = e.out[t] - first;
+#pragma unroll
+            for (int k = 0; k < N; k++) w[k] = at == k ? 0.0 : w[k];
+        }
+}
+// Its sum over the thread's AC_E neighbouring values of a segment, in order.  All loads go out first; the weights are a loop of four
+// at a time, whose values move up: straight code, and no more of it than is run often enough to have been worth fetching (the walk of
+// sixteen trees over 152064 bf16 logits: 24.5 us; 28.7 with sixteen values in a row and branches for their masks and borders).
+template <int TY, int PT>
+__device__ __forceinline__ double left_sum(const AcArgs &a, const uint8_t *row, const uint8_t *probs, const AcEnd &e, int seg) {
+    constexpr int PQ = PT < 0 ? LLM_F32 : PT;
+    const int first = seg * AC_SEG + threadIdx.x * AC_E;
+    float x[AC_E], q[AC_E];
+#pragma unroll
+    for (int k = 0; k < AC_E; k++) q[k] = 0.0f;
+    if ((seg + 1) * AC_SEG <= a.vocab) {
+#pragma unroll
+        for (int k = 0; k < AC_E; k += AC_V<TY>) values<TY, true>(row, first + k, a.vocab, -INFINITY, x + k);
+        if (PT >= 0)
+#pragma unroll
+            for (int k = 0; k < AC_E; k += AC_V<PQ>) values<PQ, true>(probs, first + k, a.vocab, 0.0f, q + k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < AC_E; k += AC_V<TY>) values<TY, false>(row, first + k, a.vocab, -INFINITY, x + k);
+        if (PT >= 0)
+#pragma unroll
+            for (int k = 0; k < AC_E; k += AC_V<PQ>) values<PQ, false>(probs, first + k, a.vocab, 0.0f, q + k);
+    }
+    double s = 0.0;
+#pragma unroll 1
+    for (int k = 0; k < AC_E; k += 4) {
+        double w[4];
+        left_of<PT>(a, e, x, q, first + k, w);
+#pragma unroll
+        for (int j = 0; j < 4; j++) s += w[j];
+#pragma unroll
+        for (int j = 0; j < AC_E - 4; j++) {
+            x[j] = x[j + 4];
+            q[j] = q[j + 4];
+        }
+    }
+    return s;
 }
 
 template <int TY, int PT> // PT: the type of the draft's probabilities, -1: none
 __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     constexpr int PQ = PT < 0 ? LLM_F32 : PT;
     __shared__ float sm_m[AC_N];
-    __shared__ int sm_best[AC_N], sm_parent[AC_N], sm_token[AC_N], sm_path[AC_N];
-    __shared__ double sm_s[AC_N], sm_p[AC_N], sm_q[AC_N], sm_sum[AC_T / 64];
+    __shared__ int sm_best[AC_N];
+    __shared__ double sm_s[AC_N], sm_sum[AC_T / 64], sm_before, sm_point;
     __shared__ AcEnd end;
+    __shared__ int sm_seg, sm_at, sm_end, sm_last;
     const int seg = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x / 64, nn = nodes(a, b);
     const int64_t at0 = (int64_t)b * a.max_n;
     if (nn == 0) {
@@ -167,198 +325,217 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
         }
         return;
     }
-    for (int r = wave; r < nn; r += AC_T / 64) {
+    const uint8_t *const x = a.x + b * a.seq, *const q = PT >= 0 ? a.q + b * a.p_seq : nullptr;
+    // a lane a node, every wave alike; every load that depends on no other first
+    AcRow rows;
+    rows.load(a, b, min((int)threadIdx.x / 16, nn - 1), 0);
+    int parent = -1, token = -1;
+    float y = 0.0f, u = 0.0f;
+    double prob = 0.0;
+    if (lane < nn) {
+        u = a.coins[at0 + lane];
+        parent = a.parents ? a.parents[at0 + lane] : lane - 1;
+        token = a.tokens[at0 + lane];
+    }
+    if (lane == 0 || parent < 0 || parent >= lane) parent = -1;
+    if (lane == 0 || token < 0 || token >= a.vocab) token = -1;
+    if (parent >= 0 && token >= 0) {
+        y = at<TY>(x + parent * a.row, token);
+        if (PT >= 0) prob = (double)at<PQ>(q + parent * a.p_row, token);
+    }
+    for (int r = threadIdx.x / 16; r - (int)threadIdx.x / 16 < nn; r += AC_T / 16) {
         float m;
         int best;
         double s;
-        row_stats(a, b, r, m, best, s);
-        if (lane == 0) sm_m[r] = m, sm_best[r] = best, sm_s[r] = s;
+        rows.join(a, b, min(r, nn - 1), m, best, s);
+        if (r < nn && (threadIdx.x & 15) == 0) sm_m[r] = m, sm_best[r] = best, sm_s[r] = s;
+        rows.load(a, b, min(r + AC_T / 16, nn - 1), 0);
     }
     __syncthreads();
-    const uint8_t *const x = a.x + b * a.seq, *const q = PT >= 0 ? a.q + b * a.p_seq : nullptr;
-    for (int i = threadIdx.x; i < a.max_n; i += AC_T) {
+    double p = 0.0;
+    if (parent >= 0 && token >= 0) p = weight_of(a, y, sm_m[parent], token, sm_best[parent]) / sm_s[parent];
+    if (seg == 0 && wave == 0 && lane > 0 && lane < a.max_n) {
         float lp = 0.0f;
-        int parent = -1, token = -1;
-        if (i > 0 && i < nn) {
-            parent = a.parents ? a.parents[at0 + i] : i - 1;
-            if (parent < 0 || parent >= i) parent = -1;
-            token = a.tokens[at0 + i];
-            if (token < 0 || token >= a.vocab) token = -1;
-            double p = 0.0;
-            if (parent >= 0) {
-                lp = -INFINITY;
-                if (token >= 0) {
-                    const float y = at<TY>(x + parent * a.row, token);
-                    p = weight(a, y, sm_m[parent], token, sm_best[parent]) / sm_s[parent];
-                    if (a.inv_t == 0.0) lp = p != p ? NAN : p > 0.0 ? 0.0f : -INFINITY;
-                    else lp = (float)(((double)y - (double)sm_m[parent]) * a.inv_t - log(sm_s[parent]));
-                    if (PT >= 0) sm_q[i] = (double)at<PQ>(q + parent * a.p_row, token);
-                }
-            }
-            sm_p[i] = p;
+        if (parent >= 0) {
+            lp = -INFINITY;
+            if (token >= 0 && a.c == 0.0) lp = p != p ? NAN : p > 0.0 ? 0.0f : -INFINITY;
+            else if (token >= 0)
+                lp = (float)((((double)y - (double)sm_m[parent]) * a.c - log2_of(sm_s[parent])) * 0.693147180559945309417);
         }
-        if (i < AC_N) sm_parent[i] = parent, sm_token[i] = token;
-        if (seg == 0 && i > 0) a.logp[at0 + i] = lp;
+        a.logp[at0 + lane] = lp;
     }
-    __syncthreads();
-    // the walk, by all threads alike
-    int node = 0, kept = 1, turned = 0;
+    // the walk: from child to child, values of a lane read by all
+    auto of = [&](double v, int i) {
+        const uint64_t w = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), i) << 32 |
+                                              (uint32_t)__builtin_amdgcn_readlane((int)w, i));
+    };
+    int node = 0;
+    uint64_t kept = 1, gone = 0; // nodes on the way; children of the node that were turned down
     double left = 1.0, aq = 0.0;
-    for (int i = 1; i < nn; i++) {
-        if (sm_parent[i] != node || sm_token[i] < 0) continue;
-        const double u = (double)a.coins[at0 + i];
-        double w = sm_p[i];
+    uint64_t open = __ballot(parent == 0 && token >= 0);
+    while (open) {
+        const int c = __ffsll((unsigned long long)open) - 1;
+        open &= open - 1;
+        const double coin = (double)__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(u), c));
+        double w = of(p, c);
         bool takes;
         if (PT >= 0) {
-            w = fmax(w - aq * sm_q[i], 0.0);
-            takes = u * sm_q[i] * left < w;
+            const double qc = of(prob, c);
+            w = fmax(w - aq * qc, 0.0);
+            takes = coin * qc * left < w;
         } else {
-            for (int t = 0; t < turned; t++)
-                if (end.out[t] == sm_token[i]) w = 0.0;
-            takes = u * left < w;
+            if (__ballot(token == __builtin_amdgcn_readlane(token, c)) & gone) w = 0.0;
+            takes = coin * left < w;
         }
         if (takes) {
-            if (threadIdx.x == 0) sm_path[kept] = i;
-            node = i, left = 1.0, aq = 0.0, turned = 0;
-            kept++;
+            node = c, left = 1.0, aq = 0.0;
+            kept |= (uint64_t)1 << c;
+            gone = 0;
+            open = __ballot(parent == node && token >= 0);
             continue;
         }
-        if (PT >= 0) {
-            aq += left;
-            bool more = false; // another child to hold against what is left
-            for (int k = i + 1; k < nn; k++) more |= sm_parent[k] == node && sm_token[k] >= 0;
-            if (more) {
-                const uint8_t *row = x + node * a.row, *probs = q + node * a.p_row;
-                double s = 0.0;
-                for (int k = threadIdx.x; k < a.vocab; k += AC_T)
-                    s += fmax(weight(a, at<TY>(row, k), sm_m[node], k, sm_best[node]) / sm_s[node] -
-                                  aq * (double)at<PQ>(probs, k), 0.0);
-                s = wave_add(s);
-                __syncthreads();
-                if (lane == 0) sm_sum[wave] = s;
-                __syncthreads();
-                left = (sm_sum[0] + sm_sum[1]) + (sm_sum[2] + sm_sum[3]);
-            }
-        } else {
+        gone |= (uint64_t)1 << c;
+        if (PT < 0) {
             left = fmax(left - w, 0.0);
-            __syncthreads();
-            if (threadIdx.x == 0) end.out[turned] = sm_token[i];
-            turned++;
-            __syncthreads();
+            continue;
         }
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        sm_path[0] = 0;
-        end.node = node, end.turned = turned, end.m = sm_m[node], end.best = sm_best[node], end.s = sm_s[node], end.a = aq;
-    }
-    __syncthreads();
-    if (seg == 0) {
-        for (int i = threadIdx.x; i < a.max_n; i += AC_T) a.path[at0 + i] = i < kept ? sm_path[i] : -1;
-        if (threadIdx.x == 0) {
-            a.kept[b] = kept;
-            a.end[b] = end;
-        }
-    }
-    double w[AC_E], s = 0.0;
-    left_of<TY, PT>(a, x + node * a.row, PT >= 0 ? q + node * a.p_row : nullptr, end, seg * AC_SEG + threadIdx.x * AC_E, w);
+        aq += left;
+        if (open) { // another child to hold against what is left
+            const uint8_t *row = x + node * a.row, *probs = q + node * a.p_row;
+            double s = 0.0;
+            const double inv = 1.0 / sm_s[node];
+            const bool greedy = a.c == 0.0;
+            const double m = (double)sm_m[node];
+            const int best = sm_best[node];
+            for (int k = threadIdx.x * 8; k < a.vocab; k += AC_T * 8) {
+                float xv[8], qv[8];
 #pragma unroll
-    for (int k = 0; k < AC_E; k++) s += w[k];
-    s = wave_add(s);
-    if (lane == 0) sm_sum[wave] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) a.sums[(int64_t)b * a.segs + seg] = (sm_sum[0] + sm_sum[1]) + (sm_sum[2] + sm_sum[3]);
-}
-
-template <int TY, int PT>
-__global__ void __launch_bounds__(AC_T) k_accept_draw(AcArgs a) {
-    __shared__ AcEnd end;
-    __shared__ double sm_sum[AC_T / 64];
-    __shared__ double sm_before;
-    __shared__ int sm_seg, sm_at, sm_last;
-    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    if (nodes(a, b) == 0) return;
-    if (threadIdx.x == 0) end = a.end[b], sm_at = 0x7fffffff, sm_last = -1;
-    __syncthreads();
-    const int64_t at0 = (int64_t)b * a.max_n;
-    const double *sums = a.sums + (int64_t)b * a.segs;
-    const AcPart *part = a.part + (at0 + end.node) * a.segs;
-    double u = 0.0;
-    if (threadIdx.x == 0) {
-        double all = 0.0;
-        for (int k = 0; k < a.segs; k++) all += sums[k];
-        bool whole = false; // nothing is left: the target's own row
-        auto sum_of = [&](int k) {
-            if (!whole) return sums[k];
-            if (a.inv_t == 0.0) return end.best / AC_SEG == k ? 1.0 : 0.0;
-            return part[k].m > -INFINITY ? part[k].s * exp(((double)part[k].m - (double)end.m) * a.inv_t) / end.s : 0.0;
-        };
-        if (all == 0.0) {
-            whole = true;
-            for (int k = 0; k < a.segs; k++) all += sum_of(k);
-            end.a = 0.0, end.turned = 0;
-        }
-        double before = 0.0;
-        int seg = -1;
-        if (all > 0.0) {
-            u = (double)a.coins[at0] * all;
-            for (seg = 0; seg < a.segs - 1; seg++) {
-                const double s = sum_of(seg);
-                if (before + s > u) break;
-                before += s;
+                for (int e = 0; e < 8; e += AC_V<TY>) values<TY>(row, k + e, a.vocab, -INFINITY, xv + e);
+#pragma unroll
+                for (int e = 0; e < 8; e += AC_V<PQ>) values<PQ>(probs, k + e, a.vocab, 0.0f, qv + e);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const double w = greedy ? k + e == best ? inv : 0.0 : weight(xv[e], m, a.c) * inv;
+                    s += fmax(w - aq * (double)qv[e], 0.0);
+                }
             }
-            while (seg > 0 && sum_of(seg) == 0.0) before -= sum_of(--seg); // (the last segments may have nothing)
-        }
-        sm_seg = seg;
-        sm_before = before;
-        sm_sum[0] = u;
-    }
-    __syncthreads();
-    const int seg = sm_seg;
-    u = sm_sum[0];
-    if (seg < 0) {
-        if (threadIdx.x == 0) a.next[b] = -1, a.logp[at0] = NAN;
-        return;
-    }
-    __syncthreads();
-    const uint8_t *row = a.x + b * a.seq + end.node * a.row;
-    double w[AC_E], s = 0.0;
-    const int first = seg * AC_SEG + threadIdx.x * AC_E;
-    left_of<TY, PT>(a, row, PT >= 0 ? a.q + b * a.p_seq + end.node * a.p_row : nullptr, end, first, w);
-#pragma unroll
-    for (int k = 0; k < AC_E; k++) s += w[k];
-    double upto = s;
-    for (int off = 1; off < 64; off <<= 1) {
-        const double y = __shfl_up(upto, off);
-        upto += lane >= off ? y : 0.0;
-    }
-    if (lane == 63) sm_sum[wave] = upto;
-    __syncthreads();
-    double c = sm_before + (upto - s);
-    for (int k = 0; k < wave; k++) c += sm_sum[k];
-    int found = 0x7fffffff, last = -1;
-#pragma unroll
-    for (int k = 0; k < AC_E; k++) {
-        c += w[k];
-        if (w[k] > 0.0) {
-            last = first + k;
-            if (c > u && found == 0x7fffffff) found = first + k;
+            left = block_add(s, sm_sum);
         }
     }
-    if (found != 0x7fffffff) atomicMin(&sm_at, found);
-    if (last >= 0) atomicMax(&sm_last, last);
+    if (wave == 0) {
+        if (lane == 0) {
+            end.node = node, end.turned = PT < 0 ? __popcll(gone) : 0;
+            end.m = sm_m[node], end.best = sm_best[node], end.s = sm_s[node], end.inv = 1.0 / sm_s[node], end.a = aq;
+        }
+        if ((gone >> lane) & 1) end.out[__popcll(gone & (((uint64_t)1 << lane) - 1))] = token;
+        if (seg == 0) {
+            const int count = __popcll(kept);
+            if (lane >= count && lane < a.max_n) a.path[at0 + lane] = -1;
+            if ((kept >> lane) & 1) a.path[at0 + __popcll(kept & (((uint64_t)1 << lane) - 1))] = lane;
+            if (lane == 0) a.kept[b] = count;
+        }
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        const int token = sm_at != 0x7fffffff ? sm_at : sm_last; // (a point at the end, by rounding)
-        a.next[b] = token;
-        if (token < 0) { // (draft probabilities that are not finite)
-            a.logp[at0] = NAN;
+    const uint8_t *const row = x + node * a.row, *const probs = PT >= 0 ? q + node * a.p_row : nullptr;
+    // Sums of segments, one after another through the same code: the workgroup's own; of the sequence's last workgroup, where nothing
+    // is left, those of the target's own row; the one that the drawn point falls into.
+    double *const sums = a.sums + (int64_t)b * a.segs;
+    auto sum_at = [&](int k) { return k < a.segs ? __hip_atomic_load(&sums[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0; };
+    int now = seg, rest = -1; // rest: the next segment of the target's own row
+    bool picked = false;
+    double s;
+#pragma unroll 1
+    for (;;) {
+        s = left_sum<TY, PT>(a, row, probs, end, now);
+        if (picked) break;
+        const double all_s = block_add(s, sm_sum);
+        if (threadIdx.x == 0) {
+            // (through to where every XCD reads it, before it is counted)
+            __hip_atomic_store(&sums[now], all_s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (rest < 0) sm_last = __hip_atomic_fetch_add(&a.done[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.segs - 1;
+        }
+        __syncthreads();
+        if (!sm_last) return;
+        if (rest >= 0 && rest < a.segs) {
+            now = rest++;
+            continue;
+        }
+        double mine = sum_at(lane), all = mine;
+        for (int k = lane + 64; k < a.segs; k += 64) all += sum_at(k);
+        all = lanes_add<64>(all);
+        if (all == 0.0 && rest < 0) {
+            __syncthreads();
+            if (threadIdx.x == 0) end.a = 0.0, end.turned = 0;
+            __syncthreads();
+            now = 0, rest = 1;
+            continue;
+        }
+        if (wave == 0) { // the point, its segment, and the sum before that, segments in order
+            const double point = (double)__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(u), 0)) * all;
+            int found = -1, last = -1; // the segment; the last one that has something (a point at the end, by rounding)
+            double before = 0.0, start = 0.0, last_start = 0.0;
+            if (all > 0.0)
+                for (int k0 = 0; k0 < a.segs && found < 0; k0 += 64) {
+                    if (k0) mine = sum_at(k0 + lane);
+                    const double to = before + upto(mine);
+                    const uint64_t over = __ballot(mine > 0.0 && to > point), some = __ballot(mine > 0.0);
+                    if (over) found = __ffsll((unsigned long long)over) - 1, start = of(to - mine, found), found += k0;
+                    if (some) last = 63 - __clzll((long long)some), last_start = of(to - mine, last), last += k0;
+                    before = of(to, 63);
+                }
+            if (lane == 0) {
+                sm_seg = found >= 0 ? found : last;
+                sm_before = found >= 0 ? start : last_start;
+                sm_point = point;
+                sm_at = 0x7fffffff, sm_end = -1;
+            }
+        }
+        __syncthreads();
+        if (sm_seg < 0) { // no probabilities, or a draft's that are not finite
+            if (threadIdx.x == 0) a.next[b] = -1, a.logp[at0] = NAN;
             return;
         }
-        double lp = 0.0;
-        if (a.inv_t != 0.0) lp = ((double)at<TY>(row, token) - (double)end.m) * a.inv_t - log(end.s);
-        else if (token != end.best) lp = -INFINITY;
-        a.logp[at0] = (float)lp;
+        now = sm_seg;
+        picked = true;
+    }
+    // the thread whose values the point falls into: the first with the sum up to its end above it (else, by rounding, the last one
+    // that has something)
+    const double to = upto(s);
+    if (lane == 63) sm_sum[wave] = to;
+    __syncthreads();
+    double c = sm_before + (to - s);
+    for (int k = 0; k < wave; k++) c += sm_sum[k];
+    if (s > 0.0 && c + s > sm_point) atomicMin(&sm_at, (int)threadIdx.x);
+    if (s > 0.0) atomicMax(&sm_end, (int)threadIdx.x);
+    __syncthreads();
+    const int thread = sm_at != 0x7fffffff ? sm_at : sm_end;
+    if ((int)threadIdx.x == thread) sm_before = c;
+    __syncthreads();
+    if (wave) return;
+    // its values, a lane each
+    const int i = sm_seg * AC_SEG + thread * AC_E + lane;
+    float value = 0.0f;
+    double w = 0.0;
+    if (thread >= 0 && lane < AC_E && i < a.vocab) {
+        value = at<TY>(row, i);
+        float qi = 0.0f;
+        if (PT >= 0) qi = at<PQ>(probs, i);
+        double one[1];
+        left_of<PT>(a, end, &value, &qi, i, one);
+        w = one[0];
+    }
+    const double sum = upto(w);
+    const uint64_t over = __ballot(w > 0.0 && sm_before + sum > sm_point), some = __ballot(w > 0.0);
+    const int drawn = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
+    if (some == 0) {
+        if (lane == 0) a.next[b] = -1, a.logp[at0] = NAN;
+    } else if (lane == drawn) {
+        float lp = i == end.best ? 0.0f : -INFINITY;
+        if (a.c != 0.0) lp = (float)((((double)value - (double)end.m) * a.c - log2_of(end.s)) * 0.693147180559945309417);
+        a.next[b] = i;
+        a.logp[at0] = lp;
     }
 }
 
@@ -369,7 +546,7 @@ int64_t ac_segs(int vocab) { return ((int64_t)vocab + AC_SEG - 1) / AC_SEG; }
 extern "C" size_t llm_draft_accept_work(int n_seq, int max_n, int vocab) {
     if (n_seq < 1 || max_n < 1 || max_n > AC_N || vocab < 1) return 0;
     const size_t segs = ac_segs(vocab);
-    return (size_t)n_seq * (max_n * segs * sizeof(AcPart) + sizeof(AcEnd) + segs * sizeof(double));
+    return (size_t)n_seq * (max_n * segs * sizeof(AcPart) + segs * sizeof(double) + sizeof(int));
 }
 
 extern "C" int llm_draft_accept(const void *logits, int type, int n_seq, int max_n, int vocab, int64_t seq, int64_t row,
@@ -404,26 +581,31 @@ extern "C" int llm_draft_accept(const void *logits, int type, int n_seq, int max
     a.x = (const uint8_t *)logits, a.q = (const uint8_t *)probs;
     a.seq = seq * xs, a.row = row * xs, a.p_seq = p_seq * ps, a.p_row = p_row * ps;
     a.max_n = max_n, a.vocab = vocab, a.segs = (int)ac_segs(vocab);
-    a.inv_t = temperature == 0.0f ? 0.0 : 1.0 / (double)temperature;
+    const int per = (int64_t)n_seq * max_n * a.segs >= 4096 ? 4 : 1;
+    a.parts = (a.segs + per - 1) / per;
+    a.c = temperature == 0.0f ? 0.0 : 1.44269504088896340736 / (double)temperature;
     a.tokens = tokens, a.parents = parents, a.n = n, a.coins = coins;
     a.kept = kept, a.path = path, a.next = next, a.logp = logp;
     a.part = (AcPart *)work;
-    a.end = (AcEnd *)(a.part + (size_t)n_seq * max_n * a.segs);
-    a.sums = (double *)(a.end + n_seq);
+    a.sums = (double *)(a.part + (size_t)n_seq * max_n * a.segs);
+    a.done = (int *)(a.sums + (size_t)n_seq * a.segs);
     hipStream_t st = (hipStream_t)stream;
-    const bool f32 = type == LLM_F32;
-    hipLaunchKernelGGL(f32 ? k_accept_rows<LLM_F32> : k_accept_rows<LLM_BF16>, dim3(a.segs, max_n, n_seq), dim3(AC_T), 0, st, a);
+    void (*rows)(AcArgs) = nullptr;
+#define ACCEPT_PICK(T, P, X) \
+    if (type == T && per == P && (probs != nullptr) == X) rows = k_accept_rows<T, P, X>;
+    ACCEPT_PICK(LLM_F32, 1, false) ACCEPT_PICK(LLM_F32, 4, false) ACCEPT_PICK(LLM_BF16, 1, false) ACCEPT_PICK(LLM_BF16, 4, false)
+    ACCEPT_PICK(LLM_F32, 1, true) ACCEPT_PICK(LLM_F32, 4, true) ACCEPT_PICK(LLM_BF16, 1, true) ACCEPT_PICK(LLM_BF16, 4, true)
+#undef ACCEPT_PICK
+    hipLaunchKernelGGL(rows, dim3(a.parts, max_n, n_seq), dim3(AC_T), 0, st, a);
     HIP_OR_FAIL(who, hipGetLastError());
-    void (*walk)(AcArgs) = nullptr, (*draw)(AcArgs) = nullptr;
+    void (*walk)(AcArgs) = nullptr;
     const int pt = probs ? p_type : -1;
 #define ACCEPT_PICK(T, P) \
-    if (type == T && pt == P) walk = k_accept_walk<T, P>, draw = k_accept_draw<T, P>;
+    if (type == T && pt == P) walk = k_accept_walk<T, P>;
     ACCEPT_PICK(LLM_F32, -1) ACCEPT_PICK(LLM_F32, LLM_F32) ACCEPT_PICK(LLM_F32, LLM_BF16)
     ACCEPT_PICK(LLM_BF16, -1) ACCEPT_PICK(LLM_BF16, LLM_F32) ACCEPT_PICK(LLM_BF16, LLM_BF16)
 #undef ACCEPT_PICK
     hipLaunchKernelGGL(walk, dim3(a.segs, n_seq), dim3(AC_T), 0, st, a);
-    HIP_OR_FAIL(who, hipGetLastError());
-    hipLaunchKernelGGL(draw, dim3(n_seq), dim3(AC_T), 0, st, a);
     HIP_OR_FAIL(who, hipGetLastError());
     return 0;
 }

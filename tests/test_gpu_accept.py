@@ -1,5 +1,8 @@
 """llm_draft_accept against its definition: the residual distributions one after another in float64.  Kept nodes, paths and drawn
-tokens have to be equal; a log probability is off by at most the rounding of its result and of the 64-bit sums before it."""
+tokens have to be equal; a log probability is off by at most the rounding of its result.  Without draft probabilities by its row's
+sum too, in 32 bits: an exponent y = (x - m) log2(e) / T is off by three roundings, 3 2^-24 |y|, which over the row is 3 2^-24 ln 2
+sum p |y| <= 3 2^-24 ln 2 log2(vocab) <= 2.2e-6; the instruction by 2^-22; eight chains of eight additions by 2^-21: 2.9e-6 <
+2^-18."""
 import math
 import random
 
@@ -47,7 +50,7 @@ def check(x, q, tokens, parents, coins, n, temperature, got):
         assert path[i].tolist() == want[1], i
         assert int(drawn[i]) == want[2], i
         for a, w in zip(logp[i].tolist(), want[3]):
-            assert a == w or (math.isnan(a) and math.isnan(w)) or abs(a - w) <= 2.0 ** -24 * abs(w) + 1e-12, (i, a, w)
+            assert a == w or (math.isnan(a) and math.isnan(w)) or abs(a - w) <= 2.0 ** -24 * abs(w) + (2.0 ** -18 if q is None else 1e-12), (i, a, w)
 
 
 @pytest.mark.parametrize("temperature", [1.0, 0.7, 0.0])
