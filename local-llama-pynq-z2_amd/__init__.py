@@ -424,29 +424,36 @@ def _pages(k, v, k_scale, v_scale):
     their scales [pages, kv heads, page / 64] (float32), with the layers before the pages or without; pages and heads may lie apart.
     And its dimensions (layers, pages, kv heads, page, head size)"""
     torch, types = _torch or _types()
-    ty, shape = types.get(k.dtype, 0), k.shape
-    many = len(shape) == 5
-    if ty < 2 or v.dtype is not k.dtype or len(shape) != 4 + many or shape[-2] % 64 or not shape[-2]:
+    dtype, shape = k.dtype, k.shape
+    ty, j = types.get(dtype, 0), len(shape) - 4  # j: where the pages are, behind the layers or first
+    if ty < 2 or v.dtype is not dtype or j not in (0, 1) or shape[-2] % 64 or not shape[-2]:
         raise ValueError("k: int8 or float8_e4m3fn codes [pages, kv heads, page, head size] are needed, v of the same type")
-    page, hs = shape[-2:]
-    rows = shape[:-2] + (page // 64,)
-    if v.shape != rows + (hs, 64):
-        raise ValueError(f"v: codes {tuple(rows) + (hs, 64)} are needed")
+    *layers, pages, h, page, hs = shape
+    rows, layers = (*layers, pages, h, page // 64), layers[0] if j else 1
+    if v.shape != (*rows, hs, 64):
+        raise ValueError(f"v: codes {(*rows, hs, 64)} are needed")
     f32 = torch.float32
     if k_scale.shape != rows or v_scale.shape != rows or k_scale.dtype is not f32 or v_scale.dtype is not f32:
-        raise ValueError(f"k_scale, v_scale: float32 {tuple(rows)} are needed")
+        raise ValueError(f"k_scale, v_scale: float32 {rows} are needed")
     sk, sv, ss, st = k.stride(), v.stride(), k_scale.stride(), v_scale.stride()
     if (sk[-1] != 1 and hs > 1) or sk[-2] != hs or sv[-1] != 1 or sv[-2] != 64 or \
             (page > 64 and (sv[-3] != 64 * hs or ss[-1] != 1 or st[-1] != 1)):
         raise ValueError("k, v and their scales: what a page holds of a head has to lie together")
-    n, at = (shape[:3] if many else (1, *shape[:2])), [0] * 6
-    for i in range(0 if many else 1, 3): # (a dimension of one has no stride that counts)
-        if n[i] > 1:
-            j = i if many else i - 1
-            if sk[j] != sv[j] or ss[j] != st[j]:
-                raise ValueError("k and v, and their scales: equal strides of layers, pages and heads are needed")
-            at[i], at[i + 3] = sk[j], ss[j]
-    return _PACK_PAGES(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, *n, hs, page, *at), (*n, page, hs)
+    layer = at = head = s_layer = s_at = s_head = 0  # (a dimension of one has no stride that counts)
+    apart = False
+    if layers > 1:
+        layer, s_layer = sk[0], ss[0]
+        apart = layer != sv[0] or s_layer != st[0]
+    if pages > 1:
+        at, s_at = sk[j], ss[j]
+        apart = apart or at != sv[j] or s_at != st[j]
+    if h > 1:
+        head, s_head = sk[j + 1], ss[j + 1]
+        apart = apart or head != sv[j + 1] or s_head != st[j + 1]
+    if apart:
+        raise ValueError("k and v, and their scales: equal strides of layers, pages and heads are needed")
+    return _PACK_PAGES(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ty, layers, pages, h, hs, page, layer, at,
+                       head, s_layer, s_at, s_head), (layers, pages, h, page, hs)
 
 
 def _table(table):

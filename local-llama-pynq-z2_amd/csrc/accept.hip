@@ -12,9 +12,10 @@
 // error of 2^-24 in the likeliest token's weight would all move by 6e-8.
 //
 // What bounds it: the rows' bytes, read once.  16 trees of 37 rows of 152064 bf16 logits, 180 MB: 26.5 us, 6.8 TB/s, for the rows (the
-// last call left a part of them in the caches) and 24.5 for the walk; a chain of 8 fp32 rows with draft probabilities: 4.3 and 16.8.
-// The walk is a chain of short steps: the parts' loads, the join, the tokens' probabilities, a segment's sum, the count, the sums of
-// the others, the drawn segment's sum again.  What is not spread is the row's pass where a child with a later sibling is turned down
+// last call left a part of them in the caches) and 21.8 for the walk; a chain of 8 fp32 rows with draft probabilities: 4.3 and 15.7.
+// The walk is a chain of short steps (of that chain, in thousands of cycles: the parts' loads 2.7, the join 2.6, the tokens'
+// probabilities 1, the walk 1.7, a segment's sum 8.6, the count 1.5, the choice of a segment 3, of a token 13), each code that runs
+// once: fetching it is a good part of the time.  What is not spread is the row's pass where a child with a later sibling is turned down
 // against draft probabilities: each workgroup takes it by itself, 25 us a time, so that none waits for another.
 #include <string.h>
 
@@ -50,7 +51,7 @@ struct AcArgs {
     int *kept, *path, *next;
     float *logp;
     AcPart *part; // [seq][row][part]
-    double *sums; // [seq][segment]
+    double *sums, *shares; // [seq][segment], [seq][segment][thread]
     int *done;    // [seq]: segments that are summed
 };
 
@@ -438,24 +439,25 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     }
     __syncthreads();
     const uint8_t *const row = x + node * a.row, *const probs = PT >= 0 ? q + node * a.p_row : nullptr;
-    // Sums of segments, one after another through the same code: the workgroup's own; of the sequence's last workgroup, where nothing
-    // is left, those of the target's own row; the one that the drawn point falls into.
-    double *const sums = a.sums + (int64_t)b * a.segs;
-    auto sum_at = [&](int k) { return k < a.segs ? __hip_atomic_load(&sums[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0; };
+    // Sums of segments through the same code: the workgroup's own; of the sequence's last workgroup, where nothing is left, those of
+    // the target's own row too.  The threads' shares are kept for the draw, which would else read the segment and sum it again (the
+    // walk of a chain of 8 fp32 rows: 15.7 us instead of 16.8, of sixteen
+    // trees of bf16 rows 21.8 instead of 24.5).
+    double *const sums = a.sums + (int64_t)b * a.segs, *const shares = a.shares + (int64_t)b * a.segs * AC_T;
+    // (through to where every XCD reads it)
+    auto put = [](double *at, double v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto get = [](double *at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto sum_at = [&](int k) { return k < a.segs ? get(&sums[k]) : 0.0; };
     int now = seg, rest = -1; // rest: the next segment of the target's own row
-    bool picked = false;
-    double s;
 #pragma unroll 1
     for (;;) {
-        s = left_sum<TY, PT>(a, row, probs, end, now);
-        if (picked) break;
-        const double all_s = block_add(s, sm_sum);
-        if (threadIdx.x == 0) {
-            // (through to where every XCD reads it, before it is counted)
-            __hip_atomic_store(&sums[now], all_s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (rest < 0) sm_last = __hip_atomic_fetch_add(&a.done[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.segs - 1;
-        }
+        const double share = left_sum<TY, PT>(a, row, probs, end, now), all_s = block_add(share, sm_sum);
+        put(&shares[now * AC_T + threadIdx.x], share);
+        if (threadIdx.x == 0) put(&sums[now], all_s);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (there before it is counted)
+        __syncthreads();
+        if (threadIdx.x == 0 && rest < 0)
+            sm_last = __hip_atomic_fetch_add(&a.done[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.segs - 1;
         __syncthreads();
         if (!sm_last) return;
         if (rest >= 0 && rest < a.segs) {
@@ -497,9 +499,9 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
             if (threadIdx.x == 0) a.next[b] = -1, a.logp[at0] = NAN;
             return;
         }
-        now = sm_seg;
-        picked = true;
+        break;
     }
+    const double s = get(&shares[sm_seg * AC_T + threadIdx.x]);
     // the thread whose values the point falls into: the first with the sum up to its end above it (else, by rounding, the last one
     // that has something)
     const double to = upto(s);
@@ -546,7 +548,7 @@ int64_t ac_segs(int vocab) { return ((int64_t)vocab + AC_SEG - 1) / AC_SEG; }
 extern "C" size_t llm_draft_accept_work(int n_seq, int max_n, int vocab) {
     if (n_seq < 1 || max_n < 1 || max_n > AC_N || vocab < 1) return 0;
     const size_t segs = ac_segs(vocab);
-    return (size_t)n_seq * (max_n * segs * sizeof(AcPart) + segs * sizeof(double) + sizeof(int));
+    return (size_t)n_seq * (max_n * segs * sizeof(AcPart) + segs * (1 + AC_T) * sizeof(double) + sizeof(int));
 }
 
 extern "C" int llm_draft_accept(const void *logits, int type, int n_seq, int max_n, int vocab, int64_t seq, int64_t row,
@@ -588,7 +590,8 @@ extern "C" int llm_draft_accept(const void *logits, int type, int n_seq, int max
     a.kept = kept, a.path = path, a.next = next, a.logp = logp;
     a.part = (AcPart *)work;
     a.sums = (double *)(a.part + (size_t)n_seq * max_n * a.segs);
-    a.done = (int *)(a.sums + (size_t)n_seq * a.segs);
+    a.shares = a.sums + (size_t)n_seq * a.segs;
+    a.done = (int *)(a.shares + (size_t)n_seq * a.segs * AC_T);
     hipStream_t st = (hipStream_t)stream;
     void (*rows)(AcArgs) = nullptr;
 #define ACCEPT_PICK(T, P, X) \
