@@ -11,12 +11,12 @@
 // Sums and exponentials that decide are in 64 bits: a token drawn in the tail of 150k stands between borders 1e-6 apart, which an
 // error of 2^-24 in the likeliest token's weight would all move by 6e-8.
 //
-// What bounds it: the rows' bytes, read once.  16 trees of 37 rows of 152064 bf16 logits, 180 MB: 26.5 us, 6.8 TB/s, for the rows (the
-// last call left a part of them in the caches) and 21.8 for the walk; a chain of 8 fp32 rows with draft probabilities: 4.3 and 15.7.
+// What bounds it: the rows' bytes, read once.  16 trees of up to 37 rows of 151936 bf16 logits, 154 MB: 26.5 us, 5.8 TB/s, for the rows (the
+// last call left a part of them in the caches) and 21.8 for the walk; a chain of 6 fp32 rows with draft probabilities: 4.3 and 15.7.
 // The walk is a chain of short steps (of that chain, in thousands of cycles: the parts' loads 2.7, the join 2.6, the tokens'
 // probabilities 1, the walk 1.7, a segment's sum 8.6, the count 1.5, the choice of a segment 3, of a token 13), each code that runs
-// once: fetching it is a good part of the time.  What is not spread is the row's pass where a child with a later sibling is turned down
-// against draft probabilities: each workgroup takes it by itself, 25 us a time, so that none waits for another.
+// once: fetching it is a good part of the time.  Trees with draft probabilities need a row's pass for each child with a later sibling that
+// is turned down: see k_accept_ask.
 #include <string.h>
 
 #include <algorithm>
@@ -28,6 +28,10 @@ namespace {
 
 constexpr int AC_T = 256, AC_E = 16, AC_SEG = AC_T * AC_E; // values of a segment
 constexpr int AC_N = 64;                                   // most nodes: a lane each
+// Least vocabulary for k_accept_ask and k_accept_left, three launches of 7 us together: a single tree of 20 nodes over 32000 logits
+// 27 us with them and 19 (nothing is asked for) or 36 without, over 151936 33 and 95, 16 trees of 37 over 8192 logits 38 and 28, over
+// 16384 43 and 40, over 32000 60 and 79, over 151936 117 and 290 (all fp32).
+constexpr int AC_ASK = 16384;
 
 struct AcPart { // of a part of a row: largest value, its first place (temperature 0), sum relative to it
     float m;
@@ -41,6 +45,11 @@ struct AcEnd { // a sequence's last node, its row's statistics, what is left of 
     double s, inv, a; // inv: 1 / s
     int out[AC_N]; // tokens turned down (no draft probabilities)
 };
+struct AcAsk { // a node whose first child is turned down and not its last one; its row's statistics; the second child
+    int node, more, best; // more: there is a third
+    float m;
+    double inv, p, q, coin;
+};
 struct AcArgs {
     const uint8_t *x, *q;
     int64_t seq, row, p_seq, p_row; // bytes
@@ -53,6 +62,9 @@ struct AcArgs {
     AcPart *part; // [seq][row][part]
     double *sums, *shares; // [seq][segment], [seq][segment][thread]
     int *done;    // [seq]: segments that are summed
+    AcAsk *asks;  // [seq][max_n]
+    int *count;   // [seq]: of them
+    double *left; // [seq][node][0, 1][segment]: what is left after the node's first and second child; NULL: not known
 };
 
 template <int TY>
@@ -247,7 +259,8 @@ __device__ __forceinline__ double log2_of(double s) {
 }
 
 // What is left of N neighbouring values from `first` on: x their logits (-infinity behind the row), q the draft's probabilities.
-template <int PT, int N>
+// A draft probability that is not finite leaves 0 for the test of a child (Z), NaN for the draw, which then has none.
+template <int PT, bool Z, int N>
 __device__ __forceinline__ void left_of(const AcArgs &a, const AcEnd &e, const float *x, const float *q, int first, double (&w)[N]) {
     const double m = (double)e.m, inv = e.inv, aq = e.a;
     if (a.c == 0.0) {
@@ -261,7 +274,7 @@ __device__ __forceinline__ void left_of(const AcArgs &a, const AcEnd &e, const f
 #pragma unroll
         for (int k = 0; k < N; k++) {
             const double d = w[k] - aq * (double)q[k];
-            w[k] = d < 0.0 ? 0.0 : d; // (NaN stays)
+            w[k] = Z ? fmax(d, 0.0) : d < 0.0 ? 0.0 : d;
         }
     if (PT < 0)
         for (int t = 0; t < e.turned; t++) {
@@ -272,8 +285,8 @@ __device__ __forceinline__ void left_of(const AcArgs &a, const AcEnd &e, const f
 }
 // Its sum over the thread's AC_E neighbouring values of a segment, in order.  All loads go out first; the weights are a loop of four
 // at a time, whose values move up: straight code, and no more of it than is run often enough to have been worth fetching (the walk of
-// sixteen trees over 152064 bf16 logits: 24.5 us; 28.7 with sixteen values in a row and branches for their masks and borders).
-template <int TY, int PT>
+// sixteen trees over 151936 bf16 logits: 24.5 us; 28.7 with sixteen values in a row and branches for their masks and borders).
+template <int TY, int PT, bool Z>
 __device__ __forceinline__ double left_sum(const AcArgs &a, const uint8_t *row, const uint8_t *probs, const AcEnd &e, int seg) {
     constexpr int PQ = PT < 0 ? LLM_F32 : PT;
     const int first = seg * AC_SEG + threadIdx.x * AC_E;
@@ -297,7 +310,7 @@ __device__ __forceinline__ double left_sum(const AcArgs &a, const uint8_t *row, 
 #pragma unroll 1
     for (int k = 0; k < AC_E; k += 4) {
         double w[4];
-        left_of<PT>(a, e, x, q, first + k, w);
+        left_of<PT, Z>(a, e, x, q, first + k, w);
 #pragma unroll
         for (int j = 0; j < 4; j++) s += w[j];
 #pragma unroll
@@ -307,6 +320,121 @@ __device__ __forceinline__ double left_sum(const AcArgs &a, const uint8_t *row, 
         }
     }
     return s;
+}
+
+// What a lane knows of its node: every wave alike.
+struct AcNode {
+    int parent, token; // -1: none
+    float y, u;        // the token's logit after its parent; the coin
+    double q, p;       // its probabilities: the draft's, the target's
+};
+// Of nn nodes, and their rows' statistics in LDS.
+template <int TY, int PT>
+__device__ __forceinline__ AcNode node_of(const AcArgs &a, int b, int nn, const uint8_t *x, const uint8_t *q, float *sm_m,
+                                          int *sm_best, double *sm_s) {
+    constexpr int PQ = PT < 0 ? LLM_F32 : PT;
+    const int lane = threadIdx.x & 63;
+    const int64_t at0 = (int64_t)b * a.max_n;
+    AcRow rows; // (every load that depends on no other first)
+    rows.load(a, b, min((int)threadIdx.x / 16, nn - 1), 0);
+    AcNode d = {-1, -1, 0.0f, 0.0f, 0.0, 0.0};
+    if (lane < nn) {
+        d.u = a.coins[at0 + lane];
+        d.parent = a.parents ? a.parents[at0 + lane] : lane - 1;
+        d.token = a.tokens[at0 + lane];
+    }
+    if (lane == 0 || d.parent < 0 || d.parent >= lane) d.parent = -1;
+    if (lane == 0 || d.token < 0 || d.token >= a.vocab) d.token = -1;
+    const bool is = d.parent >= 0 && d.token >= 0;
+    if (is) {
+        d.y = at<TY>(x + d.parent * a.row, d.token);
+        if (PT >= 0) d.q = (double)at<PQ>(q + d.parent * a.p_row, d.token);
+    }
+    for (int r = threadIdx.x / 16; r - (int)threadIdx.x / 16 < nn; r += AC_T / 16) {
+        float m;
+        int best;
+        double s;
+        rows.join(a, b, min(r, nn - 1), m, best, s);
+        if (r < nn && (threadIdx.x & 15) == 0) sm_m[r] = m, sm_best[r] = best, sm_s[r] = s;
+        rows.load(a, b, min(r + AC_T / 16, nn - 1), 0);
+    }
+    __syncthreads();
+    if (is) d.p = weight_of(a, d.y, sm_m[d.parent], d.token, sm_best[d.parent]) / sm_s[d.parent];
+    return d;
+}
+
+// What was turned down of trees with draft probabilities changes what is left of its parent's row by the number of children alone:
+// after the first a is 1, after the second 1 + z.  A pass over a row within the walk is every workgroup's own; so z of every row that
+// the walk may need it of is summed before, a workgroup a segment: k_accept_ask lists the nodes that may be reached, whose first
+// child is turned down and not the last, k_accept_left sums what is left after the first child and, launched again, after the second.
+// Third children's are left to the walk.
+template <int TY, int PT>
+__global__ void __launch_bounds__(AC_T) k_accept_ask(AcArgs a) {
+    __shared__ float sm_m[AC_N];
+    __shared__ int sm_best[AC_N];
+    __shared__ double sm_s[AC_N];
+    const int b = blockIdx.x, lane = threadIdx.x & 63, nn = nodes(a, b);
+    if (nn == 0) {
+        if (threadIdx.x == 0) a.count[b] = 0;
+        return;
+    }
+    const AcNode d = node_of<TY, PT>(a, b, nn, a.x + b * a.seq, a.q + b * a.p_seq, sm_m, sm_best, sm_s);
+    if (threadIdx.x >= 64) return;
+    const bool is = d.parent >= 0 && d.token >= 0;
+    // as the walk decides about a first child
+    const uint64_t takes = __ballot(is && (double)d.u * d.q * 1.0 < fmax(d.p - 0.0 * d.q, 0.0)), all = __ballot(is);
+    uint64_t kids = 0; // the node's
+    for (uint64_t left = all; left; left &= left - 1) {
+        const int i = __ffsll((unsigned long long)left) - 1;
+        if (__builtin_amdgcn_readlane(d.parent, i) == lane) kids |= (uint64_t)1 << i;
+    }
+    const int first = kids ? __ffsll((unsigned long long)kids) - 1 : lane;
+    const int eldest = __shfl(first, max(d.parent, 0)); // the first child of the node's parent
+    const uint64_t ok = __ballot(is && ((takes >> eldest) & 1) == (uint64_t)(lane == eldest));
+    uint64_t reach = 1;
+    for (uint64_t left = ok; left; left &= left - 1) {
+        const int i = __ffsll((unsigned long long)left) - 1;
+        reach |= ((reach >> __builtin_amdgcn_readlane(d.parent, i)) & 1) << i;
+    }
+    const uint64_t others = kids & (kids - 1);
+    const bool asks = others && !((takes >> first) & 1) && ((reach >> lane) & 1);
+    const uint64_t list = __ballot(asks);
+    const int second = others ? __ffsll((unsigned long long)others) - 1 : 0;
+    const double p = __shfl(d.p, second), q = __shfl(d.q, second);
+    const float coin = __shfl(d.u, second);
+    if (asks) {
+        AcAsk &k = a.asks[(int64_t)b * a.max_n + __popcll(list & (((uint64_t)1 << lane) - 1))];
+        k = {lane, (others & (others - 1)) != 0, sm_best[lane], sm_m[lane], 1.0 / sm_s[lane], p, q, (double)coin};
+    }
+    if (lane == 0) a.count[b] = __popcll(list);
+}
+
+// z of a node after its first (round 0) or second (1) child, by a whole wave.
+__device__ __forceinline__ double z_of(const AcArgs &a, int b, int node, int round) {
+    const double *from = a.left + (((int64_t)b * a.max_n + node) * 2 + round) * a.segs;
+    double z = 0.0;
+    for (int k = threadIdx.x & 63; k < a.segs; k += 64) z += from[k];
+    return lanes_add<64>(z);
+}
+
+template <int TY, int PT>
+__global__ void __launch_bounds__(AC_T) k_accept_left(AcArgs a, int round) {
+    __shared__ double sm_sum[AC_T / 64];
+    const int seg = blockIdx.x, b = blockIdx.z, count = a.count[b];
+    for (int i = blockIdx.y; i < count; i += gridDim.y) {
+        const AcAsk &k = a.asks[(int64_t)b * a.max_n + i];
+        const int node = k.node;
+        AcEnd e;
+        e.turned = 0, e.m = k.m, e.best = k.best, e.inv = k.inv, e.a = 1.0;
+        if (round) {
+            if (!k.more) continue;
+            const double z = z_of(a, b, node, 0);
+            if (k.coin * k.q * z < fmax(k.p - k.q, 0.0)) continue; // (as the walk decides)
+            e.a += z;
+        }
+        const double s = block_add(left_sum<TY, PT, true>(a, a.x + b * a.seq + node * a.row, a.q + b * a.p_seq + node * a.p_row, e, seg), sm_sum);
+        if (threadIdx.x == 0) a.left[(((int64_t)b * a.max_n + node) * 2 + round) * a.segs + seg] = s;
+    }
 }
 
 template <int TY, int PT> // PT: the type of the draft's probabilities, -1: none
@@ -327,34 +455,10 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
         return;
     }
     const uint8_t *const x = a.x + b * a.seq, *const q = PT >= 0 ? a.q + b * a.p_seq : nullptr;
-    // a lane a node, every wave alike; every load that depends on no other first
-    AcRow rows;
-    rows.load(a, b, min((int)threadIdx.x / 16, nn - 1), 0);
-    int parent = -1, token = -1;
-    float y = 0.0f, u = 0.0f;
-    double prob = 0.0;
-    if (lane < nn) {
-        u = a.coins[at0 + lane];
-        parent = a.parents ? a.parents[at0 + lane] : lane - 1;
-        token = a.tokens[at0 + lane];
-    }
-    if (lane == 0 || parent < 0 || parent >= lane) parent = -1;
-    if (lane == 0 || token < 0 || token >= a.vocab) token = -1;
-    if (parent >= 0 && token >= 0) {
-        y = at<TY>(x + parent * a.row, token);
-        if (PT >= 0) prob = (double)at<PQ>(q + parent * a.p_row, token);
-    }
-    for (int r = threadIdx.x / 16; r - (int)threadIdx.x / 16 < nn; r += AC_T / 16) {
-        float m;
-        int best;
-        double s;
-        rows.join(a, b, min(r, nn - 1), m, best, s);
-        if (r < nn && (threadIdx.x & 15) == 0) sm_m[r] = m, sm_best[r] = best, sm_s[r] = s;
-        rows.load(a, b, min(r + AC_T / 16, nn - 1), 0);
-    }
-    __syncthreads();
-    double p = 0.0;
-    if (parent >= 0 && token >= 0) p = weight_of(a, y, sm_m[parent], token, sm_best[parent]) / sm_s[parent];
+    const AcNode d = node_of<TY, PT>(a, b, nn, x, q, sm_m, sm_best, sm_s);
+    const int parent = d.parent, token = d.token;
+    const float y = d.y, u = d.u;
+    const double prob = d.q, p = d.p;
     if (seg == 0 && wave == 0 && lane > 0 && lane < a.max_n) {
         float lp = 0.0f;
         if (parent >= 0) {
@@ -402,7 +506,10 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
             continue;
         }
         aq += left;
-        if (open) { // another child to hold against what is left
+        const int round = __popcll(gone) - 1;
+        if (open && a.left && round < 2) { // another child to hold against what is left
+            left = z_of(a, b, node, round);
+        } else if (open) {
             const uint8_t *row = x + node * a.row, *probs = q + node * a.p_row;
             double s = 0.0;
             const double inv = 1.0 / sm_s[node];
@@ -441,8 +548,8 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     const uint8_t *const row = x + node * a.row, *const probs = PT >= 0 ? q + node * a.p_row : nullptr;
     // Sums of segments through the same code: the workgroup's own; of the sequence's last workgroup, where nothing is left, those of
     // the target's own row too.  The threads' shares are kept for the draw, which would else read the segment and sum it again (the
-    // walk of a chain of 8 fp32 rows: 15.7 us instead of 16.8, of sixteen
-    // trees of bf16 rows 21.8 instead of 24.5).
+    // walk of a chain of 6 fp32 rows: 15.7 us instead of 16.8, of 16 trees of bf16
+    // rows 21.8 instead of 24.5).
     double *const sums = a.sums + (int64_t)b * a.segs, *const shares = a.shares + (int64_t)b * a.segs * AC_T;
     // (through to where every XCD reads it)
     auto put = [](double *at, double v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
@@ -451,7 +558,7 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     int now = seg, rest = -1; // rest: the next segment of the target's own row
 #pragma unroll 1
     for (;;) {
-        const double share = left_sum<TY, PT>(a, row, probs, end, now), all_s = block_add(share, sm_sum);
+        const double share = left_sum<TY, PT, false>(a, row, probs, end, now), all_s = block_add(share, sm_sum);
         put(&shares[now * AC_T + threadIdx.x], share);
         if (threadIdx.x == 0) put(&sums[now], all_s);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (there before it is counted)
@@ -525,7 +632,7 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
         float qi = 0.0f;
         if (PT >= 0) qi = at<PQ>(probs, i);
         double one[1];
-        left_of<PT>(a, end, &value, &qi, i, one);
+        left_of<PT, false>(a, end, &value, &qi, i, one);
         w = one[0];
     }
     const double sum = upto(w);
@@ -548,7 +655,8 @@ int64_t ac_segs(int vocab) { return ((int64_t)vocab + AC_SEG - 1) / AC_SEG; }
 extern "C" size_t llm_draft_accept_work(int n_seq, int max_n, int vocab) {
     if (n_seq < 1 || max_n < 1 || max_n > AC_N || vocab < 1) return 0;
     const size_t segs = ac_segs(vocab);
-    return (size_t)n_seq * (max_n * segs * sizeof(AcPart) + segs * (1 + AC_T) * sizeof(double) + sizeof(int));
+    return (size_t)n_seq * (max_n * (segs * (sizeof(AcPart) + 2 * sizeof(double)) + sizeof(AcAsk)) +
+                            segs * (1 + AC_T) * sizeof(double) + 2 * sizeof(int));
 }
 
 extern "C" int llm_draft_accept(const void *logits, int type, int n_seq, int max_n, int vocab, int64_t seq, int64_t row,
@@ -591,7 +699,11 @@ extern "C" int llm_draft_accept(const void *logits, int type, int n_seq, int max
     a.part = (AcPart *)work;
     a.sums = (double *)(a.part + (size_t)n_seq * max_n * a.segs);
     a.shares = a.sums + (size_t)n_seq * a.segs;
-    a.done = (int *)(a.shares + (size_t)n_seq * a.segs * AC_T);
+    a.asks = (AcAsk *)(a.shares + (size_t)n_seq * a.segs * AC_T);
+    double *const z = (double *)(a.asks + (size_t)n_seq * max_n);
+    a.done = (int *)(z + (size_t)n_seq * max_n * 2 * a.segs);
+    a.count = a.done + n_seq;
+    if (probs && parents && max_n > 2 && vocab >= AC_ASK) a.left = z;
     hipStream_t st = (hipStream_t)stream;
     void (*rows)(AcArgs) = nullptr;
 #define ACCEPT_PICK(T, P, X) \
@@ -601,13 +713,21 @@ extern "C" int llm_draft_accept(const void *logits, int type, int n_seq, int max
 #undef ACCEPT_PICK
     hipLaunchKernelGGL(rows, dim3(a.parts, max_n, n_seq), dim3(AC_T), 0, st, a);
     HIP_OR_FAIL(who, hipGetLastError());
-    void (*walk)(AcArgs) = nullptr;
+    void (*walk)(AcArgs) = nullptr, (*ask)(AcArgs) = nullptr, (*sum)(AcArgs, int) = nullptr;
     const int pt = probs ? p_type : -1;
 #define ACCEPT_PICK(T, P) \
-    if (type == T && pt == P) walk = k_accept_walk<T, P>;
-    ACCEPT_PICK(LLM_F32, -1) ACCEPT_PICK(LLM_F32, LLM_F32) ACCEPT_PICK(LLM_F32, LLM_BF16)
-    ACCEPT_PICK(LLM_BF16, -1) ACCEPT_PICK(LLM_BF16, LLM_F32) ACCEPT_PICK(LLM_BF16, LLM_BF16)
+    if (type == T && pt == P) ask = k_accept_ask<T, P>, sum = k_accept_left<T, P>, walk = k_accept_walk<T, P>;
+    ACCEPT_PICK(LLM_F32, LLM_F32) ACCEPT_PICK(LLM_F32, LLM_BF16) ACCEPT_PICK(LLM_BF16, LLM_F32) ACCEPT_PICK(LLM_BF16, LLM_BF16)
 #undef ACCEPT_PICK
+    if (pt < 0) walk = type == LLM_F32 ? k_accept_walk<LLM_F32, -1> : k_accept_walk<LLM_BF16, -1>;
+    if (a.left) {
+        hipLaunchKernelGGL(ask, dim3(n_seq), dim3(AC_T), 0, st, a);
+        HIP_OR_FAIL(who, hipGetLastError());
+        for (int round = 0; round < (max_n > 3 ? 2 : 1); round++) {
+            hipLaunchKernelGGL(sum, dim3(a.segs, std::min(max_n / 2, 4), n_seq), dim3(AC_T), 0, st, a, round);
+            HIP_OR_FAIL(who, hipGetLastError());
+        }
+    }
     hipLaunchKernelGGL(walk, dim3(a.segs, n_seq), dim3(AC_T), 0, st, a);
     HIP_OR_FAIL(who, hipGetLastError());
     return 0;

@@ -177,3 +177,24 @@ def test_random_trees():
                       hot=r.choice([0.3, 2.0, 8.0]), noise=r.choice([0.1, 1.0]))
         temperature = r.choice([1.0, 0.3, 2.0, 0.0, 1e-30, 1e30])
         check(*args, None, temperature, run(*args, None, temperature))
+
+
+@pytest.mark.parametrize("kind,draft", [("fp32", "fp32"), ("bf16", "fp32"), ("fp32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("v", [5003, 16383, 16384, 20485])
+@pytest.mark.parametrize("t,wide", [(3, 2), (4, 3), (20, 3), (64, 7)])
+def test_many_children(kind, draft, v, t, wide):
+    """up to seven children of a node, most of them turned down, some without a token or twice the same one"""
+    g, b = gen(v + t + wide), 6
+    x = (torch.randn(b, t, v, generator=g) * 2.0).to(ROWS[kind])
+    q = torch.softmax(x.float() * torch.linspace(0.0, 1.0, b)[:, None, None] + 2.0 * torch.randn(b, t, v, generator=g), -1).to(ROWS[draft])
+    parents = [[-1] + [i // wide for i in range(t - 1)] for _ in range(b)]
+    tokens = torch.zeros(b, t, dtype=torch.int32)
+    for i in range(b):
+        for j in range(1, t):
+            tokens[i, j] = int(torch.multinomial(q[i, parents[i][j]].float(), 1, generator=g))
+    tokens[2, 1], tokens[3, 2] = -1, tokens[3, 1]
+    parents[4][t - 1] = -1
+    coins = torch.rand(b, t, generator=g)
+    n = [t, t, t, t, t, t - 1]
+    for temperature in (1.0, 0.6, 0.0):
+        check(x, q, tokens, parents, coins, n, temperature, run(x, q, tokens, parents, coins, n, temperature))
