@@ -551,7 +551,7 @@ def page_reserve(k, v, k_scale, v_scale, table, refs, lens, n, max_n=None):
     _no_grad(k_scale, v_scale)
     c, (_, pages, _, page, _) = _pages(k, v, k_scale, v_scale)
     (at, (b, per)), torch, L = _table(table), _torch[0], lib()
-    most = per * page if max_n is None else max_n
+    most = per * page if max_n is None else min(max_n, per * page)
     need = L.llm_page_reserve_work(c, b, per, most)
     work = torch.empty(need, dtype=torch.uint8, device=k.device)
     result = torch.empty(2, dtype=torch.int32, device=k.device)

@@ -3,6 +3,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "device.h"
 #include "operators.h"
@@ -235,8 +236,8 @@ __global__ void __launch_bounds__(256) k_page_read(RowArgs a) {
 
 int page_rows(const char *who, bool write, const llm_pages *c, const llm_rows *k, const llm_rows *v, int n_seq, const int *table,
               int per, const int *refs, const int *pos, const int *n, const int *path, int max_n, int zero_rest, void *stream) {
-    if (!c || !k || !v || max_n < 0) {
-        fprintf(stderr, "%s: bad arguments\n", who);
+    if (!c || !k || !v || max_n < 0 || max_n > 1 << 30) { // (more than a table's positions)
+        fprintf(stderr, "%s: bad arguments (%d rows a sequence)\n", who, max_n);
         return -1;
     }
     if (!op_check_pages(c, nullptr, who) || !op_check_table(table, n_seq, per, nullptr, who)) return -1;
@@ -609,11 +610,18 @@ bool op_check_pages(const llm_pages *c, OpDevice *dev, const char *who) {
                 c->type, c->n_layers, c->n_pages, c->n_kv, c->hs, c->page);
         return false;
     }
-    const int64_t codes = (int64_t)c->page * c->hs, scales = c->page / PAGE_BLOCK;
-    // (of one there is no next)
-    auto near = [](int count, int64_t stride, int64_t least) { return count > 1 && stride < least; };
-    if (near(c->n_layers, c->layer, codes) || near(c->n_pages, c->id, codes) || near(c->n_kv, c->head, codes) ||
-        near(c->n_layers, c->s_layer, scales) || near(c->n_pages, c->s_id, scales) || near(c->n_kv, c->s_head, scales)) {
+    // layers, pages and heads in the order of their strides: each lies behind what the ones before it take (of one there is no next)
+    auto apart = [&](int64_t least, int64_t layer, int64_t id, int64_t head) {
+        std::pair<int64_t, int> dim[] = {{layer, c->n_layers}, {id, c->n_pages}, {head, c->n_kv}};
+        std::sort(dim, dim + 3);
+        __int128 extent = least;
+        for (auto [stride, count] : dim) {
+            if (count > 1 && stride < extent) return false;
+            extent += (__int128)(count - 1) * stride;
+        }
+        return true;
+    };
+    if (!apart((int64_t)c->page * c->hs, c->layer, c->id, c->head) || !apart(c->page / PAGE_BLOCK, c->s_layer, c->s_id, c->s_head)) {
         fprintf(stderr, "%s: strides of the pages that lie on themselves\n", who);
         return false;
     }

@@ -103,6 +103,32 @@ def test_arguments_refused(capfd):
     assert capfd.readouterr().err.count("not device memory") == 2
 
 
+def test_more_rows_than_there_are_positions_refused(capfd):
+    """counts whose rounding up to blocks would pass an int"""
+    for n in ((1 << 30) + 1, 0x7fffffff):
+        assert write(pages(), n=n) == -1 and read(pages(), n=n) == -1
+        assert capfd.readouterr().err.count("bad arguments") == 2
+    assert write(pages(), n=1 << 30) == -1
+    assert "not device memory" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("layer,id,head,fine", [
+    (64 * 4096, 2 * 4096, 4096, True),           # [layers][pages][heads]
+    (4096, 2 * 3 * 4096, 3 * 4096, True),        # [pages][heads][layers]
+    (16 * 4096, 4096, 8 * 4096, True),           # heads before pages
+    (2 * 4096, 6 * 4096, 4096, True),            # layers between
+    (4096, 2 * 4096, 4096, False),               # layers on heads
+    (64 * 4096, 4096, 4096, False),              # pages on heads
+    (7 * 2 * 4096, 2 * 4096, 4096, False),       # the last page on the next layer's first
+    (64 * 4096, 4096, 7 * 4096, False),          # the last page of a head on the next head's first
+    (1 << 62, 1 << 61, 1 << 60, False)])         # eight pages 2^61 apart reach past 2^62; their sum passes 64 bits
+def test_pools_that_lie_on_themselves_refused(layer, id, head, fine, capfd):
+    """three layers of eight pages of two heads"""
+    c = pages(n_layers=3, layer=layer, id=id, head=head, s_layer=100, s_id=4, s_head=1)
+    assert write(c) == -1
+    assert ("not device memory" if fine else "lie on themselves") in capfd.readouterr().err
+
+
 def test_nothing_to_do():
     assert fork(count=0) == 0 and fork(seqs=0) == 0 and accept(seqs=0) == 0 and accept(n=0) == 0
 
