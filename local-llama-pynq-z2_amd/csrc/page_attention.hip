@@ -20,9 +20,10 @@ struct PagePlan {
 // How a call is cut.  Times: one call, heads of 128, int8 pages.
 // Rows.  The four waves of a workgroup share the positions, with one tile of 16 rows, or two where that is work enough: two read
 // and convert the codes half as often, one gives twice the workgroups (448 rows of bf16 over 4 x 8000 positions, 4 kv heads: 72
-// us with one, 61 with two; 259 of fp32 over 12k: 38 and 46).  Many rows over long contexts: the waves have two other tiles each of
-// the same positions, which need no join of waves, and whose pages the L1 then holds for all four (448 rows over eight sequences
-// of up to 16k: 128 us and 117; fp32 over two of 16k: 108 and 85, over eight of 3000: 62 and 63).
+// us with one, 61 with two; 259 over 12k: bf16 38.4 and 34.4, fp32 41.2 and 40.7, over 6k 27.0 and 29.5, 29.4 and 30.8).  Many
+// rows over long contexts: the waves have two other tiles each of the same positions, which need no join of waves, and whose pages
+// the L1 then holds for all four (448 rows over eight sequences of up to 16k: 128 us and 117; fp32 over two of 16k: 108 and 85,
+// over eight of 3000: 62 and 63).
 // Positions.  One sequence: as many slices as give a workgroup a CU, or two a CU where whole row blocks would leave much of the
 // chip idle.  Several: two workgroups a CU over all sequences, of equal steps (more of them cost more in find_slice and the join
 // than they even out: 32 decode steps over 0 to 8190 e4m3 positions 32 us, with four a CU 38).
@@ -32,7 +33,7 @@ PagePlan page_plan(const llm_pages *c, int n_seq, int n_heads, int max_n, int ma
     const int group = n_heads / c->n_kv, rows = group * max_n, tiles = (rows + 15) / 16;
     const int64_t heads = (int64_t)n_seq * c->n_kv, blocks = ((int64_t)std::max(max_len, 0) + PAGE_BLOCK - 1) / PAGE_BLOCK;
     const double work = p.hsp <= 128 && tiles > 1 ? (double)tiles * heads * blocks * p.hsp : 0.0;
-    p.tiles = work >= 2e6 ? 2 : 1;
+    p.tiles = work >= (n_seq > 1 ? 2e6 : 1.6e6) ? 2 : 1; // (of several sequences most are shorter than max_len)
     p.rows = work >= 6e6 && tiles > 8;
     p.block_rows = 16 * p.tiles * (p.rows ? 4 : 1);
     p.row_blocks = (rows + p.block_rows - 1) / p.block_rows;

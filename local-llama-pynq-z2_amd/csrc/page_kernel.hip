@@ -176,7 +176,7 @@ __device__ __forceinline__ bool place(const PageArgs &a, int block_rows, Place &
         a.plan[p.b * a.n_kv + p.h] = make_int2((int)id, p.slices);
     p.nn = a.n ? min(max(a.n[p.b], 0), a.max_n) : a.max_n;
     p.rows = p.nn * a.group;
-    if (a.zero_rest && p.split == 0 && p.row0 + block_rows > p.rows) // the rows behind the last token
+    if (a.zero_rest && p.split == 0 && p.rows < a.max_n * a.group && p.row0 + block_rows > p.rows) // the rows behind the last token
         for (int e = threadIdx.x * 4; e < block_rows * a.hs; e += 1024) {
             const int row = p.row0 + e / a.hs, t = row / a.group, d = e % a.hs;
             if (row >= p.rows && row < a.max_n * a.group)
@@ -218,14 +218,12 @@ __device__ __forceinline__ void put_row(const PageArgs &a, const Place &p, int r
 }
 
 // The new tokens' own rows, all in fp32: tiles of 16 tokens, from `first` on every `stride`-th.  A tile's K and V values are
-// loaded while the one before is worked on; what is not there reads a row that is.
-template <int QT>
+// loaded while the one before is worked on; what is not there reads a row that is.  EARLY: the first one's before it is known
+// whether the rows see it (one decode step of heads of 128 over 200 positions: 9.6 us instead of 10.6; two tiles would spill).
+template <int QT, bool EARLY>
 __device__ __forceinline__ void new_rows(const PageArgs &a, const Place &p, int first, int stride, const uint8_t *qp, bool ok, int tok,
                                          State &st) {
     const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4, nn = p.nn, tiles = (nn + 15) / 16;
-    uint64_t sees = 0;
-    if (ok) sees = a.mask ? a.mask[(int64_t)p.b * a.max_n + tok] : ~(uint64_t)0 >> (63 - tok);
-    if (nn < 64) sees &= ((uint64_t)1 << nn) - 1;
     const uint8_t *const kp = a.kr + p.b * a.k_seq + p.h * a.k_head, *const vp = a.vr + p.b * a.v_seq + p.h * a.v_head;
     const int part = a.hs / 4; // dimension part * j + 4 s + i is term j of product 4 s + i
     const float c = a.c * a.sign;
@@ -237,11 +235,27 @@ __device__ __forceinline__ void new_rows(const PageArgs &a, const Place &p, int 
         for (int s = 0; s < HSP / 16; s++) kx[s] = load4<QT>(krow, part * j + (4 * s < part ? 4 * s : 0));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
+            if (16 * t + i >= nn) break; // (tokens 16 t + 4 j + i, of all lane groups)
             const uint8_t *const vrow = vp + min(16 * t + 4 * j + i, nn - 1) * a.v_tok;
 #pragma unroll
             for (int d = 0; d < DT; d++) v[i][d] = load1<QT>(vrow, (16 * d < a.hs ? 16 * d : 0) + n);
         }
     };
+    auto load_q = [&] {
+#pragma unroll
+        for (int s = 0; s < HSP / 16; s++) {
+            qx[s] = load4<QT>(qp, part * j + (4 * s < part ? 4 * s : 0));
+            if (!ok || 4 * s >= part) qx[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+    if (first >= tiles) return;
+    if (EARLY) {
+        load(first);
+        load_q();
+    }
+    uint64_t sees = 0;
+    if (ok) sees = a.mask ? a.mask[(int64_t)p.b * a.max_n + tok] : ~(uint64_t)0 >> (63 - tok);
+    if (nn < 64) sees &= ((uint64_t)1 << nn) - 1;
     // (tiles of which no row sees a token are left out)
     auto next = [&](int t) {
         while (t < tiles && !__any((int)(sees >> 16 * t) & 0xffff)) t += stride;
@@ -249,12 +263,8 @@ __device__ __forceinline__ void new_rows(const PageArgs &a, const Place &p, int 
     };
     int t = next(first);
     if (t >= tiles) return;
-    load(t);
-#pragma unroll
-    for (int s = 0; s < HSP / 16; s++) {
-        qx[s] = load4<QT>(qp, part * j + (4 * s < part ? 4 * s : 0));
-        if (!ok || 4 * s >= part) qx[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
+    if (!EARLY || t != first) load(t);
+    if (!EARLY) load_q();
     for (;;) {
         f32x4 y[4];
 #pragma unroll
@@ -288,10 +298,12 @@ __device__ __forceinline__ void new_rows(const PageArgs &a, const Place &p, int 
         bool nf[4] = {false, false, false, false};
         f32x4 z[DT];
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            z[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int d = 0; d < DT; d++) z[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 4; i++) { // a value that is not finite is zero here
+        for (int i = 0; i < 4; i++) {
+            if (16 * t + i >= nn) break;
+#pragma unroll
+            for (int d = 0; d < DT; d++) { // a value that is not finite is zero here
                 const bool bad = !(fabsf(v[i][d]) < INFINITY);
                 nf[i] |= bad;
                 z[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 0.0f : v[i][d], x[i], z[d], 0, 0, 0);
@@ -410,7 +422,22 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
     };
     int step = p.first + (ROWS ? 0 : wave);
     int page = page_of(step), next = page_of(step + STRIDE);
+    // of row `row` of the wave's tile r, as they lie (what is not there reads the row's start: no load waits behind a condition)
+    float x[2 * KL][8];
+    auto load_q = [&](int r) {
+        const int row = row0 + 16 * r + n, tok = row / a.group;
+        const uint8_t *const qp = a.q + p.b * a.q_seq + (row < p.rows ? tok * a.q_tok + (p.h * a.group + row - tok * a.group) * a.q_head : 0);
+#pragma unroll
+        for (int s = 0; s < 2 * KL; s++)
+#pragma unroll
+            for (int q4 = 0; q4 < 2; q4++) {
+                const int d = 64 * (s / 2) + 16 * j + 8 * (s % 2) + 4 * q4;
+                const float4 y = load4<QT>(qp, d < a.hs ? d : 0);
+                x[s][4 * q4] = y.x, x[s][4 * q4 + 1] = y.y, x[s][4 * q4 + 2] = y.z, x[s][4 * q4 + 3] = y.w;
+            }
+    };
     if (R == 1) { // (with more rows their queries' values take the registers)
+        load_q(0);
         load_k(step, page);
         load_v(step, page);
     }
@@ -424,18 +451,9 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
     float off[R], bias[R]; // what scores and values of biased codes have too much: 128 times a query's sum, and the weights'
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const int row = row0 + 16 * r + n, tok = row / a.group;
-        const bool ok = row < p.rows;
-        const uint8_t *const qp = a.q + p.b * a.q_seq + (ok ? tok * a.q_tok + (p.h * a.group + row - tok * a.group) * a.q_head : 0);
-        float x[2 * KL][8], mx = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 2 * KL; s++)
-#pragma unroll
-            for (int q4 = 0; q4 < 2; q4++) { // (what is not there reads the row's start: no load waits behind a condition)
-                const int d = 64 * (s / 2) + 16 * j + 8 * (s % 2) + 4 * q4;
-                const float4 y = load4<QT>(qp, d < a.hs ? d : 0);
-                x[s][4 * q4] = y.x, x[s][4 * q4 + 1] = y.y, x[s][4 * q4 + 2] = y.z, x[s][4 * q4 + 3] = y.w;
-            }
+        const bool ok = row0 + 16 * r + n < p.rows;
+        float mx = 0.0f;
+        if (R > 1) load_q(r);
 #pragma unroll
         for (int s = 0; s < 2 * KL; s++)
 #pragma unroll
@@ -601,7 +619,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
         const uint8_t *const qp = a.q + p.b * a.q_seq + (ok ? tok * a.q_tok + (p.h * a.group + row - tok * a.group) * a.q_head : 0);
         if (!p.fresh || row0 + 16 * r >= p.rows) break;
         if (R > 1) park(st[R - 1 - r], true); // (the other tile's sums out of the way, over the queries)
-        new_rows<QT>(a, p, ROWS ? 0 : (wave - (p.last - p.first)) & 3, ROWS ? 1 : 4, qp, ok, tok, st[r]);
+        new_rows<QT, R == 1>(a, p, ROWS ? 0 : (wave - (p.last - p.first)) & 3, ROWS ? 1 : 4, qp, ok, tok, st[r]);
         if (R > 1) park(st[R - 1 - r], false);
     }
     if constexpr (!ROWS) { // the four waves' sums joined: each scaled to a common exponent, waves 2 and 3 into 0 and 1, then 1 into 0
