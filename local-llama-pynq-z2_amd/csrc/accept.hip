@@ -11,12 +11,12 @@
 // Sums and exponentials that decide are in 64 bits: a token drawn in the tail of 150k stands between borders 1e-6 apart, which an
 // error of 2^-24 in the likeliest token's weight would all move by 6e-8.
 //
-// What bounds it: the rows' bytes, read once.  16 trees of up to 37 rows of 151936 bf16 logits, 154 MB: 26.5 us, 5.8 TB/s, for the rows (the
-// last call left a part of them in the caches) and 21.8 for the walk; a chain of 6 fp32 rows with draft probabilities: 4.3 and 15.7.
-// The walk is a chain of short steps (of that chain, in thousands of cycles: the parts' loads 2.7, the join 2.6, the tokens'
-// probabilities 1, the walk 1.7, a segment's sum 8.6, the count 1.5, the choice of a segment 3, of a token 13), each code that runs
-// once: fetching it is a good part of the time.  Trees with draft probabilities need a row's pass for each child with a later sibling that
-// is turned down: see k_accept_ask.
+// What bounds it: the rows' bytes, read once.  16 trees of up to 37 rows of 151936 bf16 logits, 154 MB: 26.5 us, 5.8 TB/s, for
+// the rows (the last call left a part of them in the caches) and 21.8 for the walk; a chain of 6 fp32 rows with draft
+// probabilities: 4.3 and 15.7.  The walk is a chain of short steps (of that chain, in thousands of cycles: the parts' loads 2.7,
+// the join 2.6, the tokens' probabilities 1, the walk 1.7, a segment's sum 8.6, the count 1.5, the choice of a segment 3, of a
+// token 13), each code that runs once: fetching it is a good part of the time.  Trees with draft probabilities need a row's pass
+// for each child with a later sibling that is turned down: see k_accept_ask.
 #include <string.h>
 
 #include <algorithm>
@@ -28,9 +28,9 @@ namespace {
 
 constexpr int AC_T = 256, AC_E = 16, AC_SEG = AC_T * AC_E; // values of a segment
 constexpr int AC_N = 64;                                   // most nodes: a lane each
-// Least vocabulary for k_accept_ask and k_accept_left, three launches of 7 us together: a single tree of 20 nodes over 32000 logits
-// 27 us with them and 19 (nothing is asked for) or 36 without, over 151936 33 and 95, 16 trees of 37 over 8192 logits 38 and 28, over
-// 16384 43 and 40, over 32000 60 and 79, over 151936 117 and 290 (all fp32).
+// Least vocabulary for k_accept_ask and k_accept_left, three launches of 7 us together: a single tree of 20 nodes over 32000
+// logits 27 us with them and 19 (nothing is asked for) or 36 without, over 151936 33 and 95, 16 trees of 37 over 8192 logits 38
+// and 28, over 16384 43 and 40, over 32000 60 and 79, over 151936 117 and 290 (all fp32).
 constexpr int AC_ASK = 16384;
 
 struct AcPart { // of a part of a row: largest value, its first place (temperature 0), sum relative to it
@@ -283,9 +283,10 @@ __device__ __forceinline__ void left_of(const AcArgs &a, const AcEnd &e, const f
             for (int k = 0; k < N; k++) w[k] = at == k ? 0.0 : w[k];
         }
 }
-// Its sum over the thread's AC_E neighbouring values of a segment, in order.  All loads go out first; the weights are a loop of four
-// at a time, whose values move up: straight code, and no more of it than is run often enough to have been worth fetching (the walk of
-// sixteen trees over 151936 bf16 logits: 24.5 us; 28.7 with sixteen values in a row and branches for their masks and borders).
+// Its sum over the thread's AC_E neighbouring values of a segment, in order.  All loads go out first; the weights are a loop of
+// four at a time, whose values move up: straight code, and no more of it than is run often enough to have been worth fetching
+// (the walk of sixteen trees over 151936 bf16 logits: 24.5 us; 28.7 with sixteen values in a row and branches for their masks and
+// borders).
 template <int TY, int PT, bool Z>
 __device__ __forceinline__ double left_sum(const AcArgs &a, const uint8_t *row, const uint8_t *probs, const AcEnd &e, int seg) {
     constexpr int PQ = PT < 0 ? LLM_F32 : PT;
@@ -363,11 +364,11 @@ __device__ __forceinline__ AcNode node_of(const AcArgs &a, int b, int nn, const 
     return d;
 }
 
-// What was turned down of trees with draft probabilities changes what is left of its parent's row by the number of children alone:
-// after the first a is 1, after the second 1 + z.  A pass over a row within the walk is every workgroup's own; so z of every row that
-// the walk may need it of is summed before, a workgroup a segment: k_accept_ask lists the nodes that may be reached, whose first
-// child is turned down and not the last, k_accept_left sums what is left after the first child and, launched again, after the second.
-// Third children's are left to the walk.
+// What was turned down of trees with draft probabilities changes what is left of its parent's row by the number of children
+// alone: after the first a is 1, after the second 1 + z.  A pass over a row within the walk is every workgroup's own; so z of
+// every row that the walk may need it of is summed before, a workgroup a segment: k_accept_ask lists the nodes that may be
+// reached, whose first child is turned down and not the last, k_accept_left sums what is left after the first child and, launched
+// again, after the second.  Third children's are left to the walk.
 template <int TY, int PT>
 __global__ void __launch_bounds__(AC_T) k_accept_ask(AcArgs a) {
     __shared__ float sm_m[AC_N];
@@ -546,10 +547,9 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     }
     __syncthreads();
     const uint8_t *const row = x + node * a.row, *const probs = PT >= 0 ? q + node * a.p_row : nullptr;
-    // Sums of segments through the same code: the workgroup's own; of the sequence's last workgroup, where nothing is left, those of
-    // the target's own row too.  The threads' shares are kept for the draw, which would else read the segment and sum it again (the
-    // walk of a chain of 6 fp32 rows: 15.7 us instead of 16.8, of 16 trees of bf16
-    // rows 21.8 instead of 24.5).
+    // Sums of segments through the same code: the workgroup's own; of the sequence's last workgroup, where nothing is left, those
+    // of the target's own row too.  The threads' shares are kept for the draw, which would else read the segment and sum it again
+    // (the walk of a chain of 6 fp32 rows: 15.7 us instead of 16.8, of 16 trees of bf16 rows 21.8 instead of 24.5).
     double *const sums = a.sums + (int64_t)b * a.segs, *const shares = a.shares + (int64_t)b * a.segs * AC_T;
     // (through to where every XCD reads it)
     auto put = [](double *at, double v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
