@@ -135,10 +135,11 @@ struct State {
     float m, l;
     f32x4 o[DT];
 };
-// What takes the sums so far (f) and a step whose weights are relative to ms (g) to a common exponent.  It stays as it is until a step
-// is 2^8 above it, which few are: fp32 sums have that room, and the factor 1 is not multiplied by.
+// What takes the sums so far (f) and a step whose weights are relative to ms (g) to a common exponent.  It is set so that the step's
+// largest weight, 2^15, counts as 2^-8, and stays until one would count as more than 1: few steps do, and the factor 1 is not
+// multiplied by.  (Sums of weights up to 1 overflow where the values' own would.)
 __device__ __forceinline__ void join(State &s, float ms, float &f, float &g) {
-    const float mn = ms > s.m + 8.0f ? ms : s.m, mu = mn == -INFINITY ? 0.0f : mn;
+    const float mn = ms > s.m - 15.0f ? ms + 23.0f : s.m, mu = mn == -INFINITY ? 0.0f : mn;
     f = __builtin_amdgcn_exp2f(s.m - mu);
     g = __builtin_amdgcn_exp2f(ms - mu);
     s.m = mn;

@@ -89,7 +89,7 @@ def check(pool, table, q, kn, vn, lens, n, mask, scale, got, layer=0):
 
 
 def case(cache, rows, heads, h, hs, page, lens, t, n=None, masked=True, layout="plain", scale=None, own=True, seed=0, bad=False,
-         spread=1.0, k_spread=None, max_len=None, spare=0):
+         spread=1.0, k_spread=None, max_len=None, spare=0, v_top=1.0):
     g, r = gen(seed + hs + t), random.Random(seed)
     b = len(lens)
     per = -(-max(max(lens), 1) // page) + spare
@@ -97,11 +97,13 @@ def case(cache, rows, heads, h, hs, page, lens, t, n=None, masked=True, layout="
     pool = Pool(2, pages, h, page, hs, cache, g)
     for s, by in zip(pool.scale, (spread if k_spread is None else k_spread, spread)):
         s *= torch.exp(by * torch.randn(s.shape, generator=g))
+    pool.scale[1] *= v_top
     ids = torch.randperm(pages, generator=g).tolist()
     table = [[ids[i * per + j] if j * page < lens[i] else -1 for j in range(per)] for i in range(b)]
     q = torch.randn(b, t, heads, hs, generator=g).to(ROWS[rows])
     kn, vn = ((torch.randn(b, t, h, hs, generator=g) * torch.exp(torch.randn(b, t, h, 1, generator=g))).to(ROWS[rows])
               for _ in range(2))
+    vn = (vn.float() * v_top).to(ROWS[rows])
     mask = tree_masks(r, b, t) if masked else None
     nn = [t] * b if n is None else n
     tensors = pool.tensors(layout)
@@ -167,6 +169,15 @@ def test_tokens_without_rows_of_their_own(cache, rows):
 def test_scales(cache, scale):
     case(cache, "fp32", 4, 2, 64, 64, [130, 5], 3, scale=scale)
     case(cache, "bf16", 4, 2, 64, 64, [130, 5], 3, scale=scale)
+
+
+@pytest.mark.parametrize("v_top", [2.0 ** 110, 2.0 ** -100])
+@pytest.mark.parametrize("cache,rows", [("int8", "fp32"), ("int8", "bf16"), ("e4m3", "fp32"), ("e4m3", "bf16")])
+def test_values_near_the_ends_of_fp32(cache, rows, v_top):
+    """values up to about 2^110 (their scale 2^110, 0.02 and the codes), whose sums with weights up to 1 stay below 2^127"""
+    case(cache, rows, 4, 2, 64, 64, [700, 64, 3], 3, spread=0.0, v_top=v_top)
+    if v_top > 1.0:
+        case(cache, rows, 28, 4, 128, 64, [9000], 33, spread=0.0, v_top=v_top)
 
 
 @pytest.mark.parametrize("spread", [6.0, 20.0])
