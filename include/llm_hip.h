@@ -256,7 +256,7 @@ int llm_logprobs(const void *logits, int type, int rows, int vocab, int64_t stri
  * table: n_seq rows of `per` page numbers (contiguous ints); entry j of a row is the page of positions j * page and on, and a number
  * outside 0 .. n_pages - 1 is none.  refs: for each page in how many places the tables have it; 0: free.  The calls that change
  * tables keep refs right; what refs and tables that contradict each other lead to is not said, but that no memory outside the
- * arrays is touched. */
+ * arrays is touched.  A call's work memory is its own until it has run. */
 typedef struct {
     void *k, *v;
     float *k_scale, *v_scale;
