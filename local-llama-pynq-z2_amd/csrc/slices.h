@@ -17,6 +17,17 @@ __device__ __forceinline__ int slices_of_one(const A &a, int all, int &steps) {
     return (all + steps - 1) / steps;
 }
 
+// Inclusive sum over a wave: within rows of 16 lanes, then of the rows before (DPP: row_shr 1, 2, 4, 8, row_bcast 15, 31).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // The slice `id`: its sequence, kv head and number there, the slices of that head and their steps.  A sequence of n steps
 // has ceil(n / q) slices a head, the same q for all, so that long sequences do not outlast the others; q is about the least
 // at which there are no more than a.cap in all.  Every block finds it from the lengths.
@@ -46,34 +57,43 @@ __device__ __forceinline__ bool find_slice(const A &a, uint32_t id, P &p, int &s
     const int guess = __builtin_amdgcn_readfirstlane((int)(wave_sum(sum) * kv / (float)a.cap));
     const int longest = __builtin_amdgcn_readfirstlane((int)wave_max(most));
     steps = longest <= WHOLE_STEPS * a.least ? longest : max(max(a.least, guess), longest / a.each + 1);
-    int n[GROUPS];
-    for (;; steps += (steps + 15) / 16) { // (ends: at the longest sequence's steps there is a slice a head)
-        float total = 0.0f;
+    // Four lengths at once, each a sixteenth above the one before, whose chains of instructions overlap; the first at which there
+    // are few enough slices (32 sequences: 3.7k cycles for the whole function; 5.5k one after another, with the scan through LDS).
+    constexpr int AT_ONCE = 4;
+    for (bool fits = false; !fits;) { // (ends: at the longest sequence's steps there is a slice a head)
+        int q[AT_ONCE];
+        float total[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < GROUPS; i++) {
-            n[i] = 0;
-            if (64 * i < a.n_seq) {
-                n[i] = (all[i] + steps - 1) / steps;
-                total += (float)n[i];
-            }
+        for (int u = 0; u < AT_ONCE; u++) {
+            q[u] = u ? q[u - 1] + (q[u - 1] + 15) / 16 : steps;
+            total[u] = 0.0f;
         }
-        if (wave_sum(total) * kv <= (float)a.cap) break; // (exact up to 2^24)
+#pragma unroll
+        for (int i = 0; i < GROUPS; i++)
+            if (64 * i < a.n_seq)
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; u++) total[u] += (float)((all[i] + q[u] - 1) / q[u]);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) total[u] = wave_sum(total[u]) * kv; // (exact up to 2^24)
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+            if (!fits) {
+                steps = q[u];
+                fits = total[u] <= (float)a.cap;
+            }
+        if (!fits) steps += (steps + 15) / 16;
     }
+    steps = __builtin_amdgcn_readfirstlane(steps);
     int before = 0; // slices of a head of the sequences before
 #pragma unroll
     for (int i = 0; i < GROUPS; i++)
         if (64 * i < a.n_seq) {
-            int upto = n[i];
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int x = __shfl_up(upto, off);
-                upto += lane >= off ? x : 0;
-            }
+            const int n = (all[i] + steps - 1) / steps, upto = wave_scan(n);
             const int passed = __popcll(__ballot((before + upto) * a.n_kv <= (int)id));
             if (passed < 64) { // (a lane without a sequence has passed none that its neighbours have not)
                 const int at = __builtin_amdgcn_readfirstlane(passed);
                 p.b = 64 * i + at;
-                p.slices = __builtin_amdgcn_readlane(n[i], at);
+                p.slices = __builtin_amdgcn_readlane(n, at);
                 const int rest = (int)id - (before + __builtin_amdgcn_readlane(upto, at) - p.slices) * a.n_kv;
                 p.h = rest / p.slices;
                 p.split = rest - p.h * p.slices;
