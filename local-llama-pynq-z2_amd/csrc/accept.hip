@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     __shared__ int sm_best[AC_N];
     __shared__ double sm_s[AC_N], sm_sum[AC_T / 64], sm_before, sm_point;
     __shared__ AcEnd end;
-    __shared__ int sm_seg, sm_at, sm_end, sm_last;
+    __shared__ int sm_seg, sm_at[AC_T / 64], sm_end[AC_T / 64], sm_last;
     const int seg = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x / 64, nn = nodes(a, b);
     const int64_t at0 = (int64_t)b * a.max_n;
     if (nn == 0) {
@@ -598,7 +598,6 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
                 sm_seg = found >= 0 ? found : last;
                 sm_before = found >= 0 ? start : last_start;
                 sm_point = point;
-                sm_at = 0x7fffffff, sm_end = -1;
             }
         }
         __syncthreads();
@@ -616,10 +615,17 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     __syncthreads();
     double c = sm_before + (to - s);
     for (int k = 0; k < wave; k++) c += sm_sum[k];
-    if (s > 0.0 && c + s > sm_point) atomicMin(&sm_at, (int)threadIdx.x);
-    if (s > 0.0) atomicMax(&sm_end, (int)threadIdx.x);
+    // (by ballots: atomics of a wave's lanes on one address are taken one lane after another, 4 us for two)
+    {
+        const uint64_t over = __ballot(s > 0.0 && c + s > sm_point), some = __ballot(s > 0.0);
+        if (lane == 0) {
+            sm_at[wave] = over ? wave * 64 + __ffsll((unsigned long long)over) - 1 : 0x7fffffff;
+            sm_end[wave] = some ? wave * 64 + 63 - __clzll((long long)some) : -1;
+        }
+    }
     __syncthreads();
-    const int thread = sm_at != 0x7fffffff ? sm_at : sm_end;
+    const int first_at = min(min(sm_at[0], sm_at[1]), min(sm_at[2], sm_at[3]));
+    const int thread = first_at != 0x7fffffff ? first_at : max(max(sm_end[0], sm_end[1]), max(sm_end[2], sm_end[3]));
     if ((int)threadIdx.x == thread) sm_before = c;
     __syncthreads();
     if (wave) return;
