@@ -119,11 +119,26 @@ __device__ __forceinline__ double weight_of(const AcArgs &a, float x, float m, i
     return a.c == 0.0 ? i == best ? 1.0 : 0.0 : weight(x, (double)m, a.c);
 }
 
-template <int W> // over W neighbouring lanes, in a fixed order
+// A double through a DPP operand (lanes without a source, and rows that ROWS leaves out: 0).
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int i) { // i: uniform
+    const uint64_t w = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), i) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)w, i));
+}
+template <int W> // over W neighbouring lanes, 16 or 64, in a fixed order: lane ^ 1, ^ 2, mirrors of 8 and 16, then rows of 16
 __device__ __forceinline__ double lanes_add(double v) {
-#pragma unroll
-    for (int off = 1; off < W; off <<= 1) v += __shfl_xor(v, off);
-    return v;
+    v += dpp64<0xB1>(v);
+    v += dpp64<0x4E>(v);
+    v += dpp64<0x141>(v);
+    v += dpp64<0x140>(v);
+    return W == 16 ? v : (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 __device__ __forceinline__ double block_add(double v, double *sm) {
     v = lanes_add<64>(v);
@@ -132,12 +147,13 @@ __device__ __forceinline__ double block_add(double v, double *sm) {
     __syncthreads();
     return (sm[0] + sm[1]) + (sm[2] + sm[3]);
 }
-__device__ __forceinline__ double upto(double v) { // inclusive sum over a wave
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double y = __shfl_up(v, off);
-        v += (int)(threadIdx.x & 63) >= off ? y : 0.0;
-    }
+__device__ __forceinline__ double upto(double v) { // inclusive sum over a wave: row_shr 1, 2, 4, 8, row_bcast 15, 31
+    v += dpp64<0x111>(v);
+    v += dpp64<0x112>(v);
+    v += dpp64<0x114>(v);
+    v += dpp64<0x118>(v);
+    v += dpp64<0x142, 0xa>(v);
+    v += dpp64<0x143, 0xc>(v);
     return v;
 }
 
@@ -471,11 +487,6 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
         a.logp[at0 + lane] = lp;
     }
     // the walk: from child to child, values of a lane read by all
-    auto of = [&](double v, int i) {
-        const uint64_t w = __builtin_bit_cast(uint64_t, v);
-        return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), i) << 32 |
-                                              (uint32_t)__builtin_amdgcn_readlane((int)w, i));
-    };
     int node = 0;
     uint64_t kept = 1, gone = 0; // nodes on the way; children of the node that were turned down
     double left = 1.0, aq = 0.0;
@@ -484,10 +495,10 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
         const int c = __ffsll((unsigned long long)open) - 1;
         open &= open - 1;
         const double coin = (double)__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(u), c));
-        double w = of(p, c);
+        double w = lane_of(p, c);
         bool takes;
         if (PT >= 0) {
-            const double qc = of(prob, c);
+            const double qc = lane_of(prob, c);
             w = fmax(w - aq * qc, 0.0);
             takes = coin * qc * left < w;
         } else {
@@ -590,9 +601,9 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
                     if (k0) mine = sum_at(k0 + lane);
                     const double to = before + upto(mine);
                     const uint64_t over = __ballot(mine > 0.0 && to > point), some = __ballot(mine > 0.0);
-                    if (over) found = __ffsll((unsigned long long)over) - 1, start = of(to - mine, found), found += k0;
-                    if (some) last = 63 - __clzll((long long)some), last_start = of(to - mine, last), last += k0;
-                    before = of(to, 63);
+                    if (over) found = __ffsll((unsigned long long)over) - 1, start = lane_of(to - mine, found), found += k0;
+                    if (some) last = 63 - __clzll((long long)some), last_start = lane_of(to - mine, last), last += k0;
+                    before = lane_of(to, 63);
                 }
             if (lane == 0) {
                 sm_seg = found >= 0 ? found : last;
