@@ -12,11 +12,11 @@
 // error of 2^-24 in the likeliest token's weight would all move by 6e-8.
 //
 // What bounds it: the rows' bytes, read once.  16 trees of up to 37 rows of 151936 bf16 logits, 154 MB: 26.5 us, 5.8 TB/s, for
-// the rows (the last call left a part of them in the caches) and 21.8 for the walk; a chain of 6 fp32 rows with draft
-// probabilities: 4.3 and 15.7.  The walk is a chain of short steps (of that chain, in thousands of cycles: the parts' loads 2.7,
-// the join 2.6, the tokens' probabilities 1, the walk 1.7, a segment's sum 8.6, the count 1.5, the choice of a segment 3, of a
-// token 13), each code that runs once: fetching it is a good part of the time.  Trees with draft probabilities need a row's pass
-// for each child with a later sibling that is turned down: see k_accept_ask.
+// the rows (the last call left a part of them in the caches) and 17.0 for the walk; a chain of 6 fp32 rows with draft
+// probabilities: 4.1 and 10.9.  The walk is a chain of short steps (of that chain, in thousands of cycles: the parts' loads and
+// join and the tokens' probabilities 5.6, the walk 1.5, a segment's sum 7.6, the count 1.6, the choice of a segment 2.2, of a
+// token 3.5), each code that runs once: fetching it is a part of the time.  Trees with draft probabilities need a row's pass for
+// each child with a later sibling that is turned down: see k_accept_ask.
 #include <string.h>
 
 #include <algorithm>
@@ -301,8 +301,8 @@ __device__ __forceinline__ void left_of(const AcArgs &a, const AcEnd &e, const f
 }
 // Its sum over the thread's AC_E neighbouring values of a segment, in order.  All loads go out first; the weights are a loop of
 // four at a time, whose values move up: straight code, and no more of it than is run often enough to have been worth fetching
-// (the walk of sixteen trees over 151936 bf16 logits: 24.5 us; 28.7 with sixteen values in a row and branches for their masks and
-// borders).
+// (sixteen values in a row with branches for their masks and borders: 4 us more for the walk of sixteen trees over 151936 bf16
+// logits).
 template <int TY, int PT, bool Z>
 __device__ __forceinline__ double left_sum(const AcArgs &a, const uint8_t *row, const uint8_t *probs, const AcEnd &e, int seg) {
     constexpr int PQ = PT < 0 ? LLM_F32 : PT;
@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     const uint8_t *const row = x + node * a.row, *const probs = PT >= 0 ? q + node * a.p_row : nullptr;
     // Sums of segments through the same code: the workgroup's own; of the sequence's last workgroup, where nothing is left, those
     // of the target's own row too.  The threads' shares are kept for the draw, which would else read the segment and sum it again
-    // (the walk of a chain of 6 fp32 rows: 15.7 us instead of 16.8, of 16 trees of bf16 rows 21.8 instead of 24.5).
+    // (the walk of 16 trees of bf16 rows: 2.7 us less).
     double *const sums = a.sums + (int64_t)b * a.segs, *const shares = a.shares + (int64_t)b * a.segs * AC_T;
     // (through to where every XCD reads it)
     auto put = [](double *at, double v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };

@@ -18,11 +18,11 @@
 // one (11 bits, where the output has 8).  The new tokens' rows go through v_mfma_f32_16x16x4_f32 with fp32 queries and weights.
 // Maxima, sums and outputs are fp32.
 //
-// What bounds it.  Few rows: memory (32 decode steps of 7 query heads a kv head over 131 MB of e4m3 pages: 28.4 us, 4.6 TB/s), or
+// What bounds it.  Few rows: memory (32 decode steps of 7 query heads a kv head over 131 MB of e4m3 pages: 27.4 us, 4.8 TB/s), or
 // with few positions a chain of dependent loads (arguments, length, page, codes, the new row: 7.0 us for 203 positions of heads
 // of 64, 5.6 of it with none).  Many rows: vector instructions, which turn codes into fp16 and make the weights (a step of two
 // tiles of bf16 rows over int8 pages: 585, of which 192 are for the codes, beside 68 products); 448 rows of each of eight
-// sequences over up to 16k positions: 115 us, 377 TFLOP/s.
+// sequences over up to 16k positions: 112 us, 386 TFLOP/s.
 #include "device.h"
 #include "page_attention.h"
 
