@@ -57,18 +57,16 @@ __device__ __forceinline__ void split(float x, float y, uint32_t *p) {
     }
 }
 // Eight codes (two words) as fp16.  int8, its sign bit flipped, is code + 128 in a byte: 0x64 over it is 1024 + code + 128, from
-// which 1152 is taken; with BIASED it stays, a subnormal, as 2^-24 (code + 128).
-template <int CT, bool BIASED>
+// which 1152 is taken.
+template <int CT>
 __device__ __forceinline__ f16x8 codes8(uint32_t a, uint32_t b) {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t u = i < 2 ? a : b;
         if constexpr (CT == LLM_I8) {
-            const uint32_t h = __builtin_amdgcn_perm(BIASED ? 0u : 0x64646464u, u ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u);
-            r[i] = h;
-            if constexpr (!BIASED)
-                r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, h) - (f16x2){(_Float16)1152.0f, (_Float16)1152.0f});
+            const uint32_t h = __builtin_amdgcn_perm(0x64646464u, u ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u);
+            r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, h) - (f16x2){(_Float16)1152.0f, (_Float16)1152.0f});
         } else {
             r[i] = __builtin_bit_cast(uint32_t, i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u, 1.0f, 1)
                                                       : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u, 1.0f, 0));
@@ -80,10 +78,9 @@ __device__ __forceinline__ f32x4 product(f16x8 a, u32x4 b, f32x4 d) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
 }
 
-// an operand of ones, or of -128 units of biased codes
-template <bool BIASED>
-__device__ __forceinline__ f16x8 all_of() {
-    const uint32_t u = BIASED ? 0x80808080u : 0x3c003c00u; // (-2^-17, 1)
+// an operand of ones
+__device__ __forceinline__ f16x8 ones() {
+    const uint32_t u = 0x3c003c00u;
     return __builtin_bit_cast(f16x8, (u32x4){u, u, u, u});
 }
 
@@ -122,11 +119,9 @@ __device__ __forceinline__ void store4(uint8_t *row, int d, float4 y) {
 }
 
 // How 16-bit rows may hold less: their output is rounded to 8 bits.
-template <int CT, int QT>
+template <int QT>
 struct Form {
     static constexpr int Q = QT == LLM_BF16 ? 1 : 2, P = QT == LLM_BF16 ? 1 : 2; // pieces of a query, of a weight
-    static constexpr bool BIASED = QT == LLM_BF16 && CT == LLM_I8;               // codes as 2^-24 (code + 128)
-    static constexpr float UNIT = BIASED ? 0x1p24f : 1.0f;                       // what a product is short of
 };
 
 // The running state of a row: the exponent of 2 that its weights are relative to, their sum, the sums of values (dimension
@@ -359,7 +354,7 @@ constexpr size_t page_lds() {
 // loads go out as soon as a step's registers are used, its page's number a step before.
 template <int CT, int QT, int R, bool ROWS>
 __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(PageArgs a) {
-    using Fm = Form<CT, QT>;
+    using Fm = Form<QT>;
     constexpr int WAVE_LDS = page_wave_lds<R, Fm::Q>();
     constexpr int STRIDE = ROWS ? 1 : 4, BLOCK_ROWS = 16 * R * (ROWS ? 4 : 1);
     extern __shared__ __align__(16) uint8_t lds[];
@@ -458,7 +453,6 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
     u32x4 *const sm_q = mine_; // [R][2 KL][Q]
     float cq[R];
     State st[R];
-    float off[R], bias[R]; // what scores and values of biased codes have too much: 128 times a query's sum, and the weights'
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const bool ok = row0 + 16 * r + n < p.rows;
@@ -473,7 +467,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
             }
         const uint32_t e = exponent(over_groups(mx, fmax_));
         const float to = power_to(e) * a.sign;
-        cq[r] = a.c * power_from(e) * Fm::UNIT;
+        cq[r] = a.c * power_from(e);
 #pragma unroll
         for (int s = 0; s < 2 * KL; s++)
 #pragma unroll
@@ -491,13 +485,6 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
         st[r].m = -INFINITY, st[r].l = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++) st[r].o[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-        off[r] = bias[r] = 0.0f;
-        if (Fm::BIASED) {
-            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = 0; s < 2 * KL; s++) sum = product(all_of<true>(), qf[R > 1 ? 0 : r][s][0], sum);
-            off[r] = sum[0];
-        }
     }
     if (R > 1) {
         load_k(step, page);
@@ -523,7 +510,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
                 for (int k = 0; k < Fm::Q; k++) q[r][k] = R > 1 ? sm_q[((r * 2 * KL + s) * Fm::Q + k) * 64] : qf[r % (R > 1 ? 1 : R)][s][k];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-                const f16x8 kf = codes8<CT, Fm::BIASED>(kr[t][s / 2][2 * (s % 2)], kr[t][s / 2][2 * (s % 2) + 1]);
+                const f16x8 kf = codes8<CT>(kr[t][s / 2][2 * (s % 2)], kr[t][s / 2][2 * (s % 2) + 1]);
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
@@ -553,19 +540,18 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) ms = fmaxf(ms, x[r][t][i]);
-            float o = Fm::BIASED ? ks < 0.0f ? -off[r] : off[r] : 0.0f;
-            ms = (over_groups(ms, fmax_) + o) * c;
+            ms = over_groups(ms, fmax_) * c;
             // A step's largest weight is 2^15, the top of fp16's range.  Scores from 2^23 on have steps of 1 or more, and the
             // difference could be 16: those weights are few and far apart, their largest is 1, and it takes scores rounded alike.
             if (__any(fabsf(ms) >= 0x1p23f && ms != -INFINITY)) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[r][t][i] = (x[r][t][i] + o) * c;
-                c = 1.0f, o = 0.0f;
+                    for (int i = 0; i < 4; i++) x[r][t][i] *= c;
+                c = 1.0f;
             }
             ms -= fabsf(ms) < 0x1p23f ? 15.0f : 0.0f;
-            const float mu = fmaf(o, c, ms == -INFINITY ? 0.0f : -ms);
+            const float mu = ms == -INFINITY ? 0.0f : -ms;
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -576,17 +562,16 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
 #pragma unroll
                     for (int k = 0; k < Fm::P; k++) pf[r][u][k][e / 2] = w[k];
                 }
-            // the sum of the weights as the products take them: 1 or, for biased codes, -128 of their units times each
+            // the sum of the weights as the products take them
             f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int k = Fm::P - 1; k >= 0; k--)
 #pragma unroll
-                for (int u = 0; u < 2; u++) sum = product(all_of<Fm::BIASED>(), pf[r][u][k], sum);
+                for (int u = 0; u < 2; u++) sum = product(ones(), pf[r][u][k], sum);
             float f, g;
             join(st[r], ms, f, g);
-            gv[r] = g * v_size * Fm::UNIT;
-            st[r].l = fmaf(Fm::BIASED ? sum[0] * -0x1p17f : sum[0], g, st[r].l);
-            if (Fm::BIASED) bias[r] = fmaf(bias[r], f, sum[0] * gv[r]);
+            gv[r] = g * v_size;
+            st[r].l = fmaf(sum[0], g, st[r].l);
         }
         load_k(step + STRIDE, next);
         if (CT == LLM_E4M3 && left < PAGE_BLOCK) // codes past the end may be NaN: 0 * NaN
@@ -602,7 +587,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
         for (int d = 0; d < DT; d++) {
             f16x8 vf[2];
 #pragma unroll
-            for (int u = 0; u < 2; u++) vf[u] = codes8<CT, Fm::BIASED>(vr[d][2 * u], vr[d][2 * u + 1]);
+            for (int u = 0; u < 2; u++) vf[u] = codes8<CT>(vr[d][2 * u], vr[d][2 * u + 1]);
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -620,13 +605,6 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
         next = page_of(step + 2 * STRIDE);
     }
 
-    if (Fm::BIASED)
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) st[r].o[d][i] += bias[r];
     // the new tokens' rows; waves that share the rows take a tile each, from the one with the fewest steps on
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -695,7 +673,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
 PageKernel PAGE_NAME(PAGE_HSP)(int type, int q_type, int tiles, int rows, size_t *lds) {
 #define PAGE_PICK(C, QY, T, W)                                                   \
     if (type == C && q_type == QY && tiles == T && (rows != 0) == W) {            \
-        *lds = page_lds<T, W, Form<C, QY>::Q>();                                 \
+        *lds = page_lds<T, W, Form<QY>::Q>();                                 \
         return k_page_attention<C, QY, T, W>;                                    \
     }
 #define PAGE_PICK_T(T, W)                                                        \

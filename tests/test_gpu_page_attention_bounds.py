@@ -1,0 +1,120 @@
+"""llm_page_attention held between bounds that follow from its definition in float64, where scores or values are large, small, or so
+many that the tile pairs and row waves take them.
+
+Bounds.  u = 2^-24, half a step of fp32; L the positions a row sees, |q| its largest query value.
+  A score is off by at most e = (hs + 8) u |scale| sum |q k| + 2^-39 |scale| |q| sum |k| (a sum of hs products, the scales, a query's
+  pieces); d the largest over the row.
+  2 d up to 1/2: each weight is off by a factor of e^(2 d) at most, all else by (L + 64) u, relative to sum p |v|; a weight far below the
+  block's largest by 2^-39 of that: L 2^-39 max |v|; a V scale below 2^-103 loses bits to fp32's smallest numbers: 2^-118.
+  2 d above: a position whose score is 2 d + 40 below the largest has a weight of e^-40 at most.  The others' values enclose the result
+  but for (L + 64) u and L e^-40 of the largest value.
+Rounding to the output's type is monotone: the output lies between the two bounds rounded, whatever its type."""
+import math
+
+import numpy as np
+import pytest
+
+from helpers import pkg
+from pages_ref import ROWS, Pool
+from test_gpu_pages import DEV, gen, ints
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def check(pool, table, q, kn, vn, lens, n, mask, scale, got, layer=0):
+    """returns how many rows' results the bounds determine to 1% of their largest value, and all rows"""
+    b, t, heads, hs = q.shape
+    group, page = heads // pool.h, pool.page
+    val = [pool.values(0, layer), pool.values(1, layer)]
+    got, fine, rows = got.cpu(), 0, 0
+    for i in range(b):
+        at = torch.arange(min(max(lens[i], 0), len(table[i]) * page))
+        pages = torch.tensor(table[i])[at // page]
+        there = (pages >= 0) & (pages < pool.pages)
+        pages, at = pages[there], at[there] % page
+        live = min(max(n[i], 0), t)
+        assert (got[i, live:] == 0).all()
+        for h in range(pool.h):
+            k, v = val[0][pages, h, at].reshape(-1, hs), val[1][pages, h, at].reshape(-1, hs)
+            sees = torch.ones(live, k.shape[0] + (live if kn is not None else 0), dtype=torch.bool)
+            if kn is not None:
+                bits = [(1 << (j + 1)) - 1 if mask is None else int(mask[i, j]) for j in range(live)]
+                sees[:, k.shape[0]:] = torch.tensor([[bool(x >> y & 1) for y in range(live)] for x in bits], dtype=torch.bool).reshape(live, live)
+                k, v = torch.cat((k, kn[i, :live, h].double())), torch.cat((v, vn[i, :live, h].double()))
+            x = q[i, :live, h * group:(h + 1) * group].double().reshape(-1, hs)
+            y = got[i, :live, h * group:(h + 1) * group].reshape(-1, hs)
+            sees = sees.repeat_interleave(group, 0)
+            some = sees.any(1)
+            assert (y[~some] == 0).all()
+            x, y, sees = x[some], y[some], sees[some]
+            if not len(x):
+                continue
+            count = sees.sum(1, keepdim=True).double()
+            s = (x @ k.T * scale).masked_fill(~sees, -math.inf)
+            e = abs(scale) * ((hs + 8) * U * (x.abs() @ k.abs().T) + 2.0 ** -39 * x.abs().amax(1, keepdim=True) * k.abs().sum(1))
+            d = e.masked_fill(~sees, 0.0).amax(1, keepdim=True)
+            p = torch.softmax(s, 1)
+            want, size = p @ v, p @ v.abs()
+            top = torch.where(sees, v.abs().amax(1), 0.0).amax(1, keepdim=True)
+            tol = (torch.expm1((2 * d).clamp(max=1.0)) + (count + 64) * U) * size + count * 2.0 ** -39 * top + 2.0 ** -118
+            lo, hi = want - tol, want + tol
+            for j in torch.nonzero(d[:, 0] > 0.25)[:, 0].tolist():
+                near = s[j] >= s[j].max() - 2 * d[j] - 40
+                slack = ((count[j] + 64) * U + count[j] * math.exp(-40)) * top[j]
+                lo[j], hi[j] = v[near].amin(0) - slack, v[near].amax(0) + slack
+            fine += int(((hi - lo).amax(1) <= 0.01 * top[:, 0]).sum())
+            rows += len(x)
+            lo, hi = lo.to(got.dtype).double(), hi.to(got.dtype).double()
+            off = ~((y.double() >= lo) & (y.double() <= hi))
+            assert not off.any(), (i, h, int(off.sum()), off.numel(), torch.nonzero(off)[0].tolist(), y[off][0], lo[off][0], hi[off][0])
+    return fine, rows
+
+
+def run(pool, table, q, lens, kn=None, vn=None, n=None, mask=None, scale=None, max_len=None, layout="plain", tensors=None):
+    tensors = pool.tensors(layout, layers=False) if tensors is None else tensors
+    m = None if mask is None else torch.from_numpy(mask.view(np.int64)).to(DEV)
+    on = lambda x: None if x is None else x.to(DEV)  # noqa: E731
+    got = pkg().page_attention(on(q), *tensors, ints(table), ints(lens), on(kn), on(vn), n=None if n is None else ints(n), mask=m,
+                               scale=scale, max_len=max_len)
+    return check(pool, table, q, kn, vn, lens, [q.shape[1]] * q.shape[0] if n is None else n, mask,
+                 q.shape[3] ** -0.5 if scale is None else scale, got)
+
+
+TYPES = [("int8", "fp32"), ("int8", "bf16"), ("e4m3", "fp32"), ("e4m3", "bf16")]
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("q_size,k_size", [(64.0, 400.0), (8.0, 3200.0), (1.0, 1e6), (0.5, 1.0)])
+def test_queries_of_one_sign_under_large_scales(cache, rows, q_size, k_size, sign):
+    """a query's sum is far larger than its products with the rows, whose codes have both signs: scores of up to 1e6, below and above
+    where fp32 has steps of one"""
+    g, h, hs = gen(1), 2, 128
+    pool = Pool(1, 6, h, 64, hs, cache, g)
+    most = 16 if cache == "e4m3" else 20
+    pool.code[0] = torch.randint(-most, most + 1, pool.code[0].shape, generator=g).double()
+    pool.scale[0] = torch.full_like(pool.scale[0], k_size * sign)
+    for _ in range(4):
+        q = (q_size * (1.0 + torch.rand(1, 8, 4, hs, generator=g) / 4)).to(ROWS[rows])
+        run(pool, [[5, 0, 3, 1]], q, [250])
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("top", [2.0 ** 119, 2.0 ** 121])
+@pytest.mark.parametrize("slope", [0.0, 0.3, 4.0, -4.0])
+def test_values_whose_scale_is_near_the_largest(cache, rows, top, slope):
+    """values up to 2^121 under scores that rise or fall from block to block; few enough that their sums stay below 2^127"""
+    g, h, hs = gen(3), 1, 64
+    pool = Pool(1, 8, h, 64, hs, cache, g)
+    pool.code[1] = torch.randint(-3 if top < 2.0 ** 120 else -1, 2, pool.code[1].shape, generator=g).double()
+    pool.scale[1] = torch.full_like(pool.scale[1], top)
+    pool.code[0][..., 0] = 8.0
+    pool.code[0][..., 1:] = 0.0
+    pool.scale[0][0, :, 0, 0] = 0.5 + torch.arange(8) * slope
+    pool.scale[0][0, :, 0, 0] -= pool.scale[0][0, :, 0, 0].min() - 0.5
+    q = torch.ones(1, 2, 2, hs).to(ROWS[rows])
+    for lens in ([20], [500]):
+        run(pool, [list(range(8))], q, lens, scale=1.0)
