@@ -15,7 +15,8 @@
 //
 // Operands.  int8 and e4m3 codes are exact in fp16.  A query row is scaled by a power of two to the top of fp16's range: fp32
 // ones are two pieces (22 bits), bf16 ones one (their 8 bits down to 2^-39 of the largest).  Weights are two pieces, of bf16 rows
-// one (11 bits, where the output has 8).  The new tokens' rows go through v_mfma_f32_16x16x4_f32 with fp32 queries and weights.
+// too: one (11 bits) gave 3% of a batch's bf16 outputs another rounding than the exact result, two give 0.1%, at the price of 16 us in
+// 138 for eight trees of 64 over int8 pages.  The new tokens' rows go through v_mfma_f32_16x16x4_f32 with fp32 queries and weights.
 // Maxima, sums and outputs are fp32.
 //
 // What bounds it.  Few rows: memory (32 decode steps of 7 query heads a kv head over 131 MB of e4m3 pages: 27.4 us, 4.8 TB/s), or
@@ -118,11 +119,10 @@ __device__ __forceinline__ void store4(uint8_t *row, int d, float4 y) {
     else *(uint2 *)(row + (size_t)d * 2) = make_uint2(bf2(y.x, y.y), bf2(y.z, y.w));
 }
 
-// How 16-bit rows may hold less: their output is rounded to 8 bits.
+// Pieces of a query (16-bit ones are exact in one) and of a weight.
 template <int QT>
-struct Form {
-    static constexpr int Q = QT == LLM_BF16 ? 1 : 2, P = QT == LLM_BF16 ? 1 : 2; // pieces of a query, of a weight
-};
+constexpr int Q_PIECES = QT == LLM_BF16 ? 1 : 2;
+constexpr int P_PIECES = 2;
 
 // The running state of a row: the exponent of 2 that its weights are relative to, their sum, the sums of values (dimension
 // 16 d + 4 j + i).
@@ -354,8 +354,7 @@ constexpr size_t page_lds() {
 // loads go out as soon as a step's registers are used, its page's number a step before.
 template <int CT, int QT, int R, bool ROWS>
 __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(PageArgs a) {
-    using Fm = Form<QT>;
-    constexpr int WAVE_LDS = page_wave_lds<R, Fm::Q>();
+    constexpr int NQ = Q_PIECES<QT>, NP = P_PIECES, WAVE_LDS = page_wave_lds<R, NQ>();
     constexpr int STRIDE = ROWS ? 1 : 4, BLOCK_ROWS = 16 * R * (ROWS ? 4 : 1);
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, n = lane & 15, j = lane >> 4;
@@ -449,7 +448,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
 
     // the queries: value e of product s is dimension 64 (s / 2) + 16 j + 8 (s % 2) + e
     // (two tiles' queries wait in LDS, a lane's own: in registers they would spill)
-    u32x4 qf[R > 1 ? 1 : R][2 * KL][Fm::Q];
+    u32x4 qf[R > 1 ? 1 : R][2 * KL][NQ];
     u32x4 *const sm_q = mine_; // [R][2 KL][Q]
     float cq[R];
     State st[R];
@@ -472,16 +471,16 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
         for (int s = 0; s < 2 * KL; s++)
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                uint32_t w[Fm::Q];
-                split<Fm::Q>(x[s][i] * to, x[s][i + 1] * to, w);
+                uint32_t w[NQ];
+                split<NQ>(x[s][i] * to, x[s][i + 1] * to, w);
 #pragma unroll
-                for (int k = 0; k < Fm::Q; k++) qf[R > 1 ? 0 : r][s][k][i / 2] = w[k];
+                for (int k = 0; k < NQ; k++) qf[R > 1 ? 0 : r][s][k][i / 2] = w[k];
             }
         if (R > 1)
 #pragma unroll
             for (int s = 0; s < 2 * KL; s++)
 #pragma unroll
-                for (int k = 0; k < Fm::Q; k++) sm_q[((r * 2 * KL + s) * Fm::Q + k) * 64] = qf[0][s][k];
+                for (int k = 0; k < NQ; k++) sm_q[((r * 2 * KL + s) * NQ + k) * 64] = qf[0][s][k];
         st[r].m = -INFINITY, st[r].l = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++) st[r].o[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -503,18 +502,18 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
             for (int t = 0; t < 4; t++) x[r][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < 2 * KL; s++) {
-            u32x4 q[R][Fm::Q];
+            u32x4 q[R][NQ];
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int k = 0; k < Fm::Q; k++) q[r][k] = R > 1 ? sm_q[((r * 2 * KL + s) * Fm::Q + k) * 64] : qf[r % (R > 1 ? 1 : R)][s][k];
+                for (int k = 0; k < NQ; k++) q[r][k] = R > 1 ? sm_q[((r * 2 * KL + s) * NQ + k) * 64] : qf[r % (R > 1 ? 1 : R)][s][k];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 const f16x8 kf = codes8<CT>(kr[t][s / 2][2 * (s % 2)], kr[t][s / 2][2 * (s % 2) + 1]);
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
-                    for (int k = Fm::Q - 1; k >= 0; k--) x[r][t] = product(kf, q[r][k], x[r][t]); // smallest pieces first
+                    for (int k = NQ - 1; k >= 0; k--) x[r][t] = product(kf, q[r][k], x[r][t]); // smallest pieces first
             }
         }
         __builtin_amdgcn_s_setprio(0);
@@ -525,7 +524,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
 #pragma unroll
                 for (int t = 0; t < 4; t++) x[r][t] = -x[r][t];
         const float size = fabsf(ks) < INFINITY ? fabsf(ks) : 0.0f, v_size = fabsf(ks) < INFINITY ? vs : NAN;
-        u32x4 pf[R][2][Fm::P];
+        u32x4 pf[R][2][NP];
         float gv[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
@@ -556,16 +555,16 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    uint32_t w[Fm::P];
-                    split<Fm::P>(__builtin_amdgcn_exp2f(fmaf(x[r][2 * u + e / 4][e % 4], c, mu)),
+                    uint32_t w[NP];
+                    split<NP>(__builtin_amdgcn_exp2f(fmaf(x[r][2 * u + e / 4][e % 4], c, mu)),
                                  __builtin_amdgcn_exp2f(fmaf(x[r][2 * u + e / 4][e % 4 + 1], c, mu)), w);
 #pragma unroll
-                    for (int k = 0; k < Fm::P; k++) pf[r][u][k][e / 2] = w[k];
+                    for (int k = 0; k < NP; k++) pf[r][u][k][e / 2] = w[k];
                 }
             // the sum of the weights as the products take them
             f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = Fm::P - 1; k >= 0; k--)
+            for (int k = NP - 1; k >= 0; k--)
 #pragma unroll
                 for (int u = 0; u < 2; u++) sum = product(ones(), pf[r][u][k], sum);
             float f, g;
@@ -592,7 +591,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
             for (int r = 0; r < R; r++) {
                 f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int k = Fm::P - 1; k >= 0; k--)
+                for (int k = NP - 1; k >= 0; k--)
 #pragma unroll
                     for (int u = 0; u < 2; u++) y = product(vf[u], pf[r][u][k], y);
 #pragma unroll
@@ -673,7 +672,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
 PageKernel PAGE_NAME(PAGE_HSP)(int type, int q_type, int tiles, int rows, size_t *lds) {
 #define PAGE_PICK(C, QY, T, W)                                                   \
     if (type == C && q_type == QY && tiles == T && (rows != 0) == W) {            \
-        *lds = page_lds<T, W, Form<QY>::Q>();                                 \
+        *lds = page_lds<T, W, Q_PIECES<QY>>();                                 \
         return k_page_attention<C, QY, T, W>;                                    \
     }
 #define PAGE_PICK_T(T, W)                                                        \

@@ -104,7 +104,7 @@ def test_queries_of_one_sign_under_large_scales(cache, rows, q_size, k_size, sig
 
 @pytest.mark.parametrize("cache,rows", TYPES)
 @pytest.mark.parametrize("top", [2.0 ** 119, 2.0 ** 121])
-@pytest.mark.parametrize("slope", [0.0, 0.3, 4.0, -4.0])
+@pytest.mark.parametrize("slope", [0.0, 0.15, 0.3, 4.0, -4.0])
 def test_values_whose_scale_is_near_the_largest(cache, rows, top, slope):
     """values up to 2^121 under scores that rise or fall from block to block; few enough that their sums stay below 2^127"""
     g, h, hs = gen(3), 1, 64
@@ -118,3 +118,17 @@ def test_values_whose_scale_is_near_the_largest(cache, rows, top, slope):
     q = torch.ones(1, 2, 2, hs).to(ROWS[rows])
     for lens in ([20], [500]):
         run(pool, [list(range(8))], q, lens, scale=1.0)
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("hs", [64, 128, 192])
+@pytest.mark.parametrize("lens", [[2, 3, 5], [64, 67, 200]])
+def test_weights_hold_what_fp32_sums_need(cache, rows, hs, lens):
+    """nearly equal weights, of few positions: the bounds are narrow, and an output may be the other neighbour only where the exact
+    result is next to the border between two"""
+    g, h, b, heads = gen(4 + hs), 2, len(lens), 16
+    pool = Pool(1, 4 * b, h, 64, hs, cache, g)
+    q = (torch.randn(b, 4, heads, hs, generator=g) * 0.05).to(ROWS[rows])
+    table = [[4 * i + j for j in range(4)] for i in range(b)]
+    fine, all_ = run(pool, table, q, lens)
+    assert fine == all_
