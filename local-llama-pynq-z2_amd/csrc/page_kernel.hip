@@ -85,11 +85,9 @@ __device__ __forceinline__ f16x8 ones() {
     return __builtin_bit_cast(f16x8, (u32x4){u, u, u, u});
 }
 
-// The power of two that takes a magnitude to [2^14, 2^15) (magnitudes below 2^-112 to less, infinities: 2^-127 and NaN), and
-// its inverse, from the magnitude's exponent field.
-__device__ __forceinline__ uint32_t exponent(float x) { return (__float_as_uint(x) >> 23) & 0xff; }
-__device__ __forceinline__ float power_to(uint32_t e) { return __uint_as_float(min(268u - e, 253u) << 23); }
-__device__ __forceinline__ float power_from(uint32_t e) { return __uint_as_float((254u - min(268u - e, 253u)) << 23); }
+// The exponent field of a power of two that takes a magnitude to [2^14, 2^15) (magnitudes below 2^-112 to less, but all of
+// their bits into fp16's range; infinities stay).
+__device__ __forceinline__ uint32_t power_to(float x) { return min(268u - ((__float_as_uint(x) >> 23) & 0xff), 253u); }
 
 // Over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
 template <typename F>
@@ -450,7 +448,10 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
     // (two tiles' queries wait in LDS, a lane's own: in registers they would spill)
     u32x4 qf[R > 1 ? 1 : R][2 * KL][NQ];
     u32x4 *const sm_q = mine_; // [R][2 KL][Q]
-    float cq[R];
+    // A score is a product of the pieces times the softmax scale, the block's and what the queries were divided by: mantissas and
+    // exponents apart, so that nothing leaves fp32's range on the way
+    const float cm = __builtin_amdgcn_frexp_mantf(a.c);
+    int cq[R];
     State st[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -464,9 +465,9 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
                 if (!ok || 64 * (s / 2) + 16 * j + 8 * (s % 2) >= a.hs) x[s][e] = 0.0f;
                 mx = fmaxf(mx, fabsf(x[s][e]));
             }
-        const uint32_t e = exponent(over_groups(mx, fmax_));
-        const float to = power_to(e) * a.sign;
-        cq[r] = a.c * power_from(e);
+        const uint32_t e = power_to(over_groups(mx, fmax_));
+        const float to = __uint_as_float(e << 23) * a.sign;
+        cq[r] = __builtin_amdgcn_frexp_expf(a.c) + 127 - (int)e;
 #pragma unroll
         for (int s = 0; s < 2 * KL; s++)
 #pragma unroll
@@ -524,11 +525,14 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
 #pragma unroll
                 for (int t = 0; t < 4; t++) x[r][t] = -x[r][t];
         const float size = fabsf(ks) < INFINITY ? fabsf(ks) : 0.0f, v_size = fabsf(ks) < INFINITY ? vs : NAN;
+        const float sm = __builtin_amdgcn_frexp_mantf(size) * cm;
+        const int se = __builtin_amdgcn_frexp_expf(size);
         u32x4 pf[R][2][NP];
         float gv[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float c = fmaxf(cq[r] * size, 1e-45f), ms = -INFINITY; // (never 0: what is not seen is -infinity times it)
+            // (neither 0 nor infinite: what is not seen is -infinity times it, and a score may be 0)
+            float c = __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(sm, cq[r] + se), 1e-45f, 3.4e38f), ms = -INFINITY;
             if (left < PAGE_BLOCK)
 #pragma unroll
                 for (int t = 0; t < 4; t++)

@@ -103,6 +103,23 @@ def test_queries_of_one_sign_under_large_scales(cache, rows, q_size, k_size, sig
 
 
 @pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("q_top,k_top,scale", [(2.0 ** 121, 2.0 ** -118, None), (2.0 ** 126, 2.0 ** -123, None), (2.0 ** 121, 2.0 ** -121, -1.0),
+                                               (2.0 ** 60, 2.0 ** -120, 2.0 ** 60), (2.0 ** 100, 2.0 ** -136, 2.0 ** 36),
+                                               (2.0 ** -100, 2.0 ** 100, 1.0), (2.0 ** -120, 2.0 ** 112, 2.0 ** 8),
+                                               (2.0 ** -130, 2.0 ** 10, 2.0 ** 120), (2.0 ** 100, 2.0 ** 25, 2.0 ** -125),
+                                               (2.0 ** 115, 2.0 ** -143, 2.0 ** 30), (2.0 ** -113, 2.0 ** 126, 2.0 ** -12)])
+def test_scores_of_large_and_small_factors(cache, rows, q_top, k_top, scale):
+    """a query, a block's scale and the softmax scale of which two multiplied would leave fp32's range, and all three do not"""
+    g, h, hs = gen(2), 2, 64
+    pool = Pool(1, 8, h, 64, hs, cache, g)
+    pool.code[0] = (pool.code[0] / (32 if cache == "e4m3" else 8)).round().clamp(-15, 15)
+    pool.scale[0] = (torch.exp(0.5 * torch.randn(pool.scale[0].shape, generator=g)) / 8 * k_top).float()
+    q = (torch.randn(2, 3, 8, hs, generator=g).clamp(-3.5, 3.5) / 4 * q_top).to(ROWS[rows])
+    fine, all_ = run(pool, [[5, 0, 3, 1], [7, 2, 4, 6]], q, [250, 64], scale=scale)
+    assert fine == all_
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
 @pytest.mark.parametrize("top", [2.0 ** 119, 2.0 ** 121])
 @pytest.mark.parametrize("slope", [0.0, 0.15, 0.3, 4.0, -4.0])
 def test_values_whose_scale_is_near_the_largest(cache, rows, top, slope):
