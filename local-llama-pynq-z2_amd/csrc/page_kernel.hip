@@ -518,13 +518,13 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
             }
         }
         __builtin_amdgcn_s_setprio(0);
-        // a scale below zero turns the scores round; one that is not finite makes every row NaN through its values
+        // a scale below zero turns the scores round; one that is not finite, of K or V, makes every row NaN through its values
         if (ks < 0.0f)
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int t = 0; t < 4; t++) x[r][t] = -x[r][t];
-        const float size = fabsf(ks) < INFINITY ? fabsf(ks) : 0.0f, v_size = fabsf(ks) < INFINITY ? vs : NAN;
+        const float size = fabsf(ks) < INFINITY ? fabsf(ks) : 0.0f, v_size = fabsf(ks) < INFINITY && fabsf(vs) < INFINITY ? vs : NAN;
         const float sm = __builtin_amdgcn_frexp_mantf(size) * cm;
         const int se = __builtin_amdgcn_frexp_expf(size);
         u32x4 pf[R][2][NP];

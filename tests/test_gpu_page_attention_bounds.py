@@ -149,3 +149,22 @@ def test_weights_hold_what_fp32_sums_need(cache, rows, hs, lens):
     table = [[4 * i + j for j in range(4)] for i in range(b)]
     fine, all_ = run(pool, table, q, lens)
     assert fine == all_
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("what", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("side", [0, 1])
+def test_scales_that_are_not_finite(cache, rows, what, side):
+    """a block with such a scale makes all those NaN that see its positions, of its head, and changes no bit of others"""
+    g, h, hs = gen(5), 2, 64
+    pool = Pool(1, 5, h, 64, hs, cache, g)
+    tensors, table, lens = pool.tensors(layers=False), ints([[2, 0], [3, 1]]), ints([90, 70])
+    q = torch.randn(2, 3, 6, hs, generator=g).to(ROWS[rows]).to(DEV)
+    clean = pkg().page_attention(q, *tensors, table, lens)
+    for page in (2, 0):
+        old = tensors[2 + side][page, 1].clone()
+        tensors[2 + side][page, 1] = what
+        got = pkg().page_attention(q, *tensors, table, lens)
+        tensors[2 + side][page, 1] = old
+        assert torch.equal(got[1], clean[1]) and torch.equal(got[0, :, :3], clean[0, :, :3])
+        assert got[0, :, 3:].isnan().all()
