@@ -10,12 +10,14 @@ Bounds.  u = 2^-24, half a step of fp32; L the positions a row sees, |q| its lar
   but for (L + 64) u and L e^-40 of the largest value.
 Rounding to the output's type is monotone: the output lies between the two bounds rounded, whatever its type."""
 import math
+import random
 
 import numpy as np
 import pytest
 
 from helpers import pkg
 from pages_ref import ROWS, Pool
+from test_gpu_page_attention import tree_masks
 from test_gpu_pages import DEV, gen, ints
 
 torch = pytest.importorskip("torch")
@@ -168,3 +170,101 @@ def test_scales_that_are_not_finite(cache, rows, what, side):
         tensors[2 + side][page, 1] = old
         assert torch.equal(got[1], clean[1]) and torch.equal(got[0, :, :3], clean[0, :, :3])
         assert got[0, :, 3:].isnan().all()
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("by", [6.0, 20.0])
+def test_blocks_of_very_different_scales_choose_the_largest(cache, rows, by):
+    """scales from 2^-80 to 2^80: of most rows one position has all the weight, or a few"""
+    g, h, hs = gen(6), 2, 64
+    fine = all_ = 0
+    for t in (1, 5):
+        pool = Pool(1, 12, h, 64, hs, cache, g)
+        pool.scale[0] *= torch.exp(by * torch.randn(pool.scale[0].shape, generator=g))
+        q, kn, vn = (torch.randn(1, t, x, hs, generator=g).to(ROWS[rows]) for x in (6, h, h))
+        a, b = run(pool, [list(range(12))], q, [700], kn, vn)
+        fine, all_ = fine + a, all_ + b
+    assert fine >= 0.5 * all_
+
+
+# ---- tile pairs and row waves: the host's bound of the lengths chooses them, so that short contexts reach them
+
+def work_bytes(h, rows, hs, b, most, max_n, block_rows, least):
+    """what a call's work memory has where its row blocks are of so many rows, from how positions are cut"""
+    row_blocks = -(-rows // block_rows)
+    one, both = max(32 // row_blocks, 1) * 8, max(64 // row_blocks, 1) * 8
+    steps = -(-most // 64) + -(-max_n // 16)
+    sizes = set()
+    for cap in (one, both):
+        if b == 1:
+            cap = max(min(cap // h, -(-steps // least), 128), 1) * h
+        whole = cap <= b * h or steps <= 3 * least or (b > 1 and cap == one)
+        sizes.add(0 if whole else cap * rows * (hs + 2) * 4 + b * h * 8)
+    return sizes - {0}
+
+
+# (kv heads, heads, head size, positions' bound, lengths, tokens, live ones, whether waves take rows)
+PAIRS = [
+    (4, 28, 128, 16000, [300], 37, None, False),
+    (4, 28, 128, 16000, [0], 37, None, False),
+    (1, 5, 128, 170000, [130], 16, None, False),           # 80 rows: the last pair's second tile has none
+    (1, 3, 64, 240000, [1000], 33, None, False),           # 99 rows: the last pair has three
+    (2, 12, 48, 70000, [200, 0, 65], 11, [11, 5, 0], False),
+    (1, 7, 112, 52000, [64, 700, 1, 0], 10, [10, 10, 3, 1], False),
+    (4, 28, 128, 30000, [500], 64, None, True),
+    (4, 28, 128, 8192, [300, 0, 64, 129], 64, [64, 64, 2, 0], True),
+    (2, 14, 64, 54000, [128, 600], 64, [19, 64], True),    # 133 rows: of the last row block one wave has five, the others none
+    (1, 9, 96, 90000, [900, 5, 64], 21, [15, 21, 1], True),
+    (1, 64, 64, 510000, [200], 3, None, True),
+]
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("h,heads,hs,most,lens,t,n,by_rows", PAIRS)
+def test_tile_pairs(cache, rows, h, heads, hs, most, lens, t, n, by_rows):
+    """with masks, own rows, unseen places that are not finite, in a pool that lies apart"""
+    g, r, b = gen(7 + t), random.Random(t), len(lens)
+    page = 256
+    per, have = -(-most // page), [-(-x // page) for x in lens]
+    pages = sum(have) + 2
+    pool = Pool(1, pages, h, page, hs, cache, g)
+    ids = iter(torch.randperm(pages, generator=g).tolist())
+    table = [[next(ids) if j < have[i] else -1 for j in range(per)] for i in range(b)]
+    q, kn, vn = (torch.randn(b, t, x, hs, generator=g).to(ROWS[rows]) for x in (heads, h, h))
+    mask, live = tree_masks(r, b, t), [t] * b if n is None else n
+    tensors = pool.tensors("wide", layers=False)
+    nan = 0x7F if cache == "e4m3" else -128
+    spare = list(ids)
+    for pg in spare:
+        tensors[2][pg], tensors[3][pg] = math.nan, math.inf
+    for i in range(b):
+        for at in range(lens[i], -(-lens[i] // 64) * 64):
+            pg, blk = table[i][at // page], at % page // 64
+            tensors[0].view(torch.int8)[pg, :, at % page] = nan
+            tensors[1].view(torch.int8)[pg, :, blk, :, at % 64] = nan
+        kn[i, live[i]:], vn[i, live[i]:], q[i, live[i]:] = math.nan, math.inf, math.nan
+    # these sizes are of the kernels that this test is for, not of one tile a wave, nor of waves over positions
+    c = pkg()._pages(*tensors)[0]
+    need = pkg().lib().llm_page_attention_work(c, b, heads, t, most)
+    size = lambda block, least: work_bytes(h, heads // h * t, hs, b, most, t, block, least)  # noqa: E731
+    assert need in size(128 if by_rows else 32, 2 if by_rows else 4)
+    assert need not in size(16, 4) and not (by_rows and need in size(32, 4))
+    run(pool, table, q, lens, kn, vn, n, mask, max_len=most, tensors=tensors)
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("b,h,heads,hs,t", [(520, 2, 14, 64, 3), (160, 4, 8, 112, 20), (40, 4, 28, 64, 64)])
+def test_tile_pairs_without_slices(cache, rows, b, h, heads, hs, t):
+    """more than 512 sequences are not cut, nor those whose heads are as many as the slices; the last ones' waves take rows"""
+    g = gen(8)
+    lens = [(i * 37) % 90 for i in range(b)]
+    pool = Pool(1, 40, h, 64, hs, cache, g)
+    table = [[i % 40, (i + 7) % 40] + [-1] * 126 for i in range(b)]
+    q, kn, vn = (torch.randn(b, t, x, hs, generator=g).to(ROWS[rows]) for x in (heads, h, h))
+    n = [t - i % 3 for i in range(b)]
+    tensors = pool.tensors(layers=False)
+    c = pkg()._pages(*tensors)[0]
+    most = 128 * 64
+    assert pkg().lib().llm_page_attention_work(c, b, heads, t, most) == 0
+    assert heads // h * t > 16 and -(-(heads // h * t) // 16) * b * h * 128 * (-(-hs // 64) * 64) > 6e6
+    run(pool, table, q, lens, kn, vn, n, max_len=most, tensors=tensors)
