@@ -101,10 +101,6 @@ extern "C" int llm_page_attention(const llm_pages *c, const llm_rows *q, const l
         fprintf(stderr, "%s: q, out and the new rows are of different types\n", who);
         return -1;
     }
-    if (k && (k->tok > (16 << 20) / op_type_bytes(k->type) || v->tok > (16 << 20) / op_type_bytes(v->type))) {
-        fprintf(stderr, "%s: the new rows' tokens have to be at most 16 MiB from the next\n", who);
-        return -1;
-    }
     const PagePlan p = page_plan(c, n_seq, n_heads, max_n, max_len);
     if (p.bytes && (work_bytes < p.bytes || ((uintptr_t)work & 15) || !dev.holds(work, "the work memory"))) {
         fprintf(stderr, "%s: %zu bytes of work memory are needed, 16-byte aligned\n", who, p.bytes);

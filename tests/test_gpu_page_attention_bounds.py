@@ -187,6 +187,24 @@ def test_blocks_of_very_different_scales_choose_the_largest(cache, rows, by):
     assert fine >= 0.5 * all_
 
 
+@pytest.mark.parametrize("cache,rows", [("int8", torch.float32), ("e4m3", torch.bfloat16)])
+def test_new_rows_whose_tokens_lie_far_apart(cache, rows):
+    """more than 16 MiB from token to token"""
+    g, b, t, heads, h, hs = gen(2), 2, 18, 4, 2, 64
+    pool = Pool(1, 4, h, 64, hs, cache, g)
+    q, kn, vn = (torch.randn(b, t, x, hs, generator=g).to(rows) for x in (heads, h, h))
+    far = torch.zeros(t, (20 << 20) // rows.itemsize, dtype=rows, device=DEV)
+    on = []
+    for i, x in enumerate((kn, vn)):
+        y = far[:, i * 4096:i * 4096 + b * h * hs].view(t, b, h, hs).transpose(0, 1)
+        y.copy_(x)
+        on.append(y)
+    tensors, table, lens = pool.tensors(layers=False), [[3, 1], [0, 2]], [100, 7]
+    want = pkg().page_attention(q.to(DEV), *tensors, ints(table), ints(lens), kn.to(DEV), vn.to(DEV))
+    assert torch.equal(want, pkg().page_attention(q.to(DEV), *tensors, ints(table), ints(lens), *on))
+    run(pool, table, q, lens, kn, vn, tensors=tensors)
+
+
 # ---- tile pairs and row waves: the host's bound of the lengths chooses them, so that short contexts reach them
 
 def work_bytes(h, rows, hs, b, most, max_n, block_rows, least):
