@@ -335,7 +335,7 @@ int llm_page_compact(const llm_pages *c, int n_seq, int *table, int per, int *re
  * token next[b] is drawn from w (from p_r where w is zero throughout): the first whose inclusive running sum is above coins[0]
  * times the whole.  A drafted token outside 0 .. vocab - 1 is turned down and changes nothing.  coins: n_seq x max_n floats in [0, 1).
  * What is drawn from, and with probs every probability, is in 64 bits; without them those of drafted tokens are off by 2^-17 of
- * themselves at most (2^-18 up to a vocabulary of 2^22).
+ * themselves at most (2^-18 up to a vocabulary of 2^22), of what their turned-down siblings leave by four times as much.
  * kept[b]: the nodes kept, node 0 among them; path[b * max_n + j], j < kept[b]: their numbers, rising, -1 behind them (as
  * llm_page_write takes them); next[b]; logp[b * max_n + i], 0 < i < n[b]: log p of node i's token after its parent (0 without a
  * parent, -infinity outside the vocabulary), and in its place 0 the log p of next[b].  n[b] < 1: kept 0, next -1.  A row with

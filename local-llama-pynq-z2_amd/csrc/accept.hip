@@ -454,6 +454,38 @@ __global__ void __launch_bounds__(AC_T) k_accept_left(AcArgs a, int round) {
     }
 }
 
+// The sum of a row's weights without the tokens of the lanes in `gone`, by the whole workgroup.  1 less a likely token's probability
+// would be off by as much as the row's sum, however little is left; this is off by 2^-17 of itself: hardware exponentials, their
+// exponents (60 more, so that 2^-180 of the largest weight still counts) by 2^-19, and eight chains of additions.  A sequence's pass
+// over 151936 fp32 logits: 12 us more for one, 24 for sixteen.
+template <int TY>
+__device__ __forceinline__ double rest_of(const AcArgs &a, const uint8_t *row, float m, int token, uint64_t gone, double *sm) {
+    constexpr int V = AC_V<TY>, E = 32, STEP = AC_T * E;
+    const float c = (float)a.c;
+    double s = 0.0;
+    for (int k = 0; k < a.vocab; k += STEP) {
+        auto index = [&](int e) { return k + (e / V * AC_T + (int)threadIdx.x) * V + e % V; };
+        float x[E], f[8] = {};
+        if (k + STEP <= a.vocab)
+#pragma unroll
+            for (int e = 0; e < E; e += V) values<TY, true>(row, index(e), a.vocab, -INFINITY, x + e);
+        else
+#pragma unroll
+            for (int e = 0; e < E; e += V) values<TY, false>(row, index(e), a.vocab, -INFINITY, x + e);
+        for (uint64_t out = gone; out; out &= out - 1) {
+            const int t = __builtin_amdgcn_readlane(token, __ffsll((unsigned long long)out) - 1);
+            if (t >= k && t - k < STEP)
+#pragma unroll
+                for (int e = 0; e < E; e++) x[e] = t == index(e) ? -INFINITY : x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) f[e % 8] += __builtin_amdgcn_exp2f(fmaf(x[e] - m, c, 60.0f));
+#pragma unroll
+        for (int i = 0; i < 8; i++) s += (double)f[i];
+    }
+    return block_add(s, sm) * 0x1p-60;
+}
+
 template <int TY, int PT> // PT: the type of the draft's probabilities, -1: none
 __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     constexpr int PQ = PT < 0 ? LLM_F32 : PT;
@@ -489,7 +521,9 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
     // the walk: from child to child, values of a lane read by all
     int node = 0;
     uint64_t kept = 1, gone = 0; // nodes on the way; children of the node that were turned down
-    double left = 1.0, aq = 0.0;
+    // Without draft probabilities `left` is 1 less what was turned down, as far off as the row's sum: where that has become a quarter
+    // it is summed anew (rest_of), and again where three quarters of that are gone.
+    double left = 1.0, aq = 0.0, sure = 0.25;
     uint64_t open = __ballot(parent == 0 && token >= 0);
     while (open) {
         const int c = __ffsll((unsigned long long)open) - 1;
@@ -506,22 +540,26 @@ __global__ void __launch_bounds__(AC_T) k_accept_walk(AcArgs a) {
             takes = coin * left < w;
         }
         if (takes) {
-            node = c, left = 1.0, aq = 0.0;
+            node = c, left = 1.0, aq = 0.0, sure = 0.25;
             kept |= (uint64_t)1 << c;
             gone = 0;
             open = __ballot(parent == node && token >= 0);
             continue;
         }
         gone |= (uint64_t)1 << c;
-        if (PT < 0) {
-            left = fmax(left - w, 0.0);
-            continue;
-        }
-        aq += left;
+        if (PT < 0) left = fmax(left - w, 0.0);
+        else aq += left;
         const int round = __popcll(gone) - 1;
-        if (open && a.left && round < 2) { // another child to hold against what is left
+        if (!open) continue;
+        // another child to hold against what is left
+        if (PT >= 0 && a.left && round < 2) {
             left = z_of(a, b, node, round);
-        } else if (open) {
+        } else if (PT < 0) {
+            if (left < sure && a.c != 0.0) {
+                left = rest_of<TY>(a, x + node * a.row, sm_m[node], token, gone, sm_sum) / sm_s[node];
+                sure = 0.25 * left;
+            }
+        } else {
             const uint8_t *row = x + node * a.row, *probs = q + node * a.p_row;
             double s = 0.0;
             const double inv = 1.0 / sm_s[node];
