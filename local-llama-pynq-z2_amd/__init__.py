@@ -607,16 +607,14 @@ def draft_accept(logits, tokens, coins, parents=None, n=None, probs=None, temper
                 torch.full((b,), -1, dtype=i32, device=logits.device), torch.empty(b, 0, device=logits.device))
     L = lib()
     need = L.llm_draft_accept_work(b, t, vocab)
-    # one allocation: the results, and the scratch memory behind them
-    have = b * (2 + 2 * t)
-    have += -have % 4
-    mem = torch.empty(have + need // 4, dtype=i32, device=logits.device)
-    kept, drawn, path, logp, _ = mem.split_with_sizes((b, b, b * t, b * t, mem.numel() - b * (2 + 2 * t)))
+    work = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    mem = torch.empty(b * (2 + 2 * t), dtype=i32, device=logits.device)  # the results
+    kept, drawn, path, logp = mem.split_with_sizes((b, b, b * t, b * t))
     p = mem.data_ptr()
     if b and L.llm_draft_accept(x, ty, b, t, vocab, seq, row, temperature, q, qy, q_seq, q_row, _ints("tokens", tokens, b * t, i32),
                                 _ints("parents", parents, b * t, i32), _ints("n", n, b, i32),
                                 _ints("coins", coins, b * t, torch.float32), p, p + 8 * b, p + 4 * b, p + 8 * b + 4 * b * t,
-                                p + 4 * have, need, _stream(logits)) != 0:
+                                work.data_ptr(), need, _stream(logits)) != 0:
         raise RuntimeError("llm_draft_accept failed")
     return kept, path.view(b, t), drawn, logp.view(torch.float32).view(b, t)
 

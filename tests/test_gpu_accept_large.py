@@ -1,8 +1,9 @@
 """llm_draft_accept where a likely token was turned down, for large batches and vocabularies, against its definition in float64."""
 import pytest
 
+from helpers import pkg
 from test_gpu_accept import check, inputs, run
-from test_gpu_pages import gen
+from test_gpu_pages import DEV, gen
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -80,3 +81,12 @@ def test_vocabularies_of_more_than_64_segments(v, kind, draft, temperature):
         coins[i, 0] = (at[i] + 0.5) / v
     coins[3, 0], coins[0, 0] = 1.0 - 2.0 ** -24, 0.0
     check(x, q, tokens, parents, coins, None, temperature, run(x, q, tokens, parents, coins, None, temperature))
+
+
+def test_results_do_not_hold_the_work_memory():
+    """a program that keeps what a call returned keeps a few KB of it"""
+    b, t, v = 3, 5, 70001
+    x, q, tokens, parents, coins = inputs(gen(4), b, t, v, "fp32", "fp32", False)
+    got = run(x, q, tokens, parents, coins, None, 1.0)
+    assert pkg().lib().llm_draft_accept_work(b, t, v) > 65536
+    assert all(y.untyped_storage().nbytes() <= 4096 and y.device.type == DEV for y in got)
