@@ -89,6 +89,12 @@ extern "C" int llm_page_attention(const llm_pages *c, const llm_rows *q, const l
     const int count[] = {n_seq, max_n, n_heads};
     const int64_t stride[] = {out->seq, out->tok, out->head};
     if (!op_check_apart(who, "out", 3, count, stride)) return -1;
+    PagePlan p = {};
+    if (max_n && n_seq) p = page_plan(c, n_seq, n_heads, max_n, max_len);
+    if (n_seq > 65535 || c->n_kv > 65535 || (p.row_blocks && page_blocks(c, n_seq, p) >= 1 << 24)) { // (a grid has 2^32 threads)
+        fprintf(stderr, "%s: %d sequences of %d kv heads\n", who, n_seq, c->n_kv);
+        return -1;
+    }
     OpDevice dev(who);
     if (!op_check_pages(c, &dev, who)) return -1;
     if (!max_n || !n_seq) return 0;
@@ -101,13 +107,8 @@ extern "C" int llm_page_attention(const llm_pages *c, const llm_rows *q, const l
         fprintf(stderr, "%s: q, out and the new rows are of different types\n", who);
         return -1;
     }
-    const PagePlan p = page_plan(c, n_seq, n_heads, max_n, max_len);
     if (p.bytes && (work_bytes < p.bytes || ((uintptr_t)work & 15) || !dev.holds(work, "the work memory"))) {
         fprintf(stderr, "%s: %zu bytes of work memory are needed, 16-byte aligned\n", who, p.bytes);
-        return -1;
-    }
-    if (page_blocks(c, n_seq, p) > 0x7fffffff || n_seq > 65535 || c->n_kv > 65535) {
-        fprintf(stderr, "%s: %d sequences of %d kv heads\n", who, n_seq, c->n_kv);
         return -1;
     }
     if (!dev.select()) return -1;

@@ -20,7 +20,10 @@ struct RowArgs {
     int64_t r_seq[2], r_tok[2], r_head[2];     // bytes
     const int *table, *refs, *pos, *n, *path;
     int per, n_pages, n_kv, hs, page, max_n, blocks, zero_rest;
+    uint32_t units; // workgroups of a side; a row of the grid has GRID_ROW of them at most (2^32 threads would not fit)
 };
+constexpr uint32_t GRID_ROW = 1 << 22;
+__device__ __forceinline__ uint32_t unit_id() { return blockIdx.z * GRID_ROW + blockIdx.x; }
 
 // Blocks that max_n tokens from any position on can reach.
 __host__ __device__ __forceinline__ int blocks_of(int max_n) { return (max_n + PAGE_BLOCK - 2) / PAGE_BLOCK + 1; }
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(WRITE_T) k_page_write(RowArgs a) {
     __shared__ uint32_t sm_max[WRITE_T / 64];
     __shared__ __align__(4) uint8_t sm_v[256 * TURN];
     Unit u;
-    if (!find_unit(a, blockIdx.x, u) || u.page < 0 || (a.refs && a.refs[u.page] != 1)) return;
+    if (unit_id() >= a.units || !find_unit(a, unit_id(), u) || u.page < 0 || (a.refs && a.refs[u.page] != 1)) return;
     const int side = blockIdx.y, per_row = a.hs / 4, items = (u.hi - u.lo) * per_row;
     uint8_t *const dst = a.c[side] + u.page * a.id + u.h * a.head + u.blk * (PAGE_BLOCK * a.hs);
     float *const scale = a.s[side] + u.page * a.s_id + u.h * a.s_head + u.blk;
@@ -195,7 +198,9 @@ template <int CT, int RT>
 __global__ void __launch_bounds__(256) k_page_read(RowArgs a) {
     constexpr int RS = RT == LLM_F32 ? 4 : 2;
     __shared__ __align__(4) uint8_t sm_v[PAGE_BLOCK * 260]; // V's codes by position
-    const int side = blockIdx.y, h = blockIdx.x % a.n_kv, x = blockIdx.x / a.n_kv, b = x / a.blocks;
+    const uint32_t id = unit_id();
+    if (id >= a.units) return;
+    const int side = blockIdx.y, h = id % a.n_kv, x = id / a.n_kv, b = x / a.blocks;
     const int64_t p0 = a.pos[b], at = ((p0 >> 6) + x % a.blocks) * PAGE_BLOCK; // (rounded down, below 0 too)
     const int lo = (int)max((int64_t)0, p0 - at), hi = (int)min((int64_t)PAGE_BLOCK, p0 + a.max_n - at); // offsets that rows are for
     if (lo >= hi) return;
@@ -279,13 +284,14 @@ int page_rows(const char *who, bool write, const llm_pages *c, const llm_rows *k
     a.table = table, a.refs = refs, a.pos = pos, a.n = n, a.path = path;
     a.per = per, a.n_pages = c->n_pages, a.n_kv = c->n_kv, a.hs = c->hs, a.page = c->page, a.max_n = max_n;
     a.blocks = blocks, a.zero_rest = zero_rest;
-    const unsigned grid = (unsigned)(n_seq * blocks * c->n_kv);
+    a.units = (uint32_t)(n_seq * blocks * c->n_kv);
+    const dim3 grid(std::min(a.units, GRID_ROW), 2, (a.units + GRID_ROW - 1) / GRID_ROW);
     void (*kern)(RowArgs) = nullptr;
 #define PAGE_PICK(C, R)                                                                   \
     if (c->type == C && k->type == R) kern = write ? k_page_write<C, R> : k_page_read<C, R>;
     PAGE_PICK(LLM_I8, LLM_F32) PAGE_PICK(LLM_I8, LLM_BF16) PAGE_PICK(LLM_E4M3, LLM_F32) PAGE_PICK(LLM_E4M3, LLM_BF16)
 #undef PAGE_PICK
-    hipLaunchKernelGGL(kern, dim3(grid, 2), dim3(write ? WRITE_T : 256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kern, grid, dim3(write ? WRITE_T : 256), 0, (hipStream_t)stream, a);
     HIP_OR_FAIL(who, hipGetLastError());
     return 0;
 }
@@ -596,6 +602,8 @@ MoveArgs move_args(const llm_pages *c) {
     return a;
 }
 
+constexpr int64_t MOST_UNITS = 1 << 25; // layers, heads and sides of a page: a wave each, and a grid has 2^32 threads
+
 bool work_ok(const char *who, void *work, size_t have, size_t need, unsigned align, OpDevice &dev) {
     if (!need || (have >= need && !((uintptr_t)work & (align - 1)) && dev.holds(work, "the work memory"))) return true;
     fprintf(stderr, "%s: %zu bytes of work memory are needed, %u-byte aligned\n", who, need, align);
@@ -709,7 +717,7 @@ extern "C" int llm_page_reserve(const llm_pages *c, int n_seq, int *table, int p
     }
     if (!op_check_pages(c, nullptr, who) || !op_check_table(table, n_seq, per, nullptr, who)) return -1;
     const int64_t units = (int64_t)2 * c->n_kv * c->n_layers;
-    if ((int64_t)n_seq * reach(per, c->page, max_n) > 1 << 30 || n_seq > 65535 || units > 0x7fffffff) {
+    if ((int64_t)n_seq * reach(per, c->page, max_n) > 1 << 30 || n_seq > 65535 || units > MOST_UNITS) {
         fprintf(stderr, "%s: %d sequences of %d tokens, %d layers of %d heads\n", who, n_seq, max_n, c->n_layers, c->n_kv);
         return -1;
     }
@@ -750,17 +758,20 @@ extern "C" int llm_page_compact(const llm_pages *c, int n_seq, int *table, int p
         return -1;
     }
     if (!op_check_pages(c, nullptr, who) || !op_check_table(table, n_seq, per, nullptr, who)) return -1;
-    OpDevice dev(who);
-    if (!op_check_pages(c, &dev, who) || (n_seq && !op_check_table(table, n_seq, per, &dev, who)) || !dev.holds(refs, "refs") ||
-        !dev.holds(result, "result") || !work_ok(who, work, work_bytes, llm_page_compact_work(c), 4, dev))
-        return -1;
     const int64_t entries = (int64_t)n_seq * per;
     const int movers = 2048;
-    if (entries > (int64_t)1 << 32) {
-        fprintf(stderr, "%s: a table of %d x %d\n", who, n_seq, per);
+    if (entries > (int64_t)1 << 31) { // (a thread each, of 2^32; looked at before the first launch changes the counts)
+        fprintf(stderr, "%s: a table of %d sequences, %d pages each\n", who, n_seq, per);
         return -1;
     }
-    if (!dev.select()) return -1;
+    if ((int64_t)2 * c->n_kv * c->n_layers > MOST_UNITS) {
+        fprintf(stderr, "%s: %d layers of %d heads\n", who, c->n_layers, c->n_kv);
+        return -1;
+    }
+    OpDevice dev(who);
+    if (!op_check_pages(c, &dev, who) || (n_seq && !op_check_table(table, n_seq, per, &dev, who)) || !dev.holds(refs, "refs") ||
+        !dev.holds(result, "result") || !work_ok(who, work, work_bytes, llm_page_compact_work(c), 4, dev) || !dev.select())
+        return -1;
     CompactArgs a;
     memset(&a, 0, sizeof a);
     a.n_pages = c->n_pages, a.n_seq = n_seq, a.per = per, a.table = table, a.refs = refs, a.result = result;

@@ -194,3 +194,22 @@ def test_tensors_that_require_a_gradient_are_refused():
                  2: lambda: P.page_compact(*pool, table, i), 3: lambda: P.draft_accept(x, i, i)}
         with pytest.raises(ValueError, match="no gradient"):
             calls[which]()
+
+
+def test_sizes_that_no_grid_holds_are_refused_before_anything_is_launched(capfd):
+    """tables and pools whose second launch would fail after the first has changed the books"""
+    assert compact(pages(), seqs=1 << 10, per=1 << 22) == -1
+    assert "a table of" in capfd.readouterr().err
+    assert compact(pages(), seqs=1 << 9, per=(1 << 22) - 1) == -1
+    assert "not device memory" in capfd.readouterr().err
+    for layers, says in ((1 << 12, "layers of"), ((1 << 11), "not device memory")):
+        c = pages(n_layers=layers, n_pages=2, n_kv=1 << 13, hs=16, layer=1 << 24, id=1 << 23, head=1 << 10, s_layer=1 << 14,
+                  s_id=1 << 13, s_head=1)
+        for call in (compact, reserve):
+            assert call(c) == -1
+            assert says in capfd.readouterr().err
+    wide = pages(n_kv=512, hs=16, id=512 * 1024, head=1024, s_id=512, s_head=1)
+    for kw, says in ((dict(seqs=65536), "sequences of 512 kv heads"), (dict(seqs=32769), "sequences of 512 kv heads"),
+                     (dict(seqs=32767), "not device memory")):
+        assert attend(wide, heads=512, **kw) == -1
+        assert says in capfd.readouterr().err
