@@ -169,6 +169,10 @@ int kv_rows(const char *who, bool write, const llm_kv *c, const llm_rows *k, con
             if (!op_check_apart(who, "the rows", 3, count, stride)) return -1;
         }
     }
+    if ((__int128)c->n_seq * max_n * c->n_kv >= 1 << 28) { // (16 threads a row, and a grid has 2^32)
+        fprintf(stderr, "%s: %d sequences of %d rows\n", who, c->n_seq, max_n);
+        return -1;
+    }
     OpDevice dev(who);
     if (!op_check_cache(c, &dev, who)) return -1;
     if (!max_n || !c->n_seq) return 0;
@@ -181,10 +185,6 @@ int kv_rows(const char *who, bool write, const llm_kv *c, const llm_rows *k, con
     }
     if (k->type != v->type) {
         fprintf(stderr, "%s: k and v rows of different types\n", who);
-        return -1;
-    }
-    if ((int64_t)c->n_seq * max_n * c->n_kv > 0x7fffffff) {
-        fprintf(stderr, "%s: %d sequences of %d rows\n", who, c->n_seq, max_n);
         return -1;
     }
     if (!dev.select()) return -1;

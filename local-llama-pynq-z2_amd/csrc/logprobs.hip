@@ -391,18 +391,18 @@ extern "C" int llm_logprobs(const void *logits, int type, int rows, int vocab, i
         return -1;
     }
     if (!rows) return 0;
+    const LpPlan p = lp_plan(rows, vocab, top);
+    if ((int64_t)rows * p.seg * LP_T >= (int64_t)1 << 32) { // (a grid's threads)
+        fprintf(stderr, "%s: %d rows\n", who, rows);
+        return -1;
+    }
     OpDevice dev(who);
     if (!dev.holds(logits, "logits") || (n_tokens && (!dev.holds(tokens, "tokens") || !dev.holds(logp, "logp"))) ||
         (entropy && !dev.holds(entropy, "entropy")) || (lse && !dev.holds(lse, "lse")) ||
         (top && (!dev.holds(top_ids, "top_ids") || !dev.holds(top_logp, "top_logp"))))
         return -1;
-    const LpPlan p = lp_plan(rows, vocab, top);
     if (p.bytes && (work_bytes < p.bytes || ((uintptr_t)work & 15) || !dev.holds(work, "the work memory"))) {
         fprintf(stderr, "%s: %zu bytes of work memory are needed, 16-byte aligned\n", who, p.bytes);
-        return -1;
-    }
-    if ((int64_t)rows * p.seg > 0x7fffffff) {
-        fprintf(stderr, "%s: %d rows\n", who, rows);
         return -1;
     }
     if (!dev.select()) return -1;

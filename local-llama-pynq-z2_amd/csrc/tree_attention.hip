@@ -140,6 +140,13 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
     const int count[] = {c->n_seq, max_n, n_heads};
     const int64_t stride[] = {out->seq, out->tok, out->head};
     if (!op_check_apart(who, "out", 3, count, stride)) return -1;
+    TreePlan p = {};
+    if (max_n && c->n_seq) p = tree_plan(c, q->type, n_heads, max_n, max_len);
+    if (c->n_seq > 65535 || c->n_kv > 65535 ||
+        (p.row_blocks && tree_blocks(*c, p) * (p.many ? 64 * p.many : 256) >= (int64_t)1 << 32)) { // (a grid's threads)
+        fprintf(stderr, "%s: %d sequences of %d kv heads\n", who, c->n_seq, c->n_kv);
+        return -1;
+    }
     OpDevice dev(who);
     if (!op_check_cache(c, &dev, who)) return -1;
     if (!max_n || !c->n_seq) return 0;
@@ -150,13 +157,8 @@ extern "C" int llm_tree_attention(const llm_kv *c, const llm_rows *q, const llm_
         fprintf(stderr, "%s: q and out of different types\n", who);
         return -1;
     }
-    const TreePlan p = tree_plan(c, q->type, n_heads, max_n, max_len);
     if (p.bytes && (work_bytes < p.bytes || ((uintptr_t)work & 15) || !dev.holds(work, "the work memory"))) {
         fprintf(stderr, "%s: %zu bytes of work memory are needed, 16-byte aligned\n", who, p.bytes);
-        return -1;
-    }
-    if (tree_blocks(*c, p) > 0x7fffffff || c->n_seq > 65535 || c->n_kv > 65535) {
-        fprintf(stderr, "%s: %d sequences of %d kv heads\n", who, c->n_seq, c->n_kv);
         return -1;
     }
     if (!dev.select()) return -1;

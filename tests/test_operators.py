@@ -109,3 +109,20 @@ def test_models_refused():
     assert L.llm_verify(None, 0, ids, None, 2, None, None, None) == -1
     assert L.llm_keep(None, 0, ids, 2) == -1
     assert L.llm_score(None, ids, 2, 1.0, None, None, 0, None, None) == -1
+
+
+def test_sizes_that_no_grid_holds_are_refused(capfd):
+    """2^32 threads and more: such a launch would do nothing, or a part, without an error"""
+    big = dict(n_kv=1, hs=16, seq=16, head=16, pos=16, s_seq=1, s_head=1, ctx=1)
+    assert write(cache(n_seq=1 << 16, **big), n=1 << 12) == -1
+    assert "65536 sequences of 4096 rows" in capfd.readouterr().err
+    assert write(cache(n_seq=1 << 16, **big), n=(1 << 12) - 1) == -1
+    assert "not device memory" in capfd.readouterr().err
+    wide = dict(n_kv=512, hs=16, seq=512 * 16, head=16, pos=16, s_seq=512, s_head=1, ctx=1)
+    for n_seq, says in ((65536, "kv heads"), (65535, "kv heads"), (16383, "not device memory")):
+        assert attend(cache(n_seq=n_seq, **wide), heads=512) == -1
+        assert says in capfd.readouterr().err
+    assert logp(rows=1 << 25) == -1 and logp(rows=1 << 24) == -1
+    assert capfd.readouterr().err.count("rows\n") == 2
+    assert logp(rows=(1 << 24) - 1) == -1
+    assert "not device memory" in capfd.readouterr().err
