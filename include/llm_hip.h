@@ -311,7 +311,9 @@ int llm_page_fork(int n_pages, int page, int n_seq, int *table, int per, int *le
  * and replaced by a free one, into which the blocks that hold positions below lens[b] are copied, of all layers; only where all
  * that share a page ask for it in this call, the last of them (by number) keeps it.  Everything or nothing: result[0] = 1, and
  * result[1] the pages taken; or result[0] = 0, the tables as they were and result[1] the pages wanted, where so many are not
- * free, a sequence does not fit its row of the table (which wants none then) or n[b] is above max_n.  Work: llm_page_reserve_work() bytes, 16-byte aligned. */
+ * free, a sequence does not fit its row of the table (which wants none then) or n[b] is above max_n.  Rows that are written and
+ * lengths that grow without asking result[0] leave positions without a page, which nothing sees: n[b] * result[0] is what may
+ * be added.  Work: llm_page_reserve_work() bytes, 16-byte aligned. */
 size_t llm_page_reserve_work(const llm_pages *c, int n_seq, int per, int max_n);
 int llm_page_reserve(const llm_pages *c, int n_seq, int *table, int per, int *refs, const int *lens, const int *n, int max_n,
                      int *result, void *work, size_t work_bytes, void *stream);

@@ -547,7 +547,8 @@ def page_fork(table, lens, refs, to, source, page):
 def page_reserve(k, v, k_scale, v_scale, table, refs, lens, n, max_n=None):
     """Room for n[b] (int32; at most max_n, None: a table's row) more tokens of every sequence in pages of its own, shared ones
     copied in all layers (llm_page_reserve).  The pages as in page_attention, with the layers first where there are more.  Returns
-    int32 (1, pages taken), or (0, pages wanted) with nothing changed where there is no room."""
+    int32 (1, pages taken), or (0, pages wanted) with nothing changed where there is no room: what is written and added to lens
+    then is n * result[0]."""
     _no_grad(k_scale, v_scale)
     c, (_, pages, _, page, _) = _pages(k, v, k_scale, v_scale)
     (at, (b, per)), torch, L = _table(table), _torch[0], lib()
