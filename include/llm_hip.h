@@ -291,7 +291,8 @@ int llm_page_read(const llm_pages *c, const llm_rows *k, const llm_rows *v, int 
  * What is not seen changes no bit, infinities and NaN included; a new token whose V row holds one makes the tokens that see it
  * NaN, a block whose scale is one of them makes those NaN that see any of its positions.
  * Sums are fp32.  Over pages a query holds 22 bits of its largest value (bf16 queries: all their bits down to 2^-39 of it), and a
- * weight 22 bits and no finer step than 2^-39 of the row's largest weight in the block.  Over the new rows both hold fp32.
+ * weight 22 bits and no finer step than 2^-39 of the row's largest weight in the block.  Over the new rows both hold fp32.  Sums
+ * of values below 2^-90 may lose bits to fp32's smallest numbers.
  * n_heads / n_kv is at most 64.  max_len is the host's upper bound of lens[] (lens above it are right too, slower); `work`
  * has llm_page_attention_work() bytes, 16-byte aligned, and is one call's until it has run. */
 size_t llm_page_attention_work(const llm_pages *c, int n_seq, int n_heads, int max_n, int max_len);

@@ -23,7 +23,12 @@ struct RowArgs {
     uint32_t units; // workgroups of a side; a row of the grid has GRID_ROW of them at most (2^32 threads would not fit)
 };
 constexpr uint32_t GRID_ROW = 1 << 22;
-__device__ __forceinline__ uint32_t unit_id() { return blockIdx.z * GRID_ROW + blockIdx.x; }
+// The workgroup's, 0 behind the last (`over`: no branch, so that the arguments' loads stay together).
+__device__ __forceinline__ uint32_t unit_id(const RowArgs &a, bool &over) {
+    const uint32_t id = blockIdx.z * GRID_ROW + blockIdx.x;
+    over = id >= a.units;
+    return over ? 0 : id;
+}
 
 // Blocks that max_n tokens from any position on can reach.
 __host__ __device__ __forceinline__ int blocks_of(int max_n) { return (max_n + PAGE_BLOCK - 2) / PAGE_BLOCK + 1; }
@@ -33,7 +38,9 @@ struct Unit {
     int b, h, page, blk, lo, hi;
     int64_t first; // the token at offset 0 (below 0 if it is not of this call)
 };
-__device__ __forceinline__ bool find_unit(const RowArgs &a, uint32_t id, Unit &u) {
+__device__ __forceinline__ bool find_unit(const RowArgs &a, Unit &u) {
+    bool over;
+    const uint32_t id = unit_id(a, over);
     u.h = id % a.n_kv;
     const uint32_t x = id / a.n_kv;
     u.b = x / a.blocks;
@@ -42,7 +49,7 @@ __device__ __forceinline__ bool find_unit(const RowArgs &a, uint32_t id, Unit &u
     const int64_t at = (max(p0, (int64_t)0) / PAGE_BLOCK + x % a.blocks) * PAGE_BLOCK; // the block's first position
     const int64_t lo = max(p0, at), hi = min(end, at + PAGE_BLOCK);
     u.page = -1;
-    if (lo >= hi) return false;
+    if (over || lo >= hi) return false;
     u.lo = (int)(lo - at), u.hi = (int)(hi - at);
     u.first = at - p0;
     u.page = a.table[(int64_t)u.b * a.per + at / a.page];
@@ -121,7 +128,7 @@ __global__ void __launch_bounds__(WRITE_T) k_page_write(RowArgs a) {
     __shared__ uint32_t sm_max[WRITE_T / 64];
     __shared__ __align__(4) uint8_t sm_v[256 * TURN];
     Unit u;
-    if (unit_id() >= a.units || !find_unit(a, unit_id(), u) || u.page < 0 || (a.refs && a.refs[u.page] != 1)) return;
+    if (!find_unit(a, u) || u.page < 0 || (a.refs && a.refs[u.page] != 1)) return;
     const int side = blockIdx.y, per_row = a.hs / 4, items = (u.hi - u.lo) * per_row;
     uint8_t *const dst = a.c[side] + u.page * a.id + u.h * a.head + u.blk * (PAGE_BLOCK * a.hs);
     float *const scale = a.s[side] + u.page * a.s_id + u.h * a.s_head + u.blk;
@@ -198,12 +205,12 @@ template <int CT, int RT>
 __global__ void __launch_bounds__(256) k_page_read(RowArgs a) {
     constexpr int RS = RT == LLM_F32 ? 4 : 2;
     __shared__ __align__(4) uint8_t sm_v[PAGE_BLOCK * 260]; // V's codes by position
-    const uint32_t id = unit_id();
-    if (id >= a.units) return;
+    bool over;
+    const uint32_t id = unit_id(a, over);
     const int side = blockIdx.y, h = id % a.n_kv, x = id / a.n_kv, b = x / a.blocks;
     const int64_t p0 = a.pos[b], at = ((p0 >> 6) + x % a.blocks) * PAGE_BLOCK; // (rounded down, below 0 too)
     const int lo = (int)max((int64_t)0, p0 - at), hi = (int)min((int64_t)PAGE_BLOCK, p0 + a.max_n - at); // offsets that rows are for
-    if (lo >= hi) return;
+    if (over || lo >= hi) return;
     const int nn = a.n ? min(max(a.n[b], 0), a.max_n) : a.max_n;
     int page = -1;
     if (at >= 0 && at < (int64_t)a.per * a.page) page = a.table[(int64_t)b * a.per + at / a.page];
