@@ -19,21 +19,24 @@ struct PagePlan {
 
 // How a call is cut.  Times: one call, heads of 128, int8 pages.
 // Rows.  The four waves of a workgroup share the positions, with one tile of 16 rows, or two where that is work enough: two read
-// and convert the codes half as often, one gives twice the workgroups (448 rows of bf16 over 4 x 8000 positions, 4 kv heads: 72
-// us with one, 61 with two; 259 over 12k: bf16 38.4 and 34.4, fp32 41.2 and 40.7, over 6k 27.0 and 29.5, 29.4 and 30.8).  Many
-// rows over long contexts: the waves have two other tiles each of the same positions, which need no join of waves, and whose pages
-// the L1 then holds for all four (448 rows over eight sequences of up to 16k: 128 us and 117; fp32 over two of 16k: 108 and 85,
-// over eight of 3000: 62 and 63).
+// and convert the codes half as often, one gives twice the workgroups.  One sequence, one tile and two, bf16 rows and fp32: 37
+// tokens of 7 heads over 9500 positions 32.0 and 33.2, 32.3 and 32.1 us, over 10500 34.0 and 33.8, 33.5 and 32.8, over 11500 35.1
+// and 32.9, 35.4 and 34.5; 16 tokens over 26k 30.8 and 31.7, 31.5 and 33.3, over 30k 33.8 and 33.2, 34.5 and 34.5; 64 over 5000
+// 30.1 and 29.7, 30.3 and 30.5, over 6000 33.3 and 31.7, 33.7 and 32.9: they cross between 1.1e6 and 1.6e6.  Several: 448 rows over
+// 4 x 8000 70.6 and 62.0, 73.2 and 64.7.  Many rows over long contexts: the waves have two other tiles each of the same positions,
+// which need no join of waves, and whose pages the L1 then holds for all four (448 rows over eight sequences of up to 16k: 200 us
+// with waves over positions, 139 over rows; over eight of 3000 55 and 61, over two of 16k 72 and 72, fp32 58 and 62, 77 and 83).
 // Positions.  One sequence: as many slices as give a workgroup a CU, or two a CU where whole row blocks would leave much of the
 // chip idle.  Several: two workgroups a CU over all sequences, of equal steps (more of them cost more in find_slice and the join
-// than they even out: 32 decode steps over 0 to 8190 e4m3 positions 32 us, with four a CU 38).
+// than they even out: 32 decode steps over 0 to 8190 e4m3 positions 32 us, with four a CU 35; with heads of 64 15.3 and 19.1, of
+// int8 and fp32 rows 16.0 and 19.8, with six heads of 48 18.1 and 20.8).
 PagePlan page_plan(const llm_pages *c, int n_seq, int n_heads, int max_n, int max_len) {
     PagePlan p;
     p.hsp = (c->hs + 63) / 64 * 64;
     const int group = n_heads / c->n_kv, rows = group * max_n, tiles = (rows + 15) / 16;
     const int64_t heads = (int64_t)n_seq * c->n_kv, blocks = ((int64_t)std::max(max_len, 0) + PAGE_BLOCK - 1) / PAGE_BLOCK;
     const double work = p.hsp <= 128 && tiles > 1 ? (double)tiles * heads * blocks * p.hsp : 0.0;
-    p.tiles = work >= (n_seq > 1 ? 2e6 : 1.6e6) ? 2 : 1; // (of several sequences most are shorter than max_len)
+    p.tiles = work >= (n_seq > 1 ? 2e6 : 1.4e6) ? 2 : 1; // (of several sequences most are shorter than max_len)
     p.rows = work >= 6e6 && tiles > 8;
     p.block_rows = 16 * p.tiles * (p.rows ? 4 : 1);
     p.row_blocks = (rows + p.block_rows - 1) / p.block_rows;

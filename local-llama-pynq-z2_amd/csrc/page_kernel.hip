@@ -22,8 +22,8 @@
 // What bounds it.  Few rows: memory (32 decode steps of 7 query heads a kv head over 131 MB of e4m3 pages: 27.4 us, 4.8 TB/s), or
 // with few positions a chain of dependent loads (arguments, length, page, codes, the new row: 7.0 us for 203 positions of heads
 // of 64, 5.6 of it with none).  Many rows: vector instructions, which turn codes into fp16 and make the weights (a step of two
-// tiles of bf16 rows over int8 pages: 585, of which 192 are for the codes, beside 68 products); 448 rows of each of eight
-// sequences over up to 16k positions: 112 us, 386 TFLOP/s.
+// tiles of bf16 rows over int8 pages: 676, of which 320 are for the codes, beside 104 products); 448 rows of each of eight
+// sequences over up to 16k positions: 139 us, 312 TFLOP/s.
 #include "device.h"
 #include "page_attention.h"
 
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(256, (HSP <= 128 ? 2 : 1)) k_page_attention(Pa
         const int left = page < 0 ? 0 : p.len - step * PAGE_BLOCK; // positions of the block that are seen
         const int mine = left - (int)again(16 * j);                // of the lane's 16
         // (products first: of a SIMD's two waves the one that makes weights then fills in.  Eight trees of 64 fp32 rows over up to
-        // 16k int8 positions: 161 us without, 157 with it; two over e4m3 85 and 81, sixteen of 33 with heads of 64 66 and 61)
+        // 16k int8 positions: 164 us without, 156 with it, bf16 rows 145 and 139; two over e4m3 77 and 74, 69 and 66)
         __builtin_amdgcn_s_setprio(1);
         f32x4 x[R][4];
 #pragma unroll
