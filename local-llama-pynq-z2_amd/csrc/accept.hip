@@ -11,12 +11,12 @@
 // Sums and exponentials that decide are in 64 bits: a token drawn in the tail of 150k stands between borders 1e-6 apart, which an
 // error of 2^-24 in the likeliest token's weight would all move by 6e-8.
 //
-// What bounds it: the rows' bytes, read once.  16 trees of up to 37 rows of 151936 bf16 logits, 154 MB: 26.5 us, 5.8 TB/s, for
+// What bounds it: the rows' bytes, read once.  16 trees of up to 37 rows of 151936 bf16 logits, 154 MB: 25.5 us, 6.0 TB/s, for
 // the rows (the last call left a part of them in the caches) and 17.0 for the walk; a chain of 6 fp32 rows with draft
-// probabilities: 4.1 and 10.9.  The walk is a chain of short steps (of that chain, in thousands of cycles: the parts' loads and
+// probabilities: 4.1 and 10.7.  The walk is a chain of short steps (of that chain, in thousands of cycles: the parts' loads and
 // join and the tokens' probabilities 5.6, the walk 1.5, a segment's sum 7.6, the count 1.6, the choice of a segment 2.2, of a
 // token 3.5), each code that runs once: fetching it is a part of the time.  Trees with draft probabilities need a row's pass for
-// each child with a later sibling that is turned down: see k_accept_ask.
+// each child with a later sibling that is turned down: see k_accept_ask; trees without where a likely one is: see rest_of.
 #include <string.h>
 
 #include <algorithm>
@@ -161,7 +161,7 @@ __device__ __forceinline__ double upto(double v) { // inclusive sum over a wave:
 // EXACT: exponentials in 64 bits, for draft probabilities, which are held against p itself; without them a row's sum only decides
 // about its children and log probabilities, and it takes those of the hardware in 32 bits: off by 2^-18 of itself for rows up to
 // 2^22 (three roundings of the exponent, the instruction's, eight chains of additions); what is drawn from is summed in 64 bits by
-// the walk.  16 trees of 37 bf16 rows: 26.5 us, with the series in 64 bits 70.
+// the walk.  A call of 16 trees of 37 bf16 rows: 43 us, with the series in 64 bits 80.
 template <int TY, int PER, bool EXACT>
 __global__ void __launch_bounds__(AC_T) k_accept_rows(AcArgs a) {
     constexpr int V = AC_V<TY>, E = AC_E * PER;

@@ -120,8 +120,8 @@ constexpr int TURN = 68; // bytes from row to row of a turned block in LDS: rows
 
 // The rows of a block: their largest magnitude decides the scale, then their codes; a workgroup a block and side.  The rows are
 // read once, all loads at once, and wait in registers; V's codes are turned in LDS.  2048 fp32 rows of 4 heads of 128, 8.4 MB:
-// 8.6 us, bound by the codes' vector instructions (16.3 with exact quotients for all and V stored byte by byte); one row: 4.2 us,
-// dependent loads.
+// 8.6 us (16.3 with exact quotients for all and V stored byte by byte), bound by its phases one after another with a workgroup a
+// CU: of a wave's 15k cycles it waits for 8.9k, vector instructions are issued in 28% of a SIMD's; one row: 4.2 us, dependent loads.
 template <int CT, int RT>
 __global__ void __launch_bounds__(WRITE_T) k_page_write(RowArgs a) {
     constexpr int RS = RT == LLM_F32 ? 4 : 2, ITEMS = 64 * 256 / 4 / WRITE_T; // of four values a thread
@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(WRITE_T) k_page_write(RowArgs a) {
 }
 
 // The same the other way: a workgroup a block of the cache and side, its rows out of the block's codes (V's by LDS, whose rows of
-// hs + 4 bytes spread over the banks).  7069 rows of 4 heads of 128, 29 MB of fp32 out of 7.2: 10.2 us, bound by the stores.
+// hs + 4 bytes spread over the banks).  7069 rows of 4 heads of 128, 29 MB of fp32 out of 7.2: 10.0
+// us, 3.6 TB/s; of a wave's 14.5k cycles it waits for 9.2k, vector instructions are issued in a quarter of a SIMD's.
 template <int CT, int RT>
 __global__ void __launch_bounds__(256) k_page_read(RowArgs a) {
     constexpr int RS = RT == LLM_F32 ? 4 : 2;
